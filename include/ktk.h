@@ -533,6 +533,83 @@ KTK_API int ktk_paged_sv(const void* kv_cache, const int32_t* kv_indices, const 
                          void* out, const ktk_shape* shape, int32_t* status, void* stream);
 
 /*
+ * A cache of bounded size: attention that adds up what every cached token was paid, and the eviction of the tokens that were
+ * paid least.  No counterpart in the reference, whose masks (LiteSys/litesys/attention/sparsity_utils.py) choose among tokens
+ * that all stay in the cache.
+ *
+ * ktk_mass: fp32 [rows, Hkv, stride], the weights that the query heads of a group have given, so far, to the token in each place
+ * of a sequence's cache (place = its number in the order of the page table: with a sink page, token t lies in place t).  Row of
+ * sequence b: view->slot_index[b], else b; the sequences of a call have different rows.  `out` may be `in`, or memory apart from it;
+ * places behind a sequence's length are left as they are.
+ *   in, out   device pointers; where they differ, `in` is only read
+ *   rows      rows of the array: a row outside reports KTK_STATUS_BAD_TABLE and is skipped, as is a sequence longer than `stride`
+ *   decay     factor of what was there before
+ */
+typedef struct ktk_mass {
+    const float* in;
+    float* out;
+    int64_t stride;
+    int32_t rows;
+    float decay;
+} ktk_mass;
+
+/*
+ * ktk_dense_decode_v that also accumulates: with p_hq(t) the softmax weights of query head hq,
+ *   out[r, h, t] = decay * in[r, h, t] + sum_{hq of group h} p_hq(t)          for t < n - 1,
+ * and without the first term for the newest token t = n - 1, whose place may still hold what an earlier token was paid.
+ * The weights are those of fp32 scores and denominators.
+ *   total_pages  an upper bound of the entries in all lists (sizes the workspace), or -1: batch * max_pages_per_seq, which is
+ *                also what counts with view->page_count
+ *   workspace    ktk_decode_mass_workspace_bytes() bytes: the scores of all tokens, and the partials of lists that are cut
+ * q, kv_cache, o and workspace are 16-byte aligned.
+ */
+KTK_API size_t ktk_decode_mass_workspace_bytes(const ktk_shape* shape, int32_t max_pages_per_seq, int64_t total_pages);
+KTK_API int ktk_dense_decode_mass(const void* q, const void* kv_cache, const int32_t* kv_indices, const int32_t* kv_indptr,
+                                  const int32_t* kv_last_page_len, const ktk_view* view, int32_t max_pages_per_seq,
+                                  int64_t total_pages, float sm_scale, const ktk_mass* mass, void* o, void* workspace,
+                                  size_t workspace_bytes, const ktk_shape* shape, int32_t* status, void* stream);
+
+/*
+ * ktk_prefill_attention that also accumulates what the new tokens pay:
+ *   out[r, h, t] = decay * in[r, h, t] + sum over the last `window` new tokens and the heads of group h of p(t)
+ * for the tokens t that were there before, and without the first term for the sequence's new ones.  window 0: all new tokens.
+ * A sequence without new tokens is left as it is.
+ *   max_tokens   an upper bound of the tokens of any one sequence (sizes the grid)
+ *   workspace    ktk_prefill_mass_workspace_bytes() bytes: the rows' denominators
+ * q, kv_cache, o and workspace are 16-byte aligned.
+ */
+KTK_API size_t ktk_prefill_mass_workspace_bytes(const ktk_shape* shape, int64_t total_new_tokens);
+KTK_API int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr, int64_t total_new_tokens,
+                                       int32_t max_new_tokens, const void* kv_cache, const int32_t* kv_indices,
+                                       const int32_t* kv_indptr, const int32_t* kv_last_page_len, const ktk_view* view,
+                                       int64_t max_tokens, int32_t window, float sm_scale, const ktk_mass* mass, void* o,
+                                       void* workspace, size_t workspace_bytes, const ktk_shape* shape, int32_t* status,
+                                       void* stream);
+
+/*
+ * Eviction: of every (sequence, kv head) with more than `keep` tokens, `keep` stay -- the tokens at positions < sink, those of the
+ * last `recent` positions, and of the others the ones of largest mass (ties: the lowest place; NaN counts as less than all).
+ * The kept tokens behind place `keep` move, in their order, into the places in front of it that became free, in theirs: only their
+ * keys, values, masses and positions are copied.  Attention does not depend on the order of cached tokens.  The sequence then
+ * holds min(n, keep) tokens: the caller's next page table says so.  Summaries of its pages (ktk_build_summaries) are out of date.
+ *   positions_in  int32 [mass->rows, Hkv, mass->stride]: positions of the tokens in the first stored[row] places; the token in
+ *                 place t >= stored[row] of n was appended in order and has position seen[row] - n + t
+ *   positions_out the same array, or memory apart from it: receives the positions of all min(n, keep) places
+ *   stored, seen  int32 [mass->rows]: see above; tokens that the sequence has been given in all
+ *   mass->in/out  as above; `out` receives the masses of all min(n, keep) places; decay plays no part
+ *   max_pages_per_seq   an upper bound of a sequence's pages, at most 32768 (a longer sequence reports KTK_STATUS_BAD_TABLE and is
+ *                 left alone)
+ *   workspace     ktk_evict_workspace_bytes() bytes: which token moves where
+ * sink + recent <= keep, keep >= 1.  shape->group_size plays no part.
+ */
+KTK_API size_t ktk_evict_workspace_bytes(const ktk_shape* shape, int32_t max_pages_per_seq, int32_t keep);
+KTK_API int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                      const ktk_view* view, int32_t max_pages_per_seq, const ktk_mass* mass, const int32_t* positions_in,
+                      int32_t* positions_out, const int32_t* stored, const int32_t* seen, int32_t keep, int32_t sink,
+                      int32_t recent, void* workspace, size_t workspace_bytes, const ktk_shape* shape, int32_t* status,
+                      void* stream);
+
+/*
  * Host-side page pool for continuous batching.  No CUDA call, no device memory: the pool decides
  * which physical pages of the KV cache a sequence slot owns and writes the CSR arrays the kernels
  * read.  The reference has no counterpart: its benchmark uses one static interleaved table

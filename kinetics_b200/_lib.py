@@ -73,6 +73,11 @@ class View(ctypes.Structure):
                 ("slot_index", c_void_p), ("seq_order", c_void_p)]
 
 
+class Mass(ctypes.Structure):
+    """ktk_mass"""
+    _fields_ = [("in_", c_void_p), ("out", c_void_p), ("stride", c_int64), ("rows", c_int32), ("decay", c_float)]
+
+
 _i32p = c_void_p   # device pointers travel as integers
 #: host-side entry points that both libraries carry
 _HOST_SIGNATURES = {
@@ -155,6 +160,16 @@ _SIGNATURES = {
                                POINTER(Shape), _i32p, c_void_p]),
     "ktk_qkv_norm_rope": (c_int32, [c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_int64,
                                     c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p]),
+    "ktk_decode_mass_workspace_bytes": (c_size_t, [POINTER(Shape), c_int32, c_int64]),
+    "ktk_dense_decode_mass": (c_int32, [c_void_p, c_void_p, _i32p, _i32p, _i32p, POINTER(View), c_int32, c_int64, c_float,
+                                        POINTER(Mass), c_void_p, c_void_p, c_size_t, POINTER(Shape), _i32p, c_void_p]),
+    "ktk_prefill_mass_workspace_bytes": (c_size_t, [POINTER(Shape), c_int64]),
+    "ktk_prefill_attention_mass": (c_int32, [c_void_p, _i32p, c_int64, c_int32, c_void_p, _i32p, _i32p, _i32p, POINTER(View),
+                                             c_int64, c_int32, c_float, POINTER(Mass), c_void_p, c_void_p, c_size_t,
+                                             POINTER(Shape), _i32p, c_void_p]),
+    "ktk_evict_workspace_bytes": (c_size_t, [POINTER(Shape), c_int32, c_int32]),
+    "ktk_evict": (c_int32, [c_void_p, _i32p, _i32p, _i32p, POINTER(View), c_int32, POINTER(Mass), _i32p, _i32p, _i32p, _i32p,
+                            c_int32, c_int32, c_int32, c_void_p, c_size_t, POINTER(Shape), _i32p, c_void_p]),
     "ktk_silu_mul": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
     "ktk_linear_rows": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int32,
                                    c_void_p]),

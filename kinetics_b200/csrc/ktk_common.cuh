@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "ktk.h"
 
 namespace ktk {
@@ -19,6 +21,10 @@ int check_shape(const ktk_shape* s, const char* who);
 int cuda_fail(cudaError_t e, const char* who);
 int sm_count();
 int check_view(const ktk_view* v, const char* who);
+int check_mass(const ktk_mass* m, const char* who);
+// the same memory, or memory apart
+int check_apart(const void* a, const void* b, size_t bytes, const char* who, const char* what);
+int check_aligned(std::initializer_list<const void*> pointers, const char* who);      // to 16 bytes
 
 // a ktk_view with the defaults filled in
 struct View {

@@ -40,9 +40,10 @@ __device__ __forceinline__ void halve(float (&part)[kPageSize], int lane) {
     }
 }
 
-template <typename T, int G>
+// MASS: also writes the scores, and its partials whatever the number of splits.
+template <typename T, int G, bool MASS = false>
 __global__ void __launch_bounds__(kSimtWarps * 32)
-decode_simt_kernel(const DecodeParams p) {
+decode_simt_kernel(const DecodeParams p, const MassParams mp) {
     using R = typename Raw4<T>::type;
     constexpr bool kPrefetch = sizeof(T) == 2;   // a page is 64 registers in bf16, 128 in fp32
     __shared__ __align__(16) float p_sm[kSimtWarps][kPageSize * G];   // probabilities [t][g]
@@ -102,6 +103,7 @@ decode_simt_kernel(const DecodeParams p) {
     };
 
     // one page of the warp: scores, online softmax, weighted values
+    const int64_t position = MASS ? list_position(p, mp.wmax, b, h) : 0;
     auto consume = [&](int e, const R (&kr)[kPageSize], const R (&vr)[kPageSize]) {
         const int ntok = entry_tokens(el, e);
         const int tok = lane >> 1;               // the token this lane ends up holding
@@ -123,6 +125,12 @@ decode_simt_kernel(const DecodeParams p) {
             halve<1>(part, lane);
             part[0] += __shfl_xor_sync(0xffffffffu, part[0], 1);
             s[g] = (tok < ntok) ? part[0] : -INFINITY;
+        }
+        if constexpr (MASS) {
+            if ((lane & 1) == 0 && tok < ntok && position + e < mp.positions) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) mp.scores[((position + e) * kPageSize + tok) * G + g] = s[g];
+            }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -205,8 +213,9 @@ decode_simt_kernel(const DecodeParams p) {
             }
         }
         const int64_t qh = (int64_t)b * Hq + (int64_t)h * G + g;
-        if (S == 1) {
+        if (!MASS && S == 1) {
             ((T*)p.o)[qh * kHeadDim + d] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
+            if (p.lse != nullptr && d == 0) p.lse[qh] = M + log2f(L);
         } else {
             p.ws_o[(qh * S + split) * kHeadDim + d] = O;
             if (d == 0) {
@@ -240,25 +249,30 @@ combine_kernel(const float* __restrict__ ws_ml, const float* __restrict__ ws_o, 
     o[qh * kHeadDim + d] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
 }
 
-template <typename T, int G>
-static int simt_launch(const DecodeParams& p, cudaStream_t st) {
+template <typename T, int G, bool MASS>
+static int simt_launch(const DecodeParams& p, const MassParams& m, cudaStream_t st) {
     const int64_t ctas = (int64_t)p.batch * p.Hkv * p.num_splits;
-    KTK_CUDA_TRY(launch_behind(ctas <= sm_count(), decode_simt_kernel<T, G>, (unsigned)ctas, kSimtWarps * 32, 0, st, p), "ktk decode (simt)");
+    KTK_CUDA_TRY(launch_behind(ctas <= sm_count(), decode_simt_kernel<T, G, MASS>, (unsigned)ctas, kSimtWarps * 32, 0, st, p, m), "ktk decode (simt)");
     return KTK_OK;
 }
 
-template <typename T>
-static int simt_group(const DecodeParams& p, int G, cudaStream_t st) {
+template <typename T, bool MASS>
+static int simt_group(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st) {
     switch (G) {
-        case 1: return simt_launch<T, 1>(p, st);
-        case 2: return simt_launch<T, 2>(p, st);
-        case 4: return simt_launch<T, 4>(p, st);
-        default: return simt_launch<T, 8>(p, st);
+        case 1: return simt_launch<T, 1, MASS>(p, m, st);
+        case 2: return simt_launch<T, 2, MASS>(p, m, st);
+        case 4: return simt_launch<T, 4, MASS>(p, m, st);
+        default: return simt_launch<T, 8, MASS>(p, m, st);
     }
 }
 
 int launch_decode_simt(const DecodeParams& p, int dtype, int G, cudaStream_t st) {
-    return dtype == KTK_F32 ? simt_group<float>(p, G, st) : simt_group<__nv_bfloat16>(p, G, st);
+    const MassParams none{};
+    return dtype == KTK_F32 ? simt_group<float, false>(p, none, G, st) : simt_group<__nv_bfloat16, false>(p, none, G, st);
+}
+
+int launch_decode_simt_mass(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st) {
+    return simt_group<float, true>(p, m, G, st);
 }
 
 int launch_combine(const DecodeParams& p, int dtype, int G, cudaStream_t st) {

@@ -30,6 +30,21 @@ struct DecodeParams {
     int sink_tokens;             // > 0: logical page 0 holds only this many tokens and is always attended
     int local_tokens;            // the newest tokens that are always attended
     const int32_t* page_count;   // non-null: pages of sequence b (kv_indptr[b] is then only the start)
+    float* lse = nullptr;        // non-null: [B*Hq] log2 of the softmax's denominator (a list that one CTA sees whole)
+};
+
+// What the kernels that accumulate weights need beside a decode (see ktk_mass in ktk.h).
+struct MassParams {
+    const float* in;
+    float* out;
+    int64_t stride;              // floats per (row, kv head)
+    int rows;
+    const int32_t* slot_index;   // nullable: row of sequence b
+    float decay;
+    float* scores;               // log2-domain scores of every listed token: [position of its page][16 tokens][G]
+    int64_t positions;           // pages that `scores` has room for
+    int wmax;                    // positions per (sequence, kv head) where lists have a page_count view
+    int max_pages;               // the caller's bound of a list
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -135,8 +150,21 @@ __device__ __forceinline__ void page_of_pos(int pos, int first_fill, int& e, int
     slot = (pos - first_fill) % kPageSize;
 }
 
+// Position of the first page of (b, h)'s list among all lists: lists lie one behind the other, padded ones wmax apart.
+__device__ __forceinline__ int64_t list_position(const DecodeParams& p, int wmax, int b, int h) {
+    if (p.page_count) return ((int64_t)b * p.Hkv + h) * wmax;
+    const int64_t n = p.kv_indptr[b + 1] - p.kv_indptr[b];
+    return (int64_t)(p.kv_indptr[b] - p.kv_indptr[0]) * p.Hkv + h * n;
+}
+
 int launch_decode_simt(const DecodeParams& p, int dtype, int G, cudaStream_t st);
+int launch_decode_simt_mass(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st);    // fp32
 int launch_decode_mma(const DecodeParams& p, int G, cudaStream_t st);
+// What ktk_prefill_attention does, and with `lse`, for every variant but KTK_VARIANT_MMA, the denominators (log2) of all rows.
+int prefill_attention(const char* who, const void* q, const int32_t* q_indptr, int64_t total_new_tokens, int32_t max_new_tokens,
+                      const void* kv_cache, const int32_t* kv_indices, const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                      const ktk_view* view_in, float sm_scale, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                      int32_t variant, const ktk_shape* s, int32_t* status, void* stream);
 int launch_combine(const DecodeParams& p, int dtype, int G, cudaStream_t st);
 int32_t legacy_num_splits(const ktk_shape* shape, int32_t max_entries);          // per-list split count
 int32_t policy_num_splits(const ktk_shape* shape, int variant, int32_t max_entries);   // what num_splits = 0 means

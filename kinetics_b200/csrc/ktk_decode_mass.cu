@@ -1,0 +1,223 @@
+// Decode attention over a paged cache that also adds up, for every cached token, the weight that it was given:
+//     o[b, hq] = sum_t p_hq(t) V_t,     mass'[r, h, t] = decay mass[r, h, t] + sum over the group's heads of p_hq(t)
+// with p_hq(t) = 2^(s_hq(t) - lse_hq), scores s in the log2 domain; the newest token starts from 0.
+//
+// A weight needs the denominator of its whole list, which is known when every key has been read.  So the decode kernels write the
+// scores down as they go (4 G bytes per token beside the 512 of its bf16 key and value), and mass_finish_kernel turns them into
+// weights.  It also merges the pieces of lists that the decode cut.
+#include "ktk_decode_stream.cuh"
+
+namespace ktk {
+
+constexpr int kMassThreads = 256;
+constexpr int kMassTokens = 1024;                         // of a CTA
+
+// The pieces of a list: `count` of them, the k-th in row row(k) of the partials (times G heads).
+struct StreamPieces {
+    int64_t c;                                            // the CTA in which the list starts
+    int count;
+    __device__ __forceinline__ int64_t row(int k) const { return (c + k) * 2 + (k == 0 ? 1 : 0); }
+    __device__ __forceinline__ int64_t head_row(int k, int G, int g) const { return row(k) * G + g; }
+};
+struct SplitPieces {
+    int64_t unit;
+    int count;
+    __device__ __forceinline__ int64_t head_row(int k, int G, int g) const { return (unit * G + g) * count + k; }
+};
+
+// One CTA per list and kMassTokens of its tokens.  STREAM: behind the balanced partition, where a list that one CTA saw whole has its
+// output and its denominator already; otherwise behind num_splits partials of every list.
+template <typename T, bool STREAM>
+__global__ void __launch_bounds__(kMassThreads)
+mass_finish_kernel(const StreamParams p, int chunks, int decode_ctas) {
+    __shared__ float lse[8];
+    const DecodeParams& d = p.d;
+    const MassParams& m = p.m;
+    const int G = p.G, tid = threadIdx.x;
+    wait_for_front();
+    const int64_t unit = blockIdx.x / chunks;
+    const int part = (int)(blockIdx.x % chunks);
+    const int b = (int)(unit / d.Hkv), h = (int)(unit % d.Hkv);
+    bool bad;
+    EntryList el = entry_list(d, b, h, bad);
+    const int64_t qh = ((int64_t)b * d.Hkv + h) * G;
+    if (el.cnt == 0) {                                    // no token: zeros
+        if (part == 0)
+            for (int i = tid; i < G * kHeadDim; i += kMassThreads) ((T*)d.o)[qh * kHeadDim + i] = from_f32<T>(0.0f);
+        return;
+    }
+    const int64_t start = list_position(d, m.wmax, b, h);
+    if (el.cnt > m.max_pages) {
+        if (tid == 0 && part == 0) report(d.status, KTK_STATUS_BAD_TABLE);
+        if (d.page_count) el.cnt = m.max_pages;           // padded lists are clipped by the decode
+    }
+
+    const auto merge = [&](const auto& pieces) {
+        if (pieces.count == 0) {                          // whole
+            if (tid < G) lse[tid] = d.lse[qh + tid];
+            return;
+        }
+        if (part == 0) {
+            for (int i = tid; i < G * kHeadDim; i += kMassThreads) {
+                const int g = i / kHeadDim, dd = i % kHeadDim;
+                float M = -INFINITY, L = 0.0f, O = 0.0f;
+                for (int k = 0; k < pieces.count; ++k) {
+                    const int64_t row = pieces.head_row(k, G, g);
+                    const float mk = d.ws_ml[row * 2];
+                    if (mk == -INFINITY) continue;
+                    const float Mn = fmaxf(M, mk), a = exp2f(M - Mn), c = exp2f(mk - Mn);
+                    L = L * a + d.ws_ml[row * 2 + 1] * c;
+                    O = O * a + d.ws_o[row * kHeadDim + dd] * c;
+                    M = Mn;
+                }
+                ((T*)d.o)[qh * kHeadDim + i] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
+                if (dd == 0) lse[g] = M + log2f(L);
+            }
+        } else if (tid < G) {
+            float M = -INFINITY, L = 0.0f;
+            for (int k = 0; k < pieces.count; ++k) {
+                const int64_t row = pieces.head_row(k, G, tid);
+                const float mk = d.ws_ml[row * 2];
+                if (mk == -INFINITY) continue;
+                const float Mn = fmaxf(M, mk);
+                L = L * exp2f(M - Mn) + d.ws_ml[row * 2 + 1] * exp2f(mk - Mn);
+                M = Mn;
+            }
+            lse[tid] = M + log2f(L);
+        }
+    };
+    if constexpr (STREAM) {
+        int64_t total, chunk;
+        stream_extent(p, decode_ctas, total, chunk);
+        StreamPieces pieces;
+        pieces.c = start / chunk;
+        const int64_t last = (start + el.cnt - 1) / chunk;
+        pieces.count = last == pieces.c ? 0 : (int)(last - pieces.c + 1);
+        merge(pieces);
+    } else {
+        merge(SplitPieces{unit, d.num_splits});
+    }
+    __syncthreads();
+
+    const int tokens = el.cnt == 1 ? el.last : el.first + (el.cnt - 2) * kPageSize + el.last;
+    const int row = m.slot_index ? m.slot_index[b] : b;
+    if (row < 0 || row >= m.rows || tokens > m.stride || start + el.cnt > m.positions) {
+        if (tid == 0 && part == 0) report(d.status, KTK_STATUS_BAD_TABLE);
+        return;
+    }
+    const int64_t at = ((int64_t)row * d.Hkv + h) * m.stride;
+    const int t1 = (part + 1) * kMassTokens < tokens ? (part + 1) * kMassTokens : tokens;
+    for (int t = part * kMassTokens + tid; t < t1; t += kMassThreads) {
+        // a short first page leaves places of its own block free
+        const int place = t < el.first || el.cnt == 1 ? t : t + kPageSize - el.first;
+        const float* s = m.scores + (start * kPageSize + place) * G;
+        float sum = 0.0f;
+        for (int g = 0; g < G; ++g) sum += exp2f(s[g] - lse[g]);
+        m.out[at + t] = t == tokens - 1 ? sum : fmaf(m.decay, m.in[at + t], sum);
+    }
+}
+
+template <typename T, bool STREAM>
+static int launch_finish(const StreamParams& p, int decode_ctas, cudaStream_t st) {
+    const int64_t chunks = ((int64_t)p.m.max_pages * kPageSize + kMassTokens - 1) / kMassTokens;
+    const int64_t ctas = chunks * p.d.batch * p.d.Hkv;
+    if (ctas > 2147483647LL) {
+        set_error("ktk_dense_decode_mass: batch * num_kv_heads * max_pages_per_seq exceeds the grid limit");
+        return KTK_ERR_TOO_LARGE;
+    }
+    KTK_CUDA_TRY(launch_behind(true, mass_finish_kernel<T, STREAM>, (unsigned)ctas, kMassThreads, 0, st, p, (int)chunks, decode_ctas),
+                 "ktk_dense_decode_mass (finish)");
+    return KTK_OK;
+}
+
+int launch_mass_finish(const StreamParams& p, int decode_ctas, cudaStream_t st) { return launch_finish<__nv_bfloat16, true>(p, decode_ctas, st); }
+
+// Parts of the workspace, in bytes from its start
+struct MassWorkspace {
+    size_t partials, lse, scores, bytes;
+    int64_t positions;
+    int splits;
+};
+static MassWorkspace mass_workspace(const ktk_shape* s, int max_pages, int64_t total_pages) {
+    MassWorkspace w;
+    const int64_t padded = (int64_t)s->batch * max_pages;
+    if (total_pages < 0 || total_pages > padded) total_pages = padded;
+    const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    w.splits = policy_num_splits(s, KTK_VARIANT_AUTO, max_pages);
+    const size_t rows = (size_t)s->batch * s->num_kv_heads * s->group_size;
+    w.positions = total_pages * s->num_kv_heads;
+    w.partials = 0;
+    w.lse = up(w.splits == KTK_SPLITS_BALANCED ? ktk_decode_workspace_bytes(s, w.splits)
+                                               : rows * w.splits * (2 + kHeadDim) * sizeof(float));
+    w.scores = w.lse + up(rows * sizeof(float));
+    w.bytes = w.scores + up((size_t)w.positions * kPageSize * s->group_size * sizeof(float));
+    return w;
+}
+
+}  // namespace ktk
+
+using namespace ktk;
+
+extern "C" size_t ktk_decode_mass_workspace_bytes(const ktk_shape* shape, int32_t max_pages_per_seq, int64_t total_pages) {
+    if (check_shape(shape, "ktk_decode_mass_workspace_bytes") != KTK_OK || shape->batch == 0) return 0;
+    return mass_workspace(shape, max_pages_per_seq < 1 ? 1 : max_pages_per_seq, total_pages).bytes;
+}
+
+extern "C" int ktk_dense_decode_mass(const void* q, const void* kv_cache, const int32_t* kv_indices,
+                                     const int32_t* kv_indptr, const int32_t* kv_last_page_len, const ktk_view* view_in,
+                                     int32_t max_pages_per_seq, int64_t total_pages, float sm_scale, const ktk_mass* mass,
+                                     void* o, void* workspace, size_t workspace_bytes, const ktk_shape* s, int32_t* status,
+                                     void* stream) {
+    const char* who = "ktk_dense_decode_mass";
+    int rc = check_shape(s, who);
+    if (rc == KTK_OK) rc = check_view(view_in, who);
+    if (rc != KTK_OK) return rc;
+    if (s->batch == 0) return KTK_OK;
+    if (!q || !kv_cache || !kv_indices || !kv_indptr || !kv_last_page_len || !o) {
+        set_error("%s: null pointer argument", who);
+        return KTK_ERR_ARG;
+    }
+    if ((rc = check_mass(mass, who)) != KTK_OK || (rc = check_aligned({q, kv_cache, o, workspace}, who)) != KTK_OK ||
+        (rc = check_apart(mass->in, mass->out, (size_t)mass->rows * s->num_kv_heads * mass->stride * sizeof(float), who, "mass")) != KTK_OK)
+        return rc;
+    if (max_pages_per_seq < 1) max_pages_per_seq = 1;
+    const View view = make_view(view_in);
+    if (view.page_count) total_pages = -1;                // padded
+    const MassWorkspace w = mass_workspace(s, max_pages_per_seq, total_pages);
+    if (workspace == nullptr || workspace_bytes < w.bytes) {
+        set_error("%s: workspace of %zu bytes needed, got %zu", who, w.bytes, workspace ? workspace_bytes : (size_t)0);
+        return KTK_ERR_WORKSPACE;
+    }
+    if ((int64_t)s->batch * s->num_kv_heads * (w.splits > 0 ? w.splits : 1) > 2147483647LL) {
+        set_error("%s: batch * num_kv_heads * splits exceeds the grid limit", who);
+        return KTK_ERR_TOO_LARGE;
+    }
+    DecodeParams p{};
+    p.q = q; p.cache = kv_cache; p.o = o; p.entries = kv_indices;
+    p.kv_indptr = kv_indptr; p.kv_last_page_len = kv_last_page_len;
+    p.sink_tokens = view.sink_tokens; p.local_tokens = view.local_tokens; p.page_count = view.page_count;
+    p.topk = -1; p.batch = s->batch; p.Hkv = s->num_kv_heads; p.num_pages = s->num_pages;
+    p.scale_log2 = sm_scale * kLog2e;
+    p.num_splits = w.splits;
+    const bool balanced = w.splits == KTK_SPLITS_BALANCED;
+    const int64_t rows = balanced ? (int64_t)(ktk_decode_workspace_bytes(s, w.splits) / ((2 + kHeadDim) * sizeof(float)))
+                                  : (int64_t)s->batch * s->num_kv_heads * s->group_size * w.splits;
+    char* ws = (char*)workspace;
+    p.ws_ml = (float*)ws;
+    p.ws_o = (float*)ws + rows * 2;
+    p.lse = (float*)(ws + w.lse);
+    p.status = status;
+    MassParams m;
+    m.in = mass->in; m.out = mass->out; m.stride = mass->stride; m.rows = mass->rows; m.slot_index = view.slot_index;
+    m.decay = mass->decay; m.scores = (float*)(ws + w.scores); m.positions = w.positions; m.wmax = max_pages_per_seq;
+    m.max_pages = max_pages_per_seq;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (balanced) return launch_decode_stream_mass(p, m, s->group_size, max_pages_per_seq, st);
+    rc = launch_decode_simt_mass(p, m, s->group_size, st);
+    if (rc != KTK_OK) return rc;
+    StreamParams sp{};
+    sp.d = p;
+    sp.m = m;
+    sp.G = s->group_size;
+    return launch_finish<float, false>(sp, 0, st);
+}

@@ -57,10 +57,15 @@ __device__ __forceinline__ void load_q_frags(uint32_t (&qb)[8][2], const void* q
 //     O^T[128 x 8 heads]    += V^T[128 x 16] . P^T        8 x mma.m16n8k16
 // CAUSAL (prefill): the 8 columns are (query token, head) pairs with their own horizon -- column 2*tig sees
 // the first lim0 tokens of the page, column 2*tig+1 the first lim1 (both <= ntok, possibly 0).
-template <bool CAUSAL>
+// keep(s00, s01, s10, s11) gets the scores of tokens gid, gid + 8 and heads 2*tig, 2*tig+1 (log2 domain, masked ones -inf); UNROUNDED:
+// the normaliser adds the probabilities as they were before they were rounded.
+struct KeepNothing {
+    __device__ __forceinline__ void operator()(float, float, float, float) const {}
+};
+template <bool CAUSAL, bool UNROUNDED = false, class Keep = KeepNothing>
 __device__ __forceinline__ void mma_consume_page_t(MmaState& st, uint8_t* stage, int ntok,
                                                    const uint32_t (&qb)[8][2], float scale_log2, int lane,
-                                                   int lim0, int lim1) {
+                                                   int lim0, int lim1, Keep keep = Keep()) {
     const int gid = lane >> 2;
     // per-lane ldmatrix row addresses (relative to the tile): lane supplies row (lane & 7) of matrix lane >> 3
     const int mj = lane >> 3, mr = lane & 7;
@@ -99,6 +104,7 @@ __device__ __forceinline__ void mma_consume_page_t(MmaState& st, uint8_t* stage,
         if (gid >= ntok) { s00 = -INFINITY; s01 = -INFINITY; }
         if (gid + 8 >= ntok) { s10 = -INFINITY; s11 = -INFINITY; }
     }
+    keep(s00, s01, s10, s11);
     float mx0 = fmaxf(s00, s10), mx1 = fmaxf(s01, s11);
 #pragma unroll
     for (int off = 4; off <= 16; off <<= 1) {
@@ -111,10 +117,11 @@ __device__ __forceinline__ void mma_consume_page_t(MmaState& st, uint8_t* stage,
     const float b1 = (CAUSAL && mn1 == -INFINITY) ? 0.0f : mn1;
     const float al0 = exp2f(st.m0 - b0), al1 = exp2f(st.m1 - b1);
     // probabilities, rounded to bf16 once so that the normaliser matches what multiplies V
-    const uint32_t p_lo = pack_bf16(exp2f(s00 - b0), exp2f(s01 - b1));   // tokens 0-7
-    const uint32_t p_hi = pack_bf16(exp2f(s10 - b0), exp2f(s11 - b1));   // tokens 8-15
-    float sum0 = __uint_as_float(p_lo << 16) + __uint_as_float(p_hi << 16);
-    float sum1 = __uint_as_float(p_lo & 0xffff0000u) + __uint_as_float(p_hi & 0xffff0000u);
+    const float p00 = exp2f(s00 - b0), p01 = exp2f(s01 - b1), p10 = exp2f(s10 - b0), p11 = exp2f(s11 - b1);
+    const uint32_t p_lo = pack_bf16(p00, p01);   // tokens 0-7
+    const uint32_t p_hi = pack_bf16(p10, p11);   // tokens 8-15
+    float sum0 = UNROUNDED ? p00 + p10 : __uint_as_float(p_lo << 16) + __uint_as_float(p_hi << 16);
+    float sum1 = UNROUNDED ? p01 + p11 : __uint_as_float(p_lo & 0xffff0000u) + __uint_as_float(p_hi & 0xffff0000u);
 #pragma unroll
     for (int off = 4; off <= 16; off <<= 1) {
         sum0 += __shfl_xor_sync(0xffffffffu, sum0, off);
@@ -157,6 +164,7 @@ __device__ __forceinline__ void tma_load_page(uint8_t* dst, const CUtensorMap* m
 int make_kv_tensor_map(CUtensorMap* map, const DecodeParams& p);
 
 int launch_decode_stream(const DecodeParams& p, int G, int max_entries, cudaStream_t st);
+int launch_decode_stream_mass(const DecodeParams& p, const MassParams& m, int G, int max_entries, cudaStream_t st);
 int stream_grid(int64_t units, int max_entries);
 size_t stream_workspace_bytes(int G);
 

@@ -23,138 +23,22 @@
 #include <mutex>
 #include <type_traits>
 
-#include "ktk_decode_mma.cuh"
+#include "ktk_decode_stream.cuh"
 
 namespace ktk {
 
 constexpr int kStreamMaxCtasPerSm = 4;                    // the most any variant keeps resident (sizes the workspace)
-constexpr int kStreamMinChunk = 16;                       // pages: below this a CTA is not worth its start-up
 constexpr int kExchangeHeads = 4;                         // heads merged per pass through shared memory
 constexpr int kExchangeBytes = kMmaConsumers * kExchangeHeads * kHeadDim * 4;   // 8 KiB
 constexpr int stream_smem(int stages) { return stages * kStageBytes + 1024 + kExchangeBytes; }
-
-struct StreamParams {
-    DecodeParams d;
-    int G;
-    int wmax;        // padded mode: positions per unit
-    int chunk;       // padded mode: positions per CTA
-    int64_t total;   // padded mode: units * wmax
-    int exact;       // 1: dense CSR lists without a page_count view -- positions are the CSR entries themselves,
-                     //    unit (b, h) covers [(indptr[b] - indptr[0]) * Hkv + h * n(b), ... + n(b)), so ragged
-                     //    batches are cut evenly too; total and chunk are computed on the device
-};
-
-// positions [p0, p1) of CTA c; empty if p1 <= p0
-struct Range {
-    int64_t p0, p1;
-};
-
-// number of positions and positions per CTA
-__device__ __forceinline__ void stream_extent(const StreamParams& p, int64_t& total, int64_t& chunk) {
-    total = p.total;
-    chunk = p.chunk;
-    if (p.exact) {
-        total = (int64_t)(p.d.kv_indptr[p.d.batch] - p.d.kv_indptr[0]) * p.d.Hkv;
-        chunk = (total + gridDim.x - 1) / gridDim.x;
-        if (chunk < kStreamMinChunk) chunk = kStreamMinChunk;
-    }
-}
-
-__device__ __forceinline__ Range cta_range(const StreamParams& p, int64_t c) {
-    Range r;
-    int64_t total, chunk;
-    stream_extent(p, total, chunk);
-    r.p0 = c * chunk;
-    r.p1 = (r.p0 + chunk < total) ? r.p0 + chunk : total;
-    return r;
-}
-
-// The unit (b, h) whose positions are [start, start + len)
-struct Cursor {
-    int b, h, len;
-    int64_t start;
-};
-
-// exact mode: the sequence whose CSR entries contain entry q (relative to indptr[0]); all lanes of the
-// warp take part, 32 probes per round
-__device__ __forceinline__ int find_sequence(const int32_t* indptr, int B, int64_t q) {
-    const int lane = threadIdx.x & 31;
-    const int64_t base = indptr[0];
-    int lo = 0, hi = B;                                   // invariant: indptr[lo] - base <= q, answer in [lo, hi)
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32;
-        const int idx = lo + lane * step;
-        const bool ok = idx < hi && (int64_t)indptr[idx] - base <= q;
-        const unsigned m = __ballot_sync(0xffffffffu, ok);            // a prefix of the lanes: lane 0 always holds
-        const int k = 31 - __clz((int)m);
-        lo += k * step;
-        hi = (lo + step < hi) ? lo + step : hi;
-    }
-    return lo;
-}
-
-__device__ __forceinline__ Cursor cursor_at(const StreamParams& p, int64_t pos) {
-    Cursor c;
-    if (!p.exact) {
-        const int64_t u = pos / p.wmax;
-        c.b = (int)(u / p.d.Hkv);
-        c.h = (int)(u % p.d.Hkv);
-        c.start = u * p.wmax;
-        c.len = p.wmax;
-        return c;
-    }
-    const int32_t* ip = p.d.kv_indptr;
-    c.b = find_sequence(ip, p.d.batch, pos / p.d.Hkv);
-    c.len = ip[c.b + 1] - ip[c.b];
-    const int64_t first = (int64_t)(ip[c.b] - ip[0]) * p.d.Hkv;
-    c.h = (int)((pos - first) / c.len);
-    c.start = first + (int64_t)c.h * c.len;
-    return c;
-}
-
-__device__ __forceinline__ void cursor_next(const StreamParams& p, Cursor& c) {
-    c.start += c.len;
-    if (++c.h < p.d.Hkv) return;
-    c.h = 0;
-    ++c.b;
-    if (p.exact) {
-        while (c.b < p.d.batch && (c.len = p.d.kv_indptr[c.b + 1] - p.d.kv_indptr[c.b]) == 0) ++c.b;   // no positions
-    }
-}
-
-// The part of the cursor's unit that falls into the position range [p0, p1).
-struct Piece {
-    int b, h;
-    EntryList el;
-    int e_lo, e_hi;   // entries of the unit this CTA runs
-    bool first;       // the unit's positions start inside the range
-    bool bad;
-};
-
-__device__ __forceinline__ Piece get_piece(const StreamParams& p, const Cursor& c, int64_t p0, int64_t p1) {
-    Piece pc;
-    pc.b = c.b;
-    pc.h = c.h;
-    pc.el = entry_list(p.d, pc.b, pc.h, pc.bad);
-    if (pc.el.cnt > c.len) {          // a list longer than the caller's bound: flagged by the producer, clipped here
-        pc.el.cnt = c.len;
-        pc.bad = true;
-    }
-    const int lo = (p0 > c.start) ? (int)(p0 - c.start) : 0;
-    const int hi = (p1 - c.start < c.len) ? (int)(p1 - c.start) : c.len;
-    pc.first = (p0 <= c.start);
-    pc.e_lo = lo < pc.el.cnt ? lo : pc.el.cnt;
-    pc.e_hi = hi < pc.el.cnt ? hi : pc.el.cnt;
-    return pc;
-}
 
 __device__ __forceinline__ void consumer_bar() {          // the four consumer warps only
     asm volatile("bar.sync 1, %0;" ::"n"(kMmaConsumers * 32) : "memory");
 }
 
 // STAGES: ring depth (a multiple of the consumer count, so that a stage always belongs to one warp);
-// CTAS: CTAs resident per SM.
-template <int STAGES, int CTAS>
+// CTAS: CTAs resident per SM; MASS: the scores and the lists' denominators are written too (ktk_decode_mass.cu).
+template <int STAGES, int CTAS, bool MASS = false>
 __global__ void __launch_bounds__(kMmaThreads, CTAS)
 decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap kv_map) {
     static_assert(STAGES % kMmaConsumers == 0, "a stage must belong to one consumer warp");
@@ -260,9 +144,27 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                         dead = true;
                         break;
                     }
-                    if (tag > 0)
+                    if (MASS && tag > 0) {
+                        const int ntok = entry_tokens(pc.el, pc.e_lo + j);
+                        const int64_t position = cur.start + pc.e_lo + j;
+                        float* at = p.m.scores + (position * kPageSize + gid) * G + 2 * tig;
+                        const bool on = 2 * tig < G && position < p.m.positions;
+                        mma_consume_page_t<false, true>(
+                            ms, stages + s * kStageBytes, ntok, qb, d.scale_log2, lane, ntok, ntok,
+                            [&](float s00, float s01, float s10, float s11) {
+                                if (!on) return;
+                                if (G == 1) {
+                                    if (gid < ntok) at[0] = s00;
+                                    if (gid + 8 < ntok) at[8] = s10;
+                                } else {
+                                    if (gid < ntok) *reinterpret_cast<float2*>(at) = make_float2(s00, s01);
+                                    if (gid + 8 < ntok) *reinterpret_cast<float2*>(at + 8 * G) = make_float2(s10, s11);
+                                }
+                            });
+                    } else if (tag > 0) {
                         mma_consume_page(ms, stages + s * kStageBytes, entry_tokens(pc.el, pc.e_lo + j), qb,
                                          d.scale_log2, lane);
+                    }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&empty_bar[s]);
                 }
@@ -307,6 +209,7 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                     if (whole) {
                         const int64_t qh = (int64_t)pc.b * Hq + (int64_t)pc.h * G + g;
                         ((__nv_bfloat16*)d.o)[qh * kHeadDim + dd] = __float2bfloat16_rn(L > 0.0f ? O / L : 0.0f);
+                        if (MASS && dd == 0) d.lse[qh] = M + log2f(L);
                     } else {
                         const int64_t row = (int64_t)slot * G + g;
                         d.ws_o[row * kHeadDim + dd] = O;
@@ -397,6 +300,7 @@ stream_combine_kernel(const StreamParams p) {
 struct StreamVariant {
     int stages, ctas;
     void (*kernel)(const StreamParams, const CUtensorMap);
+    void (*mass_kernel)(const StreamParams, const CUtensorMap);
 };
 // Measured on a B200 at B = 4096, 32768-token context (sparse: 129 pages per list / dense: 2049), ms:
 //   4 stages x 4 CTAs per SM   0.639 / 9.53      <- default: 16 consumer warps per SM
@@ -406,8 +310,8 @@ struct StreamVariant {
 //   8 or 12 stages x 2 CTAs    0.88  / 13.5
 // The consumer warps, not the bytes in flight, set the pace: more resident warps win until registers run out.
 static const StreamVariant kStreamVariants[] = {
-    {4, 4, decode_stream_kernel<4, 4>},      // 0
-    {8, 3, decode_stream_kernel<8, 3>},      // 1
+    {4, 4, decode_stream_kernel<4, 4>, decode_stream_kernel<4, 4, true>},      // 0
+    {8, 3, decode_stream_kernel<8, 3>, decode_stream_kernel<8, 3, true>},      // 1
 };
 constexpr int kNumStreamVariants = (int)(sizeof(kStreamVariants) / sizeof(kStreamVariants[0]));
 
@@ -459,12 +363,14 @@ size_t stream_workspace_bytes(int G) {
     return (size_t)kStreamMaxCtasPerSm * sm_count() * 2 * G * (2 + kHeadDim) * sizeof(float);
 }
 
-int launch_decode_stream(const DecodeParams& p, int G, int max_entries, cudaStream_t st) {
+template <bool MASS>
+static int launch_stream(const DecodeParams& p, const MassParams& m, int G, int max_entries, cudaStream_t st) {
     CUtensorMap map;
     int rc = make_kv_tensor_map(&map, p);
     if (rc != KTK_OK) return rc;
     StreamParams sp;
     sp.d = p;
+    sp.m = m;
     sp.G = G;
     sp.wmax = max_entries;
     // dense CSR lists: cut the entries themselves (ragged batches stay balanced); selected-page tables
@@ -474,6 +380,7 @@ int launch_decode_stream(const DecodeParams& p, int G, int max_entries, cudaStre
     sp.total = units * max_entries;
     const int vi = stream_variant_index(p.topk < 0);
     const StreamVariant& var = kStreamVariants[vi];
+    const auto kernel = MASS ? var.mass_kernel : var.kernel;
     int grid = stream_grid_of(vi, units, max_entries);
     const int64_t chunk = (sp.total + grid - 1) / grid;
     if (chunk > 2147483647LL) {
@@ -483,14 +390,23 @@ int launch_decode_stream(const DecodeParams& p, int G, int max_entries, cudaStre
     sp.chunk = (int)chunk;
     if (!sp.exact) grid = (int)((sp.total + chunk - 1) / chunk);            // no empty CTA
     const int smem = stream_smem(var.stages);
-    KTK_CUDA_TRY(cudaFuncSetAttribute(var.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                  "ktk decode (balanced)");
-    KTK_CUDA_TRY(launch_behind(grid <= sm_count(), var.kernel, grid, kMmaThreads, smem, st, sp, map), "ktk decode (balanced)");
+    KTK_CUDA_TRY(launch_behind(grid <= sm_count(), kernel, grid, kMmaThreads, smem, st, sp, map), "ktk decode (balanced)");
+    if (MASS) return launch_mass_finish(sp, grid, st);
     if (grid > 1 || sp.exact) {
         KTK_CUDA_TRY(launch_behind(true, stream_combine_kernel, dim3(grid, (unsigned)sp.G), kHeadDim, 0, st, sp),
                      "ktk decode (balanced, combine)");
     }
     return KTK_OK;
+}
+
+int launch_decode_stream(const DecodeParams& p, int G, int max_entries, cudaStream_t st) {
+    return launch_stream<false>(p, MassParams{}, G, max_entries, st);
+}
+
+int launch_decode_stream_mass(const DecodeParams& p, const MassParams& m, int G, int max_entries, cudaStream_t st) {
+    return launch_stream<true>(p, m, G, max_entries, st);
 }
 
 }  // namespace ktk

@@ -57,6 +57,36 @@ int check_view(const ktk_view* v, const char* who) {
     return KTK_OK;
 }
 
+int check_mass(const ktk_mass* m, const char* who) {
+    if (m == nullptr || m->in == nullptr || m->out == nullptr) {
+        set_error("%s: mass is null", who);
+        return KTK_ERR_ARG;
+    }
+    if (m->rows < 1 || m->stride < 1) {
+        set_error("%s: mass of %d rows, %lld places each", who, m->rows, (long long)m->stride);
+        return KTK_ERR_ARG;
+    }
+    return KTK_OK;
+}
+
+int check_apart(const void* a, const void* b, size_t bytes, const char* who, const char* what) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    if (x != y && x < y + bytes && y < x + bytes) {
+        set_error("%s: %s in and out overlap: pass the same memory, or memory apart", who, what);
+        return KTK_ERR_ARG;
+    }
+    return KTK_OK;
+}
+
+int check_aligned(std::initializer_list<const void*> pointers, const char* who) {
+    for (const void* p : pointers)
+        if ((uintptr_t)p % 16 != 0) {
+            set_error("%s: queries, cache, output and workspace are 16-byte aligned", who);
+            return KTK_ERR_ARG;
+        }
+    return KTK_OK;
+}
+
 int sm_count() {
     static thread_local int cached_dev = -1;
     static thread_local int cached = 0;

@@ -357,6 +357,149 @@ def prefill_attention(q, q_indptr, max_new_tokens: int, kv_cache, kv_indices, kv
     return out
 
 
+# ---- a cache of bounded size: attention that adds up what tokens were paid, and the eviction that goes by it
+
+def _on_one_device(first, *others) -> None:
+    """The launch goes to the current device's stream: all tensors have to be there."""
+    dev = first.get_device()
+    if dev != torch.cuda.current_device():
+        raise RuntimeError(f"kinetics_b200: tensors on cuda:{dev}, current device cuda:{torch.cuda.current_device()}")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"kinetics_b200: tensors on cuda:{dev} and {t.device}")
+
+
+def _table_tensors(batch, kv_indices, kv_indptr, kv_last_page_len, view) -> None:
+    if kv_indices.dtype != torch.int32 or kv_indptr.dtype != torch.int32 or kv_last_page_len.dtype != torch.int32:
+        raise TypeError("page tables are int32")
+    if _batch_of(kv_indptr, view) != batch or kv_last_page_len.numel() < batch:
+        raise ValueError(f"page table of {_batch_of(kv_indptr, view)} sequences, {batch} expected")
+    if view is not None and any(t is not None and t.numel() < batch for t in (view.page_count, view.slot_index)):
+        raise ValueError(f"PageView: page_count and slot_index have {batch} entries")
+
+
+def _mass_args(mass, mass_out, batch, num_kv_heads, decay, view):
+    """(ktk_mass, mass_out): mass fp32 [rows, Hkv, places]; without a slot_index one row per sequence."""
+    if mass_out is None:
+        mass_out = mass
+    if mass.dtype != torch.float32 or mass_out.dtype != torch.float32:
+        raise TypeError("mass is fp32")
+    if mass.dim() != 3 or mass.shape[1] != num_kv_heads or mass_out.shape != mass.shape:
+        raise ValueError(f"mass must be [rows, {num_kv_heads}, places], got {tuple(mass.shape)} and {tuple(mass_out.shape)}")
+    if mass.shape[0] < batch and (view is None or view.slot_index is None):
+        raise ValueError(f"mass of {mass.shape[0]} rows for {batch} sequences")
+    return _lib.Mass(mass.data_ptr(), mass_out.data_ptr(), mass.shape[2], mass.shape[0], decay), mass_out
+
+
+def _scratch(need: int, workspace, device):
+    """The caller's workspace, or one from the allocator (which keeps calls on different streams, and graphs, apart)."""
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: int, mass, decay: float = 1.0,
+                      sm_scale: Optional[float] = None, mass_out=None, workspace=None, out=None, status=None, view=None):
+    """``dense_decode`` that also accumulates the weights every cached token was given.
+
+    mass fp32 [rows, Hkv, places]: what the query heads of a group have paid the token in each place of its sequence
+    (row: view.slot_index, else the sequence's number; different rows for different sequences).  Writes
+    decay * mass + the weights of this step, and the weights alone for the newest token, to mass_out (None: mass itself);
+    places behind a sequence's length are left as they are.  Returns (out, mass_out)."""
+    _cuda(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, workspace, out, status)
+    _on_one_device(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, workspace, out, status)
+    B, Hq, _ = q.shape
+    shp = _shape(B, kv_cache, Hq)
+    if q.dtype != kv_cache.dtype or out is not None and (out.dtype != q.dtype or out.shape != q.shape):
+        raise TypeError("q, kv_cache and out must share a dtype, out the shape of q")
+    _table_tensors(B, kv_indices, kv_indptr, kv_last_page_len, view)
+    m, mass_out = _mass_args(mass, mass_out, B, shp.num_kv_heads, decay, view)
+    if out is None:
+        out = torch.empty_like(q)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(q.shape[-1])
+    lib = _lib.load()
+    total = -1 if view is not None and view.page_count is not None else kv_indices.numel()
+    need = 0 if workspace is not None else int(lib.ktk_decode_mass_workspace_bytes(ctypes.byref(shp), max_pages_per_seq, total))
+    workspace, wsb = _scratch(need, workspace, q.device)
+    vp, _keep = _view_ref(view)
+    check(lib.ktk_dense_decode_mass(_ptr(q), _ptr(kv_cache), _ptr(kv_indices), _ptr(kv_indptr), _ptr(kv_last_page_len), vp,
+                                    max_pages_per_seq, total, sm_scale, ctypes.byref(m), _ptr(out), _ptr(workspace), wsb,
+                                    ctypes.byref(shp), _ptr(status), _stream()))
+    _launched(2)
+    return out, mass_out
+
+
+def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass,
+                           window: int = 0, decay: float = 1.0, sm_scale: Optional[float] = None, mass_out=None,
+                           workspace=None, out=None, status=None, view=None):
+    """``prefill_attention`` that also accumulates the weights that the last ``window`` new tokens of every sequence (0: all
+    of them) give each cached token; mass as in ``dense_decode_mass``, the sequence's new tokens start from their weights
+    alone.  Returns (out, mass_out)."""
+    _cuda(q, q_indptr, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, workspace, out, status)
+    _on_one_device(q, q_indptr, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, workspace, out, status)
+    total, Hq, _ = q.shape
+    B = q_indptr.numel() - 1
+    shp = _shape(B, kv_cache, Hq)
+    if q.dtype != kv_cache.dtype or q_indptr.dtype != torch.int32 or \
+            out is not None and (out.dtype != q.dtype or out.shape != q.shape):
+        raise TypeError("q, kv_cache and out must share a dtype, out the shape of q; q_indptr must be int32")
+    _table_tensors(B, kv_indices, kv_indptr, kv_last_page_len, view)
+    m, mass_out = _mass_args(mass, mass_out, B, shp.num_kv_heads, decay, view)
+    if out is None:
+        out = torch.empty_like(q)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(q.shape[-1])
+    lib = _lib.load()
+    need = 0 if workspace is not None else int(lib.ktk_prefill_mass_workspace_bytes(ctypes.byref(shp), total))
+    workspace, wsb = _scratch(need, workspace, q.device)
+    most = mass.shape[2] if view is not None and view.page_count is not None else kv_indices.numel() * PAGE_SIZE
+    vp, _keep = _view_ref(view)
+    check(lib.ktk_prefill_attention_mass(_ptr(q), _ptr(q_indptr), total, int(max_new_tokens), _ptr(kv_cache),
+                                         _ptr(kv_indices), _ptr(kv_indptr), _ptr(kv_last_page_len), vp, max(most, 1), window,
+                                         sm_scale, ctypes.byref(m), _ptr(out), _ptr(workspace), wsb, ctypes.byref(shp),
+                                         _ptr(status), _stream()))
+    _launched(2 if kv_cache.dtype == torch.bfloat16 else 3)
+    return out, mass_out
+
+
+def evict(kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: int, mass, positions, stored, seen, keep: int,
+          sink: int = 4, recent: int = 0, mass_out=None, positions_out=None, workspace=None, status=None, view=None):
+    """Cut every sequence with more than ``keep`` tokens down to ``keep``, per kv head: the tokens at positions < sink and of
+    the last ``recent`` positions stay, and of the others those of largest mass (ties: the lowest place).
+
+    Kept tokens behind place ``keep`` move, keys and values, into the places in front of it that became free; masses and
+    positions of the kept places go to mass_out and positions_out (None: mass and positions themselves).  positions int32
+    [rows, Hkv, places]: where the tokens of the first stored[row] places were in the sequence; those behind were appended in
+    order, up to position seen[row] - 1 (stored, seen: int32 [rows]).  Afterwards a sequence holds min(n, keep) tokens: that
+    is ``stored`` of the next call, and what the next page table has to say.  Page summaries have to be rebuilt.
+    Returns (mass_out, positions_out)."""
+    _cuda(kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, positions, stored, seen, mass_out, positions_out, workspace,
+          status)
+    _on_one_device(kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, positions, stored, seen, mass_out, positions_out,
+                   workspace, status)
+    B = _batch_of(kv_indptr, view)
+    shp = _shape(B, kv_cache, kv_cache.shape[3])
+    _table_tensors(B, kv_indices, kv_indptr, kv_last_page_len, view)
+    m, mass_out = _mass_args(mass, mass_out, B, shp.num_kv_heads, 1.0, view)
+    if positions_out is None:
+        positions_out = positions
+    if any(t.dtype != torch.int32 for t in (positions, positions_out, stored, seen)):
+        raise TypeError("positions, stored and seen are int32")
+    if positions.shape != mass.shape or positions_out.shape != mass.shape or stored.numel() != mass.shape[0] or \
+            seen.numel() != mass.shape[0]:
+        raise ValueError("positions have the shape of mass, stored and seen one entry per row")
+    lib = _lib.load()
+    need = 0 if workspace is not None else int(lib.ktk_evict_workspace_bytes(ctypes.byref(shp), max_pages_per_seq, keep))
+    workspace, wsb = _scratch(need, workspace, kv_cache.device)
+    vp, _keep = _view_ref(view)
+    check(lib.ktk_evict(_ptr(kv_cache), _ptr(kv_indices), _ptr(kv_indptr), _ptr(kv_last_page_len), vp, max_pages_per_seq,
+                        ctypes.byref(m), _ptr(positions), _ptr(positions_out), _ptr(stored), _ptr(seen), keep, sink, recent,
+                        _ptr(workspace), wsb, ctypes.byref(shp), _ptr(status), _stream()))
+    _launched(2)
+    return mass_out, positions_out
+
+
 def paged_qk(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, logits, sm_scale: Optional[float] = None,
              status=None, view=None):
     """Scaled logits of q [B, Hq, D] against every key of each sequence, read through the page table, into the
