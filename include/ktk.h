@@ -574,17 +574,19 @@ KTK_API int ktk_dense_decode_mass(const void* q, const void* kv_cache, const int
  *   out[r, h, t] = decay * in[r, h, t] + sum over the last `window` new tokens and the heads of group h of p(t)
  * for the tokens t that were there before, and without the first term for the sequence's new ones.  window 0: all new tokens.
  * A sequence without new tokens is left as it is.
- *   max_tokens   an upper bound of the tokens of any one sequence (sizes the grid)
- *   workspace    ktk_prefill_mass_workspace_bytes() bytes: the rows' denominators
+ *   max_pages_per_seq, total_pages   upper bounds of one list's entries and of all lists' together (-1: batch * max_pages_per_seq,
+ *                as with view->page_count); they size the grid and the workspace
+ *   workspace    ktk_prefill_mass_workspace_bytes() bytes: the rows' denominators, and sums over parts of the rows
  * q, kv_cache, o and workspace are 16-byte aligned.
  */
-KTK_API size_t ktk_prefill_mass_workspace_bytes(const ktk_shape* shape, int64_t total_new_tokens);
+KTK_API size_t ktk_prefill_mass_workspace_bytes(const ktk_shape* shape, int64_t total_new_tokens, int32_t max_new_tokens,
+                                                int64_t max_pages_per_seq, int64_t total_pages, int32_t window);
 KTK_API int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr, int64_t total_new_tokens,
                                        int32_t max_new_tokens, const void* kv_cache, const int32_t* kv_indices,
                                        const int32_t* kv_indptr, const int32_t* kv_last_page_len, const ktk_view* view,
-                                       int64_t max_tokens, int32_t window, float sm_scale, const ktk_mass* mass, void* o,
-                                       void* workspace, size_t workspace_bytes, const ktk_shape* shape, int32_t* status,
-                                       void* stream);
+                                       int64_t max_pages_per_seq, int64_t total_pages, int32_t window, float sm_scale,
+                                       const ktk_mass* mass, void* o, void* workspace, size_t workspace_bytes,
+                                       const ktk_shape* shape, int32_t* status, void* stream);
 
 /*
  * Eviction: of every (sequence, kv head) with more than `keep` tokens, `keep` stay -- the tokens at positions < sink, those of the

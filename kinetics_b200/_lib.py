@@ -163,10 +163,10 @@ _SIGNATURES = {
     "ktk_decode_mass_workspace_bytes": (c_size_t, [POINTER(Shape), c_int32, c_int64]),
     "ktk_dense_decode_mass": (c_int32, [c_void_p, c_void_p, _i32p, _i32p, _i32p, POINTER(View), c_int32, c_int64, c_float,
                                         POINTER(Mass), c_void_p, c_void_p, c_size_t, POINTER(Shape), _i32p, c_void_p]),
-    "ktk_prefill_mass_workspace_bytes": (c_size_t, [POINTER(Shape), c_int64]),
+    "ktk_prefill_mass_workspace_bytes": (c_size_t, [POINTER(Shape), c_int64, c_int32, c_int64, c_int64, c_int32]),
     "ktk_prefill_attention_mass": (c_int32, [c_void_p, _i32p, c_int64, c_int32, c_void_p, _i32p, _i32p, _i32p, POINTER(View),
-                                             c_int64, c_int32, c_float, POINTER(Mass), c_void_p, c_void_p, c_size_t,
-                                             POINTER(Shape), _i32p, c_void_p]),
+                                             c_int64, c_int64, c_int32, c_float, POINTER(Mass), c_void_p, c_void_p,
+                                             c_size_t, POINTER(Shape), _i32p, c_void_p]),
     "ktk_evict_workspace_bytes": (c_size_t, [POINTER(Shape), c_int32, c_int32]),
     "ktk_evict": (c_int32, [c_void_p, _i32p, _i32p, _i32p, POINTER(View), c_int32, POINTER(Mass), _i32p, _i32p, _i32p, _i32p,
                             c_int32, c_int32, c_int32, c_void_p, c_size_t, POINTER(Shape), _i32p, c_void_p]),

@@ -451,12 +451,16 @@ def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indice
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])
     lib = _lib.load()
-    need = 0 if workspace is not None else int(lib.ktk_prefill_mass_workspace_bytes(ctypes.byref(shp), total))
+    if view is not None and view.page_count is not None:
+        most, pages = mass.shape[2] // PAGE_SIZE + 2, -1
+    else:
+        most, pages = max(kv_indices.numel(), 1), kv_indices.numel()
+    need = 0 if workspace is not None else int(lib.ktk_prefill_mass_workspace_bytes(ctypes.byref(shp), total, max_new_tokens,
+                                                                                    most, pages, window))
     workspace, wsb = _scratch(need, workspace, q.device)
-    most = mass.shape[2] if view is not None and view.page_count is not None else kv_indices.numel() * PAGE_SIZE
     vp, _keep = _view_ref(view)
     check(lib.ktk_prefill_attention_mass(_ptr(q), _ptr(q_indptr), total, int(max_new_tokens), _ptr(kv_cache),
-                                         _ptr(kv_indices), _ptr(kv_indptr), _ptr(kv_last_page_len), vp, max(most, 1), window,
+                                         _ptr(kv_indices), _ptr(kv_indptr), _ptr(kv_last_page_len), vp, most, pages, window,
                                          sm_scale, ctypes.byref(m), _ptr(out), _ptr(workspace), wsb, ctypes.byref(shp),
                                          _ptr(status), _stream()))
     _launched(2 if kv_cache.dtype == torch.bfloat16 else 3)
