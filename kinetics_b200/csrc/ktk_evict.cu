@@ -1,11 +1,11 @@
 // Eviction from a paged cache by accumulated attention weight: of every (sequence, kv head) with more than `keep` tokens the ones
 // of largest mass stay, with the first and the newest.  The kept tokens behind place `keep` move into the holes in front of it.
 //
-// evict_plan_kernel, one CTA per (sequence, kv head): every token has a 32-bit key whose order is that of the masses (the
-// first and newest: the largest key, NaN: the smallest).  The keep-th largest key is found two bits at a time, by counting the keys
-// that reach each of three thresholds; tokens at exactly that key stay from the lowest place on.  Which tokens stay is held as one bit
-// each, and prefix sums over the bits' words number the holes and the tokens that move.
-// evict_move_kernel copies keys and values, a warp to a token.
+// One CTA per (sequence, kv head) plans: every token has a 32-bit key whose order is that of the masses (the first and newest:
+// the largest key, NaN: the smallest).  The keep-th largest key is found two bits at a time, by counting the keys that reach each of
+// three thresholds, until a threshold is reached by exactly `keep` keys; tokens at exactly the last threshold stay from the lowest
+// place on.  Which tokens stay is held as one bit each, and prefix sums over the bits' words number the holes and the tokens that move.
+// Keys and values are copied a warp to a token, by the planning CTA or by a launch of their own (evict_move_kernel).
 #include "ktk_decode.cuh"
 
 namespace ktk {
@@ -34,7 +34,7 @@ struct EvictParams {
     int32_t* from;                    // [units][max_moves] their places
     int32_t* to;                      // [units][max_moves] the holes
     int max_moves;
-    int smem_keys;                    // keys that shared memory holds (0: they are made again in every pass)
+    int smem_keys;                    // of evict_long_kernel: keys that shared memory holds (0: none)
     int32_t* status;
 };
 
@@ -44,21 +44,22 @@ __device__ __forceinline__ uint32_t evict_key(float mass) {
     return mass != mass ? 0u : score_to_key(mass);        // NaN less than -inf (whose key is above 0)
 }
 
-// Sum over the block of up to three 21-bit counts packed in 64 bits; every thread gets it.  Two buffers in turn: one barrier each.
+// Sums over the block of three counts, up to 2^21 each, packed in 64 bits; every thread gets them.  Two buffers in turn: one barrier each.
 template <int THREADS>
-__device__ __forceinline__ uint64_t block_sum(uint64_t x, uint64_t (*buf)[32], int& turn) {
+__device__ __forceinline__ uint64_t block_sum(uint32_t n1, uint32_t n2, uint32_t n3, uint64_t (*buf)[32], int& turn) {
     constexpr int W = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    if (lane == 0) buf[turn][warp] = x;
+    n1 = __reduce_add_sync(0xffffffffu, n1);
+    n2 = __reduce_add_sync(0xffffffffu, n2);
+    n3 = __reduce_add_sync(0xffffffffu, n3);
+    if (lane == 0) buf[turn][warp] = (uint64_t)n1 | (uint64_t)n2 << 21 | (uint64_t)n3 << 42;
     __syncthreads();
-    x = lane < W ? buf[turn][lane] : 0;
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    x = __shfl_sync(0xffffffffu, x, 0);
+    const uint64_t x = lane < W ? buf[turn][lane] : 0;
+    n1 = __reduce_add_sync(0xffffffffu, (uint32_t)(x & 0x1fffff));
+    n2 = __reduce_add_sync(0xffffffffu, (uint32_t)(x >> 21 & 0x1fffff));
+    n3 = __reduce_add_sync(0xffffffffu, (uint32_t)(x >> 42));
     turn ^= 1;
-    return x;
+    return (uint64_t)n1 | (uint64_t)n2 << 21 | (uint64_t)n3 << 42;
 }
 
 // Exclusive prefix sum over the block's threads, and the total
@@ -86,172 +87,321 @@ __device__ __forceinline__ uint64_t block_prefix(uint64_t x, uint64_t (*buf)[32]
     return before + incl - x;
 }
 
-template <int THREADS>
+// A (sequence, kv head) and its tokens; false: nothing is evicted from it
+struct EvictUnit {
+    int n, stored, seen, start, first_fill;
+    int64_t at;                                      // of its row in masses and positions
+    const float* mass;
+    const int32_t* pos;
+    __device__ __forceinline__ int position(int t) const { return t < stored ? pos[t] : seen - n + t; }
+};
+__device__ __forceinline__ bool evict_unit(const EvictParams& p, int64_t unit, int most, EvictUnit& u) {
+    const int b = (int)(unit / p.Hkv), h = (int)(unit % p.Hkv);
+    const SeqPages sp = seq_pages(p.kv_indptr, p.page_count, p.kv_last_page_len, p.sink_tokens, b);
+    const int row = p.slot_index ? p.slot_index[b] : b;
+    u.n = sp.total;
+    u.start = sp.start;
+    u.first_fill = sp.first_fill;
+    if (sp.bad || row < 0 || row >= p.rows || u.n > p.stride || sp.n_pages > p.max_pages || u.n > most) {
+        if (threadIdx.x == 0) report(p.status, KTK_STATUS_BAD_TABLE);
+        return false;
+    }
+    if (u.n <= 0) return false;
+    u.at = ((int64_t)row * p.Hkv + h) * p.stride;
+    u.mass = p.mass_in + u.at;
+    u.pos = p.pos_in + u.at;
+    u.stored = p.stored[row];
+    u.seen = p.seen[row];
+    return true;
+}
+__device__ __forceinline__ uint32_t key_at(const EvictParams& p, const EvictUnit& u, int t) {
+    const int at = u.position(t);
+    const float mass = u.mass[t];
+    return at < p.sink || at >= u.seen - p.recent ? 0xffffffffu : evict_key(mass);
+}
+// What stays in its place: to be read (before anything is written), to be written
+struct EvictCopy {
+    float mass;
+    int pos;
+};
+__device__ __forceinline__ EvictCopy copy_read(const EvictParams& p, const EvictUnit& u, int t) {
+    return {p.mass_in == p.mass_out ? 0.0f : u.mass[t], p.pos_in == p.pos_out && t < u.stored ? 0 : u.position(t)};
+}
+__device__ __forceinline__ void copy_write(const EvictParams& p, const EvictUnit& u, int t, const EvictCopy& c) {
+    if (p.mass_in != p.mass_out) p.mass_out[u.at + t] = c.mass;
+    if (p.pos_in != p.pos_out || t >= u.stored) p.pos_out[u.at + t] = c.pos;
+}
+
+// ITEMS keys per thread, t = j * THREADS + thread: visit(j, t) for those that there are
+template <int THREADS, int ITEMS, class Visit>
+__device__ __forceinline__ void each_item(int n, Visit visit) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+        if (j * THREADS >= n) break;                 // uniform
+        visit(j, j * THREADS + (int)threadIdx.x);
+    }
+}
+
+// The words of places in front of `keep`
+__device__ __forceinline__ uint32_t in_front(int w, int keep) {
+    return w * 32 + 32 <= keep ? 0xffffffffu : w * 32 >= keep ? 0u : (1u << (keep - w * 32)) - 1u;
+}
+
+// above, level: one bit per token, its key is above the threshold, at it.  Numbers the holes and the tokens that move, in the order of
+// their places: hole(i, t), mover(i, t).  `above` becomes: the token stays.  Returns how many move.
+template <int THREADS, class Hole, class Mover>
+__device__ __forceinline__ int number_moves(uint32_t* above, const uint32_t* level, int words, int keep, int need, uint64_t (*buf)[32],
+                                            int& turn, Hole hole, Mover mover) {
+    const int tid = threadIdx.x;
+    // words of a thread: consecutive ones, so that prefix sums over threads go by place
+    const int each = (words + THREADS - 1) / THREADS;
+    const int w0 = tid * each < words ? tid * each : words, w1 = w0 + each < words ? w0 + each : words;
+    uint64_t total;
+    int left = 0;                                    // how many at the threshold the thread's words may still keep
+    if (need > 0) {
+        uint32_t ties = 0;
+        for (int w = w0; w < w1; ++w) ties += __popc(level[w]);
+        left = need - (int)block_prefix<THREADS>(ties, buf, turn, total);
+    }
+    uint32_t holes = 0, movers = 0;
+    for (int w = w0; w < w1; ++w) {
+        uint32_t stay = above[w];
+        if (need > 0) {
+            for (uint32_t l = level[w]; l != 0 && left > 0; l &= l - 1, --left) stay |= l & (0u - l);      // the lowest places first
+            above[w] = stay;
+        }
+        holes += __popc(~stay & in_front(w, keep));
+        movers += __popc(stay & ~in_front(w, keep));
+    }
+    const uint64_t first = block_prefix<THREADS>((uint64_t)holes | (uint64_t)movers << 32, buf, turn, total);
+    int i = (int)(uint32_t)first, k = (int)(first >> 32);
+    for (int w = w0; w < w1; ++w) {
+        for (uint32_t x = ~above[w] & in_front(w, keep); x != 0; x &= x - 1) hole(i++, w * 32 + __ffs((int)x) - 1);
+        for (uint32_t x = above[w] & ~in_front(w, keep); x != 0; x &= x - 1) mover(k++, w * 32 + __ffs((int)x) - 1);
+    }
+    return (int)(uint32_t)total;
+}
+
+// Two bits of the threshold from the counts of keys that reach it plus 1, 2, 3 steps; whether exactly `keep` keys reach it now
+__device__ __forceinline__ bool next_bits(uint64_t counts, int keep, int shift, uint32_t& threshold) {
+    const auto count = [&](int i) { return (int)(counts >> (21 * i) & 0x1fffff); };
+    const int step = count(2) >= keep ? 3 : count(1) >= keep ? 2 : count(0) >= keep ? 1 : 0;
+    threshold += (uint32_t)step << shift;
+    return step > 0 && count(step - 1) == keep;
+}
+
+// Tokens of a warp's copies, their loads in flight together
+constexpr int kEvEach = 4;
+// Copies keys and values of moves first .. first + kEvEach - 1 (of `moves`): from(i) -> to(i).  CHUNKS: 16-byte pieces of a token's key
+// (as many of its value)
+template <int CHUNKS, class From, class To>
+__device__ __forceinline__ void copy_tokens(const EvictParams& p, int h, int start, int first_fill, int first, int moves, From from, To to) {
+    constexpr int kLoads = 2 * CHUNKS / 32;
+    const int lane = threadIdx.x & 31;
+    uint4* cache = (uint4*)p.cache;
+    // the 16-byte piece `c` of the token in place t: its key's, then its value's; -1: no such page
+    const auto piece = [&](int t, int c) -> int64_t {
+        int e, slot;
+        page_of_pos(t, first_fill, e, slot);
+        const int64_t page = __ldg(p.kv_indices + start + e);
+        if (page < 0 || page >= p.num_pages) return -1;
+        return (((page * 2 + c / CHUNKS) * kPageSize + slot) * p.Hkv + h) * CHUNKS + c % CHUNKS;
+    };
+    uint4 v[kEvEach][kLoads];
+    int64_t dst[kEvEach][kLoads];
+#pragma unroll
+    for (int i = 0; i < kEvEach; ++i) {
+        const bool on = first + i < moves;
+        const int s = on ? from(first + i) : 0, d = on ? to(first + i) : 0;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            dst[i][j] = -1;
+            if (!on) continue;
+            const int64_t src = piece(s, j * 32 + lane);
+            if (src >= 0) dst[i][j] = piece(d, j * 32 + lane);
+            if (dst[i][j] >= 0) v[i][j] = cache[src];
+            else report(p.status, KTK_STATUS_BAD_PAGE);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kEvEach; ++i)
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j)
+            if (dst[i][j] >= 0) cache[dst[i][j]] = v[i][j];
+}
+
+// Sequences of at most THREADS * ITEMS tokens: keys in registers.  CHUNKS 0: keys and values are left to evict_move_kernel.
+template <int THREADS, int ITEMS, int CHUNKS>
 __global__ void __launch_bounds__(THREADS)
-evict_plan_kernel(const EvictParams p) {
+evict_kernel(const EvictParams p) {
+    constexpr int kMost = THREADS * ITEMS, kWords = kMost / 32;
+    __shared__ uint64_t buf[2][32];
+    __shared__ uint32_t above[kWords], level[kWords];
+    extern __shared__ uint16_t ev_lists[];           // [max_moves] from, [max_moves] to
+    uint16_t *from = ev_lists, *to = from + p.max_moves;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    wait_for_front();
+    const int64_t unit = blockIdx.x;
+    EvictUnit u;
+    if (!evict_unit(p, unit, kMost, u)) {
+        if (CHUNKS == 0 && tid == 0) p.count[unit] = 0;
+        return;
+    }
+    const int n = u.n, keep = p.keep;
+    uint32_t key[ITEMS];
+    if (n > keep) {
+        each_item<THREADS, ITEMS>(n, [&](int j, int t) { key[j] = t < n ? key_at(p, u, t) : 0; });
+    }
+    // what stays is read early as well: the copies are written behind the search
+    EvictCopy stay[ITEMS];
+    const int front = n < keep ? n : keep;
+    each_item<THREADS, ITEMS>(front, [&](int j, int t) { if (t < front) stay[j] = copy_read(p, u, t); });
+    if (n <= keep) {
+        each_item<THREADS, ITEMS>(n, [&](int j, int t) { if (t < n) copy_write(p, u, t, stay[j]); });
+        if (CHUNKS == 0 && tid == 0) p.count[unit] = 0;
+        return;
+    }
+    int turn = 0;
+    uint32_t threshold = 0;                          // the largest, of the bits so far, that at least `keep` keys reach
+    bool exact = false;
+    for (int shift = 30; shift >= 0 && !exact; shift -= 2) {
+        const uint32_t c1 = threshold + (1u << shift), c2 = threshold + (2u << shift), c3 = threshold + (3u << shift);
+        uint32_t n1 = 0, n2 = 0, n3 = 0;
+        each_item<THREADS, ITEMS>(n, [&](int j, int) {       // a key of 0 reaches none
+            n1 += key[j] >= c1;
+            n2 += key[j] >= c2;
+            n3 += key[j] >= c3;
+        });
+        exact = next_bits(block_sum<THREADS>(n1, n2, n3, buf, turn), keep, shift, threshold);
+    }
+    uint32_t over = 0;
+    each_item<THREADS, ITEMS>(n, [&](int j, int t) {
+        const uint32_t a = __ballot_sync(0xffffffffu, t < n && (key[j] > threshold || (exact && key[j] == threshold)));
+        const uint32_t l = __ballot_sync(0xffffffffu, t < n && !exact && key[j] == threshold);
+        if (lane == 0) {
+            above[t / 32] = a;
+            level[t / 32] = l;
+            over += __popc(a);
+        }
+    });
+    const int need = keep - (int)(block_sum<THREADS>(over, 0, 0, buf, turn) & 0x1fffff);
+    const int moves = number_moves<THREADS>(above, level, (n + 31) / 32, keep, need, buf, turn,
+                                            [&](int i, int t) { to[i] = (uint16_t)t; }, [&](int i, int t) { from[i] = (uint16_t)t; });
+    __syncthreads();
+    if constexpr (CHUNKS > 0) {
+        for (int i = warp * kEvEach; i < moves; i += THREADS / 32 * kEvEach)
+            copy_tokens<CHUNKS>(p, (int)(unit % p.Hkv), u.start, u.first_fill, i, moves, [&](int k) { return (int)from[k]; },
+                                [&](int k) { return (int)to[k]; });
+    } else {
+        if (tid == 0) p.count[unit] = moves;
+        for (int i = tid; i < moves; i += THREADS) {
+            p.from[unit * p.max_moves + i] = from[i];
+            p.to[unit * p.max_moves + i] = to[i];
+        }
+    }
+    each_item<THREADS, ITEMS>(front, [&](int j, int t) {
+        if (t < front && (above[t >> 5] >> (t & 31) & 1u)) copy_write(p, u, t, stay[j]);
+    });
+    for (int i = tid; i < moves; i += THREADS) {
+        const float mass = u.mass[from[i]];
+        const int at = u.position(from[i]);
+        p.mass_out[u.at + to[i]] = mass;
+        p.pos_out[u.at + to[i]] = at;
+    }
+}
+
+// Longer ones: keys in shared memory, or made again in every pass.
+constexpr int kEvLong = 1024;
+__global__ void __launch_bounds__(kEvLong)
+evict_long_kernel(const EvictParams p) {
     extern __shared__ __align__(16) uint32_t ev_smem[];
     __shared__ uint64_t buf[2][32];
     const int tid = threadIdx.x, lane = tid & 31;
     wait_for_front();
     const int64_t unit = blockIdx.x;
-    const int b = (int)(unit / p.Hkv), h = (int)(unit % p.Hkv);
-    const SeqPages sp = seq_pages(p.kv_indptr, p.page_count, p.kv_last_page_len, p.sink_tokens, b);
-    const int n = sp.total, row = p.slot_index ? p.slot_index[b] : b;
-    const bool bad = sp.bad || row < 0 || row >= p.rows || n > p.stride || sp.n_pages > p.max_pages;
-    if (bad || n <= 0) {
-        if (tid == 0) {
-            if (bad) report(p.status, KTK_STATUS_BAD_TABLE);
-            p.count[unit] = 0;
-        }
+    EvictUnit u;
+    if (!evict_unit(p, unit, kEvMaxPages * kPageSize, u)) {
+        if (tid == 0) p.count[unit] = 0;
         return;
     }
-    const int64_t at = ((int64_t)row * p.Hkv + h) * p.stride;
-    const float* mass = p.mass_in + at;
-    const int32_t* pos = p.pos_in + at;
-    const int stored = p.stored[row], seen = p.seen[row], keep = p.keep;
-    const auto position = [&](int t) { return t < stored ? pos[t] : seen - n + t; };
-    const bool same_mass = p.mass_in == p.mass_out, same_pos = p.pos_in == p.pos_out;
-    // what stays in its place
-    const auto copy = [&](int t) {
-        if (!same_mass) p.mass_out[at + t] = mass[t];
-        if (!same_pos || t >= stored) p.pos_out[at + t] = position(t);
-    };
+    const int n = u.n, keep = p.keep;
     if (n <= keep) {
-        for (int t = tid; t < n; t += THREADS) copy(t);
+        for (int t = tid; t < n; t += kEvLong) copy_write(p, u, t, copy_read(p, u, t));
         if (tid == 0) p.count[unit] = 0;
         return;
     }
     const int words = (n + 31) / 32;
-    uint32_t* above = ev_smem;                       // one bit per token: its key is above the threshold; later: it stays
-    uint32_t* level = above + words;                 // its key is the threshold
-    uint32_t* keys = level + words;
+    uint32_t *above = ev_smem, *level = above + words, *keys = level + words;
     const bool held = n <= p.smem_keys;
-    const auto make_key = [&](int t) -> uint32_t {
-        const int at_pos = position(t);
-        return at_pos < p.sink || at_pos >= seen - p.recent ? 0xffffffffu : evict_key(mass[t]);
-    };
     if (held) {
-        for (int t = tid; t < n; t += THREADS) keys[t] = make_key(t);
+        for (int t = tid; t < n; t += kEvLong) keys[t] = key_at(p, u, t);
         __syncthreads();
     }
-    const auto key_of = [&](int t) { return held ? keys[t] : make_key(t); };
-
+    const auto key_of = [&](int t) { return held ? keys[t] : key_at(p, u, t); };
     int turn = 0;
-    uint32_t threshold = 0;                          // the largest that at least `keep` keys reach
-    for (int shift = 30; shift >= 0; shift -= 2) {
+    uint32_t threshold = 0;
+    bool exact = false;
+    for (int shift = 30; shift >= 0 && !exact; shift -= 2) {
         const uint32_t c1 = threshold + (1u << shift), c2 = threshold + (2u << shift), c3 = threshold + (3u << shift);
         uint32_t n1 = 0, n2 = 0, n3 = 0;
-        for (int t = tid; t < n; t += THREADS) {
+        for (int t = tid; t < n; t += kEvLong) {
             const uint32_t k = key_of(t);
             n1 += k >= c1;
             n2 += k >= c2;
             n3 += k >= c3;
         }
-        const uint64_t sum = block_sum<THREADS>((uint64_t)n1 | (uint64_t)n2 << 21 | (uint64_t)n3 << 42, buf, turn);
-        const auto reach = [&](int i) { return (int)(sum >> (21 * i) & 0x1fffff) >= keep; };
-        if (reach(2)) threshold = c3;
-        else if (reach(1)) threshold = c2;
-        else if (reach(0)) threshold = c1;
+        exact = next_bits(block_sum<kEvLong>(n1, n2, n3, buf, turn), keep, shift, threshold);
     }
     uint32_t over = 0;
-    for (int t0 = tid - lane; t0 < words * 32; t0 += THREADS) {
+    for (int t0 = tid - lane; t0 < words * 32; t0 += kEvLong) {
         const int t = t0 + lane;
         const uint32_t k = t < n ? key_of(t) : 0;
-        const uint32_t a = __ballot_sync(0xffffffffu, t < n && k > threshold), l = __ballot_sync(0xffffffffu, t < n && k == threshold);
+        const uint32_t a = __ballot_sync(0xffffffffu, t < n && (k > threshold || (exact && k == threshold)));
+        const uint32_t l = __ballot_sync(0xffffffffu, t < n && !exact && k == threshold);
         if (lane == 0) {
             above[t0 / 32] = a;
             level[t0 / 32] = l;
             over += __popc(a);
         }
     }
-    const int need = keep - (int)block_sum<THREADS>(over, buf, turn);          // how many at the threshold stay
-    // words of a thread: consecutive ones, so that prefix sums over threads go by place
-    const int each = (words + THREADS - 1) / THREADS;
-    const int w0 = tid * each < words ? tid * each : words, w1 = w0 + each < words ? w0 + each : words;
-    uint32_t ties = 0;
-    for (int w = w0; w < w1; ++w) ties += __popc(level[w]);
-    uint64_t total;
-    int left = need - (int)block_prefix<THREADS>(ties, buf, turn, total);      // that the thread's words may still give
-    uint32_t holes = 0, movers = 0;
-    const auto in_front = [&](int w) { return w * 32 + 32 <= keep ? 0xffffffffu : w * 32 >= keep ? 0u : (1u << (keep - w * 32)) - 1u; };
-    for (int w = w0; w < w1; ++w) {
-        uint32_t l = level[w], stay = above[w];
-        while (l != 0 && left > 0) {                 // the lowest places first
-            stay |= l & (0u - l);
-            l &= l - 1;
-            --left;
-        }
-        above[w] = stay;
-        holes += __popc(~stay & in_front(w));
-        movers += __popc(stay & ~in_front(w));
-    }
-    const uint64_t first = block_prefix<THREADS>((uint64_t)holes | (uint64_t)movers << 32, buf, turn, total);
-    int hole = (int)(uint32_t)first, mover = (int)(first >> 32);
-    int32_t* from = p.from + unit * p.max_moves;
-    int32_t* to = p.to + unit * p.max_moves;
-    for (int w = w0; w < w1; ++w) {
-        for (uint32_t x = ~above[w] & in_front(w); x != 0; x &= x - 1) to[hole++] = w * 32 + __ffs((int)x) - 1;
-        for (uint32_t x = above[w] & ~in_front(w); x != 0; x &= x - 1) from[mover++] = w * 32 + __ffs((int)x) - 1;
-    }
+    const int need = keep - (int)(block_sum<kEvLong>(over, 0, 0, buf, turn) & 0x1fffff);
+    int32_t *from = p.from + unit * p.max_moves, *to = p.to + unit * p.max_moves;
+    const int moves = number_moves<kEvLong>(above, level, words, keep, need, buf, turn, [&](int i, int t) { to[i] = t; },
+                                            [&](int i, int t) { from[i] = t; });
     __syncthreads();
-    const int moves = (int)(uint32_t)total;
     if (tid == 0) p.count[unit] = moves;
-    for (int t = tid; t < keep; t += THREADS)
-        if (above[t >> 5] >> (t & 31) & 1u) copy(t);
-    for (int i = tid; i < moves; i += THREADS) {
+    for (int t = tid; t < keep; t += kEvLong)
+        if (above[t >> 5] >> (t & 31) & 1u) copy_write(p, u, t, copy_read(p, u, t));
+    for (int i = tid; i < moves; i += kEvLong) {
         const int s = from[i], d = to[i];
-        p.mass_out[at + d] = mass[s];
-        p.pos_out[at + d] = position(s);
+        p.mass_out[u.at + d] = u.mass[s];
+        p.pos_out[u.at + d] = u.position(s);
     }
 }
 
 constexpr int kEvWarps = 8;
-constexpr int kEvEach = 4;            // tokens of a warp, their loads in flight together
-
-// CHUNKS: 16-byte pieces of a token's key (as many of its value)
 template <int CHUNKS>
 __global__ void __launch_bounds__(kEvWarps * 32)
 evict_move_kernel(const EvictParams p, int parts) {
-    constexpr int kLoads = 2 * CHUNKS / 32;
     wait_for_front();
     const int64_t unit = blockIdx.x / parts;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int first = ((int)(blockIdx.x % parts) * kEvWarps + warp) * kEvEach;
+    const int first = ((int)(blockIdx.x % parts) * kEvWarps + (threadIdx.x >> 5)) * kEvEach;
     const int moves = p.count[unit];
     if (first >= moves) return;
-    const int b = (int)(unit / p.Hkv), h = (int)(unit % p.Hkv);
-    const int start = p.kv_indptr[b], first_fill = p.sink_tokens > 0 ? p.sink_tokens : kPageSize;
-    uint4* cache = (uint4*)p.cache;
-    // the 16-byte piece `c` of the token in place t: its key's, then its value's; -1: no such page
-    const auto piece = [&](int t, int c) -> int64_t {
-        int e, slot;
-        page_of_pos(t, first_fill, e, slot);
-        const int64_t page = p.kv_indices[start + e];
-        if (page < 0 || page >= p.num_pages) return -1;
-        return (((page * 2 + c / CHUNKS) * kPageSize + slot) * p.Hkv + h) * CHUNKS + c % CHUNKS;
-    };
-    const int n = moves - first < kEvEach ? moves - first : kEvEach;
-    uint4 v[kEvEach][kLoads];
-    int64_t dst[kEvEach][kLoads];
-#pragma unroll
-    for (int i = 0; i < kEvEach; ++i) {
-        if (i >= n) break;
-        const int s = p.from[unit * p.max_moves + first + i], d = p.to[unit * p.max_moves + first + i];
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const int64_t src = piece(s, j * 32 + lane);
-            dst[i][j] = src < 0 ? -1 : piece(d, j * 32 + lane);
-            if (dst[i][j] >= 0) v[i][j] = cache[src];
-            else report(p.status, KTK_STATUS_BAD_PAGE);
-        }
+    const int32_t *from = p.from + unit * p.max_moves, *to = p.to + unit * p.max_moves;
+    copy_tokens<CHUNKS>(p, (int)(unit % p.Hkv), p.kv_indptr[unit / p.Hkv], p.sink_tokens > 0 ? p.sink_tokens : kPageSize, first, moves,
+                        [&](int k) { return from[k]; }, [&](int k) { return to[k]; });
+}
+
+template <int THREADS, int ITEMS>
+static cudaError_t launch_evict(const EvictParams& p, int64_t units, bool fused, bool f32, cudaStream_t st) {
+    const auto kernel = !fused ? evict_kernel<THREADS, ITEMS, 0> : f32 ? evict_kernel<THREADS, ITEMS, 32> : evict_kernel<THREADS, ITEMS, 16>;
+    const size_t smem = (size_t)p.max_moves * 2 * sizeof(uint16_t);
+    if (smem > 32 * 1024) {                          // beside the static words
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
     }
-#pragma unroll
-    for (int i = 0; i < kEvEach; ++i) {
-        if (i >= n) break;
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j)
-            if (dst[i][j] >= 0) cache[dst[i][j]] = v[i][j];
-    }
+    return launch_behind(units <= sm_count(), kernel, (unsigned)units, THREADS, smem, st, p);
 }
 
 static int64_t evict_max_moves(int max_pages, int keep) {
@@ -318,22 +468,26 @@ extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_
     p.to = p.from + units * p.max_moves;
 
     const int64_t most = (int64_t)max_pages_per_seq * kPageSize;
-    const size_t bits = (size_t)((most + 31) / 32) * 2 * sizeof(uint32_t), room = 200 * 1024;
-    p.smem_keys = bits + most * sizeof(uint32_t) <= room ? (int)most : 0;
-    const size_t smem = bits + (size_t)p.smem_keys * sizeof(uint32_t);
     cudaStream_t st = (cudaStream_t)stream;
-    const bool wide = most > 4096;
-    const auto kernel = wide ? evict_plan_kernel<1024> : evict_plan_kernel<256>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
-    KTK_CUDA_TRY(launch_behind(false, kernel, (unsigned)units, wide ? 1024 : 256, smem, st, p), who);
     const int parts = (p.max_moves + kEvWarps * kEvEach - 1) / (kEvWarps * kEvEach);
     if (units * parts > 2147483647LL) {
         set_error("%s: too many tokens to move in one launch", who);
         return KTK_ERR_TOO_LARGE;
     }
-    if (s->dtype == KTK_F32)
-        KTK_CUDA_TRY(launch_behind(true, evict_move_kernel<32>, (unsigned)(units * parts), kEvWarps * 32, 0, st, p, parts), who);
-    else
-        KTK_CUDA_TRY(launch_behind(true, evict_move_kernel<16>, (unsigned)(units * parts), kEvWarps * 32, 0, st, p, parts), who);
+    const bool fused = most <= 32768 && (units >= sm_count() || p.max_moves <= 256);
+    const bool f32 = s->dtype == KTK_F32;
+    if (most <= 4096) KTK_CUDA_TRY((launch_evict<512, 8>(p, units, fused, f32, st)), who);
+    else if (most <= 16384) KTK_CUDA_TRY((launch_evict<1024, 16>(p, units, fused, f32, st)), who);
+    else if (most <= 32768) KTK_CUDA_TRY((launch_evict<1024, 32>(p, units, fused, f32, st)), who);
+    else {
+        const size_t bits = (size_t)((most + 31) / 32) * 2 * sizeof(uint32_t), room = 200 * 1024;
+        p.smem_keys = bits + most * sizeof(uint32_t) <= room ? (int)most : 0;
+        const size_t smem = bits + (size_t)p.smem_keys * sizeof(uint32_t);
+        KTK_CUDA_TRY(cudaFuncSetAttribute(evict_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+        KTK_CUDA_TRY(launch_behind(false, evict_long_kernel, (unsigned)units, kEvLong, smem, st, p), who);
+    }
+    if (fused) return KTK_OK;
+    const auto move = f32 ? evict_move_kernel<32> : evict_move_kernel<16>;
+    KTK_CUDA_TRY(launch_behind(true, move, (unsigned)(units * parts), kEvWarps * 32, 0, st, p, parts), who);
     return KTK_OK;
 }

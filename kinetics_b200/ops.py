@@ -358,18 +358,29 @@ def prefill_attention(q, q_indptr, max_new_tokens: int, kv_cache, kv_indices, kv
 
 
 # ---- a cache of bounded size: attention that adds up what tokens were paid, and the eviction that goes by it
+# A decode step of few sequences takes the device some ten microseconds: these calls look at their tensors once and hand plain
+# integers to the library.
 
-def _on_one_device(first, *others) -> None:
-    """The launch goes to the current device's stream: all tensors have to be there."""
-    dev = first.get_device()
-    if dev != torch.cuda.current_device():
-        raise RuntimeError(f"kinetics_b200: tensors on cuda:{dev}, current device cuda:{torch.cuda.current_device()}")
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            raise RuntimeError(f"kinetics_b200: tensors on cuda:{dev} and {t.device}")
+def _addresses(*tensors):
+    """Addresses of contiguous tensors on the current device (None: 0), and that device's stream."""
+    dev = torch.cuda.current_device()
+    at = []
+    for t in tensors:
+        if t is None:
+            at.append(0)
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("kinetics_b200 ops need CUDA tensors: this path has no CPU fallback")
+        if not t.is_contiguous():
+            raise RuntimeError("kinetics_b200 ops need contiguous tensors")
+        if t.get_device() != dev:
+            raise RuntimeError(f"kinetics_b200: a tensor on {t.device}, the current device is cuda:{dev}")
+        at.append(t.data_ptr())
+    at.append(torch._C._cuda_getCurrentRawStream(dev))
+    return at
 
 
-def _table_tensors(batch, kv_indices, kv_indptr, kv_last_page_len, view) -> None:
+def _check_table(batch, kv_indices, kv_indptr, kv_last_page_len, view) -> None:
     if kv_indices.dtype != torch.int32 or kv_indptr.dtype != torch.int32 or kv_last_page_len.dtype != torch.int32:
         raise TypeError("page tables are int32")
     if _batch_of(kv_indptr, view) != batch or kv_last_page_len.numel() < batch:
@@ -378,24 +389,29 @@ def _table_tensors(batch, kv_indices, kv_indptr, kv_last_page_len, view) -> None
         raise ValueError(f"PageView: page_count and slot_index have {batch} entries")
 
 
-def _mass_args(mass, mass_out, batch, num_kv_heads, decay, view):
-    """(ktk_mass, mass_out): mass fp32 [rows, Hkv, places]; without a slot_index one row per sequence."""
-    if mass_out is None:
-        mass_out = mass
+def _check_queries(q, kv_cache, out) -> None:
+    if q.dim() != 3 or q.shape[2] != kv_cache.shape[-1]:
+        raise ValueError(f"q must be [rows, Hq, {kv_cache.shape[-1]}], got {tuple(q.shape)}")
+    if q.dtype != kv_cache.dtype or out.dtype != q.dtype or out.shape != q.shape:
+        raise TypeError("q, kv_cache and out must share a dtype, out the shape of q")
+
+
+def _check_mass(mass, mass_out, batch, num_kv_heads, view) -> None:
+    """mass fp32 [rows, Hkv, places]; without a slot_index one row per sequence."""
     if mass.dtype != torch.float32 or mass_out.dtype != torch.float32:
         raise TypeError("mass is fp32")
     if mass.dim() != 3 or mass.shape[1] != num_kv_heads or mass_out.shape != mass.shape:
         raise ValueError(f"mass must be [rows, {num_kv_heads}, places], got {tuple(mass.shape)} and {tuple(mass_out.shape)}")
     if mass.shape[0] < batch and (view is None or view.slot_index is None):
         raise ValueError(f"mass of {mass.shape[0]} rows for {batch} sequences")
-    return _lib.Mass(mass.data_ptr(), mass_out.data_ptr(), mass.shape[2], mass.shape[0], decay), mass_out
 
 
-def _scratch(need: int, workspace, device):
-    """The caller's workspace, or one from the allocator (which keeps calls on different streams, and graphs, apart)."""
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    return workspace, workspace.numel() * workspace.element_size()
+def _list_bounds(mass, kv_indices, view):
+    """Pages of the longest list, pages of all lists (-1: unknown), as far as the tensors' sizes tell."""
+    if view is not None and view.page_count is not None:
+        return mass.shape[2] // PAGE_SIZE + 2, -1
+    pages = kv_indices.numel()
+    return max(pages, 1), pages
 
 
 def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: int, mass, decay: float = 1.0,
@@ -405,27 +421,25 @@ def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_
     mass fp32 [rows, Hkv, places]: what the query heads of a group have paid the token in each place of its sequence
     (row: view.slot_index, else the sequence's number; different rows for different sequences).  Writes
     decay * mass + the weights of this step, and the weights alone for the newest token, to mass_out (None: mass itself);
-    places behind a sequence's length are left as they are.  Returns (out, mass_out)."""
-    _cuda(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, workspace, out, status)
-    _on_one_device(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, workspace, out, status)
-    B, Hq, _ = q.shape
-    shp = _shape(B, kv_cache, Hq)
-    if q.dtype != kv_cache.dtype or out is not None and (out.dtype != q.dtype or out.shape != q.shape):
-        raise TypeError("q, kv_cache and out must share a dtype, out the shape of q")
-    _table_tensors(B, kv_indices, kv_indptr, kv_last_page_len, view)
-    m, mass_out = _mass_args(mass, mass_out, B, shp.num_kv_heads, decay, view)
+    places behind a sequence's length are left as they are.  workspace: ``ktk_decode_mass_workspace_bytes`` bytes, not shared
+    by calls that may overlap (None: from the allocator, which keeps streams and graphs apart).  Returns (out, mass_out)."""
     if out is None:
         out = torch.empty_like(q)
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(q.shape[-1])
-    lib = _lib.load()
-    total = -1 if view is not None and view.page_count is not None else kv_indices.numel()
-    need = 0 if workspace is not None else int(lib.ktk_decode_mass_workspace_bytes(ctypes.byref(shp), max_pages_per_seq, total))
-    workspace, wsb = _scratch(need, workspace, q.device)
-    vp, _keep = _view_ref(view)
-    check(lib.ktk_dense_decode_mass(_ptr(q), _ptr(kv_cache), _ptr(kv_indices), _ptr(kv_indptr), _ptr(kv_last_page_len), vp,
-                                    max_pages_per_seq, total, sm_scale, ctypes.byref(m), _ptr(out), _ptr(workspace), wsb,
-                                    ctypes.byref(shp), _ptr(status), _stream()))
+    if mass_out is None:
+        mass_out = mass
+    lib, cv = _lib.load(), None if view is None else view.c()
+    _check_queries(q, kv_cache, out)
+    B, Hq, D = q.shape
+    shp = _shape(B, kv_cache, Hq)
+    _check_table(B, kv_indices, kv_indptr, kv_last_page_len, view)
+    _check_mass(mass, mass_out, B, shp.num_kv_heads, view)
+    total = _list_bounds(mass, kv_indices, view)[1]
+    if workspace is None:
+        workspace = torch.empty(lib.ktk_decode_mass_workspace_bytes(shp, max_pages_per_seq, total), dtype=torch.uint8, device=q.device)
+    q_, kv_, i_, p_, l_, m_, mo_, o_, w_, s_, stream = _addresses(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out,
+                                                                 out, workspace, status)
+    check(lib.ktk_dense_decode_mass(q_, kv_, i_, p_, l_, cv, max_pages_per_seq, total, D ** -0.5 if sm_scale is None else sm_scale,
+                                    _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], decay), o_, w_, workspace.nbytes, shp, s_, stream))
     _launched(2)
     return out, mass_out
 
@@ -434,35 +448,30 @@ def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indice
                            window: int = 0, decay: float = 1.0, sm_scale: Optional[float] = None, mass_out=None,
                            workspace=None, out=None, status=None, view=None):
     """``prefill_attention`` that also accumulates the weights that the last ``window`` new tokens of every sequence (0: all
-    of them) give each cached token; mass as in ``dense_decode_mass``, the sequence's new tokens start from their weights
-    alone.  Returns (out, mass_out)."""
-    _cuda(q, q_indptr, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, workspace, out, status)
-    _on_one_device(q, q_indptr, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, workspace, out, status)
-    total, Hq, _ = q.shape
-    B = q_indptr.numel() - 1
-    shp = _shape(B, kv_cache, Hq)
-    if q.dtype != kv_cache.dtype or q_indptr.dtype != torch.int32 or \
-            out is not None and (out.dtype != q.dtype or out.shape != q.shape):
-        raise TypeError("q, kv_cache and out must share a dtype, out the shape of q; q_indptr must be int32")
-    _table_tensors(B, kv_indices, kv_indptr, kv_last_page_len, view)
-    m, mass_out = _mass_args(mass, mass_out, B, shp.num_kv_heads, decay, view)
+    of them) give each cached token; mass and workspace as in ``dense_decode_mass``, the sequence's new tokens start from their
+    weights alone.  Returns (out, mass_out)."""
     if out is None:
         out = torch.empty_like(q)
-    if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(q.shape[-1])
-    lib = _lib.load()
-    if view is not None and view.page_count is not None:
-        most, pages = mass.shape[2] // PAGE_SIZE + 2, -1
-    else:
-        most, pages = max(kv_indices.numel(), 1), kv_indices.numel()
-    need = 0 if workspace is not None else int(lib.ktk_prefill_mass_workspace_bytes(ctypes.byref(shp), total, max_new_tokens,
-                                                                                    most, pages, window))
-    workspace, wsb = _scratch(need, workspace, q.device)
-    vp, _keep = _view_ref(view)
-    check(lib.ktk_prefill_attention_mass(_ptr(q), _ptr(q_indptr), total, int(max_new_tokens), _ptr(kv_cache),
-                                         _ptr(kv_indices), _ptr(kv_indptr), _ptr(kv_last_page_len), vp, most, pages, window,
-                                         sm_scale, ctypes.byref(m), _ptr(out), _ptr(workspace), wsb, ctypes.byref(shp),
-                                         _ptr(status), _stream()))
+    if mass_out is None:
+        mass_out = mass
+    lib, cv = _lib.load(), None if view is None else view.c()
+    _check_queries(q, kv_cache, out)
+    total, Hq, D = q.shape
+    B = q_indptr.numel() - 1
+    shp = _shape(B, kv_cache, Hq)
+    if q_indptr.dtype != torch.int32:
+        raise TypeError("q_indptr must be int32")
+    _check_table(B, kv_indices, kv_indptr, kv_last_page_len, view)
+    _check_mass(mass, mass_out, B, shp.num_kv_heads, view)
+    most, pages = _list_bounds(mass, kv_indices, view)
+    if workspace is None:
+        workspace = torch.empty(lib.ktk_prefill_mass_workspace_bytes(shp, total, max_new_tokens, most, pages, window), dtype=torch.uint8,
+                                device=q.device)
+    q_, n_, kv_, i_, p_, l_, m_, mo_, o_, w_, s_, stream = _addresses(q, q_indptr, kv_cache, kv_indices, kv_indptr, kv_last_page_len,
+                                                                     mass, mass_out, out, workspace, status)
+    check(lib.ktk_prefill_attention_mass(q_, n_, total, max_new_tokens, kv_, i_, p_, l_, cv, most, pages, window,
+                                         D ** -0.5 if sm_scale is None else sm_scale,
+                                         _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], decay), o_, w_, workspace.nbytes, shp, s_, stream))
     _launched(2 if kv_cache.dtype == torch.bfloat16 else 3)
     return out, mass_out
 
@@ -477,29 +486,27 @@ def evict(kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: 
     [rows, Hkv, places]: where the tokens of the first stored[row] places were in the sequence; those behind were appended in
     order, up to position seen[row] - 1 (stored, seen: int32 [rows]).  Afterwards a sequence holds min(n, keep) tokens: that
     is ``stored`` of the next call, and what the next page table has to say.  Page summaries have to be rebuilt.
-    Returns (mass_out, positions_out)."""
-    _cuda(kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, positions, stored, seen, mass_out, positions_out, workspace,
-          status)
-    _on_one_device(kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, positions, stored, seen, mass_out, positions_out,
-                   workspace, status)
-    B = _batch_of(kv_indptr, view)
-    shp = _shape(B, kv_cache, kv_cache.shape[3])
-    _table_tensors(B, kv_indices, kv_indptr, kv_last_page_len, view)
-    m, mass_out = _mass_args(mass, mass_out, B, shp.num_kv_heads, 1.0, view)
+    workspace: ``ktk_evict_workspace_bytes`` bytes, as in ``dense_decode_mass``.  Returns (mass_out, positions_out)."""
+    if mass_out is None:
+        mass_out = mass
     if positions_out is None:
         positions_out = positions
+    lib, cv = _lib.load(), None if view is None else view.c()
+    B = _batch_of(kv_indptr, view)
+    shp = _shape(B, kv_cache, kv_cache.shape[3])
+    _check_table(B, kv_indices, kv_indptr, kv_last_page_len, view)
+    _check_mass(mass, mass_out, B, shp.num_kv_heads, view)
     if any(t.dtype != torch.int32 for t in (positions, positions_out, stored, seen)):
         raise TypeError("positions, stored and seen are int32")
     if positions.shape != mass.shape or positions_out.shape != mass.shape or stored.numel() != mass.shape[0] or \
             seen.numel() != mass.shape[0]:
         raise ValueError("positions have the shape of mass, stored and seen one entry per row")
-    lib = _lib.load()
-    need = 0 if workspace is not None else int(lib.ktk_evict_workspace_bytes(ctypes.byref(shp), max_pages_per_seq, keep))
-    workspace, wsb = _scratch(need, workspace, kv_cache.device)
-    vp, _keep = _view_ref(view)
-    check(lib.ktk_evict(_ptr(kv_cache), _ptr(kv_indices), _ptr(kv_indptr), _ptr(kv_last_page_len), vp, max_pages_per_seq,
-                        ctypes.byref(m), _ptr(positions), _ptr(positions_out), _ptr(stored), _ptr(seen), keep, sink, recent,
-                        _ptr(workspace), wsb, ctypes.byref(shp), _ptr(status), _stream()))
+    if workspace is None:
+        workspace = torch.empty(lib.ktk_evict_workspace_bytes(shp, max_pages_per_seq, keep), dtype=torch.uint8, device=kv_cache.device)
+    kv_, i_, p_, l_, m_, mo_, at_, ato_, st_, se_, w_, s_, stream = _addresses(
+        kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, positions, positions_out, stored, seen, workspace, status)
+    check(lib.ktk_evict(kv_, i_, p_, l_, cv, max_pages_per_seq, _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], 1.0), at_, ato_, st_, se_,
+                        keep, sink, recent, w_, workspace.nbytes, shp, s_, stream))
     _launched(2)
     return mass_out, positions_out
 
