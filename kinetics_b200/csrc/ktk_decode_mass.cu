@@ -10,122 +10,147 @@
 namespace ktk {
 
 constexpr int kMassThreads = 256;
-constexpr int kMassTokens = 1024;                         // of a CTA
+constexpr int kMassEach = 4;                              // tokens of a thread, their loads in flight together
+constexpr int kMassTokens = kMassThreads * kMassEach;     // of a CTA
 
-// The pieces of a list: `count` of them, the k-th in row row(k) of the partials (times G heads).
-struct StreamPieces {
-    int64_t c;                                            // the CTA in which the list starts
+// The pieces of a list: `count` of them, 0 for a list that one CTA saw whole.  STREAM: behind the balanced partition; otherwise
+// num_splits partials of every list.
+template <bool STREAM> struct Pieces {
+    int64_t first;                                        // the CTA in which the list starts; the list's number
     int count;
-    __device__ __forceinline__ int64_t row(int k) const { return (c + k) * 2 + (k == 0 ? 1 : 0); }
-    __device__ __forceinline__ int64_t head_row(int k, int G, int g) const { return row(k) * G + g; }
-};
-struct SplitPieces {
-    int64_t unit;
-    int count;
-    __device__ __forceinline__ int64_t head_row(int k, int G, int g) const { return (unit * G + g) * count + k; }
+    __device__ __forceinline__ int64_t row(int k, int G, int g) const {
+        return STREAM ? ((first + k) * 2 + (k == 0 ? 1 : 0)) * G + g : (first * G + g) * count + k;
+    }
 };
 
-// One CTA per list and kMassTokens of its tokens.  STREAM: behind the balanced partition, where a list that one CTA saw whole has its
-// output and its denominator already; otherwise behind num_splits partials of every list.
-template <typename T, bool STREAM>
+// One CTA per list and kMassTokens of its tokens, and one per list for its output.
+template <typename T, bool STREAM, int G>
 __global__ void __launch_bounds__(kMassThreads)
 mass_finish_kernel(const StreamParams p, int chunks, int decode_ctas) {
-    __shared__ float lse[8];
+    __shared__ float lse[G];
     const DecodeParams& d = p.d;
     const MassParams& m = p.m;
-    const int G = p.G, tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31;
     wait_for_front();
-    const int64_t unit = blockIdx.x / chunks;
-    const int part = (int)(blockIdx.x % chunks);
+    const int64_t unit = blockIdx.x / (chunks + 1);
+    const int part = (int)(blockIdx.x % (chunks + 1));
     const int b = (int)(unit / d.Hkv), h = (int)(unit % d.Hkv);
     bool bad;
     EntryList el = entry_list(d, b, h, bad);
     const int64_t qh = ((int64_t)b * d.Hkv + h) * G;
     if (el.cnt == 0) {                                    // no token: zeros
-        if (part == 0)
+        if (part == chunks)
             for (int i = tid; i < G * kHeadDim; i += kMassThreads) ((T*)d.o)[qh * kHeadDim + i] = from_f32<T>(0.0f);
         return;
     }
     const int64_t start = list_position(d, m.wmax, b, h);
     if (el.cnt > m.max_pages) {
-        if (tid == 0 && part == 0) report(d.status, KTK_STATUS_BAD_TABLE);
+        if (tid == 0 && part == chunks) report(d.status, KTK_STATUS_BAD_TABLE);
         if (d.page_count) el.cnt = m.max_pages;           // padded lists are clipped by the decode
     }
-
-    const auto merge = [&](const auto& pieces) {
-        if (pieces.count == 0) {                          // whole
-            if (tid < G) lse[tid] = d.lse[qh + tid];
-            return;
-        }
-        if (part == 0) {
-            for (int i = tid; i < G * kHeadDim; i += kMassThreads) {
-                const int g = i / kHeadDim, dd = i % kHeadDim;
-                float M = -INFINITY, L = 0.0f, O = 0.0f;
-                for (int k = 0; k < pieces.count; ++k) {
-                    const int64_t row = pieces.head_row(k, G, g);
-                    const float mk = d.ws_ml[row * 2];
-                    if (mk == -INFINITY) continue;
-                    const float Mn = fmaxf(M, mk), a = exp2f(M - Mn), c = exp2f(mk - Mn);
-                    L = L * a + d.ws_ml[row * 2 + 1] * c;
-                    O = O * a + d.ws_o[row * kHeadDim + dd] * c;
-                    M = Mn;
-                }
-                ((T*)d.o)[qh * kHeadDim + i] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
-                if (dd == 0) lse[g] = M + log2f(L);
-            }
-        } else if (tid < G) {
-            float M = -INFINITY, L = 0.0f;
-            for (int k = 0; k < pieces.count; ++k) {
-                const int64_t row = pieces.head_row(k, G, tid);
-                const float mk = d.ws_ml[row * 2];
-                if (mk == -INFINITY) continue;
-                const float Mn = fmaxf(M, mk);
-                L = L * exp2f(M - Mn) + d.ws_ml[row * 2 + 1] * exp2f(mk - Mn);
-                M = Mn;
-            }
-            lse[tid] = M + log2f(L);
-        }
-    };
+    Pieces<STREAM> pieces;
     if constexpr (STREAM) {
         int64_t total, chunk;
         stream_extent(p, decode_ctas, total, chunk);
-        StreamPieces pieces;
-        pieces.c = start / chunk;
+        pieces.first = start / chunk;
         const int64_t last = (start + el.cnt - 1) / chunk;
-        pieces.count = last == pieces.c ? 0 : (int)(last - pieces.c + 1);
-        merge(pieces);
+        pieces.count = last == pieces.first ? 0 : (int)(last - pieces.first + 1);
     } else {
-        merge(SplitPieces{unit, d.num_splits});
+        pieces.first = unit;
+        pieces.count = d.num_splits;
     }
-    __syncthreads();
+    if (part == chunks) {
+        if (pieces.count == 0) return;
+        for (int i = tid; i < G * kHeadDim; i += kMassThreads) {
+            const int g = i / kHeadDim, dd = i % kHeadDim;
+            float M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll 4
+            for (int k = 0; k < pieces.count; ++k) {
+                const int64_t row = pieces.row(k, G, g);
+                const float2 ml = *reinterpret_cast<const float2*>(d.ws_ml + row * 2);
+                const float o = d.ws_o[row * kHeadDim + dd];
+                if (ml.x == -INFINITY) continue;          // nothing seen: its partial row is unspecified
+                const float Mn = fmaxf(M, ml.x), a = exp2f(M - Mn), c = exp2f(ml.x - Mn);
+                L = L * a + ml.y * c;
+                O = O * a + o * c;
+                M = Mn;
+            }
+            ((T*)d.o)[qh * kHeadDim + i] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
+        }
+        return;
+    }
 
     const int tokens = el.cnt == 1 ? el.last : el.first + (el.cnt - 2) * kPageSize + el.last;
     const int row = m.slot_index ? m.slot_index[b] : b;
+    if (part * kMassTokens >= tokens) return;
     if (row < 0 || row >= m.rows || tokens > m.stride || start + el.cnt > m.positions) {
         if (tid == 0 && part == 0) report(d.status, KTK_STATUS_BAD_TABLE);
         return;
     }
     const int64_t at = ((int64_t)row * d.Hkv + h) * m.stride;
-    const int t1 = (part + 1) * kMassTokens < tokens ? (part + 1) * kMassTokens : tokens;
-    for (int t = part * kMassTokens + tid; t < t1; t += kMassThreads) {
+    float s[kMassEach][G], before[kMassEach];
+#pragma unroll
+    for (int i = 0; i < kMassEach; ++i) {
+        const int t = part * kMassTokens + i * kMassThreads + tid;
+        if (t >= tokens) continue;
         // a short first page leaves places of its own block free
         const int place = t < el.first || el.cnt == 1 ? t : t + kPageSize - el.first;
-        const float* s = m.scores + (start * kPageSize + place) * G;
+        const float* from = m.scores + (start * kPageSize + place) * G;
+        if constexpr (G >= 4) {
+#pragma unroll
+            for (int g = 0; g < G; g += 4) *reinterpret_cast<float4*>(&s[i][g]) = *reinterpret_cast<const float4*>(from + g);
+        } else if constexpr (G == 2) {
+            *reinterpret_cast<float2*>(s[i]) = *reinterpret_cast<const float2*>(from);
+        } else {
+            s[i][0] = *from;
+        }
+        before[i] = t == tokens - 1 ? 0.0f : m.in[at + t];
+    }
+    if (tid < 32) {                                       // lanes of a head: pieces lane / G, lane / G + 32 / G, ...
+        const int g = lane % G;
+        float M = -INFINITY, L = 0.0f;
+        const auto join = [&](float m2, float l2) {
+            const float Mn = fmaxf(M, m2);
+            if (Mn == -INFINITY) return;
+            L = L * exp2f(M - Mn) + l2 * exp2f(m2 - Mn);
+            M = Mn;
+        };
+        for (int k = lane / G; k < pieces.count; k += 32 / G) {
+            const float2 ml = *reinterpret_cast<const float2*>(d.ws_ml + pieces.row(k, G, g) * 2);
+            join(ml.x, ml.y);
+        }
+#pragma unroll
+        for (int o = G; o < 32; o <<= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
+            join(m2, l2);
+        }
+        if (lane < G) lse[lane] = pieces.count == 0 ? d.lse[qh + lane] : M + log2f(L);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMassEach; ++i) {
+        const int t = part * kMassTokens + i * kMassThreads + tid;
+        if (t >= tokens) continue;
         float sum = 0.0f;
-        for (int g = 0; g < G; ++g) sum += exp2f(s[g] - lse[g]);
-        m.out[at + t] = t == tokens - 1 ? sum : fmaf(m.decay, m.in[at + t], sum);
+#pragma unroll
+        for (int g = 0; g < G; ++g) sum += exp2f(s[i][g] - lse[g]);
+        m.out[at + t] = t == tokens - 1 ? sum : fmaf(m.decay, before[i], sum);
     }
 }
 
 template <typename T, bool STREAM>
 static int launch_finish(const StreamParams& p, int decode_ctas, cudaStream_t st) {
     const int64_t chunks = ((int64_t)p.m.max_pages * kPageSize + kMassTokens - 1) / kMassTokens;
-    const int64_t ctas = chunks * p.d.batch * p.d.Hkv;
+    const int64_t ctas = (chunks + 1) * p.d.batch * p.d.Hkv;
     if (ctas > 2147483647LL) {
         set_error("ktk_dense_decode_mass: batch * num_kv_heads * max_pages_per_seq exceeds the grid limit");
         return KTK_ERR_TOO_LARGE;
     }
-    KTK_CUDA_TRY(launch_behind(true, mass_finish_kernel<T, STREAM>, (unsigned)ctas, kMassThreads, 0, st, p, (int)chunks, decode_ctas),
+    const auto go = [&](auto kernel) {
+        return launch_behind(true, kernel, (unsigned)ctas, kMassThreads, 0, st, p, (int)chunks, decode_ctas);
+    };
+    KTK_CUDA_TRY(p.G == 1 ? go(mass_finish_kernel<T, STREAM, 1>) : p.G == 2 ? go(mass_finish_kernel<T, STREAM, 2>)
+                 : p.G == 4 ? go(mass_finish_kernel<T, STREAM, 4>) : go(mass_finish_kernel<T, STREAM, 8>),
                  "ktk_dense_decode_mass (finish)");
     return KTK_OK;
 }

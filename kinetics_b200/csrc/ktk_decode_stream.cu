@@ -347,16 +347,18 @@ static int stream_slots(int vi) {
     return slots[dev][vi];
 }
 
-static int stream_grid_of(int vi, int64_t units, int max_entries) {
+static int stream_grid_of(int vi, int64_t units, int max_entries, int min_chunk) {
     const int64_t total = units * (int64_t)max_entries;
-    int64_t grid = (total + kStreamMinChunk - 1) / kStreamMinChunk;
+    int64_t grid = (total + min_chunk - 1) / min_chunk;
     const int64_t slots = stream_slots(vi);
     if (grid > slots) grid = slots;
     if (grid < 1) grid = 1;
     return (int)grid;
 }
 
-int stream_grid(int64_t units, int max_entries) { return stream_grid_of(stream_variant_index(false), units, max_entries); }
+int stream_grid(int64_t units, int max_entries) {
+    return stream_grid_of(stream_variant_index(false), units, max_entries, kStreamMinChunk);
+}
 
 size_t stream_workspace_bytes(int G) {
     // two slots per CTA of the largest grid, each G rows of (m, l) + 128 floats
@@ -381,7 +383,8 @@ static int launch_stream(const DecodeParams& p, const MassParams& m, int G, int 
     const int vi = stream_variant_index(p.topk < 0);
     const StreamVariant& var = kStreamVariants[vi];
     const auto kernel = MASS ? var.mass_kernel : var.kernel;
-    int grid = stream_grid_of(vi, units, max_entries);
+    sp.min_chunk = MASS ? kStreamMinChunkMass : kStreamMinChunk;
+    int grid = stream_grid_of(vi, units, max_entries, sp.min_chunk);
     const int64_t chunk = (sp.total + grid - 1) / grid;
     if (chunk > 2147483647LL) {
         set_error("ktk decode: %lld page positions per CTA exceed the balanced partition's limit", (long long)chunk);

@@ -6,12 +6,15 @@
 
 namespace ktk {
 
-constexpr int kStreamMinChunk = 16;                       // pages: below this a CTA is not worth its start-up
+// Pages: below this a CTA is not worth its start-up.  Behind the form that accumulates weights pieces are joined by more CTAs, and one
+// page per consumer warp is (one sequence of 517 tokens, 8 kv heads: MEASURE).
+constexpr int kStreamMinChunk = 16, kStreamMinChunkMass = kMmaConsumers;
 
 struct StreamParams {
     DecodeParams d;
     MassParams m;    // read by the kernels that accumulate weights
     int G;
+    int min_chunk;   // kStreamMinChunk, or that of the form that accumulates weights
     int wmax;        // padded mode: positions per unit
     int chunk;       // padded mode: positions per CTA
     int64_t total;   // padded mode: units * wmax
@@ -32,7 +35,7 @@ __device__ __forceinline__ void stream_extent(const StreamParams& p, int64_t cta
     if (p.exact) {
         total = (int64_t)(p.d.kv_indptr[p.d.batch] - p.d.kv_indptr[0]) * p.d.Hkv;
         chunk = (total + ctas - 1) / ctas;
-        if (chunk < kStreamMinChunk) chunk = kStreamMinChunk;
+        if (chunk < p.min_chunk) chunk = p.min_chunk;
     }
 }
 __device__ __forceinline__ void stream_extent(const StreamParams& p, int64_t& total, int64_t& chunk) {

@@ -1,11 +1,14 @@
 // Eviction from a paged cache by accumulated attention weight: of every (sequence, kv head) with more than `keep` tokens the ones
 // of largest mass stay, with the first and the newest.  The kept tokens behind place `keep` move into the holes in front of it.
 //
-// One CTA per (sequence, kv head) plans: every token has a 32-bit key whose order is that of the masses (the first and newest:
-// the largest key, NaN: the smallest).  The keep-th largest key is found two bits at a time, by counting the keys that reach each of
-// three thresholds, until a threshold is reached by exactly `keep` keys; tokens at exactly the last threshold stay from the lowest
-// place on.  Which tokens stay is held as one bit each, and prefix sums over the bits' words number the holes and the tokens that move.
-// Keys and values are copied a warp to a token, by the planning CTA or by a launch of their own (evict_move_kernel).
+// A CTA per (sequence, kv head), or a cluster of them, plans: every token has a 32-bit key whose order is that of the masses (the
+// first and newest: the largest key, NaN: the smallest).  The keep-th largest key is found by its digits, the first of 11 bits, from
+// counts of the keys with each digit; tokens at exactly that key stay from the lowest place on.  Which tokens stay is held as one bit
+// each, and prefix sums over the bits' words number the holes and the tokens that move.
+// Keys and values are copied a warp to a token: by the planning CTA where few can move, else by a launch of their own, whose many
+// warps hide the chain of loads (list, page table, cache) that each copy is.
+#include <cooperative_groups.h>
+
 #include "ktk_decode.cuh"
 
 namespace ktk {
@@ -30,7 +33,7 @@ struct EvictParams {
     const int32_t* stored;
     const int32_t* seen;
     int keep, sink, recent;
-    int32_t* count;                   // [units] tokens that move
+    int32_t* count;                   // of evict_long_kernel: [units] tokens that move
     int32_t* from;                    // [units][max_moves] their places
     int32_t* to;                      // [units][max_moves] the holes
     int max_moves;
@@ -44,47 +47,29 @@ __device__ __forceinline__ uint32_t evict_key(float mass) {
     return mass != mass ? 0u : score_to_key(mass);        // NaN less than -inf (whose key is above 0)
 }
 
-// Sums over the block of three counts, up to 2^21 each, packed in 64 bits; every thread gets them.  Two buffers in turn: one barrier each.
-template <int THREADS>
-__device__ __forceinline__ uint64_t block_sum(uint32_t n1, uint32_t n2, uint32_t n3, uint64_t (*buf)[32], int& turn) {
+// Exclusive prefix sum over the block's threads, and the total.  Two buffers in turn: one barrier each.
+template <int THREADS, typename T>
+__device__ __forceinline__ T block_prefix(T x, uint64_t (*buf)[32], int& turn, T& total) {
     constexpr int W = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    n1 = __reduce_add_sync(0xffffffffu, n1);
-    n2 = __reduce_add_sync(0xffffffffu, n2);
-    n3 = __reduce_add_sync(0xffffffffu, n3);
-    if (lane == 0) buf[turn][warp] = (uint64_t)n1 | (uint64_t)n2 << 21 | (uint64_t)n3 << 42;
-    __syncthreads();
-    const uint64_t x = lane < W ? buf[turn][lane] : 0;
-    n1 = __reduce_add_sync(0xffffffffu, (uint32_t)(x & 0x1fffff));
-    n2 = __reduce_add_sync(0xffffffffu, (uint32_t)(x >> 21 & 0x1fffff));
-    n3 = __reduce_add_sync(0xffffffffu, (uint32_t)(x >> 42));
-    turn ^= 1;
-    return (uint64_t)n1 | (uint64_t)n2 << 21 | (uint64_t)n3 << 42;
-}
-
-// Exclusive prefix sum over the block's threads, and the total
-template <int THREADS>
-__device__ __forceinline__ uint64_t block_prefix(uint64_t x, uint64_t (*buf)[32], int& turn, uint64_t& total) {
-    constexpr int W = THREADS / 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint64_t incl = x;
+    T incl = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        const T y = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += y;
     }
     if (lane == 31) buf[turn][warp] = incl;
     __syncthreads();
-    uint64_t w = lane < W ? buf[turn][lane] : 0, wi = w;
+    const T w = lane < W ? (T)buf[turn][lane] : 0;
+    T wi = w;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, wi, o);
+    for (int o = 1; o < W; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, wi, o);
         if (lane >= o) wi += y;
     }
-    total = __shfl_sync(0xffffffffu, wi, 31);
-    const uint64_t before = __shfl_sync(0xffffffffu, wi - w, warp);
+    total = __shfl_sync(0xffffffffu, wi, W - 1);
     turn ^= 1;
-    return before + incl - x;
+    return __shfl_sync(0xffffffffu, wi - w, warp) + incl - x;
 }
 
 // A (sequence, kv head) and its tokens; false: nothing is evicted from it
@@ -93,7 +78,11 @@ struct EvictUnit {
     int64_t at;                                      // of its row in masses and positions
     const float* mass;
     const int32_t* pos;
-    __device__ __forceinline__ int position(int t) const { return t < stored ? pos[t] : seen - n + t; }
+    // both loads are always made, so that those of several tokens can be in flight together
+    __device__ __forceinline__ int position(int t) const {
+        const int at = pos[t < stored ? t : 0];
+        return t < stored ? at : seen - n + t;
+    }
 };
 __device__ __forceinline__ bool evict_unit(const EvictParams& p, int64_t unit, int most, EvictUnit& u) {
     const int b = (int)(unit / p.Hkv), h = (int)(unit % p.Hkv);
@@ -114,32 +103,18 @@ __device__ __forceinline__ bool evict_unit(const EvictParams& p, int64_t unit, i
     u.seen = p.seen[row];
     return true;
 }
-__device__ __forceinline__ uint32_t key_at(const EvictParams& p, const EvictUnit& u, int t) {
-    const int at = u.position(t);
-    const float mass = u.mass[t];
-    return at < p.sink || at >= u.seen - p.recent ? 0xffffffffu : evict_key(mass);
-}
-// What stays in its place: to be read (before anything is written), to be written
-struct EvictCopy {
+// What a token in front of place `keep` has if it stays; holes are written over later.  The key of a token.
+struct EvictToken {
     float mass;
     int pos;
 };
-__device__ __forceinline__ EvictCopy copy_read(const EvictParams& p, const EvictUnit& u, int t) {
-    return {p.mass_in == p.mass_out ? 0.0f : u.mass[t], p.pos_in == p.pos_out && t < u.stored ? 0 : u.position(t)};
+__device__ __forceinline__ EvictToken read_token(const EvictUnit& u, int t) { return {u.mass[t], u.position(t)}; }
+__device__ __forceinline__ void keep_token(const EvictParams& p, const EvictUnit& u, int t, const EvictToken& x) {
+    if (p.mass_in != p.mass_out) p.mass_out[u.at + t] = x.mass;
+    if (p.pos_in != p.pos_out || t >= u.stored) p.pos_out[u.at + t] = x.pos;
 }
-__device__ __forceinline__ void copy_write(const EvictParams& p, const EvictUnit& u, int t, const EvictCopy& c) {
-    if (p.mass_in != p.mass_out) p.mass_out[u.at + t] = c.mass;
-    if (p.pos_in != p.pos_out || t >= u.stored) p.pos_out[u.at + t] = c.pos;
-}
-
-// ITEMS keys per thread, t = j * THREADS + thread: visit(j, t) for those that there are
-template <int THREADS, int ITEMS, class Visit>
-__device__ __forceinline__ void each_item(int n, Visit visit) {
-#pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-        if (j * THREADS >= n) break;                 // uniform
-        visit(j, j * THREADS + (int)threadIdx.x);
-    }
+__device__ __forceinline__ uint32_t key_of(const EvictParams& p, const EvictUnit& u, const EvictToken& x) {
+    return x.pos < p.sink || x.pos >= u.seen - p.recent ? 0xffffffffu : evict_key(x.mass);
 }
 
 // The words of places in front of `keep`
@@ -147,47 +122,177 @@ __device__ __forceinline__ uint32_t in_front(int w, int keep) {
     return w * 32 + 32 <= keep ? 0xffffffffu : w * 32 >= keep ? 0u : (1u << (keep - w * 32)) - 1u;
 }
 
-// above, level: one bit per token, its key is above the threshold, at it.  Numbers the holes and the tokens that move, in the order of
-// their places: hole(i, t), mover(i, t).  `above` becomes: the token stays.  Returns how many move.
-template <int THREADS, class Hole, class Mover>
-__device__ __forceinline__ int number_moves(uint32_t* above, const uint32_t* level, int words, int keep, int need, uint64_t (*buf)[32],
-                                            int& turn, Hole hole, Mover mover) {
+// The CTAs of a cluster, and an array that each of them has
+struct Cluster {
+    int size, rank;
+    __device__ __forceinline__ void sync() const {
+        if (size > 1) cooperative_groups::this_cluster().sync();
+        else __syncthreads();
+    }
+    template <typename T> __device__ __forceinline__ const T* of(const T* mine, int r) const {
+        return size > 1 ? cooperative_groups::this_cluster().map_shared_rank(mine, r) : mine;
+    }
+};
+
+// The keep-th largest key and how many keys are above it, digit by digit.  walk(visit): calls visit(key, there) for the CTA's keys, whole
+// warps together.  hist: zeros, kEvBins for each digit, the first twice; one, then the other half of a warp counts there, since many keys
+// share a first digit.  found: three words.  All CTAs of the cluster find the same.
+constexpr int kEvBins = 2048, kEvHists = 4;
+struct Threshold {
+    uint32_t key;
+    int above;
+};
+template <int THREADS, class Walk>
+__device__ __forceinline__ Threshold find_threshold(int keep, const Cluster& cl, uint32_t (*hist)[kEvBins], uint32_t* found,
+                                                    uint64_t (*buf)[32], int& turn, Walk walk) {
+    constexpr int kEach = kEvBins / THREADS;
+    const int tid = threadIdx.x, lane = tid & 31;
+    Threshold r{0, 0};
+    uint32_t known = 0;                              // mask of the digits found
+    for (int digit = 0; ; ++digit) {
+        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+        const uint32_t digits = digit == 2 ? 1023u : 2047u;
+        uint32_t* mine = hist[digit == 0 ? 0 : digit + 1];
+        if (digit == 0) {
+            uint32_t* copy = hist[lane >> 4];
+            walk([&](uint32_t key, bool on) {
+                if (on) atomicAdd(&copy[key >> 21], 1u);
+            });
+        } else {
+            walk([&](uint32_t key, bool on) {
+                on = on && (key & known) == r.key;
+                const unsigned active = __ballot_sync(0xffffffffu, on);
+                if (active == 0) return;
+                // a warp whose keys share a digit (the same mass) adds once
+                const uint32_t bin = key >> shift & digits, one = __shfl_sync(0xffffffffu, bin, __ffs((int)active) - 1);
+                if (__all_sync(0xffffffffu, !on || bin == one)) {
+                    if (lane == 0) atomicAdd(&mine[one], (uint32_t)__popc(active));
+                } else if (on) {
+                    atomicAdd(&mine[bin], 1u);
+                }
+            });
+        }
+        if (cl.size > 1) {
+            if (digit == 0) {
+                __syncthreads();
+                for (int i = tid; i < kEvBins; i += THREADS) hist[0][i] += hist[1][i];
+            }
+            cl.sync();
+            uint32_t sums[kEach];
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                sums[k] = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < cl.size) sums[k] += cl.of(mine, i)[k * THREADS + tid];
+            }
+            cl.sync();                               // all have read
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) mine[k * THREADS + tid] = sums[k];
+        }
+        __syncthreads();
+        // from the largest digit on, kEach to a thread
+        const int bin0 = kEvBins - (tid + 1) * kEach;
+        uint32_t c[kEach], sum = 0, total;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            c[k] = mine[bin0 + k];
+            if (digit == 0 && cl.size == 1) c[k] += hist[1][bin0 + k];
+            sum += c[k];
+        }
+        const uint32_t need = (uint32_t)(keep - r.above);
+        uint32_t before = block_prefix<THREADS>(sum, buf, turn, total);
+        if (before < need && need <= before + sum) {             // one thread
+#pragma unroll
+            for (int k = kEach - 1; k >= 0; --k) {
+                if (before < need && need <= before + c[k]) {
+                    found[0] = (uint32_t)(bin0 + k);
+                    found[1] = before;
+                    found[2] = c[k];
+                }
+                before += c[k];
+            }
+        }
+        __syncthreads();
+        r.key |= found[0] << shift;
+        r.above += (int)found[1];
+        known |= digits << shift;
+        const uint32_t here = found[2];
+        if (digit == 2) return r;
+        if (here == (uint32_t)(keep - r.above) && r.key != 0) return {r.key - 1, keep};          // all keys with these digits stay
+        __syncthreads();                             // found may be written again
+    }
+}
+
+// The CTA's words of stay, level: one bit per token, its key is above the threshold, at it; `need` of the latter, over the cluster,
+// stay.  Afterwards `stay` says which tokens stay and `level` holds, for words in front of place `keep`, the holes in words before, for
+// those behind the tokens that move.  first: number of the CTA's first word; shared: two words that the cluster's CTAs read of each
+// other.  Returns how many tokens of the cluster move.
+template <int THREADS>
+__device__ __forceinline__ int number_moves(uint32_t* stay, uint32_t* level, int first, int words, int keep, int need, const Cluster& cl,
+                                            uint64_t* shared, uint64_t (*buf)[32], int& turn) {
     const int tid = threadIdx.x;
     // words of a thread: consecutive ones, so that prefix sums over threads go by place
     const int each = (words + THREADS - 1) / THREADS;
     const int w0 = tid * each < words ? tid * each : words, w1 = w0 + each < words ? w0 + each : words;
-    uint64_t total;
-    int left = 0;                                    // how many at the threshold the thread's words may still keep
-    if (need > 0) {
-        uint32_t ties = 0;
-        for (int w = w0; w < w1; ++w) ties += __popc(level[w]);
-        left = need - (int)block_prefix<THREADS>(ties, buf, turn, total);
-    }
-    uint32_t holes = 0, movers = 0;
-    for (int w = w0; w < w1; ++w) {
-        uint32_t stay = above[w];
-        if (need > 0) {
-            for (uint32_t l = level[w]; l != 0 && left > 0; l &= l - 1, --left) stay |= l & (0u - l);      // the lowest places first
-            above[w] = stay;
+    // sums over the CTAs in front, and over all
+    const auto over_cluster = [&](uint64_t* mine, uint64_t total, uint64_t& all) -> uint64_t {
+        if (cl.size == 1) {
+            all = total;
+            return 0;
         }
-        holes += __popc(~stay & in_front(w, keep));
-        movers += __popc(stay & ~in_front(w, keep));
+        if (tid == 0) *mine = total;
+        cl.sync();
+        uint64_t before = 0;
+        all = 0;
+        for (int i = 0; i < cl.size; ++i) {
+            const uint64_t x = *cl.of(mine, i);
+            if (i < cl.rank) before += x;
+            all += x;
+        }
+        return before;
+    };
+    uint64_t all, total;
+    if (need > 0) {
+        uint64_t ties = 0;
+        for (int w = w0; w < w1; ++w) ties += __popc(level[w]);
+        const uint64_t before = block_prefix<THREADS>(ties, buf, turn, total);
+        int left = need - (int)(before + over_cluster(&shared[0], total, all));
+        for (int w = w0; w < w1; ++w) {
+            uint32_t l = level[w], more = 0;
+            if (left >= __popc(l)) {
+                more = l;
+                left -= __popc(l);
+            } else {
+                for (; left > 0; l &= l - 1, --left) more |= l & (0u - l);       // the lowest places first
+            }
+            stay[w] |= more;
+        }
     }
-    const uint64_t first = block_prefix<THREADS>((uint64_t)holes | (uint64_t)movers << 32, buf, turn, total);
-    int i = (int)(uint32_t)first, k = (int)(first >> 32);
+    uint64_t count = 0;                              // holes | tokens that move
+    const auto add = [&](int w) {
+        count += (uint64_t)__popc(~stay[w] & in_front(first + w, keep)) | (uint64_t)__popc(stay[w] & ~in_front(first + w, keep)) << 32;
+    };
+    for (int w = w0; w < w1; ++w) add(w);
+    count = block_prefix<THREADS>(count, buf, turn, total);
+    count += over_cluster(&shared[1], total, all);
     for (int w = w0; w < w1; ++w) {
-        for (uint32_t x = ~above[w] & in_front(w, keep); x != 0; x &= x - 1) hole(i++, w * 32 + __ffs((int)x) - 1);
-        for (uint32_t x = above[w] & ~in_front(w, keep); x != 0; x &= x - 1) mover(k++, w * 32 + __ffs((int)x) - 1);
+        level[w] = (first + w) * 32 < keep ? (uint32_t)count : (uint32_t)(count >> 32);
+        add(w);
     }
-    return (int)(uint32_t)total;
+    return (int)(uint32_t)all;
 }
-
-// Two bits of the threshold from the counts of keys that reach it plus 1, 2, 3 steps; whether exactly `keep` keys reach it now
-__device__ __forceinline__ bool next_bits(uint64_t counts, int keep, int shift, uint32_t& threshold) {
-    const auto count = [&](int i) { return (int)(counts >> (21 * i) & 0x1fffff); };
-    const int step = count(2) >= keep ? 3 : count(1) >= keep ? 2 : count(0) >= keep ? 1 : 0;
-    threshold += (uint32_t)step << shift;
-    return step > 0 && count(step - 1) == keep;
+// What becomes of the token in place t: hole(i) the i-th hole is there, mover(i) it is the i-th token that moves
+template <class Hole, class Mover>
+__device__ __forceinline__ void token_move(const uint32_t* stay, const uint32_t* level, int first, int t, int keep, Hole hole, Mover mover) {
+    const int w = t >> 5;
+    const uint32_t s = stay[w - first], bit = 1u << (t & 31), below = bit - 1;
+    if (t < keep) {
+        if (!(s & bit)) hole((int)level[w - first] + __popc(~s & below));
+    } else if (s & bit) {
+        const uint32_t front = in_front(w, keep);
+        mover((front ? 0 : (int)level[w - first]) + __popc(s & below & ~front));         // only words in front lie before one that is cut
+    }
 }
 
 // Tokens of a warp's copies, their loads in flight together
@@ -230,83 +335,81 @@ __device__ __forceinline__ void copy_tokens(const EvictParams& p, int h, int sta
             if (dst[i][j] >= 0) cache[dst[i][j]] = v[i][j];
 }
 
-// Sequences of at most THREADS * ITEMS tokens: keys in registers.  CHUNKS 0: keys and values are left to evict_move_kernel.
+// Sequences of at most THREADS * ITEMS tokens per CTA of the cluster, keys in registers.  CHUNKS: 16-byte pieces of a token's key; 0:
+// keys and values are left to evict_move_kernel.
 template <int THREADS, int ITEMS, int CHUNKS>
 __global__ void __launch_bounds__(THREADS)
-evict_kernel(const EvictParams p) {
-    constexpr int kMost = THREADS * ITEMS, kWords = kMost / 32;
-    __shared__ uint64_t buf[2][32];
-    __shared__ uint32_t above[kWords], level[kWords];
-    extern __shared__ uint16_t ev_lists[];           // [max_moves] from, [max_moves] to
-    uint16_t *from = ev_lists, *to = from + p.max_moves;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+evict_kernel(const EvictParams p, int cluster) {
+    constexpr int kMost = THREADS * ITEMS, kWords = kMost / 32, kBatch = 8;
+    __shared__ uint64_t buf[2][32], shared[2];
+    __shared__ uint32_t hist[kEvHists][kEvBins], found[3], stay[kWords], level[kWords];
+    const int tid = threadIdx.x;
+    for (int i = tid; i < kEvHists * kEvBins; i += THREADS) hist[0][i] = 0;
     wait_for_front();
-    const int64_t unit = blockIdx.x;
+    const Cluster cl{cluster, (int)(blockIdx.x % cluster)};
+    const int64_t unit = blockIdx.x / cluster;
     EvictUnit u;
-    if (!evict_unit(p, unit, kMost, u)) {
-        if (CHUNKS == 0 && tid == 0) p.count[unit] = 0;
-        return;
-    }
-    const int n = u.n, keep = p.keep;
+    const bool there = evict_unit(p, unit, kMost * cluster, u);                  // the same for the cluster
+    if (CHUNKS == 0 && (!there || u.n <= p.keep) && tid == 0) p.count[unit] = 0;
+    if (!there) return;
+    const int keep = p.keep, front = u.n < keep ? u.n : keep;
+    // the CTA's tokens: whole words
+    const int words = ((u.n + 31) / 32 + cluster - 1) / cluster, first = cl.rank * words, t0 = first * 32;
+    const int n = min(u.n - t0, words * 32);         // may be negative
     uint32_t key[ITEMS];
-    if (n > keep) {
-        each_item<THREADS, ITEMS>(n, [&](int j, int t) { key[j] = t < n ? key_at(p, u, t) : 0; });
-    }
-    // what stays is read early as well: the copies are written behind the search
-    EvictCopy stay[ITEMS];
-    const int front = n < keep ? n : keep;
-    each_item<THREADS, ITEMS>(front, [&](int j, int t) { if (t < front) stay[j] = copy_read(p, u, t); });
-    if (n <= keep) {
-        each_item<THREADS, ITEMS>(n, [&](int j, int t) { if (t < n) copy_write(p, u, t, stay[j]); });
-        if (CHUNKS == 0 && tid == 0) p.count[unit] = 0;
-        return;
-    }
-    int turn = 0;
-    uint32_t threshold = 0;                          // the largest, of the bits so far, that at least `keep` keys reach
-    bool exact = false;
-    for (int shift = 30; shift >= 0 && !exact; shift -= 2) {
-        const uint32_t c1 = threshold + (1u << shift), c2 = threshold + (2u << shift), c3 = threshold + (3u << shift);
-        uint32_t n1 = 0, n2 = 0, n3 = 0;
-        each_item<THREADS, ITEMS>(n, [&](int j, int) {       // a key of 0 reaches none
-            n1 += key[j] >= c1;
-            n2 += key[j] >= c2;
-            n3 += key[j] >= c3;
-        });
-        exact = next_bits(block_sum<THREADS>(n1, n2, n3, buf, turn), keep, shift, threshold);
-    }
-    uint32_t over = 0;
-    each_item<THREADS, ITEMS>(n, [&](int j, int t) {
-        const uint32_t a = __ballot_sync(0xffffffffu, t < n && (key[j] > threshold || (exact && key[j] == threshold)));
-        const uint32_t l = __ballot_sync(0xffffffffu, t < n && !exact && key[j] == threshold);
-        if (lane == 0) {
-            above[t / 32] = a;
-            level[t / 32] = l;
-            over += __popc(a);
+#pragma unroll
+    for (int j0 = 0; j0 < ITEMS; j0 += kBatch) {     // reads of a batch, then its writes
+        if (j0 * THREADS >= n) break;
+        EvictToken x[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) x[j] = read_token(u, min(t0 + (j0 + j) * THREADS + tid, u.n - 1));
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int i = (j0 + j) * THREADS + tid;
+            key[j0 + j] = key_of(p, u, x[j]);
+            if (i < n && t0 + i < front) keep_token(p, u, t0 + i, x[j]);
         }
-    });
-    const int need = keep - (int)(block_sum<THREADS>(over, 0, 0, buf, turn) & 0x1fffff);
-    const int moves = number_moves<THREADS>(above, level, (n + 31) / 32, keep, need, buf, turn,
-                                            [&](int i, int t) { to[i] = (uint16_t)t; }, [&](int i, int t) { from[i] = (uint16_t)t; });
+    }
+    if (u.n <= keep) return;
     __syncthreads();
-    if constexpr (CHUNKS > 0) {
-        for (int i = warp * kEvEach; i < moves; i += THREADS / 32 * kEvEach)
-            copy_tokens<CHUNKS>(p, (int)(unit % p.Hkv), u.start, u.first_fill, i, moves, [&](int k) { return (int)from[k]; },
-                                [&](int k) { return (int)to[k]; });
-    } else {
-        if (tid == 0) p.count[unit] = moves;
-        for (int i = tid; i < moves; i += THREADS) {
-            p.from[unit * p.max_moves + i] = from[i];
-            p.to[unit * p.max_moves + i] = to[i];
+    const auto each_item = [&](auto visit) {         // of the CTA's tokens, whole warps
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            if (j * THREADS >= n) break;             // uniform
+            visit(j, j * THREADS + tid);
         }
-    }
-    each_item<THREADS, ITEMS>(front, [&](int j, int t) {
-        if (t < front && (above[t >> 5] >> (t & 31) & 1u)) copy_write(p, u, t, stay[j]);
+    };
+    int turn = 0;
+    const Threshold at = find_threshold<THREADS>(keep, cl, hist, found, buf, turn, [&](auto visit) {
+        each_item([&](int j, int i) { visit(key[j], i < n); });
     });
-    for (int i = tid; i < moves; i += THREADS) {
-        const float mass = u.mass[from[i]];
-        const int at = u.position(from[i]);
-        p.mass_out[u.at + to[i]] = mass;
-        p.pos_out[u.at + to[i]] = at;
+    each_item([&](int j, int i) {
+        const uint32_t a = __ballot_sync(0xffffffffu, i < n && key[j] > at.key), l = __ballot_sync(0xffffffffu, i < n && key[j] == at.key);
+        if ((tid & 31) == 0) {
+            stay[i / 32] = a;
+            level[i / 32] = l;
+        }
+    });
+    __syncthreads();
+    const int moves = number_moves<THREADS>(stay, level, first, n > 0 ? (n + 31) / 32 : 0, keep, keep - at.above, cl, shared, buf, turn);
+    __syncthreads();
+    int32_t *from = p.from + unit * p.max_moves, *to = p.to + unit * p.max_moves;
+    each_item([&](int, int i) {
+        if (i < n) token_move(stay, level, first, t0 + i, keep, [&](int k) { to[k] = t0 + i; }, [&](int k) { from[k] = t0 + i; });
+    });
+    cl.sync();
+    if constexpr (CHUNKS > 0) {                      // one CTA
+        constexpr int W = THREADS / 32;
+        for (int i = (tid >> 5) * kEvEach; i < moves; i += W * kEvEach)
+            copy_tokens<CHUNKS>(p, (int)(unit % p.Hkv), u.start, u.first_fill, i, moves, [&](int k) { return from[k]; },
+                                [&](int k) { return to[k]; });
+    } else {
+        if (cl.rank == 0 && tid == 0) p.count[unit] = moves;
+    }
+    for (int i = cl.rank * THREADS + tid; i < moves; i += cluster * THREADS) {
+        const EvictToken x = read_token(u, from[i]);
+        p.mass_out[u.at + to[i]] = x.mass;
+        p.pos_out[u.at + to[i]] = x.pos;
     }
 }
 
@@ -316,7 +419,10 @@ __global__ void __launch_bounds__(kEvLong)
 evict_long_kernel(const EvictParams p) {
     extern __shared__ __align__(16) uint32_t ev_smem[];
     __shared__ uint64_t buf[2][32];
+    __shared__ uint32_t hist[kEvHists][kEvBins], found[3];
     const int tid = threadIdx.x, lane = tid & 31;
+    const Cluster alone{1, 0};
+    for (int i = tid; i < kEvHists * kEvBins; i += kEvLong) hist[0][i] = 0;
     wait_for_front();
     const int64_t unit = blockIdx.x;
     EvictUnit u;
@@ -324,61 +430,51 @@ evict_long_kernel(const EvictParams p) {
         if (tid == 0) p.count[unit] = 0;
         return;
     }
-    const int n = u.n, keep = p.keep;
+    const int n = u.n, keep = p.keep, words = (n + 31) / 32;
+    uint32_t *stay = ev_smem, *level = stay + words, *keys = level + words;
+    const bool held = n <= p.smem_keys;
+    for (int t = tid; t < n; t += kEvLong) {
+        const EvictToken x = read_token(u, t);
+        if (held && n > keep) keys[t] = key_of(p, u, x);
+        if (t < keep) keep_token(p, u, t, x);
+    }
     if (n <= keep) {
-        for (int t = tid; t < n; t += kEvLong) copy_write(p, u, t, copy_read(p, u, t));
         if (tid == 0) p.count[unit] = 0;
         return;
     }
-    const int words = (n + 31) / 32;
-    uint32_t *above = ev_smem, *level = above + words, *keys = level + words;
-    const bool held = n <= p.smem_keys;
-    if (held) {
-        for (int t = tid; t < n; t += kEvLong) keys[t] = key_at(p, u, t);
-        __syncthreads();
-    }
-    const auto key_of = [&](int t) { return held ? keys[t] : key_at(p, u, t); };
+    __syncthreads();
+    // a key made again may not see what was written: positions behind `stored` are not read, and masses in place are not written
+    const auto each = [&](auto visit) {
+        for (int t0 = tid - lane; t0 < n; t0 += kEvLong) {
+            const int t = t0 + lane;
+            visit(t, t >= n ? 0 : held ? keys[t] : key_of(p, u, read_token(u, t)));
+        }
+    };
     int turn = 0;
-    uint32_t threshold = 0;
-    bool exact = false;
-    for (int shift = 30; shift >= 0 && !exact; shift -= 2) {
-        const uint32_t c1 = threshold + (1u << shift), c2 = threshold + (2u << shift), c3 = threshold + (3u << shift);
-        uint32_t n1 = 0, n2 = 0, n3 = 0;
-        for (int t = tid; t < n; t += kEvLong) {
-            const uint32_t k = key_of(t);
-            n1 += k >= c1;
-            n2 += k >= c2;
-            n3 += k >= c3;
-        }
-        exact = next_bits(block_sum<kEvLong>(n1, n2, n3, buf, turn), keep, shift, threshold);
-    }
-    uint32_t over = 0;
-    for (int t0 = tid - lane; t0 < words * 32; t0 += kEvLong) {
-        const int t = t0 + lane;
-        const uint32_t k = t < n ? key_of(t) : 0;
-        const uint32_t a = __ballot_sync(0xffffffffu, t < n && (k > threshold || (exact && k == threshold)));
-        const uint32_t l = __ballot_sync(0xffffffffu, t < n && !exact && k == threshold);
+    const Threshold at = find_threshold<kEvLong>(keep, alone, hist, found, buf, turn, [&](auto visit) {
+        each([&](int t, uint32_t key) { visit(key, t < n); });
+    });
+    each([&](int t, uint32_t key) {
+        const uint32_t a = __ballot_sync(0xffffffffu, t < n && key > at.key), l = __ballot_sync(0xffffffffu, t < n && key == at.key);
         if (lane == 0) {
-            above[t0 / 32] = a;
-            level[t0 / 32] = l;
-            over += __popc(a);
+            stay[t / 32] = a;
+            level[t / 32] = l;
         }
-    }
-    const int need = keep - (int)(block_sum<kEvLong>(over, 0, 0, buf, turn) & 0x1fffff);
+    });
+    __syncthreads();
+    const int moves = number_moves<kEvLong>(stay, level, 0, words, keep, keep - at.above, alone, nullptr, buf, turn);
+    __syncthreads();
     int32_t *from = p.from + unit * p.max_moves, *to = p.to + unit * p.max_moves;
-    const int moves = number_moves<kEvLong>(above, level, words, keep, need, buf, turn, [&](int i, int t) { to[i] = t; },
-                                            [&](int i, int t) { from[i] = t; });
+    for (int t = tid; t < n; t += kEvLong)
+        token_move(stay, level, 0, t, keep, [&](int i) { to[i] = t; }, [&](int i) { from[i] = t; });
     __syncthreads();
     if (tid == 0) p.count[unit] = moves;
-    for (int t = tid; t < keep; t += kEvLong)
-        if (above[t >> 5] >> (t & 31) & 1u) copy_write(p, u, t, copy_read(p, u, t));
     for (int i = tid; i < moves; i += kEvLong) {
-        const int s = from[i], d = to[i];
-        p.mass_out[u.at + d] = u.mass[s];
-        p.pos_out[u.at + d] = u.position(s);
+        const EvictToken x = read_token(u, from[i]);
+        p.mass_out[u.at + to[i]] = x.mass;
+        p.pos_out[u.at + to[i]] = x.pos;
     }
 }
-
 constexpr int kEvWarps = 8;
 template <int CHUNKS>
 __global__ void __launch_bounds__(kEvWarps * 32)
@@ -394,15 +490,34 @@ evict_move_kernel(const EvictParams p, int parts) {
 }
 
 template <int THREADS, int ITEMS>
-static cudaError_t launch_evict(const EvictParams& p, int64_t units, bool fused, bool f32, cudaStream_t st) {
+static cudaError_t launch_evict(const EvictParams& p, int64_t units, int cluster, bool fused, bool f32, cudaStream_t st) {
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = (unsigned)(units * cluster);
+    cfg.blockDim = THREADS;
+    cfg.stream = st;
+    cfg.attrs = units * cluster <= sm_count() ? attr : attr + 1;                 // early, as launch_behind
+    cfg.numAttrs = (units * cluster <= sm_count() ? 1 : 0) + 1;
     const auto kernel = !fused ? evict_kernel<THREADS, ITEMS, 0> : f32 ? evict_kernel<THREADS, ITEMS, 32> : evict_kernel<THREADS, ITEMS, 16>;
-    const size_t smem = (size_t)p.max_moves * 2 * sizeof(uint16_t);
-    if (smem > 32 * 1024) {                          // beside the static words
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
-    return launch_behind(units <= sm_count(), kernel, (unsigned)units, THREADS, smem, st, p);
+    return cudaLaunchKernelEx(&cfg, kernel, p, cluster);
 }
+
+// CTAs per (sequence, kv head): more than one for long sequences where SMs would idle.  Two sequences of 32768 tokens, 8 kv heads, the
+// plan alone: 48 us with one CTA of 1024 threads each, 30 with two, 26 with four, 46 with eight of 256 threads (which read 2048
+// counts of seven others, three times).
+static int evict_cluster(int64_t units, int64_t most) {
+    int c = 1;
+    while (c < 4 && most > 4096 * c && units * c * 2 <= sm_count()) c *= 2;
+    return most > 16384 * c ? 4 : c;
+}
+// The planning CTA copies at most this many tokens; more go to a launch of their own.  2049 tokens cut to 2048, 8 kv heads: 11.8 us in
+// one launch, 14 in two; 48 sequences of 2304 tokens cut to 2048: 48 us and 37; 7 of 700 cut to 333, fp32: 28 us and 13.
+constexpr int kEvFused = 64;
 
 static int64_t evict_max_moves(int max_pages, int keep) {
     const int64_t behind = (int64_t)max_pages * kPageSize - keep;
@@ -470,21 +585,21 @@ extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_
     const int64_t most = (int64_t)max_pages_per_seq * kPageSize;
     cudaStream_t st = (cudaStream_t)stream;
     const int parts = (p.max_moves + kEvWarps * kEvEach - 1) / (kEvWarps * kEvEach);
-    if (units * parts > 2147483647LL) {
+    if (units * (parts > 8 ? parts : 8) > 2147483647LL) {
         set_error("%s: too many tokens to move in one launch", who);
         return KTK_ERR_TOO_LARGE;
     }
-    const bool fused = most <= 32768 && (units >= sm_count() || p.max_moves <= 256);
     const bool f32 = s->dtype == KTK_F32;
-    if (most <= 4096) KTK_CUDA_TRY((launch_evict<512, 8>(p, units, fused, f32, st)), who);
-    else if (most <= 16384) KTK_CUDA_TRY((launch_evict<1024, 16>(p, units, fused, f32, st)), who);
-    else if (most <= 32768) KTK_CUDA_TRY((launch_evict<1024, 32>(p, units, fused, f32, st)), who);
+    const int cluster = evict_cluster(units, most);
+    const bool fused = cluster == 1 && most <= 16384 && p.max_moves <= kEvFused;
+    if (most <= 4096) KTK_CUDA_TRY((launch_evict<256, 16>(p, units, cluster, fused, f32, st)), who);
+    else if (most <= 16384 * cluster) KTK_CUDA_TRY((launch_evict<1024, 16>(p, units, cluster, fused, f32, st)), who);
     else {
-        const size_t bits = (size_t)((most + 31) / 32) * 2 * sizeof(uint32_t), room = 200 * 1024;
-        p.smem_keys = bits + most * sizeof(uint32_t) <= room ? (int)most : 0;
-        const size_t smem = bits + (size_t)p.smem_keys * sizeof(uint32_t);
-        KTK_CUDA_TRY(cudaFuncSetAttribute(evict_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
-        KTK_CUDA_TRY(launch_behind(false, evict_long_kernel, (unsigned)units, kEvLong, smem, st, p), who);
+    const size_t bits = (size_t)((most + 31) / 32) * 2 * sizeof(uint32_t), room = 190 * 1024;
+    p.smem_keys = bits + most * sizeof(uint32_t) <= room ? (int)most : 0;
+    const size_t smem = bits + (size_t)p.smem_keys * sizeof(uint32_t);
+    KTK_CUDA_TRY(cudaFuncSetAttribute(evict_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+    KTK_CUDA_TRY(launch_behind(false, evict_long_kernel, (unsigned)units, kEvLong, smem, st, p), who);
     }
     if (fused) return KTK_OK;
     const auto move = f32 ? evict_move_kernel<32> : evict_move_kernel<16>;
