@@ -11,7 +11,7 @@ namespace ktk {
 
 constexpr int kMassThreads = 256;
 constexpr int kMassEach = 4;                              // tokens of a thread, their loads in flight together
-constexpr int kMassTokens = kMassThreads * kMassEach;     // of a CTA
+constexpr int kMassTokens = kMassThreads * kMassEach;     // of a CTA at a time
 
 // The pieces of a list: `count` of them, 0 for a list that one CTA saw whole.  STREAM: behind the balanced partition; otherwise
 // num_splits partials of every list.
@@ -23,10 +23,11 @@ template <bool STREAM> struct Pieces {
     }
 };
 
-// One CTA per list and kMassTokens of its tokens, and one per list for its output.
+// One CTA per list and `rounds` times kMassTokens of its tokens, and one per list for its output.  A CTA's first loads, one behind the
+// other, take longer than a round does: about as many CTAs as the device holds, and the next round's loads in flight.
 template <typename T, bool STREAM, int G>
 __global__ void __launch_bounds__(kMassThreads)
-mass_finish_kernel(const StreamParams p, int chunks, int decode_ctas) {
+mass_finish_kernel(const StreamParams p, int chunks, int rounds, int decode_ctas) {
     __shared__ float lse[G];
     const DecodeParams& d = p.d;
     const MassParams& m = p.m;
@@ -82,30 +83,37 @@ mass_finish_kernel(const StreamParams p, int chunks, int decode_ctas) {
 
     const int tokens = el.cnt == 1 ? el.last : el.first + (el.cnt - 2) * kPageSize + el.last;
     const int row = m.slot_index ? m.slot_index[b] : b;
-    if (part * kMassTokens >= tokens) return;
+    const int t_begin = part * rounds * kMassTokens, t_end = min(t_begin + rounds * kMassTokens, tokens);
+    if (t_begin >= t_end) return;
     if (row < 0 || row >= m.rows || tokens > m.stride || start + el.cnt > m.positions) {
         if (tid == 0 && part == 0) report(d.status, KTK_STATUS_BAD_TABLE);
         return;
     }
     const int64_t at = ((int64_t)row * d.Hkv + h) * m.stride;
     float s[kMassEach][G], before[kMassEach];
+    const auto load = [&](int t0) {
 #pragma unroll
-    for (int i = 0; i < kMassEach; ++i) {
-        const int t = part * kMassTokens + i * kMassThreads + tid;
-        if (t >= tokens) continue;
-        // a short first page leaves places of its own block free
-        const int place = t < el.first || el.cnt == 1 ? t : t + kPageSize - el.first;
-        const float* from = m.scores + (start * kPageSize + place) * G;
-        if constexpr (G >= 4) {
+        for (int i = 0; i < kMassEach; ++i) {
+            const int t = min(t0 + i * kMassThreads + tid, tokens - 1);
+            // a short first page leaves places of its own block free
+            const int place = t < el.first || el.cnt == 1 ? t : t + kPageSize - el.first;
+            const float* from = m.scores + (start * kPageSize + place) * G;
+            if constexpr (G >= 4) {
 #pragma unroll
-            for (int g = 0; g < G; g += 4) *reinterpret_cast<float4*>(&s[i][g]) = *reinterpret_cast<const float4*>(from + g);
-        } else if constexpr (G == 2) {
-            *reinterpret_cast<float2*>(s[i]) = *reinterpret_cast<const float2*>(from);
-        } else {
-            s[i][0] = *from;
+                for (int g = 0; g < G; g += 4) {
+                    const float4 v = __ldcs(reinterpret_cast<const float4*>(from + g));
+                    s[i][g] = v.x; s[i][g + 1] = v.y; s[i][g + 2] = v.z; s[i][g + 3] = v.w;
+                }
+            } else if constexpr (G == 2) {
+                const float2 v = __ldcs(reinterpret_cast<const float2*>(from));
+                s[i][0] = v.x; s[i][1] = v.y;
+            } else {
+                s[i][0] = __ldcs(from);
+            }
+            before[i] = m.in[at + t];
         }
-        before[i] = t == tokens - 1 ? 0.0f : m.in[at + t];
-    }
+    };
+    load(t_begin);
     if (tid < 32) {                                       // lanes of a head: pieces lane / G, lane / G + 32 / G, ...
         const int g = lane % G;
         float M = -INFINITY, L = 0.0f;
@@ -127,27 +135,39 @@ mass_finish_kernel(const StreamParams p, int chunks, int decode_ctas) {
         if (lane < G) lse[lane] = pieces.count == 0 ? d.lse[qh + lane] : M + log2f(L);
     }
     __syncthreads();
+    float mine[G];
 #pragma unroll
-    for (int i = 0; i < kMassEach; ++i) {
-        const int t = part * kMassTokens + i * kMassThreads + tid;
-        if (t >= tokens) continue;
-        float sum = 0.0f;
+    for (int g = 0; g < G; ++g) mine[g] = lse[g];
+    for (int t0 = t_begin; t0 < t_end; t0 += kMassTokens) {
+        float sum[kMassEach], old[kMassEach];
 #pragma unroll
-        for (int g = 0; g < G; ++g) sum += exp2f(s[i][g] - lse[g]);
-        m.out[at + t] = t == tokens - 1 ? sum : fmaf(m.decay, before[i], sum);
+        for (int i = 0; i < kMassEach; ++i) {
+            sum[i] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) sum[i] += exp2f(s[i][g] - mine[g]);
+            old[i] = before[i];
+        }
+        if (t0 + kMassTokens < t_end) load(t0 + kMassTokens);
+#pragma unroll
+        for (int i = 0; i < kMassEach; ++i) {
+            const int t = t0 + i * kMassThreads + tid;
+            if (t < t_end) m.out[at + t] = t == tokens - 1 ? sum[i] : fmaf(m.decay, old[i], sum[i]);
+        }
     }
 }
 
 template <typename T, bool STREAM>
 static int launch_finish(const StreamParams& p, int decode_ctas, cudaStream_t st) {
-    const int64_t chunks = ((int64_t)p.m.max_pages * kPageSize + kMassTokens - 1) / kMassTokens;
-    const int64_t ctas = (chunks + 1) * p.d.batch * p.d.Hkv;
+    const int64_t units = (int64_t)p.d.batch * p.d.Hkv, all = ((int64_t)p.m.max_pages * kPageSize + kMassTokens - 1) / kMassTokens;
+    int64_t rounds = (units * all + sm_count() * 3 - 1) / (sm_count() * 3);      // CTAs that the device holds at once
+    rounds = rounds < 1 ? 1 : rounds > all ? all : rounds;
+    const int64_t chunks = (all + rounds - 1) / rounds, ctas = (chunks + 1) * units;
     if (ctas > 2147483647LL) {
         set_error("ktk_dense_decode_mass: batch * num_kv_heads * max_pages_per_seq exceeds the grid limit");
         return KTK_ERR_TOO_LARGE;
     }
     const auto go = [&](auto kernel) {
-        return launch_behind(true, kernel, (unsigned)ctas, kMassThreads, 0, st, p, (int)chunks, decode_ctas);
+        return launch_behind(true, kernel, (unsigned)ctas, kMassThreads, 0, st, p, (int)chunks, (int)rounds, decode_ctas);
     };
     KTK_CUDA_TRY(p.G == 1 ? go(mass_finish_kernel<T, STREAM, 1>) : p.G == 2 ? go(mass_finish_kernel<T, STREAM, 2>)
                  : p.G == 4 ? go(mass_finish_kernel<T, STREAM, 4>) : go(mass_finish_kernel<T, STREAM, 8>),

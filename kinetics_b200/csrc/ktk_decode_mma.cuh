@@ -148,15 +148,16 @@ __device__ __forceinline__ void mma_consume_page(MmaState& st, uint8_t* stage, i
     mma_consume_page_t<false>(st, stage, ntok, qb, scale_log2, lane, ntok, ntok);
 }
 
-// The four TMA tile loads of one page (K and V, each as two 16-row x 128-byte boxes) into a stage.
+// The four TMA tile loads of one page (K and V, each as two 16-row x 128-byte boxes) into a stage.  `policy`: nothing, or read_once_policy().
+template <class... Policy>
 __device__ __forceinline__ void tma_load_page(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int64_t page,
-                                              int h) {
+                                              int h, Policy... policy) {
     const int y = (int)(page * (2 * kPageSize));      // token row of K slot 0
     mbar_arrive_expect_tx(bar, kStageBytes);
-    tma_load_3d(dst, map, bar, 0, h, y);
-    tma_load_3d(dst + kHalfTile, map, bar, 64, h, y);
-    tma_load_3d(dst + 2 * kHalfTile, map, bar, 0, h, y + kPageSize);
-    tma_load_3d(dst + 3 * kHalfTile, map, bar, 64, h, y + kPageSize);
+    tma_load_3d(dst, map, bar, 0, h, y, policy...);
+    tma_load_3d(dst + kHalfTile, map, bar, 64, h, y, policy...);
+    tma_load_3d(dst + 2 * kHalfTile, map, bar, 0, h, y + kPageSize, policy...);
+    tma_load_3d(dst + 3 * kHalfTile, map, bar, 64, h, y + kPageSize, policy...);
 }
 
 // Tensor map over the cache seen as [token rows = pages*2*16][Hkv][128], innermost first, in boxes of

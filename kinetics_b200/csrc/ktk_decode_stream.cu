@@ -103,7 +103,8 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                             issued = i + 1;
                         } else {
                             stage_tag[s] = i + 1;
-                            tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h);
+                            if (MASS) tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h, read_once_policy());
+                            else tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h);
                             issued = i + 1;
                         }
                     }

@@ -16,6 +16,7 @@ no CPU implementation and no PyTorch fallback: a CPU tensor raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -358,8 +359,9 @@ def prefill_attention(q, q_indptr, max_new_tokens: int, kv_cache, kv_indices, kv
 
 
 # ---- a cache of bounded size: attention that adds up what tokens were paid, and the eviction that goes by it
-# A decode step of few sequences takes the device some ten microseconds: these calls look at their tensors once and hand plain
-# integers to the library.
+# A decode step of few sequences takes the device some ten microseconds, a Python attribute a tenth of one: these calls look at each
+# tensor once, and what follows from sizes and types alone (checks, the C struct, the workspace's size) is worked out once per set
+# of them.
 
 def _addresses(*tensors):
     """Addresses of contiguous tensors on the current device (None: 0), and that device's stream."""
@@ -369,49 +371,97 @@ def _addresses(*tensors):
         if t is None:
             at.append(0)
             continue
-        if not t.is_cuda:
-            raise RuntimeError("kinetics_b200 ops need CUDA tensors: this path has no CPU fallback")
+        if t.get_device() != dev:
+            if not t.is_cuda:
+                raise RuntimeError("kinetics_b200 ops need CUDA tensors: this path has no CPU fallback")
+            raise RuntimeError(f"kinetics_b200: a tensor on {t.device}, the current device is cuda:{dev}")
         if not t.is_contiguous():
             raise RuntimeError("kinetics_b200 ops need contiguous tensors")
-        if t.get_device() != dev:
-            raise RuntimeError(f"kinetics_b200: a tensor on {t.device}, the current device is cuda:{dev}")
         at.append(t.data_ptr())
     at.append(torch._C._cuda_getCurrentRawStream(dev))
     return at
 
 
-def _check_table(batch, kv_indices, kv_indptr, kv_last_page_len, view) -> None:
-    if kv_indices.dtype != torch.int32 or kv_indptr.dtype != torch.int32 or kv_last_page_len.dtype != torch.int32:
-        raise TypeError("page tables are int32")
-    if _batch_of(kv_indptr, view) != batch or kv_last_page_len.numel() < batch:
-        raise ValueError(f"page table of {_batch_of(kv_indptr, view)} sequences, {batch} expected")
-    if view is not None and any(t is not None and t.numel() < batch for t in (view.page_count, view.slot_index)):
-        raise ValueError(f"PageView: page_count and slot_index have {batch} entries")
+def _needs_cuda(t) -> None:
+    if not t.is_cuda:
+        raise RuntimeError("kinetics_b200 ops need CUDA tensors: this path has no CPU fallback")
 
 
-def _check_queries(q, kv_cache, out) -> None:
-    if q.dim() != 3 or q.shape[2] != kv_cache.shape[-1]:
-        raise ValueError(f"q must be [rows, Hq, {kv_cache.shape[-1]}], got {tuple(q.shape)}")
-    if q.dtype != kv_cache.dtype or out.dtype != q.dtype or out.shape != q.shape:
-        raise TypeError("q, kv_cache and out must share a dtype, out the shape of q")
-
-
-def _check_mass(mass, mass_out, batch, num_kv_heads, view) -> None:
-    """mass fp32 [rows, Hkv, places]; without a slot_index one row per sequence."""
-    if mass.dtype != torch.float32 or mass_out.dtype != torch.float32:
+def _mass_shape(batch, kv_shape, dtype, num_q_heads, mass_shape, mass_dtype, slots, tables) -> Shape:
+    """The sizes of a call over `batch` sequences, checked.  mass fp32 [rows, Hkv, places]; without slots (view.slot_index) one row
+    per sequence.  tables: (dtype, entries wanted or None, entries) of index tensors."""
+    if len(kv_shape) != 5 or kv_shape[1] != 2:
+        raise ValueError("kv_cache must be [num_pages, 2, page_size, num_kv_heads, head_dim]")
+    hkv = kv_shape[3]
+    if num_q_heads % hkv:
+        raise ValueError(f"{num_q_heads} query heads do not divide into {hkv} kv heads")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"kinetics_b200: dtype {dtype} not supported (float32 or bfloat16)")
+    if mass_dtype != torch.float32:
         raise TypeError("mass is fp32")
-    if mass.dim() != 3 or mass.shape[1] != num_kv_heads or mass_out.shape != mass.shape:
-        raise ValueError(f"mass must be [rows, {num_kv_heads}, places], got {tuple(mass.shape)} and {tuple(mass_out.shape)}")
-    if mass.shape[0] < batch and (view is None or view.slot_index is None):
-        raise ValueError(f"mass of {mass.shape[0]} rows for {batch} sequences")
+    if len(mass_shape) != 3 or mass_shape[1] != hkv:
+        raise ValueError(f"mass must be [rows, {hkv}, places], got {tuple(mass_shape)}")
+    if mass_shape[0] < batch and not slots:
+        raise ValueError(f"mass of {mass_shape[0]} rows for {batch} sequences")
+    for index_dtype, want, have in tables:
+        if index_dtype != torch.int32:
+            raise TypeError("page tables, counts and positions are int32")
+        if want is not None and have < want:
+            raise ValueError(f"a table of {have} entries, {want} expected")
+    return Shape(batch, hkv, num_q_heads // hkv, kv_shape[4], kv_shape[2],
+                 _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32, kv_shape[0])
 
 
-def _list_bounds(mass, kv_indices, view):
-    """Pages of the longest list, pages of all lists (-1: unknown), as far as the tensors' sizes tell."""
-    if view is not None and view.page_count is not None:
-        return mass.shape[2] // PAGE_SIZE + 2, -1
-    pages = kv_indices.numel()
-    return max(pages, 1), pages
+def _check_queries(q_shape, q_dtype, kv_shape, kv_dtype) -> None:
+    if len(q_shape) != 3 or q_shape[2] != kv_shape[-1]:
+        raise ValueError(f"q must be [rows, Hq, {kv_shape[-1]}], got {tuple(q_shape)}")
+    if q_dtype != kv_dtype:
+        raise TypeError("q and kv_cache must share a dtype")
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dtype, slots, padded, tables, max_pages):
+    """(sizes, pages of all lists or -1, workspace bytes)"""
+    _check_queries(q_shape, q_dtype, kv_shape, kv_dtype)
+    shp = _mass_shape(q_shape[0], kv_shape, kv_dtype, q_shape[1], mass_shape, mass_dtype, slots, tables)
+    pages = -1 if padded else tables[0][2]
+    return shp, pages, int(_lib.load().ktk_decode_mass_workspace_bytes(shp, max_pages, pages))
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefill_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dtype, slots, padded, tables, max_new, window):
+    """(sizes, pages of the longest list, of all lists or -1, workspace bytes)"""
+    _check_queries(q_shape, q_dtype, kv_shape, kv_dtype)
+    batch = tables[3][2] - 1
+    shp = _mass_shape(batch, kv_shape, kv_dtype, q_shape[1], mass_shape, mass_dtype, slots, tables)
+    pages = -1 if padded else tables[0][2]
+    most = mass_shape[2] // PAGE_SIZE + 2 if padded else max(pages, 1)
+    return shp, most, pages, int(_lib.load().ktk_prefill_mass_workspace_bytes(shp, q_shape[0], max_new, most, pages, window))
+
+
+@functools.lru_cache(maxsize=1024)
+def _evict_plan(batch, kv_shape, kv_dtype, mass_shape, mass_dtype, positions_shape, slots, tables, max_pages, keep):
+    """(sizes, workspace bytes)"""
+    shp = _mass_shape(batch, kv_shape, kv_dtype, kv_shape[3], mass_shape, mass_dtype, slots, tables)
+    if positions_shape != mass_shape:
+        raise ValueError(f"positions {tuple(positions_shape)} must have the shape of mass {tuple(mass_shape)}")
+    return shp, int(_lib.load().ktk_evict_workspace_bytes(shp, max_pages, keep))
+
+
+def _tables(batch, kv_indices, kv_indptr, kv_last_page_len, view):
+    """Types and sizes of a page table: ((dtype, entries wanted, entries), ...)."""
+    if view is None:
+        return ((kv_indices.dtype, None, kv_indices.numel()), (kv_indptr.dtype, batch + 1, kv_indptr.numel()),
+                (kv_last_page_len.dtype, batch, kv_last_page_len.numel()))
+    padded = view.page_count is not None
+    more = tuple((t.dtype, batch, t.numel()) for t in (view.page_count, view.slot_index) if t is not None)
+    return ((kv_indices.dtype, None, kv_indices.numel()), (kv_indptr.dtype, batch if padded else batch + 1, kv_indptr.numel()),
+            (kv_last_page_len.dtype, batch, kv_last_page_len.numel())) + more
+
+
+def _same(t, like, what) -> None:
+    if t.dtype != like.dtype or t.shape != like.shape:
+        raise TypeError(f"{what} must have the dtype and shape {like.dtype} {tuple(like.shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
 def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: int, mass, decay: float = 1.0,
@@ -423,23 +473,26 @@ def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_
     decay * mass + the weights of this step, and the weights alone for the newest token, to mass_out (None: mass itself);
     places behind a sequence's length are left as they are.  workspace: ``ktk_decode_mass_workspace_bytes`` bytes, not shared
     by calls that may overlap (None: from the allocator, which keeps streams and graphs apart).  Returns (out, mass_out)."""
+    _needs_cuda(q)
+    slots = view is not None and view.slot_index is not None
+    padded = view is not None and view.page_count is not None
+    shp, pages, need = _decode_mass_plan(q.shape, q.dtype, kv_cache.shape, kv_cache.dtype, mass.shape, mass.dtype, slots, padded,
+                                         _tables(len(q), kv_indices, kv_indptr, kv_last_page_len, view), max_pages_per_seq)
     if out is None:
         out = torch.empty_like(q)
+    else:
+        _same(out, q, "out")
     if mass_out is None:
         mass_out = mass
-    lib, cv = _lib.load(), None if view is None else view.c()
-    _check_queries(q, kv_cache, out)
-    B, Hq, D = q.shape
-    shp = _shape(B, kv_cache, Hq)
-    _check_table(B, kv_indices, kv_indptr, kv_last_page_len, view)
-    _check_mass(mass, mass_out, B, shp.num_kv_heads, view)
-    total = _list_bounds(mass, kv_indices, view)[1]
+    else:
+        _same(mass_out, mass, "mass_out")
     if workspace is None:
-        workspace = torch.empty(lib.ktk_decode_mass_workspace_bytes(shp, max_pages_per_seq, total), dtype=torch.uint8, device=q.device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     q_, kv_, i_, p_, l_, m_, mo_, o_, w_, s_, stream = _addresses(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out,
                                                                  out, workspace, status)
-    check(lib.ktk_dense_decode_mass(q_, kv_, i_, p_, l_, cv, max_pages_per_seq, total, D ** -0.5 if sm_scale is None else sm_scale,
-                                    _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], decay), o_, w_, workspace.nbytes, shp, s_, stream))
+    check(_lib.load().ktk_dense_decode_mass(
+        q_, kv_, i_, p_, l_, None if view is None else view.c(), max_pages_per_seq, pages, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
+        _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], decay), o_, w_, workspace.nbytes, shp, s_, stream))
     _launched(2)
     return out, mass_out
 
@@ -450,29 +503,29 @@ def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indice
     """``prefill_attention`` that also accumulates the weights that the last ``window`` new tokens of every sequence (0: all
     of them) give each cached token; mass and workspace as in ``dense_decode_mass``, the sequence's new tokens start from their
     weights alone.  Returns (out, mass_out)."""
+    _needs_cuda(q)
+    slots = view is not None and view.slot_index is not None
+    padded = view is not None and view.page_count is not None
+    i_, p_, l_, *more = _tables(q_indptr.numel() - 1, kv_indices, kv_indptr, kv_last_page_len, view)
+    shp, most, pages, need = _prefill_mass_plan(q.shape, q.dtype, kv_cache.shape, kv_cache.dtype, mass.shape, mass.dtype, slots, padded,
+                                                (i_, p_, l_, (q_indptr.dtype, None, q_indptr.numel()), *more), max_new_tokens, window)
     if out is None:
         out = torch.empty_like(q)
+    else:
+        _same(out, q, "out")
     if mass_out is None:
         mass_out = mass
-    lib, cv = _lib.load(), None if view is None else view.c()
-    _check_queries(q, kv_cache, out)
-    total, Hq, D = q.shape
-    B = q_indptr.numel() - 1
-    shp = _shape(B, kv_cache, Hq)
-    if q_indptr.dtype != torch.int32:
-        raise TypeError("q_indptr must be int32")
-    _check_table(B, kv_indices, kv_indptr, kv_last_page_len, view)
-    _check_mass(mass, mass_out, B, shp.num_kv_heads, view)
-    most, pages = _list_bounds(mass, kv_indices, view)
+    else:
+        _same(mass_out, mass, "mass_out")
     if workspace is None:
-        workspace = torch.empty(lib.ktk_prefill_mass_workspace_bytes(shp, total, max_new_tokens, most, pages, window), dtype=torch.uint8,
-                                device=q.device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     q_, n_, kv_, i_, p_, l_, m_, mo_, o_, w_, s_, stream = _addresses(q, q_indptr, kv_cache, kv_indices, kv_indptr, kv_last_page_len,
                                                                      mass, mass_out, out, workspace, status)
-    check(lib.ktk_prefill_attention_mass(q_, n_, total, max_new_tokens, kv_, i_, p_, l_, cv, most, pages, window,
-                                         D ** -0.5 if sm_scale is None else sm_scale,
-                                         _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], decay), o_, w_, workspace.nbytes, shp, s_, stream))
-    _launched(2 if kv_cache.dtype == torch.bfloat16 else 3)
+    check(_lib.load().ktk_prefill_attention_mass(
+        q_, n_, q.shape[0], max_new_tokens, kv_, i_, p_, l_, None if view is None else view.c(), most, pages, window,
+        HEAD_DIM ** -0.5 if sm_scale is None else sm_scale, _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], decay), o_, w_,
+        workspace.nbytes, shp, s_, stream))
+    _launched(2 if shp.dtype == _lib.KTK_BF16 else 3)
     return out, mass_out
 
 
@@ -487,26 +540,28 @@ def evict(kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: 
     order, up to position seen[row] - 1 (stored, seen: int32 [rows]).  Afterwards a sequence holds min(n, keep) tokens: that
     is ``stored`` of the next call, and what the next page table has to say.  Page summaries have to be rebuilt.
     workspace: ``ktk_evict_workspace_bytes`` bytes, as in ``dense_decode_mass``.  Returns (mass_out, positions_out)."""
+    _needs_cuda(kv_cache)
+    slots = view is not None and view.slot_index is not None
+    batch, rows = _batch_of(kv_indptr, view), mass.shape[0]
+    shp, need = _evict_plan(batch, kv_cache.shape, kv_cache.dtype, mass.shape, mass.dtype, positions.shape, slots,
+                            _tables(batch, kv_indices, kv_indptr, kv_last_page_len, view) +
+                            ((positions.dtype, None, 0), (stored.dtype, rows, stored.numel()), (seen.dtype, rows, seen.numel())),
+                            max_pages_per_seq, keep)
     if mass_out is None:
         mass_out = mass
+    else:
+        _same(mass_out, mass, "mass_out")
     if positions_out is None:
         positions_out = positions
-    lib, cv = _lib.load(), None if view is None else view.c()
-    B = _batch_of(kv_indptr, view)
-    shp = _shape(B, kv_cache, kv_cache.shape[3])
-    _check_table(B, kv_indices, kv_indptr, kv_last_page_len, view)
-    _check_mass(mass, mass_out, B, shp.num_kv_heads, view)
-    if any(t.dtype != torch.int32 for t in (positions, positions_out, stored, seen)):
-        raise TypeError("positions, stored and seen are int32")
-    if positions.shape != mass.shape or positions_out.shape != mass.shape or stored.numel() != mass.shape[0] or \
-            seen.numel() != mass.shape[0]:
-        raise ValueError("positions have the shape of mass, stored and seen one entry per row")
+    else:
+        _same(positions_out, positions, "positions_out")
     if workspace is None:
-        workspace = torch.empty(lib.ktk_evict_workspace_bytes(shp, max_pages_per_seq, keep), dtype=torch.uint8, device=kv_cache.device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=kv_cache.device)
     kv_, i_, p_, l_, m_, mo_, at_, ato_, st_, se_, w_, s_, stream = _addresses(
         kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out, positions, positions_out, stored, seen, workspace, status)
-    check(lib.ktk_evict(kv_, i_, p_, l_, cv, max_pages_per_seq, _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], 1.0), at_, ato_, st_, se_,
-                        keep, sink, recent, w_, workspace.nbytes, shp, s_, stream))
+    check(_lib.load().ktk_evict(
+        kv_, i_, p_, l_, None if view is None else view.c(), max_pages_per_seq, _lib.Mass(m_, mo_, mass.shape[2], rows, 1.0), at_, ato_,
+        st_, se_, keep, sink, recent, w_, workspace.nbytes, shp, s_, stream))
     _launched(2)
     return mass_out, positions_out
 
