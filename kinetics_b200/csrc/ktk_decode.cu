@@ -215,7 +215,7 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
         const int64_t qh = (int64_t)b * Hq + (int64_t)h * G + g;
         if (!MASS && S == 1) {
             ((T*)p.o)[qh * kHeadDim + d] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
-            if (p.lse != nullptr && d == 0) p.lse[qh] = M + log2f(L);
+            if (p.neg_lse != nullptr && d == 0) p.neg_lse[qh] = -(M + log2f(L));
         } else {
             p.ws_o[(qh * S + split) * kHeadDim + d] = O;
             if (d == 0) {

@@ -28,7 +28,7 @@ template <bool STREAM> struct Pieces {
 template <typename T, bool STREAM, int G>
 __global__ void __launch_bounds__(kMassThreads)
 mass_finish_kernel(const StreamParams p, int chunks, int rounds, int decode_ctas) {
-    __shared__ float lse[G];
+    __shared__ float neg_lse[G];
     const DecodeParams& d = p.d;
     const MassParams& m = p.m;
     const int tid = threadIdx.x, lane = tid & 31;
@@ -132,19 +132,19 @@ mass_finish_kernel(const StreamParams p, int chunks, int rounds, int decode_ctas
             const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
             join(m2, l2);
         }
-        if (lane < G) lse[lane] = pieces.count == 0 ? d.lse[qh + lane] : M + log2f(L);
+        if (lane < G) neg_lse[lane] = pieces.count == 0 ? d.neg_lse[qh + lane] : -(M + log2f(L));
     }
     __syncthreads();
     float mine[G];
 #pragma unroll
-    for (int g = 0; g < G; ++g) mine[g] = lse[g];
+    for (int g = 0; g < G; ++g) mine[g] = neg_lse[g];
     for (int t0 = t_begin; t0 < t_end; t0 += kMassTokens) {
         float sum[kMassEach], old[kMassEach];
 #pragma unroll
         for (int i = 0; i < kMassEach; ++i) {
             sum[i] = 0.0f;
 #pragma unroll
-            for (int g = 0; g < G; ++g) sum[i] += exp2f(s[i][g] - mine[g]);
+            for (int g = 0; g < G; ++g) sum[i] += exp2f(s[i][g] + mine[g]);
             old[i] = before[i];
         }
         if (t0 + kMassTokens < t_end) load(t0 + kMassTokens);
@@ -250,7 +250,7 @@ extern "C" int ktk_dense_decode_mass(const void* q, const void* kv_cache, const 
     char* ws = (char*)workspace;
     p.ws_ml = (float*)ws;
     p.ws_o = (float*)ws + rows * 2;
-    p.lse = (float*)(ws + w.lse);
+    p.neg_lse = (float*)(ws + w.lse);
     p.status = status;
     MassParams m;
     m.in = mass->in; m.out = mass->out; m.stride = mass->stride; m.rows = mass->rows; m.slot_index = view.slot_index;

@@ -210,7 +210,7 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                     if (whole) {
                         const int64_t qh = (int64_t)pc.b * Hq + (int64_t)pc.h * G + g;
                         ((__nv_bfloat16*)d.o)[qh * kHeadDim + dd] = __float2bfloat16_rn(L > 0.0f ? O / L : 0.0f);
-                        if (MASS && dd == 0) d.lse[qh] = M + log2f(L);
+                        if (MASS && dd == 0) d.neg_lse[qh] = -(M + log2f(L));
                     } else {
                         const int64_t row = (int64_t)slot * G + g;
                         d.ws_o[row * kHeadDim + dd] = O;

@@ -55,7 +55,7 @@ prefill_mass_simt_kernel(const PrefillMassParams p, int chunks) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) rows[r][c * 8 + k] = f[k];
         }
-        if (tid < n) row_lse[tid] = p.lse[(int64_t)(s.q0 + tok0 + (r0 + tid) / G) * Hq + h * G + (r0 + tid) % G];
+        if (tid < n) row_lse[tid] = p.neg_lse[(int64_t)(s.q0 + tok0 + (r0 + tid) / G) * Hq + h * G + (r0 + tid) % G];
         __syncthreads();
         for (int r = 0; r < n; ++r) {
             float dot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -68,7 +68,7 @@ prefill_mass_simt_kernel(const PrefillMassParams p, int chunks) {
                 dot[3] = fmaf(v.w, key[i + 3], dot[3]);
             }
             const float x = (dot[0] + dot[1]) + (dot[2] + dot[3]);
-            if (t <= s.base_pos + tok0 + (r0 + r) / G) sum += exp2f(x * p.scale_log2 - row_lse[r]);
+            if (t <= s.base_pos + tok0 + (r0 + r) / G) sum += exp2f(x * p.scale_log2 + row_lse[r]);
         }
     }
     if (on) {
@@ -139,14 +139,15 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
     p.q = q; p.cache = kv_cache; p.q_indptr = q_indptr; p.kv_indices = kv_indices; p.kv_indptr = kv_indptr;
     p.kv_last_page_len = kv_last_page_len; p.page_count = view.page_count; p.sink_tokens = view.sink_tokens;
     p.batch = s->batch; p.Hkv = s->num_kv_heads; p.G = s->group_size; p.num_pages = s->num_pages; p.total_new = total_new_tokens;
-    p.scale_log2 = sm_scale * kLog2e; p.lse = lse; p.window = window; p.status = status;
+    p.scale_log2 = sm_scale * kLog2e; p.neg_lse = lse; p.window = window; p.status = status;
     p.m.in = mass->in; p.m.out = mass->out; p.m.stride = mass->stride; p.m.rows = mass->rows;
     p.m.slot_index = view.slot_index; p.m.decay = mass->decay;
     cudaStream_t st = (cudaStream_t)stream;
     if (s->dtype == KTK_BF16) {
         const MassPlan plan = mass_plan(s, max_new_tokens, max_pages_per_seq, total_pages, window);
-        p.groups = plan.groups; p.splits = plan.splits; p.tiles = plan.tiles; p.partial = (float*)behind;
-        return launch_prefill_mass_umma(p, st);
+        p.splits = plan.splits;
+        p.partial = (float*)behind;
+        return launch_prefill_mass_umma(p, plan.groups, st);
     }
     KTK_CUDA_TRY(launch_behind(false, prefill_mass_simt_kernel, (unsigned)ctas, kPsKeys, 0, st, p, (int)chunks), who);
     return KTK_OK;

@@ -18,15 +18,13 @@ struct PrefillMassParams {
     int64_t num_pages;
     int64_t total_new;
     float scale_log2;
-    const float* lse;           // [total_new, Hq]
+    const float* neg_lse;       // [total_new, Hq]: minus log2 of the rows' denominators
     int window;
     int32_t* status;
     MassParams m;
     // of the tcgen05 form (mass_plan)
-    int groups;                 // groups of pages per sequence, at most
-    int splits;                 // parts that a sequence's rows are cut into
-    int tiles;                  // tiles of 128 rows per part
-    float* partial;             // splits > 1: [batch * Hkv][splits][groups * 256] sums by key
+    int splits;                 // parts that the rows of a group of pages are cut into
+    float* partial;             // splits > 1: [groups of all sequences][Hkv][splits][256] sums by key
 };
 
 // What a CTA's sequence is, and where it lies in the mass array; false: nothing to do
@@ -50,12 +48,13 @@ __device__ __forceinline__ bool mass_sequence(const PrefillMassParams& p, int b,
     return true;
 }
 
-// How the tcgen05 form cuts its work, and the floats of its partial sums
+// How the tcgen05 form cuts its work: groups of 16 pages of all sequences (at most), parts of each, floats of their sums
 struct MassPlan {
-    int groups, splits, tiles;
+    int64_t groups;
+    int splits;
     size_t partial;
 };
 MassPlan mass_plan(const ktk_shape* s, int max_new_tokens, int64_t max_pages, int64_t total_pages, int window);
-int launch_prefill_mass_umma(const PrefillMassParams& p, cudaStream_t st);
+int launch_prefill_mass_umma(const PrefillMassParams& p, int64_t groups, cudaStream_t st);
 
 }  // namespace ktk

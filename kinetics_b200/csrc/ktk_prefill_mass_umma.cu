@@ -1,14 +1,17 @@
 // Weights of a chunk's rows summed by keys, on the fifth-generation tensor cores: with the rows' denominators known,
 //     sum[t] = sum over rows of 2^(s(t, row) - lse_row)
-// One CTA per (sequence, kv head, 16 pages = 256 keys, part of the rows).  The scores are computed transposed,
-// S^T[128 keys x 128 rows] = K . Q^T, so that a thread holds a key and sums along its own lane of tensor memory: no exchange between
-// threads, and one value per key at the end.  The rows of a tile are the (token, head) pairs of 128 / G new tokens.
+// One CTA per (sequence, kv head, 16 pages = 256 keys, part of the rows that see them), two CTAs per SM.  The scores are computed
+// transposed, S^T[128 keys x 64 rows] = K . Q^T, so that a thread holds a key and sums along its own lane of tensor memory: no exchange
+// between threads, and one value per key at the end.  The rows of a tile are the (token, head) pairs of 64 / G new tokens.
 //
 // Roles of the 320 threads:
 //     warps 0..3, 4..7   exponentials and sums of the first, the second 128 keys
-//     warp 8             matrix instructions: per tile of rows and 128 keys, into one of two buffers of 128 columns each
+//     warp 8             matrix instructions: per tile of rows and 128 keys, into one of two buffers of 64 columns each
 //     warp 9             the keys' pages (once), then tiles of queries (TMA) and their rows' denominators, kPmStages in flight
 // Every wait is bounded.
+//
+// Bound by the exponentials: 1024 cycles of the special-function units (16 a cycle) per 128 keys and 128 rows, 512 to 768 of the tensor
+// cores.  So kPmPoly of every eight pairs are computed by a polynomial on the FMA pipes.
 #include "ktk_prefill_mass.cuh"
 #include "ktk_umma.cuh"
 
@@ -19,16 +22,18 @@ namespace ktk {
 constexpr int kPmThreads = 320;
 constexpr int kPmPages = 8;                               // of 128 keys
 constexpr int kPmBlock = kUmRows;                         // keys of a block
-constexpr int kPmTile = kUmRows * 128;                    // [128 rows][64 columns]
-constexpr int kPmStages = 4;
-constexpr int kPmSmem = (2 + kPmStages) * 2 * kPmTile + 1024;
-constexpr int kPmTmemCols = 512;
+constexpr int kPmRows = 64;                               // rows of a tile
+constexpr int kPmKTile = kPmBlock * 128, kPmQTile = kPmRows * 128;      // [128 keys], [64 rows][64 columns]
+constexpr int kPmStages = 2;
+constexpr int kPmSmem = 2 * 2 * kPmKTile + kPmStages * 2 * kPmQTile + 1024;
+constexpr int kPmTmemCols = 256;
+constexpr int kPmPoly = 2;
 
 struct PmShared {
     uint64_t k, full[kPmStages], empty[kPmStages], s[2][2], s_free[2][2];
     uint32_t tmem;
     int abort;
-    alignas(16) float neg_lse[kPmStages][kUmRows];
+    alignas(16) float neg_lse[kPmStages][kPmRows];
 };
 
 // first tile of rows, counted from the first counted token, in which some row sees the token in place t
@@ -37,37 +42,94 @@ __device__ __forceinline__ int first_tile(const MassSequence& s, int tpc, int t)
     return tok > 0 ? tok / tpc : 0;
 }
 
-__global__ void __launch_bounds__(kPmThreads, 1)
+// 2^x for x <= 126 (smaller than 2^-126: that), two at a time: x = n + f, 2^f by the polynomial of degree 5 with the least relative error
+// over [-1/2, 1/2] (7.5e-8; 2.3e-7 in fp32), times 2^n.  n + 1.5 2^23 has n in its lowest bits.  NaN stays NaN.
+__device__ __forceinline__ float at_least(float x, float low) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(low));
+    return r;
+}
+__device__ __forceinline__ void exp2_poly(float& x, float& y) {
+    const float magic = 12582912.0f;
+    const uint64_t v = pack2(at_least(x, -126.0f), at_least(y, -126.0f));
+    const uint64_t t = add2(v, pack2(magic, magic)), n = add2(t, pack2(-magic, -magic)), f = fma2(n, pack2(-1.0f, -1.0f), v);
+    uint64_t r = fma2(f, pack2(0.0013276472f, 0.0013276472f), pack2(0.009675541f, 0.009675541f));
+    r = fma2(r, f, pack2(0.05550713f, 0.05550713f));
+    r = fma2(r, f, pack2(0.2402212f, 0.2402212f));
+    r = fma2(r, f, pack2(0.69314694f, 0.69314694f));
+    r = fma2(r, f, pack2(1.0000001f, 1.0000001f));
+    float t0, t1;
+    unpack2(t, t0, t1);
+    const auto power = [](float n) { return __uint_as_float((__float_as_uint(n) << 23) + 0x3f800000u); };
+    unpack2(mul2(r, pack2(power(t0), power(t1))), x, y);
+}
+
+// The group-th 16 pages among those of all sequences with new tokens: its sequence and its number there, by a whole warp; false: there
+// are fewer.
+__device__ __forceinline__ bool find_group(const PrefillMassParams& p, int group, int& b, int& g) {
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int i = b0 + lane;
+        int mine = 0;
+        if (i < p.batch && p.q_indptr[i + 1] > p.q_indptr[i]) {
+            const int pages = p.page_count ? p.page_count[i] : p.kv_indptr[i + 1] - p.kv_indptr[i];
+            mine = pages > 0 ? (pages + 2 * kPmPages - 1) / (2 * kPmPages) : 0;
+        }
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, group < upto);
+        if (here != 0) {
+            const int at = __ffs((int)here) - 1;
+            b = b0 + at;
+            g = group - __shfl_sync(0xffffffffu, upto - mine, at);
+            return true;
+        }
+        group -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+// Tiles of rows of a group of pages: those from the first that sees its first key on, cut into equal parts
+struct PmTiles {
+    int first, all, each;
+};
+__device__ __forceinline__ PmTiles tiles_of(const PrefillMassParams& p, const MassSequence& s, int g, int tpc) {
+    PmTiles t;
+    t.all = ((s.n_new - s.counted) + tpc - 1) / tpc;
+    t.first = first_tile(s, tpc, page_first_pos(g * 2 * kPmPages, s.sp.first_fill));
+    t.each = (t.all - t.first + p.splits - 1) / p.splits;
+    return t;
+}
+
+__global__ void __launch_bounds__(kPmThreads, 2)
 prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUtensorMap kv_map,
                          const __grid_constant__ CUtensorMap q_map) {
     extern __shared__ uint8_t pm_raw[];
     __shared__ __align__(16) PmShared sh;
     uint8_t* k_sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pm_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* q_sm = k_sm + 2 * 2 * kPmTile;
+    uint8_t* q_sm = k_sm + 2 * 2 * kPmKTile;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     wait_for_front();
-    const int h = blockIdx.x % p.Hkv, split = (int)(blockIdx.x / p.Hkv) % p.splits, group = (int)(blockIdx.x / p.Hkv) / p.splits;
-    const int b = blockIdx.y, G = p.G, Hq = p.Hkv * G, tpc = kUmRows / G;
+    const int h = blockIdx.x % p.Hkv, split = (int)(blockIdx.x / p.Hkv) % p.splits, item = (int)(blockIdx.x / p.Hkv) / p.splits;
+    const int G = p.G, Hq = p.Hkv * G, tpc = kPmRows / G;
+    int b, group;
+    const int items = (int)(gridDim.x / p.Hkv) / p.splits;
+    if (item == items - 1 && h == 0 && split == 0 && find_group(p, items, b, group) && tid == 0)
+        report(p.status, KTK_STATUS_BAD_TABLE);           // more than the caller's bounds
+    if (!find_group(p, item, b, group)) return;           // uniform for the CTA, as all that follows: nothing set up yet
     MassSequence s;
     if (!mass_sequence(p, b, group == 0 && split == 0 && h == 0, s)) return;
     const int e0 = group * 2 * kPmPages;
-    if (e0 >= s.sp.n_pages) return;                       // uniform for the CTA: nothing set up yet
-    const int n_tiles = ((s.n_new - s.counted) + tpc - 1) / tpc;
-    const int t_end = (split + 1) * p.tiles < n_tiles ? (split + 1) * p.tiles : n_tiles;
-    if (tid == 0 && group == 0 && split == 0 && h == 0 && (n_tiles > p.splits * p.tiles || s.sp.n_pages > p.groups * 2 * kPmPages))
-        report(p.status, KTK_STATUS_BAD_TABLE);           // more than the caller's bounds
-    int begin[2];                                         // first tile of each block of keys
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        begin[m] = t_end;
-        if (e0 + m * kPmPages < s.sp.n_pages) {
-            const int f = first_tile(s, tpc, page_first_pos(e0 + m * kPmPages, s.sp.first_fill));
-            begin[m] = f > split * p.tiles ? f : split * p.tiles;
-            if (begin[m] > t_end) begin[m] = t_end;
-        }
-    }
-    const int t_begin = begin[0];                         // the first block's keys are seen first
+    const PmTiles tiles = tiles_of(p, s, group, tpc);
+    const int t_begin = tiles.first + split * tiles.each, t_end = min(t_begin + tiles.each, tiles.all);
     if (t_begin >= t_end) return;
+    int begin[2] = {t_begin, t_end};                      // first tile of each block of keys: the first block's are seen first
+    if (e0 + kPmPages < s.sp.n_pages)
+        begin[1] = min(max(first_tile(s, tpc, page_first_pos(e0 + kPmPages, s.sp.first_fill)), t_begin), t_end);
 
     if (warp == 8) {
         tmem_alloc(&sh.tmem, kPmTmemCols);
@@ -77,7 +139,7 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
             prefetch_tensormap(&q_map);
             mbar_init(&sh.k, 1);
             for (int i = 0; i < kPmStages; ++i) {
-                mbar_init(&sh.full[i], 1);
+                mbar_init(&sh.full[i], 1 + 32);           // the queries' bytes, every lane's denominators
                 mbar_init(&sh.empty[i], 1 + 8);           // matrix instructions, the warps that read the denominators
             }
             for (int i = 0; i < 4; ++i) {
@@ -106,44 +168,44 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
         }
         __syncwarp();
         if (on) {
-            uint8_t* dst = k_sm + (lane / kPmPages) * 2 * kPmTile + (lane % kPmPages) * (kPageSize * 128);
+            uint8_t* dst = k_sm + (lane / kPmPages) * 2 * kPmKTile + (lane % kPmPages) * (kPageSize * 128);
             const int z = (int)page * (2 * kPageSize);    // token row of slot 0
             tma_load_3d(dst, &kv_map, &sh.k, 0, h, z);
-            tma_load_3d(dst + kPmTile, &kv_map, &sh.k, 64, h, z);
+            tma_load_3d(dst + kPmKTile, &kv_map, &sh.k, 64, h, z);
         }
         __syncwarp();
+        const int shift = 31 - __clz(G);              // 1, 2, 4 or 8
         bool alive = true;
         for (int i = t_begin; i < t_end; ++i, ++issued) {
             const int st = issued % kPmStages, tok0 = s.counted + i * tpc;
-            float nl[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int r = k * 32 + lane, tok = tok0 + r / G;
-                nl[k] = tok < s.n_new ? -p.lse[(int64_t)(s.q0 + tok) * Hq + h * G + r % G] : 0.0f;
-            }
             if (issued >= kPmStages) alive = mbar_wait_all(&sh.empty[st], ((issued / kPmStages) - 1) & 1, &sh.abort);
             if (!alive) break;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sh.neg_lse[st][k * 32 + lane] = nl[k];
-            __syncwarp();
+            for (int k = 0; k < kPmRows / 32; ++k) {
+                const int r = k * 32 + lane, tok = tok0 + (r >> shift);
+                const float* src = p.neg_lse + ((int64_t)(s.q0 + tok) * Hq + h * G + (r & (G - 1)));
+                const bool row = tok < s.n_new;
+                cp_async4(smem_u32(&sh.neg_lse[st][r]), row ? src : p.neg_lse, row ? 4 : 0);
+            }
+            cp_async_arrive(&sh.full[st]);
             if (lane == 0) {
-                mbar_arrive_expect_tx(&sh.full[st], 2 * kPmTile);
-                uint8_t* dst = q_sm + st * 2 * kPmTile;
+                mbar_arrive_expect_tx(&sh.full[st], 2 * kPmQTile);
+                uint8_t* dst = q_sm + st * 2 * kPmQTile;
                 tma_load_3d(dst, &q_map, &sh.full[st], 0, h * G, s.q0 + tok0);
-                tma_load_3d(dst + kPmTile, &q_map, &sh.full[st], 64, h * G, s.q0 + tok0);
+                tma_load_3d(dst + kPmQTile, &q_map, &sh.full[st], 64, h * G, s.q0 + tok0);
             }
             __syncwarp();
         }
     } else if (warp == 8) {
         // ---------------- matrix instructions ----------------
-        const uint32_t tmem = sh.tmem, idesc = umma_idesc(kUmRows, false);
+        const uint32_t tmem = sh.tmem, idesc = umma_idesc(kPmRows, false);
         const uint64_t k_desc = umma_desc(smem_u32(k_sm), 0, 1024), q_desc = umma_desc(smem_u32(q_sm), 0, 1024);
         bool alive = mbar_wait_all(&sh.k, 0, &sh.abort);
         for (int i = t_begin; i < t_end && alive; ++i) {
             const int n = i - t_begin, st = n % kPmStages;
             alive = mbar_wait_all(&sh.full[st], (n / kPmStages) & 1, &sh.abort);
             tc_fence_after();
-            const uint64_t qb = umma_desc_at(q_desc, st * 2 * kPmTile);
+            const uint64_t qb = umma_desc_at(q_desc, st * 2 * kPmQTile);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 if (!alive || i < begin[m]) continue;
@@ -154,13 +216,13 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
                     if (!alive) continue;
                 }
                 if (elect_one()) {
-                    const uint64_t ka = umma_desc_at(k_desc, m * 2 * kPmTile);
+                    const uint64_t ka = umma_desc_at(k_desc, m * 2 * kPmKTile);
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
-                            umma_f16(tmem + m * 256 + (j & 1) * 128, umma_desc_at(ka, c * kPmTile + x * 32),
-                                     umma_desc_at(qb, c * kPmTile + x * 32), idesc, (c > 0 || x > 0) ? 1u : 0u);
+                            umma_f16(tmem + m * 128 + (j & 1) * kPmRows, umma_desc_at(ka, c * kPmKTile + x * 32),
+                                     umma_desc_at(qb, c * kPmQTile + x * 32), idesc, (c > 0 || x > 0) ? 1u : 0u);
                     umma_commit(&sh.s[m][j & 1]);
                 }
                 __syncwarp();
@@ -175,7 +237,7 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
         const bool on = e < s.sp.n_pages && slot < (e == s.sp.n_pages - 1 ? s.sp.last_fill : (e == 0 ? s.sp.first_fill : kPageSize));
         const int t = page_first_pos(e, s.sp.first_fill) + slot;
         const int t_last = page_first_pos(e0 + (m + 1) * kPmPages, s.sp.first_fill);      // behind the block's last key
-        const uint32_t my = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16) + m * 256;
+        const uint32_t my = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16) + m * 128;
         const uint64_t c2 = pack2(p.scale_log2, p.scale_log2);
         float total = 0.0f, lost = 0.0f;                  // the sum, and what its rounding lost
         bool alive = true;
@@ -191,40 +253,39 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
                 const int tok0 = s.counted + i * tpc;
                 // columns that see the key, and those that are rows at all
                 const int c_lo = (t - s.base_pos - tok0) * G, c_hi = (s.n_new - tok0) * G;
-                const bool cut = s.base_pos + tok0 < t_last || c_hi < kUmRows;             // uniform for the block
+                const bool cut = s.base_pos + tok0 < t_last || c_hi < kPmRows;             // uniform for the block
                 uint64_t acc[4] = {0, 0, 0, 0};
+                float v[2][32];
+                tmem_ld64(my + (j & 1) * kPmRows, v[0], v[1]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.s_free[m][j & 1]);
+                const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(sh.neg_lse[st]);
+                auto sum = [&](auto masked) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float v[2][32];
-                    tmem_ld64(my + (j & 1) * 128 + half * 64, v[0], v[1]);
-                    if (half == 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.s_free[m][j & 1]);
-                    }
-                    const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(&sh.neg_lse[st][half * 64]);
-                    auto sum = [&](auto masked) {
+                    for (int c = 0; c < kPmRows; c += 4) {
+                        const ulonglong2 l = nl[c / 4];
 #pragma unroll
-                        for (int c = 0; c < 64; c += 4) {
-                            const ulonglong2 l = nl[c / 4];
-                            float x[4];
-                            unpack2(fma2(pack2(v[c / 32][c % 32], v[c / 32][c % 32 + 1]), c2, l.x), x[0], x[1]);
-                            unpack2(fma2(pack2(v[c / 32][c % 32 + 2], v[c / 32][c % 32 + 3]), c2, l.y), x[2], x[3]);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                x[k] = ex2(x[k]);
-                                if (masked) {
-                                    const int col = half * 64 + c + k;
-                                    x[k] = col >= c_lo && col < c_hi ? x[k] : 0.0f;
-                                }
+                        for (int k = 0; k < 4; k += 2) {
+                            const int col = c + k, pair = col / 2 % 8;
+                            float x, y;
+                            unpack2(fma2(pack2(v[col / 32][col % 32], v[col / 32][col % 32 + 1]), c2, k == 0 ? l.x : l.y), x, y);
+                            if (pair * kPmPoly % 8 + kPmPoly > 7) {      // kPmPoly of eight, evenly spread
+                                exp2_poly(x, y);
+                            } else {
+                                x = ex2(x);
+                                y = ex2(y);
                             }
-                            acc[c / 4 % 2 * 2] = add2(acc[c / 4 % 2 * 2], pack2(x[0], x[1]));
-                            acc[c / 4 % 2 * 2 + 1] = add2(acc[c / 4 % 2 * 2 + 1], pack2(x[2], x[3]));
+                            if (masked) {
+                                x = col >= c_lo && col < c_hi ? x : 0.0f;
+                                y = col + 1 >= c_lo && col + 1 < c_hi ? y : 0.0f;
+                            }
+                            acc[col / 2 % 4] = add2(acc[col / 2 % 4], pack2(x, y));
                         }
-                    };
-                    if (cut) sum(std::true_type{});
-                    else sum(std::false_type{});
-                }
+                    }
+                };
+                if (cut) sum(std::true_type{});
+                else sum(std::false_type{});
                 float a, c;
                 unpack2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), a, c);
                 const float x = a + c - lost, y = total + x;
@@ -236,7 +297,7 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
         }
         if (alive && on) {
             if (p.splits > 1) {
-                p.partial[(((int64_t)b * p.Hkv + h) * p.splits + split) * p.groups * (2 * kPmBlock) + e * kPageSize + slot] = total;
+                p.partial[(((int64_t)item * p.Hkv + h) * p.splits + split) * (2 * kPmBlock) + m * kPmBlock + key] = total;
             } else {
                 const int64_t at = ((int64_t)s.row * p.Hkv + h) * p.m.stride + t;
                 p.m.out[at] = t >= s.base_pos ? total : fmaf(p.m.decay, p.m.in[at], total);
@@ -258,44 +319,44 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
     }
 }
 
-// Adds the parts' sums, in their order
-__global__ void __launch_bounds__(256)
+// Adds the parts' sums, in their order: a CTA per group of pages and kv head
+__global__ void __launch_bounds__(2 * kPmBlock)
 prefill_mass_add_kernel(const PrefillMassParams p) {
     wait_for_front();
-    const int b = blockIdx.z, h = blockIdx.y, tpc = kUmRows / p.G;
+    const int h = blockIdx.x % p.Hkv, item = blockIdx.x / p.Hkv, tid = threadIdx.x;
+    int b, group;
     MassSequence s;
-    if (!mass_sequence(p, b, false, s)) return;
-    const int place = blockIdx.x * 256 + threadIdx.x, e = place / kPageSize, slot = place % kPageSize;
+    if (!find_group(p, item, b, group) || !mass_sequence(p, b, false, s)) return;
+    const int e = group * 2 * kPmPages + tid / kPageSize, slot = tid % kPageSize;
     if (e >= s.sp.n_pages || slot >= (e == s.sp.n_pages - 1 ? s.sp.last_fill : (e == 0 ? s.sp.first_fill : kPageSize))) return;
     const int t = page_first_pos(e, s.sp.first_fill) + slot;
-    const int n_tiles = ((s.n_new - s.counted) + tpc - 1) / tpc;
-    const int first = first_tile(s, tpc, page_first_pos(e / (2 * kPmPages) * (2 * kPmPages), s.sp.first_fill)) / p.tiles;
-    const int64_t width = (int64_t)p.groups * (2 * kPmBlock);
-    const float* part = p.partial + ((int64_t)b * p.Hkv + h) * p.splits * width + place;
+    const PmTiles tiles = tiles_of(p, s, group, kPmRows / p.G);
+    const float* part = p.partial + ((int64_t)item * p.Hkv + h) * p.splits * (2 * kPmBlock) + tid;
     float sum = 0.0f;
-    for (int i = first; i < p.splits && i * p.tiles < n_tiles; ++i) sum += part[i * width];
+#pragma unroll 4
+    for (int i = 0; i < p.splits; ++i)
+        if (tiles.first + i * tiles.each < tiles.all) sum += part[i * (2 * kPmBlock)];
     const int64_t at = ((int64_t)s.row * p.Hkv + h) * p.m.stride + t;
     p.m.out[at] = t >= s.base_pos ? sum : fmaf(p.m.decay, p.m.in[at], sum);
 }
 
+// Parts: some four rounds of the CTAs that the device holds (two per SM), of 512 rows at least.  The parts of early keys, which the most
+// rows see, start first.
 MassPlan mass_plan(const ktk_shape* s, int max_new_tokens, int64_t max_pages, int64_t total_pages, int window) {
     MassPlan plan;
-    const int tpc = kUmRows / s->group_size, counted = window > 0 && window < max_new_tokens ? window : max_new_tokens;
-    const int tiles = (counted + tpc - 1) / tpc;
-    plan.groups = (int)((max_pages + 2 * kPmPages - 1) / (2 * kPmPages));
-    int64_t about = (int64_t)plan.groups * s->batch;      // groups of all sequences
-    if (total_pages >= 0 && total_pages / (2 * kPmPages) + s->batch < about) about = total_pages / (2 * kPmPages) + s->batch;
-    about *= s->num_kv_heads;
-    int64_t want = (4 * (int64_t)sm_count() + about - 1) / about, most = (tiles + 3) / 4;
-    if (want > most) want = most;
-    if (want < 1) want = 1;
-    plan.tiles = (int)((tiles + want - 1) / want);
-    plan.splits = (tiles + plan.tiles - 1) / plan.tiles;
-    plan.partial = plan.splits > 1 ? (size_t)s->batch * s->num_kv_heads * plan.splits * plan.groups * (2 * kPmBlock) : 0;
+    const int64_t each = (max_pages + 2 * kPmPages - 1) / (2 * kPmPages);
+    plan.groups = each * s->batch;
+    if (total_pages >= 0 && total_pages / (2 * kPmPages) + s->batch < plan.groups) plan.groups = total_pages / (2 * kPmPages) + s->batch;
+    const int64_t rows = (int64_t)(window > 0 && window < max_new_tokens ? window : max_new_tokens) * s->group_size;
+    const int64_t ctas = plan.groups * s->num_kv_heads;
+    int64_t splits = (8 * (int64_t)sm_count() + ctas - 1) / ctas, most = (rows + 511) / 512;
+    if (splits > most) splits = most;
+    plan.splits = splits < 1 ? 1 : (int)splits;
+    plan.partial = plan.splits > 1 ? (size_t)ctas * plan.splits * (2 * kPmBlock) : 0;
     return plan;
 }
 
-int launch_prefill_mass_umma(const PrefillMassParams& p, cudaStream_t st) {
+int launch_prefill_mass_umma(const PrefillMassParams& p, int64_t groups, cudaStream_t st) {
     const char* who = "ktk_prefill_attention_mass";
     DecodeParams d{};                                     // only what the tensor map needs
     d.cache = p.cache; d.Hkv = p.Hkv; d.num_pages = p.num_pages;
@@ -305,20 +366,18 @@ int launch_prefill_mass_umma(const PrefillMassParams& p, cudaStream_t st) {
     const uint64_t Hq = (uint64_t)p.Hkv * p.G;
     const uint64_t dims[3] = {(uint64_t)kHeadDim, Hq, (uint64_t)p.total_new};
     const uint64_t strides[2] = {(uint64_t)kHeadDim * 2, Hq * kHeadDim * 2};
-    const uint32_t box[3] = {64, (uint32_t)p.G, (uint32_t)(kUmRows / p.G)};
+    const uint32_t box[3] = {64, (uint32_t)p.G, (uint32_t)(kPmRows / p.G)};
     rc = make_tensor_map_3d(&q_map, p.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, who);
     if (rc != KTK_OK) return rc;
-    const int64_t items = (int64_t)p.groups * p.splits * p.Hkv;
-    if (items > 2147483647LL) {
+    const int64_t units = groups * p.Hkv;
+    if (units * p.splits > 2147483647LL) {
         set_error("%s: num_kv_heads * tokens exceed the grid limit", who);
         return KTK_ERR_TOO_LARGE;
     }
     KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_mass_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem), who);
-    KTK_CUDA_TRY(launch_behind(false, prefill_mass_umma_kernel, dim3((unsigned)items, (unsigned)p.batch), kPmThreads, kPmSmem, st, p,
-                               kv_map, q_map), who);
+    KTK_CUDA_TRY(launch_behind(false, prefill_mass_umma_kernel, (unsigned)(units * p.splits), kPmThreads, kPmSmem, st, p, kv_map, q_map), who);
     if (p.splits > 1)
-        KTK_CUDA_TRY(launch_behind(true, prefill_mass_add_kernel, dim3((unsigned)p.groups, (unsigned)p.Hkv, (unsigned)p.batch), 256, 0,
-                                   st, p), who);
+        KTK_CUDA_TRY(launch_behind(true, prefill_mass_add_kernel, (unsigned)units, 2 * kPmBlock, 0, st, p), who);
     return KTK_OK;
 }
 

@@ -215,7 +215,7 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
         const bool done = fl.softmax<false>(tile, p.scale_log2, m_ref, l_run, prepare, [](float&, float&) {}, clear);
         if (done && fl.blocks_of(tile) > 0) {
             const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-            if (p.lse != nullptr && row_on) p.lse[(int64_t)(q0 + my_tok) * Hq + my_head] = m_ref + log2f(l_run);
+            if (p.neg_lse != nullptr && row_on) p.neg_lse[(int64_t)(q0 + my_tok) * Hq + my_head] = -(m_ref + log2f(l_run));
             const uint32_t o_at = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16) + kFlColO + tile * 128;
             __nv_bfloat16* dst = (__nv_bfloat16*)p.o + ((int64_t)(q0 + (row_on ? my_tok : 0)) * Hq + my_head) * kHeadDim;
 #pragma unroll
