@@ -265,7 +265,7 @@ extern "C" int ktk_prefill_attention(const void* q, const int32_t* q_indptr, int
 
 int ktk::prefill_attention(const char* who, const void* q, const int32_t* q_indptr, int64_t total_new_tokens, int32_t max_new_tokens,
                            const void* kv_cache, const int32_t* kv_indices, const int32_t* kv_indptr,
-                           const int32_t* kv_last_page_len, const ktk_view* view_in, float sm_scale, void* o, float* neg_lse,
+                           const int32_t* kv_last_page_len, const ktk_view* view_in, float sm_scale, void* o, void* lse,
                            void* workspace, size_t workspace_bytes, int32_t variant, const ktk_shape* s, int32_t* status,
                            void* stream) {
     int rc = check_shape(s, who);
@@ -301,7 +301,7 @@ int ktk::prefill_attention(const char* who, const void* q, const int32_t* q_indp
             u.q = q; u.o = o; u.cache = kv_cache; u.q_indptr = q_indptr; u.kv_indices = kv_indices;
             u.kv_indptr = kv_indptr; u.kv_last_page_len = kv_last_page_len; u.page_count = view.page_count;
             u.sink_tokens = view.sink_tokens; u.batch = s->batch; u.total_new = total_new_tokens; u.Hkv = s->num_kv_heads; u.G = G;
-            u.num_pages = s->num_pages; u.scale_log2 = sm_scale * kLog2e; u.status = status; u.neg_lse = neg_lse;
+            u.num_pages = s->num_pages; u.scale_log2 = sm_scale * kLog2e; u.status = status; u.lse = (uint4*)lse;
             return launch_prefill_umma(u, max_new_tokens, st);
         }
         PrefillParams p;
@@ -333,7 +333,7 @@ int ktk::prefill_attention(const char* who, const void* q, const int32_t* q_indp
     d.kv_indptr = rows; d.page_count = rows + total_new_tokens; d.kv_last_page_len = rows + 2 * total_new_tokens;
     d.topk = -1; d.entry_stride = 0; d.batch = (int)total_new_tokens; d.Hkv = s->num_kv_heads;
     d.num_pages = s->num_pages; d.scale_log2 = sm_scale * kLog2e; d.num_splits = 1;
-    d.ws_ml = nullptr; d.ws_o = nullptr; d.status = status; d.neg_lse = neg_lse;
+    d.ws_ml = nullptr; d.ws_o = nullptr; d.status = status; d.neg_lse = (float*)lse;
     d.sink_tokens = view.sink_tokens; d.local_tokens = view.local_tokens;
     return launch_decode_simt(d, s->dtype, G, st);
 }

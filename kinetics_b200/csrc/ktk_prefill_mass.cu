@@ -55,7 +55,7 @@ prefill_mass_simt_kernel(const PrefillMassParams p, int chunks) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) rows[r][c * 8 + k] = f[k];
         }
-        if (tid < n) row_lse[tid] = p.neg_lse[(int64_t)(s.q0 + tok0 + (r0 + tid) / G) * Hq + h * G + (r0 + tid) % G];
+        if (tid < n) row_lse[tid] = ((const float*)p.lse)[(int64_t)(s.q0 + tok0 + (r0 + tid) / G) * Hq + h * G + (r0 + tid) % G];
         __syncthreads();
         for (int r = 0; r < n; ++r) {
             float dot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -84,7 +84,7 @@ using namespace ktk;
 namespace {
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 size_t lse_bytes(const ktk_shape* s, int64_t total_new) {
-    return up((size_t)total_new * s->num_kv_heads * s->group_size * sizeof(float));
+    return up((size_t)total_new * s->num_kv_heads * s->group_size * (s->dtype == KTK_F32 ? sizeof(float) : 16));
 }
 }  // namespace
 
@@ -113,6 +113,10 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
     if ((rc = check_mass(mass, who)) != KTK_OK || (rc = check_aligned({q, kv_cache, o, workspace}, who)) != KTK_OK ||
         (rc = check_apart(mass->in, mass->out, (size_t)mass->rows * s->num_kv_heads * mass->stride * sizeof(float), who, "mass")) != KTK_OK)
         return rc;
+    if (!(sm_scale != 0.0f && sm_scale - sm_scale == 0.0f)) {
+        set_error("%s: sm_scale %g: finite, and not 0", who, (double)sm_scale);
+        return KTK_ERR_ARG;
+    }
     if (total_new_tokens < 0 || max_new_tokens < 1 || window < 0 || max_pages_per_seq < 1) {
         set_error("%s: total_new_tokens %lld, max_new_tokens %d, window %d, max_pages_per_seq %lld", who,
                   (long long)total_new_tokens, max_new_tokens, window, (long long)max_pages_per_seq);
@@ -130,7 +134,7 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
         set_error("%s: batch * num_kv_heads * max_pages_per_seq exceeds the grid limit", who);
         return KTK_ERR_TOO_LARGE;
     }
-    float* lse = (float*)workspace;
+    void* lse = workspace;
     char* behind = (char*)workspace + lse_bytes(s, total_new_tokens);
     rc = prefill_attention(who, q, q_indptr, total_new_tokens, max_new_tokens, kv_cache, kv_indices, kv_indptr, kv_last_page_len,
                            view_in, sm_scale, o, lse, behind, need - lse_bytes(s, total_new_tokens), KTK_VARIANT_AUTO, s, status, stream);
@@ -139,7 +143,7 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
     p.q = q; p.cache = kv_cache; p.q_indptr = q_indptr; p.kv_indices = kv_indices; p.kv_indptr = kv_indptr;
     p.kv_last_page_len = kv_last_page_len; p.page_count = view.page_count; p.sink_tokens = view.sink_tokens;
     p.batch = s->batch; p.Hkv = s->num_kv_heads; p.G = s->group_size; p.num_pages = s->num_pages; p.total_new = total_new_tokens;
-    p.scale_log2 = sm_scale * kLog2e; p.neg_lse = lse; p.window = window; p.status = status;
+    p.scale_log2 = sm_scale * kLog2e; p.lse = lse; p.window = window; p.status = status;
     p.m.in = mass->in; p.m.out = mass->out; p.m.stride = mass->stride; p.m.rows = mass->rows;
     p.m.slot_index = view.slot_index; p.m.decay = mass->decay;
     cudaStream_t st = (cudaStream_t)stream;

@@ -18,7 +18,7 @@ struct PrefillMassParams {
     int64_t num_pages;
     int64_t total_new;
     float scale_log2;
-    const float* neg_lse;       // [total_new, Hq]: minus log2 of the rows' denominators
+    const void* lse;            // of the rows [total_new, Hq], see prefill_attention (ktk_decode.cuh)
     int window;
     int32_t* status;
     MassParams m;

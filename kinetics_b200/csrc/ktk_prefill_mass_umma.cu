@@ -3,15 +3,18 @@
 // One CTA per (sequence, kv head, 16 pages = 256 keys, part of the rows that see them), two CTAs per SM.  The scores are computed
 // transposed, S^T[128 keys x 64 rows] = K . Q^T, so that a thread holds a key and sums along its own lane of tensor memory: no exchange
 // between threads, and one value per key at the end.  The rows of a tile are the (token, head) pairs of 64 / G new tokens.
+// A row's denominator is the same for all threads; read from shared memory it would take as much of it as the matrix instructions do
+// (a word for each of 32 lanes: 4 cycles per four columns and warp).  So it is one more step of the product: minus lse over the
+// scale, as three bf16 that add up to its 24 bits (written so by the attention kernel), times keys of three ones.
 //
 // Roles of the 320 threads:
 //     warps 0..3, 4..7   exponentials and sums of the first, the second 128 keys
 //     warp 8             matrix instructions: per tile of rows and 128 keys, into one of two buffers of 64 columns each
-//     warp 9             the keys' pages (once), then tiles of queries (TMA) and their rows' denominators, kPmStages in flight
+//     warp 9             TMA: the keys' pages (once), then tiles of queries and their rows' denominators, kPmStages in flight
 // Every wait is bounded.
 //
-// Bound by the exponentials: 1024 cycles of the special-function units (16 a cycle) per 128 keys and 128 rows, 512 to 768 of the tensor
-// cores.  So kPmPoly of every eight pairs are computed by a polynomial on the FMA pipes.
+// Per 128 keys and 128 rows: 1024 cycles of the special-function units (16 exponentials a cycle), 864 of shared memory for the operands
+// (72 per instruction of 64 rows).
 #include "ktk_prefill_mass.cuh"
 #include "ktk_umma.cuh"
 
@@ -25,16 +28,21 @@ constexpr int kPmBlock = kUmRows;                         // keys of a block
 constexpr int kPmRows = 64;                               // rows of a tile
 constexpr int kPmKTile = kPmBlock * 128, kPmQTile = kPmRows * 128;      // [128 keys], [64 rows][64 columns]
 constexpr int kPmStages = 2;
-constexpr int kPmSmem = 2 * 2 * kPmKTile + kPmStages * 2 * kPmQTile + 1024;
+constexpr int kPmOnes = kPmBlock * 16, kPmLse = kPmRows * 16;         // [128 keys], [64 rows][8 columns]: the first 8 of the last step
+constexpr int kPmSmem = 2 * 2 * kPmKTile + kPmStages * (2 * kPmQTile + kPmLse) + 2 * kPmOnes + 1024;
 constexpr int kPmTmemCols = 256;
-constexpr int kPmPoly = 2;
+constexpr int kPmPoly = 1;
 
 struct PmShared {
     uint64_t k, full[kPmStages], empty[kPmStages], s[2][2], s_free[2][2];
     uint32_t tmem;
     int abort;
-    alignas(16) float neg_lse[kPmStages][kPmRows];
 };
+
+// Operand descriptor without a swizzle, K-major: rows of 16 bytes, eight to 128 bytes; `next`: bytes to the next 8 columns
+__device__ __forceinline__ uint64_t umma_desc_rows16(uint32_t saddr, uint32_t next) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)((next >> 4) & 0x3FFFu) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
 
 // first tile of rows, counted from the first counted token, in which some row sees the token in place t
 __device__ __forceinline__ int first_tile(const MassSequence& s, int tpc, int t) {
@@ -107,11 +115,13 @@ __device__ __forceinline__ PmTiles tiles_of(const PrefillMassParams& p, const Ma
 
 __global__ void __launch_bounds__(kPmThreads, 2)
 prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUtensorMap kv_map,
-                         const __grid_constant__ CUtensorMap q_map) {
+                         const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap lse_map) {
     extern __shared__ uint8_t pm_raw[];
     __shared__ __align__(16) PmShared sh;
     uint8_t* k_sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_sm = k_sm + 2 * 2 * kPmKTile;
+    uint8_t* lse_sm = q_sm + kPmStages * 2 * kPmQTile;
+    uint8_t* ones_sm = lse_sm + kPmStages * kPmLse;       // then as many zeros: the other 8 columns of the last step
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     wait_for_front();
     const int h = blockIdx.x % p.Hkv, split = (int)(blockIdx.x / p.Hkv) % p.splits, item = (int)(blockIdx.x / p.Hkv) / p.splits;
@@ -137,10 +147,11 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
         if (lane == 0) {
             prefetch_tensormap(&kv_map);
             prefetch_tensormap(&q_map);
+            prefetch_tensormap(&lse_map);
             mbar_init(&sh.k, 1);
             for (int i = 0; i < kPmStages; ++i) {
-                mbar_init(&sh.full[i], 1 + 32);           // the queries' bytes, every lane's denominators
-                mbar_init(&sh.empty[i], 1 + 8);           // matrix instructions, the warps that read the denominators
+                mbar_init(&sh.full[i], 1);
+                mbar_init(&sh.empty[i], 1);
             }
             for (int i = 0; i < 4; ++i) {
                 mbar_init(&sh.s[i >> 1][i & 1], 1);
@@ -149,6 +160,11 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
             sh.abort = 0;
             mbar_init_fence();
         }
+    } else if (tid < kPmBlock) {
+        const uint4 ones = make_uint4(0x3F803F80u, 0x00003F80u, 0u, 0u);
+        *reinterpret_cast<uint4*>(ones_sm + tid * 16) = ones;
+        *reinterpret_cast<uint4*>(ones_sm + kPmOnes + tid * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async();
     }
     tc_fence_before();
     __syncthreads();
@@ -174,38 +190,33 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
             tma_load_3d(dst + kPmKTile, &kv_map, &sh.k, 64, h, z);
         }
         __syncwarp();
-        const int shift = 31 - __clz(G);              // 1, 2, 4 or 8
-        bool alive = true;
-        for (int i = t_begin; i < t_end; ++i, ++issued) {
-            const int st = issued % kPmStages, tok0 = s.counted + i * tpc;
-            if (issued >= kPmStages) alive = mbar_wait_all(&sh.empty[st], ((issued / kPmStages) - 1) & 1, &sh.abort);
-            if (!alive) break;
-#pragma unroll
-            for (int k = 0; k < kPmRows / 32; ++k) {
-                const int r = k * 32 + lane, tok = tok0 + (r >> shift);
-                const float* src = p.neg_lse + ((int64_t)(s.q0 + tok) * Hq + h * G + (r & (G - 1)));
-                const bool row = tok < s.n_new;
-                cp_async4(smem_u32(&sh.neg_lse[st][r]), row ? src : p.neg_lse, row ? 4 : 0);
-            }
-            cp_async_arrive(&sh.full[st]);
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&sh.full[st], 2 * kPmQTile);
+        if (lane == 0) {
+            bool alive = true;
+            for (int i = t_begin; i < t_end; ++i, ++issued) {
+                const int st = issued % kPmStages, token = s.q0 + s.counted + i * tpc;
+                if (issued >= kPmStages) alive = mbar_wait_fast(&sh.empty[st], ((issued / kPmStages) - 1) & 1, &sh.abort);
+                if (!alive) break;
                 uint8_t* dst = q_sm + st * 2 * kPmQTile;
-                tma_load_3d(dst, &q_map, &sh.full[st], 0, h * G, s.q0 + tok0);
-                tma_load_3d(dst + kPmQTile, &q_map, &sh.full[st], 64, h * G, s.q0 + tok0);
+                mbar_arrive_expect_tx(&sh.full[st], 2 * kPmQTile + kPmLse);
+                tma_load_3d(dst, &q_map, &sh.full[st], 0, h * G, token);
+                tma_load_3d(dst + kPmQTile, &q_map, &sh.full[st], 64, h * G, token);
+                tma_load_3d(lse_sm + st * kPmLse, &lse_map, &sh.full[st], 0, h * G, token);
             }
-            __syncwarp();
         }
+        __syncwarp();
     } else if (warp == 8) {
         // ---------------- matrix instructions ----------------
         const uint32_t tmem = sh.tmem, idesc = umma_idesc(kPmRows, false);
         const uint64_t k_desc = umma_desc(smem_u32(k_sm), 0, 1024), q_desc = umma_desc(smem_u32(q_sm), 0, 1024);
+        const uint64_t ones_desc = umma_desc_rows16(smem_u32(ones_sm), kPmOnes);
         bool alive = mbar_wait_all(&sh.k, 0, &sh.abort);
         for (int i = t_begin; i < t_end && alive; ++i) {
             const int n = i - t_begin, st = n % kPmStages;
             alive = mbar_wait_all(&sh.full[st], (n / kPmStages) & 1, &sh.abort);
             tc_fence_after();
             const uint64_t qb = umma_desc_at(q_desc, st * 2 * kPmQTile);
+            const uint32_t lse_at = smem_u32(lse_sm + st * kPmLse);
+            const uint64_t lse_desc = umma_desc_rows16(lse_at, smem_u32(ones_sm + kPmOnes) - lse_at);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 if (!alive || i < begin[m]) continue;
@@ -223,6 +234,8 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
                         for (int x = 0; x < 4; ++x)
                             umma_f16(tmem + m * 128 + (j & 1) * kPmRows, umma_desc_at(ka, c * kPmKTile + x * 32),
                                      umma_desc_at(qb, c * kPmQTile + x * 32), idesc, (c > 0 || x > 0) ? 1u : 0u);
+                    // last: what was added before is rounded to the size of a score, not of lse
+                    umma_f16(tmem + m * 128 + (j & 1) * kPmRows, ones_desc, lse_desc, idesc, 1u);
                     umma_commit(&sh.s[m][j & 1]);
                 }
                 __syncwarp();
@@ -241,59 +254,45 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
         const uint64_t c2 = pack2(p.scale_log2, p.scale_log2);
         float total = 0.0f, lost = 0.0f;                  // the sum, and what its rounding lost
         bool alive = true;
-        for (int i = t_begin; i < t_end && alive; ++i) {
-            const int n = i - t_begin, st = n % kPmStages;
-            alive = mbar_wait_all(&sh.full[st], (n / kPmStages) & 1, &sh.abort);
+        for (int i = begin[m]; i < t_end; ++i) {
+            const int j = i - begin[m], tok0 = s.counted + i * tpc;
+            alive = mbar_wait_all(&sh.s[m][j & 1], (j >> 1) & 1, &sh.abort);
             if (!alive) break;
-            if (i >= begin[m]) {
-                const int j = i - begin[m];
-                alive = mbar_wait_all(&sh.s[m][j & 1], (j >> 1) & 1, &sh.abort);
-                if (!alive) break;
-                tc_fence_after();
-                const int tok0 = s.counted + i * tpc;
-                // columns that see the key, and those that are rows at all
-                const int c_lo = (t - s.base_pos - tok0) * G, c_hi = (s.n_new - tok0) * G;
-                const bool cut = s.base_pos + tok0 < t_last || c_hi < kPmRows;             // uniform for the block
-                uint64_t acc[4] = {0, 0, 0, 0};
-                float v[2][32];
-                tmem_ld64(my + (j & 1) * kPmRows, v[0], v[1]);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.s_free[m][j & 1]);
-                const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(sh.neg_lse[st]);
-                auto sum = [&](auto masked) {
-#pragma unroll
-                    for (int c = 0; c < kPmRows; c += 4) {
-                        const ulonglong2 l = nl[c / 4];
-#pragma unroll
-                        for (int k = 0; k < 4; k += 2) {
-                            const int col = c + k, pair = col / 2 % 8;
-                            float x, y;
-                            unpack2(fma2(pack2(v[col / 32][col % 32], v[col / 32][col % 32 + 1]), c2, k == 0 ? l.x : l.y), x, y);
-                            if (pair * kPmPoly % 8 + kPmPoly > 7) {      // kPmPoly of eight, evenly spread
-                                exp2_poly(x, y);
-                            } else {
-                                x = ex2(x);
-                                y = ex2(y);
-                            }
-                            if (masked) {
-                                x = col >= c_lo && col < c_hi ? x : 0.0f;
-                                y = col + 1 >= c_lo && col + 1 < c_hi ? y : 0.0f;
-                            }
-                            acc[col / 2 % 4] = add2(acc[col / 2 % 4], pack2(x, y));
-                        }
-                    }
-                };
-                if (cut) sum(std::true_type{});
-                else sum(std::false_type{});
-                float a, c;
-                unpack2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), a, c);
-                const float x = a + c - lost, y = total + x;
-                lost = (y - total) - x;
-                total = y;
-            }
+            tc_fence_after();
+            float v[2][32];
+            tmem_ld64(my + (j & 1) * kPmRows, v[0], v[1]);
+            tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.empty[st]);
+            if (lane == 0) mbar_arrive(&sh.s_free[m][j & 1]);
+            // columns that see the key, and those that are rows at all
+            const int c_lo = (t - s.base_pos - tok0) * G, c_hi = (s.n_new - tok0) * G;
+            uint64_t acc[4] = {0, 0, 0, 0};
+            auto sum = [&](auto masked) {
+#pragma unroll
+                for (int col = 0; col < kPmRows; col += 2) {
+                    const int pair = col / 2 % 8;
+                    float x, y;
+                    unpack2(mul2(pack2(v[col / 32][col % 32], v[col / 32][col % 32 + 1]), c2), x, y);
+                    if (pair * kPmPoly % 8 + kPmPoly > 7) {              // kPmPoly of eight, evenly spread
+                        exp2_poly(x, y);
+                    } else {
+                        x = ex2(x);
+                        y = ex2(y);
+                    }
+                    if (masked) {
+                        x = col >= c_lo && col < c_hi ? x : 0.0f;
+                        y = col + 1 >= c_lo && col + 1 < c_hi ? y : 0.0f;
+                    }
+                    acc[col / 2 % 4] = add2(acc[col / 2 % 4], pack2(x, y));
+                }
+            };
+            if (s.base_pos + tok0 < t_last || c_hi < kPmRows) sum(std::true_type{});      // uniform for the block
+            else sum(std::false_type{});
+            float a, c;
+            unpack2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), a, c);
+            const float x = a + c - lost, y = total + x;
+            lost = (y - total) - x;
+            total = y;
         }
         if (alive && on) {
             if (p.splits > 1) {
@@ -360,7 +359,7 @@ int launch_prefill_mass_umma(const PrefillMassParams& p, int64_t groups, cudaStr
     const char* who = "ktk_prefill_attention_mass";
     DecodeParams d{};                                     // only what the tensor map needs
     d.cache = p.cache; d.Hkv = p.Hkv; d.num_pages = p.num_pages;
-    CUtensorMap kv_map, q_map;
+    CUtensorMap kv_map, q_map, lse_map;
     int rc = make_kv_tensor_map(&kv_map, d);
     if (rc != KTK_OK) return rc;
     const uint64_t Hq = (uint64_t)p.Hkv * p.G;
@@ -369,13 +368,19 @@ int launch_prefill_mass_umma(const PrefillMassParams& p, int64_t groups, cudaStr
     const uint32_t box[3] = {64, (uint32_t)p.G, (uint32_t)(kPmRows / p.G)};
     rc = make_tensor_map_3d(&q_map, p.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, who);
     if (rc != KTK_OK) return rc;
+    const uint64_t lse_dims[3] = {8, Hq, (uint64_t)p.total_new}, lse_strides[2] = {16, Hq * 16};
+    const uint32_t lse_box[3] = {8, (uint32_t)p.G, (uint32_t)(kPmRows / p.G)};
+    rc = make_tensor_map_3d(&lse_map, p.lse, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, lse_dims, lse_strides, lse_box, CU_TENSOR_MAP_SWIZZLE_NONE,
+                            who);
+    if (rc != KTK_OK) return rc;
     const int64_t units = groups * p.Hkv;
     if (units * p.splits > 2147483647LL) {
         set_error("%s: num_kv_heads * tokens exceed the grid limit", who);
         return KTK_ERR_TOO_LARGE;
     }
     KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_mass_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem), who);
-    KTK_CUDA_TRY(launch_behind(false, prefill_mass_umma_kernel, (unsigned)(units * p.splits), kPmThreads, kPmSmem, st, p, kv_map, q_map), who);
+    KTK_CUDA_TRY(launch_behind(false, prefill_mass_umma_kernel, (unsigned)(units * p.splits), kPmThreads, kPmSmem, st, p, kv_map, q_map,
+                               lse_map), who);
     if (p.splits > 1)
         KTK_CUDA_TRY(launch_behind(true, prefill_mass_add_kernel, (unsigned)units, 2 * kPmBlock, 0, st, p), who);
     return KTK_OK;

@@ -215,7 +215,11 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
         const bool done = fl.softmax<false>(tile, p.scale_log2, m_ref, l_run, prepare, [](float&, float&) {}, clear);
         if (done && fl.blocks_of(tile) > 0) {
             const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-            if (p.neg_lse != nullptr && row_on) p.neg_lse[(int64_t)(q0 + my_tok) * Hq + my_head] = -(m_ref + log2f(l_run));
+            if (p.lse != nullptr && row_on) {
+                const float v = -(m_ref + log2f(l_run)) / p.scale_log2;
+                const float hi = __bfloat162float(__float2bfloat16_rn(v)), mid = __bfloat162float(__float2bfloat16_rn(v - hi));
+                p.lse[(int64_t)(q0 + my_tok) * Hq + my_head] = make_uint4(pack_bf16(hi, mid), pack_bf16(v - hi - mid, 0.0f), 0u, 0u);
+            }
             const uint32_t o_at = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16) + kFlColO + tile * 128;
             __nv_bfloat16* dst = (__nv_bfloat16*)p.o + ((int64_t)(q0 + (row_on ? my_tok : 0)) * Hq + my_head) * kHeadDim;
 #pragma unroll

@@ -21,7 +21,7 @@ struct PrefillUmmaParams {
     int64_t num_pages;
     float scale_log2;
     int32_t* status;
-    float* neg_lse = nullptr;  // non-null: [total_new, Hq], minus log2 of the softmax's denominators
+    uint4* lse = nullptr;      // non-null: [total_new, Hq], see prefill_attention (ktk_decode.cuh)
 };
 
 int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st);
