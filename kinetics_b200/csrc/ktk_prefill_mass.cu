@@ -6,74 +6,84 @@
 
 namespace ktk {
 
-constexpr int kPsKeys = 128;    // keys of a CTA, one per thread
-constexpr int kPsRows = 32;     // rows of a stage
+constexpr int kPsKeys = 64, kPsRows = 64;     // keys of a CTA, rows of a tile
+constexpr int kPsThreads = 256;               // 16 x 16, four keys and four rows each
+constexpr int kPsDims = 32;                   // dimensions of a stage
+constexpr int kPsLd = kPsKeys + 4;            // floats between dimensions in shared memory (16-byte aligned, writes spread over banks)
 
-// One CTA per (sequence, kv head, 128 keys): a thread holds a key and walks the rows that see it.
-__global__ void __launch_bounds__(kPsKeys)
+// One CTA per (sequence, kv head, 64 keys): tiles of 64 rows against its keys, 32 dimensions at a time through shared memory
+// ([dimension][key or row]), four by four products in registers.  FMA-bound: 4096 cycles per tile and SM.
+__global__ void __launch_bounds__(kPsThreads)
 prefill_mass_simt_kernel(const PrefillMassParams p, int chunks) {
-    __shared__ __align__(16) float rows[kPsRows][kHeadDim];
-    __shared__ float row_lse[kPsRows];
+    __shared__ __align__(16) float keys[kPsDims][kPsLd], rows[kPsDims][kPsLd];
+    __shared__ float row_lse[kPsRows], sums[16][kPsKeys];
     wait_for_front();
     const int64_t unit = blockIdx.x / chunks;
-    const int part = (int)(blockIdx.x % chunks), tid = threadIdx.x;
+    const int part = (int)(blockIdx.x % chunks), tid = threadIdx.x, tk = tid % 16, tr = tid / 16;
     const int b = (int)(unit / p.Hkv), h = (int)(unit % p.Hkv), G = p.G, Hq = p.Hkv * G;
     MassSequence s;
     if (!mass_sequence(p, b, part == 0 && h == 0, s)) return;
-    const int t0 = part * kPsKeys, t = t0 + tid;
+    const int t0 = part * kPsKeys;
     if (t0 >= s.sp.total) return;
-    float key[kHeadDim];
-    bool on = t < s.sp.total;
-    if (on) {
+    // a thread brings a quarter of a key's and of a row's dimensions of a stage: 8 floats
+    const int mine = tid / 4, quarter = tid % 4 * 8;
+    const float* key = nullptr;
+    if (t0 + mine < s.sp.total) {
         int e, slot;
-        page_of_pos(t, s.sp.first_fill, e, slot);
+        page_of_pos(t0 + mine, s.sp.first_fill, e, slot);
         const int64_t page = p.kv_indices[s.sp.start + e];
-        if (page < 0 || page >= p.num_pages) {
-            report(p.status, KTK_STATUS_BAD_PAGE);
-            on = false;
-        } else {
-            const float* src = (const float*)p.cache + ((page * 2 * kPageSize + slot) * p.Hkv + h) * kHeadDim;
-#pragma unroll
-            for (int i = 0; i < kHeadDim; i += 8) load8(src + i, *reinterpret_cast<float(*)[8]>(key + i));
-        }
-    }
-    if (!on) {
-#pragma unroll
-        for (int i = 0; i < kHeadDim; ++i) key[i] = 0.0f;
+        if (page < 0 || page >= p.num_pages) report(p.status, KTK_STATUS_BAD_PAGE);
+        else key = (const float*)p.cache + ((page * 2 * kPageSize + slot) * p.Hkv + h) * kHeadDim;
     }
     // tokens that are counted and see the chunk's first key
-    const int tok0 = max(s.counted, t0 - s.base_pos);
-    const int n_rows = (s.n_new - tok0) * G;
-    float sum = 0.0f;
+    const int tok0 = max(s.counted, t0 - s.base_pos), n_rows = (s.n_new - tok0) * G;
+    float sum[4] = {};
     for (int r0 = 0; r0 < n_rows; r0 += kPsRows) {
-        const int n = n_rows - r0 < kPsRows ? n_rows - r0 : kPsRows;
-        __syncthreads();
-        for (int i = tid; i < n * (kHeadDim / 8); i += kPsKeys) {
-            const int r = i / (kHeadDim / 8), c = i % (kHeadDim / 8), tok = tok0 + (r0 + r) / G, g = (r0 + r) % G;
-            float f[8];
-            load8((const float*)p.q + ((int64_t)(s.q0 + tok) * Hq + h * G + g) * kHeadDim + c * 8, f);
+        const int r = r0 + mine;
+        const float* row = r < n_rows ? (const float*)p.q + ((int64_t)(s.q0 + tok0 + r / G) * Hq + h * G + r % G) * kHeadDim : nullptr;
+        float dot[4][4] = {};                     // [row][key]
+        for (int d0 = 0; d0 < kHeadDim; d0 += kPsDims) {
+            float kv[8] = {}, qv[8] = {};
+            if (key) load8(key + d0 + quarter, kv);
+            if (row) load8(row + d0 + quarter, qv);
+            __syncthreads();
 #pragma unroll
-            for (int k = 0; k < 8; ++k) rows[r][c * 8 + k] = f[k];
-        }
-        if (tid < n) row_lse[tid] = ((const float*)p.lse)[(int64_t)(s.q0 + tok0 + (r0 + tid) / G) * Hq + h * G + (r0 + tid) % G];
-        __syncthreads();
-        for (int r = 0; r < n; ++r) {
-            float dot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < kHeadDim; i += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(&rows[r][i]);
-                dot[0] = fmaf(v.x, key[i], dot[0]);
-                dot[1] = fmaf(v.y, key[i + 1], dot[1]);
-                dot[2] = fmaf(v.z, key[i + 2], dot[2]);
-                dot[3] = fmaf(v.w, key[i + 3], dot[3]);
+            for (int i = 0; i < 8; ++i) {
+                keys[quarter + i][mine] = kv[i];
+                rows[quarter + i][mine] = qv[i];
             }
-            const float x = (dot[0] + dot[1]) + (dot[2] + dot[3]);
-            if (t <= s.base_pos + tok0 + (r0 + r) / G) sum += exp2f(x * p.scale_log2 + row_lse[r]);
+            if (d0 == 0 && tid < kPsRows)
+                row_lse[tid] = r0 + tid < n_rows ? ((const float*)p.lse)[(int64_t)(s.q0 + tok0 + (r0 + tid) / G) * Hq + h * G + (r0 + tid) % G] : 0.0f;
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < kPsDims; ++d) {
+                const float4 k4 = *reinterpret_cast<const float4*>(&keys[d][tk * 4]), q4 = *reinterpret_cast<const float4*>(&rows[d][tr * 4]);
+                const float k[4] = {k4.x, k4.y, k4.z, k4.w}, q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) dot[i][j] = fmaf(q[i], k[j], dot[i][j]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = r0 + tr * 4 + i, sees = at < n_rows ? s.base_pos + tok0 + at / G : -1;
+            const float lse = row_lse[tr * 4 + i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (t0 + tk * 4 + j <= sees) sum[j] += exp2f(fmaf(dot[i][j], p.scale_log2, lse));
         }
     }
-    if (on) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[tr][tk * 4 + j] = sum[j];
+    __syncthreads();
+    if (tid < kPsKeys && t0 + tid < s.sp.total) {
+        const int t = t0 + tid;
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) total += sums[i][tid];
         const int64_t at = ((int64_t)s.row * p.Hkv + h) * p.m.stride + t;
-        p.m.out[at] = t >= s.base_pos ? sum : fmaf(p.m.decay, p.m.in[at], sum);
+        p.m.out[at] = t >= s.base_pos ? total : fmaf(p.m.decay, p.m.in[at], total);
     }
 }
 
@@ -153,6 +163,6 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
         p.partial = (float*)behind;
         return launch_prefill_mass_umma(p, plan.groups, st);
     }
-    KTK_CUDA_TRY(launch_behind(false, prefill_mass_simt_kernel, (unsigned)ctas, kPsKeys, 0, st, p, (int)chunks), who);
+    KTK_CUDA_TRY(launch_behind(false, prefill_mass_simt_kernel, (unsigned)ctas, kPsThreads, 0, st, p, (int)chunks), who);
     return KTK_OK;
 }

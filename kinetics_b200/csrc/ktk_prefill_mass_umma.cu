@@ -7,14 +7,18 @@
 // (a word for each of 32 lanes: 4 cycles per four columns and warp).  So it is one more step of the product: minus lse over the
 // scale, as three bf16 that add up to its 24 bits (written so by the attention kernel), times keys of three ones.
 //
+// The keys go on to tensor memory, an instruction's other operand then is all that it reads from shared memory: 32 cycles for 64 rows,
+// 48 with the keys there.
+//
 // Roles of the 320 threads:
-//     warps 0..3, 4..7   exponentials and sums of the first, the second 128 keys
-//     warp 8             matrix instructions: per tile of rows and 128 keys, into one of two buffers of 64 columns each
-//     warp 9             TMA: the keys' pages (once), then tiles of queries and their rows' denominators, kPmStages in flight
+//     warps 0..3, 4..7   the first, the second 128 keys to tensor memory; exponentials and sums
+//     warp 8             matrix instructions: per tile of rows and 128 keys, as soon as the last tile's scores are in registers
+//     warp 9             TMA: the keys' pages (once), then tiles of queries and their rows' denominators, kPmStages in flight, all but the
+//                        first kPmFirst of them where the keys were
 // Every wait is bounded.
 //
-// Per 128 keys and 128 rows: 1024 cycles of the special-function units (16 exponentials a cycle), 864 of shared memory for the operands
-// (72 per instruction of 64 rows).
+// Per 128 keys and 128 rows: 1024 cycles of the special-function units (16 exponentials a cycle) without kPmPoly, some 600 of the tensor
+// cores.
 #include "ktk_prefill_mass.cuh"
 #include "ktk_umma.cuh"
 
@@ -27,14 +31,16 @@ constexpr int kPmPages = 8;                               // of 128 keys
 constexpr int kPmBlock = kUmRows;                         // keys of a block
 constexpr int kPmRows = 64;                               // rows of a tile
 constexpr int kPmKTile = kPmBlock * 128, kPmQTile = kPmRows * 128;      // [128 keys], [64 rows][64 columns]
-constexpr int kPmStages = 2;
 constexpr int kPmOnes = kPmBlock * 16, kPmLse = kPmRows * 16;         // [128 keys], [64 rows][8 columns]: the first 8 of the last step
-constexpr int kPmSmem = 2 * 2 * kPmKTile + kPmStages * (2 * kPmQTile + kPmLse) + 2 * kPmOnes + 1024;
-constexpr int kPmTmemCols = 256;
-constexpr int kPmPoly = 1;
+constexpr int kPmStage = 2 * kPmQTile + kPmLse;
+constexpr int kPmFirst = 2, kPmStages = 5;
+static_assert((kPmStages - kPmFirst) * kPmStage <= 4 * kPmKTile, "stages where the keys were");
+constexpr int kPmSmem = 4 * kPmKTile + kPmFirst * kPmStage + 2 * kPmOnes + 1024;
+constexpr int kPmTmemCols = 256, kPmColS = 128;          // keys m at column 64 m, scores m at 128 + 64 m
+constexpr int kPmPoly = 2;
 
 struct PmShared {
-    uint64_t k, full[kPmStages], empty[kPmStages], s[2][2], s_free[2][2];
+    uint64_t k, k_moved, full[kPmStages], empty[kPmStages], s[2], s_free[2];
     uint32_t tmem;
     int abort;
 };
@@ -119,9 +125,9 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
     extern __shared__ uint8_t pm_raw[];
     __shared__ __align__(16) PmShared sh;
     uint8_t* k_sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pm_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* q_sm = k_sm + 2 * 2 * kPmKTile;
-    uint8_t* lse_sm = q_sm + kPmStages * 2 * kPmQTile;
-    uint8_t* ones_sm = lse_sm + kPmStages * kPmLse;       // then as many zeros: the other 8 columns of the last step
+    uint8_t* first_sm = k_sm + 4 * kPmKTile;
+    uint8_t* ones_sm = first_sm + kPmFirst * kPmStage;    // then as many zeros: the other 8 columns of the last step
+    const auto stage = [&](int st) { return st < kPmFirst ? first_sm + st * kPmStage : k_sm + (st - kPmFirst) * kPmStage; };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     wait_for_front();
     const int h = blockIdx.x % p.Hkv, split = (int)(blockIdx.x / p.Hkv) % p.splits, item = (int)(blockIdx.x / p.Hkv) / p.splits;
@@ -153,9 +159,10 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
                 mbar_init(&sh.full[i], 1);
                 mbar_init(&sh.empty[i], 1);
             }
-            for (int i = 0; i < 4; ++i) {
-                mbar_init(&sh.s[i >> 1][i & 1], 1);
-                mbar_init(&sh.s_free[i >> 1][i & 1], 4);
+            mbar_init(&sh.k_moved, 8);
+            for (int m = 0; m < 2; ++m) {
+                mbar_init(&sh.s[m], 1);
+                mbar_init(&sh.s_free[m], 4);
             }
             sh.abort = 0;
             mbar_init_fence();
@@ -194,49 +201,49 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
             bool alive = true;
             for (int i = t_begin; i < t_end; ++i, ++issued) {
                 const int st = issued % kPmStages, token = s.q0 + s.counted + i * tpc;
-                if (issued >= kPmStages) alive = mbar_wait_fast(&sh.empty[st], ((issued / kPmStages) - 1) & 1, &sh.abort);
+                if (issued == kPmFirst) alive = mbar_wait_fast(&sh.k_moved, 0, &sh.abort);
+                if (issued >= kPmStages) alive = alive && mbar_wait_fast(&sh.empty[st], ((issued / kPmStages) - 1) & 1, &sh.abort);
                 if (!alive) break;
-                uint8_t* dst = q_sm + st * 2 * kPmQTile;
-                mbar_arrive_expect_tx(&sh.full[st], 2 * kPmQTile + kPmLse);
+                uint8_t* dst = stage(st);
+                mbar_arrive_expect_tx(&sh.full[st], kPmStage);
                 tma_load_3d(dst, &q_map, &sh.full[st], 0, h * G, token);
                 tma_load_3d(dst + kPmQTile, &q_map, &sh.full[st], 64, h * G, token);
-                tma_load_3d(lse_sm + st * kPmLse, &lse_map, &sh.full[st], 0, h * G, token);
+                tma_load_3d(dst + 2 * kPmQTile, &lse_map, &sh.full[st], 0, h * G, token);
             }
         }
         __syncwarp();
     } else if (warp == 8) {
         // ---------------- matrix instructions ----------------
         const uint32_t tmem = sh.tmem, idesc = umma_idesc(kPmRows, false);
-        const uint64_t k_desc = umma_desc(smem_u32(k_sm), 0, 1024), q_desc = umma_desc(smem_u32(q_sm), 0, 1024);
-        const uint64_t ones_desc = umma_desc_rows16(smem_u32(ones_sm), kPmOnes);
-        bool alive = mbar_wait_all(&sh.k, 0, &sh.abort);
+        const uint64_t q_desc = umma_desc(smem_u32(k_sm), 0, 1024), ones_desc = umma_desc_rows16(smem_u32(ones_sm), kPmOnes);
+        bool alive = mbar_wait_all(&sh.k_moved, 0, &sh.abort);
         for (int i = t_begin; i < t_end && alive; ++i) {
             const int n = i - t_begin, st = n % kPmStages;
             alive = mbar_wait_all(&sh.full[st], (n / kPmStages) & 1, &sh.abort);
             tc_fence_after();
-            const uint64_t qb = umma_desc_at(q_desc, st * 2 * kPmQTile);
-            const uint32_t lse_at = smem_u32(lse_sm + st * kPmLse);
+            const uint64_t qb = umma_desc_at(q_desc, (uint32_t)(stage(st) - k_sm));
+            const uint32_t lse_at = smem_u32(stage(st) + 2 * kPmQTile);
             const uint64_t lse_desc = umma_desc_rows16(lse_at, smem_u32(ones_sm + kPmOnes) - lse_at);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 if (!alive || i < begin[m]) continue;
                 const int j = i - begin[m];
-                if (j >= 2) {
-                    alive = mbar_wait_all(&sh.s_free[m][j & 1], ((j >> 1) - 1) & 1, &sh.abort);
+                if (j > 0) {
+                    alive = mbar_wait_all(&sh.s_free[m], (j - 1) & 1, &sh.abort);
                     tc_fence_after();
                     if (!alive) continue;
                 }
                 if (elect_one()) {
-                    const uint64_t ka = umma_desc_at(k_desc, m * 2 * kPmKTile);
+                    const uint32_t to = tmem + kPmColS + m * kPmRows;
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
-                            umma_f16(tmem + m * 128 + (j & 1) * kPmRows, umma_desc_at(ka, c * kPmKTile + x * 32),
-                                     umma_desc_at(qb, c * kPmQTile + x * 32), idesc, (c > 0 || x > 0) ? 1u : 0u);
+                            umma_f16_ts(to, tmem + m * 64 + c * 32 + x * 8, umma_desc_at(qb, c * kPmQTile + x * 32), idesc,
+                                        (c > 0 || x > 0) ? 1u : 0u);
                     // last: what was added before is rounded to the size of a score, not of lse
-                    umma_f16(tmem + m * 128 + (j & 1) * kPmRows, ones_desc, lse_desc, idesc, 1u);
-                    umma_commit(&sh.s[m][j & 1]);
+                    umma_f16(to, ones_desc, lse_desc, idesc, 1u);
+                    umma_commit(&sh.s[m]);
                 }
                 __syncwarp();
             }
@@ -250,20 +257,35 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
         const bool on = e < s.sp.n_pages && slot < (e == s.sp.n_pages - 1 ? s.sp.last_fill : (e == 0 ? s.sp.first_fill : kPageSize));
         const int t = page_first_pos(e, s.sp.first_fill) + slot;
         const int t_last = page_first_pos(e0 + (m + 1) * kPmPages, s.sp.first_fill);      // behind the block's last key
-        const uint32_t my = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16) + m * 128;
+        const uint32_t my = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint64_t c2 = pack2(p.scale_log2, p.scale_log2);
         float total = 0.0f, lost = 0.0f;                  // the sum, and what its rounding lost
-        bool alive = true;
-        for (int i = begin[m]; i < t_end; ++i) {
+        bool alive = mbar_wait_all(&sh.k, 0, &sh.abort);
+        if (alive) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {                 // a row of 64 columns, two to a word
+                uint32_t w[32];
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    *reinterpret_cast<uint4*>(w + 4 * x) = *reinterpret_cast<const uint4*>(k_sm + (2 * m + c) * kPmKTile + swz(key, x));
+                tmem_st32_u32(my + m * 64 + c * 32, w);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            fence_proxy_async();                          // TMA writes there next
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.k_moved);
+        }
+        for (int i = begin[m]; i < t_end && alive; ++i) {
             const int j = i - begin[m], tok0 = s.counted + i * tpc;
-            alive = mbar_wait_all(&sh.s[m][j & 1], (j >> 1) & 1, &sh.abort);
+            alive = mbar_wait_all(&sh.s[m], j & 1, &sh.abort);
             if (!alive) break;
             tc_fence_after();
             float v[2][32];
-            tmem_ld64(my + (j & 1) * kPmRows, v[0], v[1]);
+            tmem_ld64(my + kPmColS + m * kPmRows, v[0], v[1]);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.s_free[m][j & 1]);
+            if (lane == 0) mbar_arrive(&sh.s_free[m]);
             // columns that see the key, and those that are rows at all
             const int c_lo = (t - s.base_pos - tok0) * G, c_hi = (s.n_new - tok0) * G;
             uint64_t acc[4] = {0, 0, 0, 0};
