@@ -2,89 +2,142 @@
 //     mass'[r, h, t] = decay mass[r, h, t] + sum over (token, head) rows of 2^(s_row(t) - lse_row)
 // The attention itself is that of ktk_prefill.cu, which writes the rows' denominators down; the weights are then summed by keys: bf16
 // in ktk_prefill_mass_umma.cu, fp32 here.
+#include <cooperative_groups.h>
+
 #include "ktk_prefill_mass.cuh"
 
 namespace ktk {
 
-constexpr int kPsKeys = 64, kPsRows = 64;     // keys of a CTA, rows of a tile
-constexpr int kPsThreads = 256;               // 16 x 16, four keys and four rows each
-constexpr int kPsDims = 32;                   // dimensions of a stage
-constexpr int kPsLd = kPsKeys + 4;            // floats between dimensions in shared memory (16-byte aligned, writes spread over banks)
+constexpr int kPsKeys = 32, kPsRows = 64;     // keys of a CTA, rows of a tile
+constexpr int kPsThreads = 128;               // 8 x 16, four keys and four rows each
+constexpr int kPsLd = kHeadDim + 4;           // floats between keys or rows in shared memory: eight of them lie in different banks
+constexpr int kPsSmem = (kPsKeys + 2 * kPsRows) * kPsLd * 4;
 
-// One CTA per (sequence, kv head, 64 keys): tiles of 64 rows against its keys, 32 dimensions at a time through shared memory
-// ([dimension][key or row]), four by four products in registers.  FMA-bound: 4096 cycles per tile and SM.
+// One CTA per (sequence, kv head, 32 keys), its keys and two tiles of 64 rows in shared memory: a tile is multiplied, four by four
+// products in a thread's registers, while the next one comes.  Bound by shared memory: 32 cycles per dimension and tile.  Stages of 32
+// dimensions instead of whole tiles were bound by the loads' latency, 2 us each.
+// Where that leaves SMs idle, a cluster of CTAs takes the tiles in turn and its first one adds the sums.
 __global__ void __launch_bounds__(kPsThreads)
-prefill_mass_simt_kernel(const PrefillMassParams p, int chunks) {
-    __shared__ __align__(16) float keys[kPsDims][kPsLd], rows[kPsDims][kPsLd];
-    __shared__ float row_lse[kPsRows], sums[16][kPsKeys];
+prefill_mass_simt_kernel(const PrefillMassParams p, int chunks, int cluster) {
+    extern __shared__ __align__(16) float ps_smem[];
+    __shared__ float sums[kPsThreads / 8][kPsKeys], totals[kPsKeys];
+    float* keys = ps_smem;                        // [key][kPsLd], then [tile][row][kPsLd]
     wait_for_front();
-    const int64_t unit = blockIdx.x / chunks;
-    const int part = (int)(blockIdx.x % chunks), tid = threadIdx.x, tk = tid % 16, tr = tid / 16;
-    const int b = (int)(unit / p.Hkv), h = (int)(unit % p.Hkv), G = p.G, Hq = p.Hkv * G;
+    const int64_t item = blockIdx.x / cluster, unit = item / chunks;
+    const int part = (int)(item % chunks), rank = (int)(blockIdx.x % cluster), tid = threadIdx.x, tk = tid % 8, tr = tid / 8;
+    const int b = (int)(unit / p.Hkv), h = (int)(unit % p.Hkv), G = p.G, Hq = p.Hkv * G, shift = 31 - __clz(G);    // 1, 2, 4 or 8
     MassSequence s;
-    if (!mass_sequence(p, b, part == 0 && h == 0, s)) return;
+    if (!mass_sequence(p, b, part == 0 && h == 0 && rank == 0, s)) return;      // the same for the cluster
     const int t0 = part * kPsKeys;
     if (t0 >= s.sp.total) return;
-    // a thread brings a quarter of a key's and of a row's dimensions of a stage: 8 floats
-    const int mine = tid / 4, quarter = tid % 4 * 8;
-    const float* key = nullptr;
-    if (t0 + mine < s.sp.total) {
-        int e, slot;
-        page_of_pos(t0 + mine, s.sp.first_fill, e, slot);
-        const int64_t page = p.kv_indices[s.sp.start + e];
-        if (page < 0 || page >= p.num_pages) report(p.status, KTK_STATUS_BAD_PAGE);
-        else key = (const float*)p.cache + ((page * 2 * kPageSize + slot) * p.Hkv + h) * kHeadDim;
-    }
     // tokens that are counted and see the chunk's first key
     const int tok0 = max(s.counted, t0 - s.base_pos), n_rows = (s.n_new - tok0) * G;
-    float sum[4] = {};
-    for (int r0 = 0; r0 < n_rows; r0 += kPsRows) {
-        const int r = r0 + mine;
-        const float* row = r < n_rows ? (const float*)p.q + ((int64_t)(s.q0 + tok0 + r / G) * Hq + h * G + r % G) * kHeadDim : nullptr;
-        float dot[4][4] = {};                     // [row][key]
-        for (int d0 = 0; d0 < kHeadDim; d0 += kPsDims) {
-            float kv[8] = {}, qv[8] = {};
-            if (key) load8(key + d0 + quarter, kv);
-            if (row) load8(row + d0 + quarter, qv);
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                keys[quarter + i][mine] = kv[i];
-                rows[quarter + i][mine] = qv[i];
-            }
-            if (d0 == 0 && tid < kPsRows)
-                row_lse[tid] = r0 + tid < n_rows ? ((const float*)p.lse)[(int64_t)(s.q0 + tok0 + (r0 + tid) / G) * Hq + h * G + (r0 + tid) % G] : 0.0f;
-            __syncthreads();
-#pragma unroll
-            for (int d = 0; d < kPsDims; ++d) {
-                const float4 k4 = *reinterpret_cast<const float4*>(&keys[d][tk * 4]), q4 = *reinterpret_cast<const float4*>(&rows[d][tr * 4]);
-                const float k[4] = {k4.x, k4.y, k4.z, k4.w}, q[4] = {q4.x, q4.y, q4.z, q4.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) dot[i][j] = fmaf(q[i], k[j], dot[i][j]);
-            }
+    const auto row_of = [&](int r) { return (int64_t)(s.q0 + tok0 + (r >> shift)) * Hq + h * G + (r & (G - 1)); };
+    // a warp brings a key or a row at a time, 16 bytes a lane; places without one get zeros
+    const int warp = tid / 32, lane = tid % 32;
+    for (int k = warp; k < kPsKeys; k += kPsThreads / 32) {
+        const float* src = nullptr;
+        if (t0 + k < s.sp.total) {
+            int e, slot;
+            page_of_pos(t0 + k, s.sp.first_fill, e, slot);
+            const int64_t page = p.kv_indices[s.sp.start + e];
+            if (page < 0 || page >= p.num_pages) report(p.status, KTK_STATUS_BAD_PAGE);
+            else src = (const float*)p.cache + ((page * 2 * kPageSize + slot) * p.Hkv + h) * kHeadDim;
         }
+        cp_async16(smem_u32(keys + k * kPsLd + lane * 4), src ? src + lane * 4 : (const float*)p.cache, src ? 16 : 0);
+    }
+    const auto load_rows = [&](int r0, int tile) {
+        float* rows = keys + (kPsKeys + tile * kPsRows) * kPsLd;
+        for (int r = warp; r < kPsRows; r += kPsThreads / 32) {
+            const bool on = r0 + r < n_rows;
+            cp_async16(smem_u32(rows + r * kPsLd + lane * 4), (const float*)p.q + (on ? row_of(r0 + r) * kHeadDim + lane * 4 : 0), on ? 16 : 0);
+        }
+        cp_async_commit();
+    };
+    load_rows(rank * kPsRows, 0);
+    float sum[4] = {};
+    for (int r0 = rank * kPsRows, tile = 0; r0 < n_rows; r0 += cluster * kPsRows, tile ^= 1) {
+        if (r0 + cluster * kPsRows < n_rows) load_rows(r0 + cluster * kPsRows, tile ^ 1);
+        else cp_async_commit();
+        int sees[4];
+        float lse[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int at = r0 + tr * 4 + i, sees = at < n_rows ? s.base_pos + tok0 + at / G : -1;
-            const float lse = row_lse[tr * 4 + i];
+            const int r = r0 + tr + 16 * i;
+            sees[i] = r < n_rows ? s.base_pos + tok0 + (r >> shift) : -1;
+            lse[i] = r < n_rows ? ((const float*)p.lse)[row_of(r)] : 0.0f;
+        }
+        cp_async_wait<1>();
+        __syncthreads();
+        const float* rows = keys + (kPsKeys + tile * kPsRows) * kPsLd;
+        float dot[4][4] = {};                     // [row tr + 16 i][key tk + 8 j]
+#pragma unroll 4
+        for (int d = 0; d < kHeadDim; d += 4) {
+            float4 k[4], q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(keys + (tk + 8 * j) * kPsLd + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(rows + (tr + 16 * i) * kPsLd + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    dot[i][j] = fmaf(q[i].x, k[j].x, dot[i][j]);
+                    dot[i][j] = fmaf(q[i].y, k[j].y, dot[i][j]);
+                    dot[i][j] = fmaf(q[i].z, k[j].z, dot[i][j]);
+                    dot[i][j] = fmaf(q[i].w, k[j].w, dot[i][j]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (t0 + tk * 4 + j <= sees) sum[j] += exp2f(fmaf(dot[i][j], p.scale_log2, lse));
-        }
+                if (t0 + tk + 8 * j <= sees[i]) sum[j] += exp2f(fmaf(dot[i][j], p.scale_log2, lse[i]));
+        __syncthreads();                          // the tile is free
     }
+    cp_async_wait<0>();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums[tr][tk * 4 + j] = sum[j];
+    for (int j = 0; j < 4; ++j) sums[tr][tk + 8 * j] = sum[j];
     __syncthreads();
-    if (tid < kPsKeys && t0 + tid < s.sp.total) {
-        const int t = t0 + tid;
-        float total = 0.0f;
+    float total = 0.0f;
+    if (tid < kPsKeys) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) total += sums[i][tid];
+        for (int i = 0; i < kPsThreads / 8; ++i) total += sums[i][tid];
+        totals[tid] = total;
+    }
+    if (cluster > 1) {
+        auto cl = cooperative_groups::this_cluster();
+        cl.sync();
+        if (rank == 0 && tid < kPsKeys)
+            for (int i = 1; i < cluster; ++i) total += *cl.map_shared_rank(&totals[tid], i);
+        cl.sync();                                // the others stay until theirs are read
+    }
+    if (rank == 0 && tid < kPsKeys && t0 + tid < s.sp.total) {
+        const int t = t0 + tid;
         const int64_t at = ((int64_t)s.row * p.Hkv + h) * p.m.stride + t;
         p.m.out[at] = t >= s.base_pos ? total : fmaf(p.m.decay, p.m.in[at], total);
     }
+}
+
+static int launch_prefill_mass_simt(const PrefillMassParams& p, int64_t ctas, int chunks, int max_new, cudaStream_t st) {
+    const char* who = "ktk_prefill_attention_mass";
+    const int64_t rows = (int64_t)(p.window > 0 && p.window < max_new ? p.window : max_new) * p.G;
+    int cluster = 1;
+    while (cluster < 8 && ctas * cluster < 2 * sm_count() && rows > (int64_t)kPsRows * cluster) cluster *= 2;
+    KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_mass_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPsSmem), who);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = (unsigned)(ctas * cluster);
+    cfg.blockDim = kPsThreads;
+    cfg.dynamicSmemBytes = kPsSmem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    KTK_CUDA_TRY(cudaLaunchKernelEx(&cfg, prefill_mass_simt_kernel, p, chunks, cluster), who);
+    return KTK_OK;
 }
 
 }  // namespace ktk
@@ -140,7 +193,7 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
         return KTK_ERR_WORKSPACE;
     }
     const int64_t chunks = (max_pages_per_seq * kPageSize + kPsKeys - 1) / kPsKeys, ctas = chunks * s->batch * s->num_kv_heads;
-    if (max_pages_per_seq > (1 << 27) || ctas > 2147483647LL) {
+    if (max_pages_per_seq > (1 << 27) || ctas > 2147483647LL / 8) {
         set_error("%s: batch * num_kv_heads * max_pages_per_seq exceeds the grid limit", who);
         return KTK_ERR_TOO_LARGE;
     }
@@ -163,6 +216,5 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
         p.partial = (float*)behind;
         return launch_prefill_mass_umma(p, plan.groups, st);
     }
-    KTK_CUDA_TRY(launch_behind(false, prefill_mass_simt_kernel, (unsigned)ctas, kPsThreads, 0, st, p, (int)chunks), who);
-    return KTK_OK;
+    return launch_prefill_mass_simt(p, ctas, (int)chunks, max_new_tokens, st);
 }
