@@ -119,7 +119,7 @@ class DecoderStack:
         logits = torch.mm(n, self.lm_head.t())
         if self.logits_dtype is not None:
             logits = logits.to(self.logits_dtype)
-        return logits.view(bsz, seq_len, -1)
+        return logits.view(bsz, seq_len, logits.shape[-1])             # also of no rows: all portions of a prompt but the last
 
     @torch.no_grad()
     def next_tokens(self, input_ids, position_ids, batch_idx, kv, last_only: bool = False):
