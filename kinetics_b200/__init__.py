@@ -16,6 +16,7 @@ from . import ops  # noqa: E402  (registers the torch ops)
 from .config import LayerConfig, get_config  # noqa: E402
 from .layers import BlockTopkDecoderLayer, DecoderLayer, init_weights  # noqa: E402
 from .batch_cache import BatchKVManager  # noqa: E402
+from .evicting_cache import EvictingKVManager  # noqa: E402
 from .engine import Engine, PagePool, PooledKVManager, PoolExhausted  # noqa: E402
 from .decoder_stack import DecoderStack  # noqa: E402
 from .layer_cache import LayeredKVManager  # noqa: E402
@@ -24,5 +25,5 @@ from .munadra import Munadra, MunadraConfig  # noqa: E402
 from .registry import load_model, model_class  # noqa: E402
 
 __all__ = ["ops", "LayerConfig", "get_config", "BlockTopkDecoderLayer", "DecoderLayer", "init_weights",
-           "BatchKVManager", "DecoderStack", "Engine", "Gifetar", "GifetarConfig", "LayeredKVManager", "load_model",
+           "BatchKVManager", "DecoderStack", "Engine", "EvictingKVManager", "Gifetar", "GifetarConfig", "LayeredKVManager", "load_model",
            "model_class", "Munadra", "MunadraConfig", "PagePool", "PooledKVManager", "PoolExhausted"]

@@ -464,6 +464,14 @@ def _same(t, like, what) -> None:
         raise TypeError(f"{what} must have the dtype and shape {like.dtype} {tuple(like.shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
+def decode_mass_workspace_bytes(batch: int, num_kv_heads: int, group_size: int, max_pages_per_seq: int, dtype=torch.bfloat16,
+                                total_pages: int = -1) -> int:
+    """Bytes of workspace that ``dense_decode_mass`` needs; total_pages: entries of all page lists (-1, and always with a
+    view.page_count: batch * max_pages_per_seq)."""
+    shp = Shape(batch, num_kv_heads, group_size, HEAD_DIM, PAGE_SIZE, _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32, 0)
+    return int(_lib.load().ktk_decode_mass_workspace_bytes(shp, max_pages_per_seq, total_pages))
+
+
 def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: int, mass, decay: float = 1.0,
                       sm_scale: Optional[float] = None, mass_out=None, workspace=None, out=None, status=None, view=None):
     """``dense_decode`` that also accumulates the weights every cached token was given.
