@@ -560,7 +560,9 @@ typedef struct ktk_mass {
  * The weights are those of fp32 scores and denominators.
  *   total_pages  an upper bound of the entries in all lists (sizes the workspace), or -1: batch * max_pages_per_seq, which is
  *                also what counts with view->page_count
- *   workspace    ktk_decode_mass_workspace_bytes() bytes: the scores of all tokens, and the partials of lists that are cut
+ *   max_pages_per_seq  at least every sequence's page count; a longer list reports KTK_STATUS_BAD_TABLE and its results are void
+ *   workspace    ktk_decode_mass_workspace_bytes() bytes: the scores of all tokens, and the partials of lists that are cut; 0, and then
+ *                it may be null, for lists that the device holds all at once (a cluster of CTAs each)
  * q, kv_cache, o and workspace are 16-byte aligned.
  */
 KTK_API size_t ktk_decode_mass_workspace_bytes(const ktk_shape* shape, int32_t max_pages_per_seq, int64_t total_pages);

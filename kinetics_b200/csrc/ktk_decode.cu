@@ -7,6 +7,7 @@
 // row is one coalesced 256-byte (bf16) warp load straight from HBM, and the
 // next page of the warp is already in flight in registers while the current
 // one is being reduced.  The four warps merge through shared memory.
+#include "ktk_decode_mass.cuh"
 #include "ktk_decode_mma.cuh"
 
 namespace ktk {
@@ -40,8 +41,10 @@ __device__ __forceinline__ void halve(float (&part)[kPageSize], int lane) {
     }
 }
 
-// MASS: also writes the scores, and its partials whatever the number of splits.
-template <typename T, int G, bool MASS = false>
+// MASS: weights are accumulated too.  kMassLong: the scores go to memory and all partials with them (ktk_decode_mass.cu); kMassCluster:
+// the splits of a list are a cluster, scores stay in (dynamic) shared memory.
+enum SimtMass { kMassNone, kMassLong, kMassCluster };
+template <typename T, int G, SimtMass MASS>
 __global__ void __launch_bounds__(kSimtWarps * 32)
 decode_simt_kernel(const DecodeParams p, const MassParams mp) {
     using R = typename Raw4<T>::type;
@@ -59,7 +62,11 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
     const int Hq = p.Hkv * G;
 
     bool bad;
-    const EntryList el = entry_list(p, b, h, bad);
+    EntryList el = entry_list(p, b, h, bad);
+    if (MASS == kMassCluster && el.cnt > mp.max_pages) {      // the scores of more do not fit
+        el.cnt = mp.max_pages;
+        bad = true;
+    }
     if (bad && tid == 0 && split == 0) report(p.status, KTK_STATUS_BAD_TABLE);
     const int per = (el.cnt + S - 1) / S;
     const int e0 = split * per;
@@ -103,7 +110,8 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
     };
 
     // one page of the warp: scores, online softmax, weighted values
-    const int64_t position = MASS ? list_position(p, mp.wmax, b, h) : 0;
+    extern __shared__ __align__(16) float simt_scores[];                      // kMassCluster
+    const int64_t position = MASS == kMassLong ? list_position(p, mp.wmax, b, h) : 0;
     auto consume = [&](int e, const R (&kr)[kPageSize], const R (&vr)[kPageSize]) {
         const int ntok = entry_tokens(el, e);
         const int tok = lane >> 1;               // the token this lane ends up holding
@@ -126,10 +134,16 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
             part[0] += __shfl_xor_sync(0xffffffffu, part[0], 1);
             s[g] = (tok < ntok) ? part[0] : -INFINITY;
         }
-        if constexpr (MASS) {
+        if constexpr (MASS == kMassLong) {
             if ((lane & 1) == 0 && tok < ntok && position + e < mp.positions) {
 #pragma unroll
                 for (int g = 0; g < G; ++g) mp.scores[((position + e) * kPageSize + tok) * G + g] = s[g];
+            }
+        }
+        if constexpr (MASS == kMassCluster) {
+            if ((lane & 1) == 0) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) simt_scores[((e - e0) * kPageSize + tok) * G + g] = s[g];
             }
         }
 #pragma unroll
@@ -196,6 +210,7 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
         if (lane == 0) { red_m[warp][g] = m[g]; red_l[warp][g] = l[g]; }
         *reinterpret_cast<float4*>(&red_o[warp][g][lane * 4]) = make_float4(o[g][0], o[g][1], o[g][2], o[g][3]);
     }
+    __shared__ MassShared<MASS == kMassCluster ? G : 1> shared;
     __syncthreads();
     const int d = tid;   // 128 threads, one per head-dim element
 #pragma unroll
@@ -213,7 +228,10 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
             }
         }
         const int64_t qh = (int64_t)b * Hq + (int64_t)h * G + g;
-        if (!MASS && S == 1) {
+        if constexpr (MASS == kMassCluster) {
+            shared.o[g][d] = O;
+            if (d == 0) { shared.ml[g][0] = M; shared.ml[g][1] = L; }
+        } else if (MASS == kMassNone && S == 1) {
             ((T*)p.o)[qh * kHeadDim + d] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
             if (p.neg_lse != nullptr && d == 0) p.neg_lse[qh] = -(M + log2f(L));
         } else {
@@ -223,6 +241,10 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
                 p.ws_ml[(qh * S + split) * 2 + 1] = L;
             }
         }
+    }
+    if constexpr (MASS == kMassCluster) {
+        __syncthreads();
+        finish_cluster<T>(p, mp, b, h, G, S, split, shared, simt_scores, ListShare{el, e0 < el.cnt ? e0 : el.cnt, e1 > e0 ? e1 : (e0 < el.cnt ? e0 : el.cnt)});
     }
 }
 
@@ -249,14 +271,21 @@ combine_kernel(const float* __restrict__ ws_ml, const float* __restrict__ ws_o, 
     o[qh * kHeadDim + d] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
 }
 
-template <typename T, int G, bool MASS>
+template <typename T, int G, SimtMass MASS>
 static int simt_launch(const DecodeParams& p, const MassParams& m, cudaStream_t st) {
     const int64_t ctas = (int64_t)p.batch * p.Hkv * p.num_splits;
+    if constexpr (MASS == kMassCluster) {
+        const size_t smem = (size_t)((m.max_pages + p.num_splits - 1) / p.num_splits) * kPageSize * G * sizeof(float);
+        KTK_CUDA_TRY(cudaFuncSetAttribute(decode_simt_kernel<T, G, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "ktk decode (simt)");
+        KTK_CUDA_TRY(launch_cluster(ctas <= sm_count(), decode_simt_kernel<T, G, MASS>, (unsigned)ctas, kSimtWarps * 32, smem, p.num_splits, st, p, m),
+                     "ktk decode (simt)");
+        return KTK_OK;
+    }
     KTK_CUDA_TRY(launch_behind(ctas <= sm_count(), decode_simt_kernel<T, G, MASS>, (unsigned)ctas, kSimtWarps * 32, 0, st, p, m), "ktk decode (simt)");
     return KTK_OK;
 }
 
-template <typename T, bool MASS>
+template <typename T, SimtMass MASS>
 static int simt_group(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st) {
     switch (G) {
         case 1: return simt_launch<T, 1, MASS>(p, m, st);
@@ -268,11 +297,11 @@ static int simt_group(const DecodeParams& p, const MassParams& m, int G, cudaStr
 
 int launch_decode_simt(const DecodeParams& p, int dtype, int G, cudaStream_t st) {
     const MassParams none{};
-    return dtype == KTK_F32 ? simt_group<float, false>(p, none, G, st) : simt_group<__nv_bfloat16, false>(p, none, G, st);
+    return dtype == KTK_F32 ? simt_group<float, kMassNone>(p, none, G, st) : simt_group<__nv_bfloat16, kMassNone>(p, none, G, st);
 }
 
-int launch_decode_simt_mass(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st) {
-    return simt_group<float, true>(p, m, G, st);
+int launch_decode_simt_mass(const DecodeParams& p, const MassParams& m, int G, bool cluster, cudaStream_t st) {
+    return cluster ? simt_group<float, kMassCluster>(p, m, G, st) : simt_group<float, kMassLong>(p, m, G, st);
 }
 
 int launch_combine(const DecodeParams& p, int dtype, int G, cudaStream_t st) {

@@ -158,7 +158,8 @@ __device__ __forceinline__ int64_t list_position(const DecodeParams& p, int wmax
 }
 
 int launch_decode_simt(const DecodeParams& p, int dtype, int G, cudaStream_t st);
-int launch_decode_simt_mass(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st);    // fp32
+int launch_decode_simt_mass(const DecodeParams& p, const MassParams& m, int G, bool cluster, cudaStream_t st);    // fp32
+int launch_decode_mma_mass(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st);                   // bf16, a cluster per list
 int launch_decode_mma(const DecodeParams& p, int G, cudaStream_t st);
 // What ktk_prefill_attention does, and with `lse`, for every variant but KTK_VARIANT_MMA, the logarithms of the rows' denominators
 // [total_new, Hq]: fp32 minus log2 of them; bf16 minus log2 of them over scale_log2, as 16 bytes: three bf16 that add up to it, and zeros.

@@ -2,9 +2,13 @@
 //     o[b, hq] = sum_t p_hq(t) V_t,     mass'[r, h, t] = decay mass[r, h, t] + sum over the group's heads of p_hq(t)
 // with p_hq(t) = 2^(s_hq(t) - lse_hq), scores s in the log2 domain; the newest token starts from 0.
 //
-// A weight needs the denominator of its whole list, which is known when every key has been read.  So the decode kernels write the
-// scores down as they go (4 G bytes per token beside the 512 of its bf16 key and value), and mass_finish_kernel turns them into
-// weights.  It also merges the pieces of lists that the decode cut.
+// A weight needs the denominator of its whole list, which is known when every key has been read.  Two forms:
+//   a cluster of CTAs per (sequence, kv head) whose scores stay in shared memory: one launch (ktk_decode_mass.cuh), for lists that the
+//     device holds all at once;
+//   the balanced partition (bf16) or splits (fp32): the decode kernels write the scores down as they go (4 G bytes per token beside
+//     the 512 of its bf16 key and value), and mass_finish_kernel turns them into weights.  It also merges the pieces of lists that
+//     the decode cut.
+#include "ktk_decode_mass.cuh"
 #include "ktk_decode_stream.cuh"
 
 namespace ktk {
@@ -177,21 +181,49 @@ static int launch_finish(const StreamParams& p, int decode_ctas, cudaStream_t st
 
 int launch_mass_finish(const StreamParams& p, int decode_ctas, cudaStream_t st) { return launch_finish<__nv_bfloat16, true>(p, decode_ctas, st); }
 
+// CTAs per list of the form that needs no workspace; 0: the other form
+static int mass_cluster(const ktk_shape* s, int max_pages) {
+    const int64_t units = (int64_t)s->batch * s->num_kv_heads, sms = sm_count();
+    const int G = s->group_size;
+    if (s->dtype == KTK_F32) {
+        // as many splits as the plain decode takes, as far as a cluster goes
+        const int splits = legacy_num_splits(s, max_pages);
+        int c = 1;
+        const auto bytes = [&](int k) { return (int64_t)(max_pages + k - 1) / k * kPageSize * G * (int64_t)sizeof(float); };
+        while (c < kMassMaxCluster && (c < splits || bytes(c) > 64 * 1024)) c *= 2;
+        return bytes(c) <= 160 * 1024 && splits <= 2 * kMassMaxCluster ? c : 0;
+    }
+    int best = 0;
+    for (int c = 1; c <= kMassMaxCluster; c *= 2) {
+        const int64_t per_sm = mma_mass_per_sm(4, max_pages, c, G);
+        if (units * c > (per_sm < 4 ? per_sm : 4) * sms || (c > 1 && max_pages < kMmaConsumers * c)) continue;
+        best = c;
+    }
+    if (best == 0) return 0;
+    // the balanced partition where it would spread the pages over many more CTAs
+    const int64_t mine = (max_pages + best - 1) / best, even = units * max_pages / (4 * sms);
+    return mine <= 2 * even + 16 ? best : 0;
+}
+
 // Parts of the workspace, in bytes from its start
 struct MassWorkspace {
-    size_t partials, lse, scores, bytes;
+    size_t lse, scores, bytes;
     int64_t positions;
-    int splits;
+    int cluster, splits;
 };
 static MassWorkspace mass_workspace(const ktk_shape* s, int max_pages, int64_t total_pages) {
-    MassWorkspace w;
+    MassWorkspace w{};
+    w.cluster = mass_cluster(s, max_pages);
+    if (w.cluster > 0) {
+        w.splits = w.cluster;
+        return w;
+    }
     const int64_t padded = (int64_t)s->batch * max_pages;
     if (total_pages < 0 || total_pages > padded) total_pages = padded;
     const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     w.splits = policy_num_splits(s, KTK_VARIANT_AUTO, max_pages);
     const size_t rows = (size_t)s->batch * s->num_kv_heads * s->group_size;
     w.positions = total_pages * s->num_kv_heads;
-    w.partials = 0;
     w.lse = up(w.splits == KTK_SPLITS_BALANCED ? ktk_decode_workspace_bytes(s, w.splits)
                                                : rows * w.splits * (2 + kHeadDim) * sizeof(float));
     w.scores = w.lse + up(rows * sizeof(float));
@@ -229,7 +261,7 @@ extern "C" int ktk_dense_decode_mass(const void* q, const void* kv_cache, const 
     const View view = make_view(view_in);
     if (view.page_count) total_pages = -1;                // padded
     const MassWorkspace w = mass_workspace(s, max_pages_per_seq, total_pages);
-    if (workspace == nullptr || workspace_bytes < w.bytes) {
+    if (w.bytes > 0 && (workspace == nullptr || workspace_bytes < w.bytes)) {
         set_error("%s: workspace of %zu bytes needed, got %zu", who, w.bytes, workspace ? workspace_bytes : (size_t)0);
         return KTK_ERR_WORKSPACE;
     }
@@ -244,6 +276,13 @@ extern "C" int ktk_dense_decode_mass(const void* q, const void* kv_cache, const 
     p.topk = -1; p.batch = s->batch; p.Hkv = s->num_kv_heads; p.num_pages = s->num_pages;
     p.scale_log2 = sm_scale * kLog2e;
     p.num_splits = w.splits;
+    MassParams m{};
+    m.in = mass->in; m.out = mass->out; m.stride = mass->stride; m.rows = mass->rows; m.slot_index = view.slot_index;
+    m.decay = mass->decay; m.wmax = max_pages_per_seq; m.max_pages = max_pages_per_seq;
+    p.status = status;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (w.cluster > 0)
+        return s->dtype == KTK_F32 ? launch_decode_simt_mass(p, m, s->group_size, true, st) : launch_decode_mma_mass(p, m, s->group_size, st);
     const bool balanced = w.splits == KTK_SPLITS_BALANCED;
     const int64_t rows = balanced ? (int64_t)(ktk_decode_workspace_bytes(s, w.splits) / ((2 + kHeadDim) * sizeof(float)))
                                   : (int64_t)s->batch * s->num_kv_heads * s->group_size * w.splits;
@@ -251,14 +290,10 @@ extern "C" int ktk_dense_decode_mass(const void* q, const void* kv_cache, const 
     p.ws_ml = (float*)ws;
     p.ws_o = (float*)ws + rows * 2;
     p.neg_lse = (float*)(ws + w.lse);
-    p.status = status;
-    MassParams m;
-    m.in = mass->in; m.out = mass->out; m.stride = mass->stride; m.rows = mass->rows; m.slot_index = view.slot_index;
-    m.decay = mass->decay; m.scores = (float*)(ws + w.scores); m.positions = w.positions; m.wmax = max_pages_per_seq;
-    m.max_pages = max_pages_per_seq;
-    cudaStream_t st = (cudaStream_t)stream;
+    m.scores = (float*)(ws + w.scores);
+    m.positions = w.positions;
     if (balanced) return launch_decode_stream_mass(p, m, s->group_size, max_pages_per_seq, st);
-    rc = launch_decode_simt_mass(p, m, s->group_size, st);
+    rc = launch_decode_simt_mass(p, m, s->group_size, false, st);
     if (rc != KTK_OK) return rc;
     StreamParams sp{};
     sp.d = p;

@@ -13,17 +13,24 @@
 // S^T accumulators through movmatrix.  Softmax runs in base 2 with an online
 // maximum per head; each warp keeps its own (m, l, O^T) and the four warps merge
 // through shared memory at the end.  HBM traffic is exactly the listed pages.
+#include "ktk_decode_mass.cuh"
 #include "ktk_decode_mma.cuh"
 
 namespace ktk {
 
 struct MmaParams {
     DecodeParams d;
+    MassParams m;        // read by the MASS form
     int G;
 };
 
-__global__ void __launch_bounds__(kMmaThreads, 3)
+// MASS: weights are accumulated too; the splits of a list are a cluster, and the scores of a CTA's tokens stay in shared memory, behind the
+// stages.
+template <int STAGES, int CTAS, bool MASS>
+__global__ void __launch_bounds__(kMmaThreads, CTAS)
 decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map) {
+    static_assert(STAGES % kMmaConsumers == 0, "a stage must belong to one consumer warp");
+    constexpr int kMmaStages = STAGES;                     // shadows the default
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kMmaStages];
     __shared__ __align__(8) uint64_t empty_bar[kMmaStages];
@@ -34,6 +41,7 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
 
     // the swizzle pattern is a function of the shared-memory address: stages start on 1 KiB
     uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* scores = reinterpret_cast<float*>(stages + kMmaStages * kStageBytes);              // MASS: [token of the split][G]
 
     const DecodeParams& d = p.d;
     const int G = p.G;
@@ -46,12 +54,17 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
     const int Hq = d.Hkv * G;
 
     bool bad;
-    const EntryList el = entry_list(d, b, h, bad);
+    EntryList el = entry_list(d, b, h, bad);
+    if (MASS && el.cnt > p.m.max_pages) {                     // the scores of more do not fit
+        el.cnt = p.m.max_pages;
+        bad = true;
+    }
     if (bad && tid == 0 && split == 0) report(d.status, KTK_STATUS_BAD_TABLE);
     const int per = (el.cnt + S - 1) / S;
     const int e0 = split * per;
     const int e1 = (e0 + per < el.cnt) ? e0 + per : el.cnt;
     const int n_entries = (e1 > e0) ? e1 - e0 : 0;
+    __shared__ MassShared<MASS ? 8 : 1> shared;
 
     if (tid == 0) {
         for (int s = 0; s < kMmaStages; ++s) {
@@ -92,7 +105,8 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
                         issued = i + 1;
                     } else {
                         stage_tag[s] = i + 1;
-                        tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, h);
+                        if (MASS) tma_load_whole_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, h);
+                        else tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, h);
                         issued = i + 1;
                     }
                 }
@@ -115,8 +129,22 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
                 if (lane == 0) { report(d.status, KTK_STATUS_INTERNAL); abort_flag = 1; }
                 break;
             }
-            if (tag > 0)
+            if (MASS && tag > 0) {
+                const int ntok = entry_tokens(el, e0 + i);
+                float* at = scores + (i * kPageSize + gid) * G + 2 * tig;
+                mma_consume_page_t<false, true, true>(ms, stages + s * kStageBytes, ntok, qb, d.scale_log2, lane, ntok, ntok,
+                                                [&](float s00, float s01, float s10, float s11) {
+                                                    if (2 * tig >= G) return;
+                                                    at[0] = s00;
+                                                    at[8 * G] = s10;
+                                                    if (G > 1) {
+                                                        at[1] = s01;
+                                                        at[8 * G + 1] = s11;
+                                                    }
+                                                });
+            } else if (tag > 0) {
                 mma_consume_page(ms, stages + s * kStageBytes, entry_tokens(el, e0 + i), qb, d.scale_log2, lane);
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_bar[s]);
         }
@@ -132,7 +160,8 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
             for (int i = (total > kMmaStages ? total - kMmaStages : 0); i < total; ++i)
                 mbar_wait(&full_bar[i % kMmaStages], (i / kMmaStages) & 1, &never);
         }
-        return;
+        if (!MASS) return;
+        __syncthreads();                                      // the cluster's other CTAs wait for this one: its results are void
     }
 
     // ---- merge the consumer warps (stage memory reused as the exchange buffer) ----
@@ -168,7 +197,10 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
                 }
             }
             const int64_t qh = (int64_t)b * Hq + (int64_t)h * G + g;
-            if (S == 1) {
+            if constexpr (MASS) {
+                shared.o[g][dd] = O;
+                if (dd == 0) { shared.ml[g][0] = M; shared.ml[g][1] = L; }
+            } else if (S == 1) {
                 ((__nv_bfloat16*)d.o)[qh * kHeadDim + dd] = __float2bfloat16_rn(L > 0.0f ? O / L : 0.0f);
             } else {
                 d.ws_o[(qh * S + split) * kHeadDim + dd] = O;
@@ -178,6 +210,11 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
                 }
             }
         }
+    }
+    if constexpr (MASS) {
+        __syncthreads();
+        const int at = e0 < el.cnt ? e0 : el.cnt;
+        finish_cluster<__nv_bfloat16>(d, p.m, b, h, G, S, split, shared, scores, ListShare{el, at, at + n_entries});
     }
 }
 
@@ -193,18 +230,48 @@ int make_kv_tensor_map(CUtensorMap* map, const DecodeParams& p) {
                               CU_TENSOR_MAP_SWIZZLE_128B, "ktk decode");
 }
 
+int make_page_tensor_map(CUtensorMap* map, const DecodeParams& p) {
+    const uint64_t dims[4] = {64, (uint64_t)p.num_pages * 2 * kPageSize, 2, (uint64_t)p.Hkv};
+    const uint64_t strides[3] = {(uint64_t)p.Hkv * kHeadDim * 2, 128, (uint64_t)kHeadDim * 2};
+    const uint32_t box[4] = {64, 2 * kPageSize, 2, 1};
+    if (dims[1] >= (1ull << 31)) {
+        set_error("ktk decode: %lld pages exceed the tensor-core variant's 2^26-page limit", (long long)p.num_pages);
+        return KTK_ERR_TOO_LARGE;
+    }
+    return make_tensor_map(map, p.cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                           "ktk decode");
+}
+
 int launch_decode_mma(const DecodeParams& p, int G, cudaStream_t st) {
     CUtensorMap map;
     int rc = make_kv_tensor_map(&map, p);
     if (rc != KTK_OK) return rc;
     const int smem = kMmaStages * kStageBytes + 1024;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(decode_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                 "ktk decode (mma)");
+    const auto kernel = decode_mma_kernel<kMmaStages, 3, false>;
+    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "ktk decode (mma)");
     MmaParams mp;
     mp.d = p;
+    mp.m = MassParams{};
     mp.G = G;
     const int64_t ctas = (int64_t)p.batch * p.Hkv * p.num_splits;
-    KTK_CUDA_TRY(launch_behind(ctas <= sm_count(), decode_mma_kernel, (unsigned)ctas, kMmaThreads, smem, st, mp, map), "ktk decode (mma)");
+    KTK_CUDA_TRY(launch_behind(ctas <= sm_count(), kernel, (unsigned)ctas, kMmaThreads, smem, st, mp, map), "ktk decode (mma)");
+    return KTK_OK;
+}
+
+int launch_decode_mma_mass(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st) {
+    const char* who = "ktk_dense_decode_mass";
+    CUtensorMap map;
+    int rc = make_page_tensor_map(&map, p);
+    if (rc != KTK_OK) return rc;
+    const int64_t ctas = (int64_t)p.batch * p.Hkv * p.num_splits;
+    const int per_sm = (int)((ctas + sm_count() - 1) / sm_count());
+    const auto fits = [&](int stages) { return mma_mass_per_sm(stages, m.max_pages, p.num_splits, G) >= per_sm; };
+    const int stages = fits(16) ? 16 : fits(8) ? 8 : 4;
+    const int smem = mma_mass_smem(stages, m.max_pages, p.num_splits, G);
+    const auto kernel = stages == 16 ? decode_mma_kernel<16, 1, true> : stages == 8 ? decode_mma_kernel<8, 3, true> : decode_mma_kernel<4, 4, true>;
+    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
+    const MmaParams mp{p, m, G};
+    KTK_CUDA_TRY(launch_cluster(ctas <= sm_count(), kernel, (unsigned)ctas, kMmaThreads, smem, p.num_splits, st, mp, map), who);
     return KTK_OK;
 }
 

@@ -20,8 +20,9 @@ static_assert(kMmaStages % kMmaConsumers == 0, "a stage must belong to one consu
 
 // byte offset of 16-byte chunk `c16` (0..15 across the 256-byte row) of token row `tok`
 // inside a K or V tile stored as two 128-byte-swizzled half tiles
+template <int HALF = kHalfTile>
 __device__ __forceinline__ uint32_t tile_off(int tok, int c16) {
-    return (uint32_t)((c16 >> 3) * kHalfTile + tok * 128 + (((c16 & 7) ^ (tok & 7)) << 4));
+    return (uint32_t)((c16 >> 3) * HALF + tok * 128 + (((c16 & 7) ^ (tok & 7)) << 4));
 }
 
 // A consumer warp's running softmax state for the two heads 2*tig, 2*tig+1 it holds
@@ -58,27 +59,29 @@ __device__ __forceinline__ void load_q_frags(uint32_t (&qb)[8][2], const void* q
 // CAUSAL (prefill): the 8 columns are (query token, head) pairs with their own horizon -- column 2*tig sees
 // the first lim0 tokens of the page, column 2*tig+1 the first lim1 (both <= ntok, possibly 0).
 // keep(s00, s01, s10, s11) gets the scores of tokens gid, gid + 8 and heads 2*tig, 2*tig+1 (log2 domain, masked ones -inf); UNROUNDED:
-// the normaliser adds the probabilities as they were before they were rounded.
+// the normaliser adds the probabilities as they were before they were rounded.  WHOLE: the stage holds the page as tma_load_whole_page
+// brings it: the first halves of K's and V's rows, then the second ones.
 struct KeepNothing {
     __device__ __forceinline__ void operator()(float, float, float, float) const {}
 };
-template <bool CAUSAL, bool UNROUNDED = false, class Keep = KeepNothing>
+template <bool CAUSAL, bool UNROUNDED = false, bool WHOLE = false, class Keep = KeepNothing>
 __device__ __forceinline__ void mma_consume_page_t(MmaState& st, uint8_t* stage, int ntok,
                                                    const uint32_t (&qb)[8][2], float scale_log2, int lane,
                                                    int lim0, int lim1, Keep keep = Keep()) {
+    constexpr int kHalf = WHOLE ? 2 * kHalfTile : kHalfTile, kV = WHOLE ? kHalfTile : 2 * kHalfTile;     // bytes to the second half, to V
     const int gid = lane >> 2;
     // per-lane ldmatrix row addresses (relative to the tile): lane supplies row (lane & 7) of matrix lane >> 3
     const int mj = lane >> 3, mr = lane & 7;
     const int k_tok = mr + 8 * (mj & 1), k_c = mj >> 1;     // K:  matrices (tok 0-7 | 8-15) x (chunk 2ks | 2ks+1)
     const int v_tok = mr + 8 * (mj >> 1), v_c = mj & 1;     // V^T: matrices (chunk 2mt | 2mt+1) x (tok 0-7 | 8-15)
     const uint32_t kt = smem_u32(stage);
-    const uint32_t vt = kt + 2 * kHalfTile;
+    const uint32_t vt = kt + kV;
     if (ntok < kPageSize) {
         // rows past the fill level may hold anything: clear them in V so that 0 * x stays 0
-        uint8_t* vrow = stage + 2 * kHalfTile;
+        uint8_t* vrow = stage + kV;
         for (int c = lane; c < (kPageSize - ntok) * 16; c += 32) {
             const int t = ntok + (c >> 4), cc = c & 15;
-            *reinterpret_cast<uint4*>(vrow + (cc >> 3) * kHalfTile + t * 128 + ((cc & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vrow + (cc >> 3) * kHalf + t * 128 + ((cc & 7) << 4)) = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
     }
@@ -87,8 +90,8 @@ __device__ __forceinline__ void mma_consume_page_t(MmaState& st, uint8_t* stage,
 #pragma unroll
     for (int ks = 0; ks < 8; ks += 2) {
         uint32_t ka[4], kb[4];
-        ldmatrix_x4(ka, kt + tile_off(k_tok, 2 * ks + k_c));
-        ldmatrix_x4(kb, kt + tile_off(k_tok, 2 * ks + 2 + k_c));
+        ldmatrix_x4(ka, kt + tile_off<kHalf>(k_tok, 2 * ks + k_c));
+        ldmatrix_x4(kb, kt + tile_off<kHalf>(k_tok, 2 * ks + 2 + k_c));
         mma_bf16(s_a, ka, qb[ks][0], qb[ks][1]);
         mma_bf16(s_b, kb, qb[ks + 1][0], qb[ks + 1][1]);
     }
@@ -136,7 +139,7 @@ __device__ __forceinline__ void mma_consume_page_t(MmaState& st, uint8_t* stage,
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
         uint32_t va[4];
-        ldmatrix_x4_trans(va, vt + tile_off(v_tok, 2 * mt + v_c));
+        ldmatrix_x4_trans(va, vt + tile_off<kHalf>(v_tok, 2 * mt + v_c));
         st.acc[mt][0] *= al0; st.acc[mt][1] *= al1; st.acc[mt][2] *= al0; st.acc[mt][3] *= al1;
         mma_bf16(st.acc[mt], va, pb0, pb1);
     }
@@ -148,21 +151,29 @@ __device__ __forceinline__ void mma_consume_page(MmaState& st, uint8_t* stage, i
     mma_consume_page_t<false>(st, stage, ntok, qb, scale_log2, lane, ntok, ntok);
 }
 
-// The four TMA tile loads of one page (K and V, each as two 16-row x 128-byte boxes) into a stage.  `policy`: nothing, or read_once_policy().
-template <class... Policy>
+// The four TMA tile loads of one page (K and V, each as two 16-row x 128-byte boxes) into a stage.
 __device__ __forceinline__ void tma_load_page(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int64_t page,
-                                              int h, Policy... policy) {
+                                              int h) {
     const int y = (int)(page * (2 * kPageSize));      // token row of K slot 0
     mbar_arrive_expect_tx(bar, kStageBytes);
-    tma_load_3d(dst, map, bar, 0, h, y, policy...);
-    tma_load_3d(dst + kHalfTile, map, bar, 64, h, y, policy...);
-    tma_load_3d(dst + 2 * kHalfTile, map, bar, 0, h, y + kPageSize, policy...);
-    tma_load_3d(dst + 3 * kHalfTile, map, bar, 64, h, y + kPageSize, policy...);
+    tma_load_3d(dst, map, bar, 0, h, y);
+    tma_load_3d(dst + kHalfTile, map, bar, 64, h, y);
+    tma_load_3d(dst + 2 * kHalfTile, map, bar, 0, h, y + kPageSize);
+    tma_load_3d(dst + 3 * kHalfTile, map, bar, 64, h, y + kPageSize);
+}
+
+// A page by one load, through make_page_tensor_map's map; it is read once: it makes way in L2 before what is kept there.  The issuing
+// thread is what a CTA that streams alone waits for: MEASURE.
+__device__ __forceinline__ void tma_load_whole_page(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int64_t page, int h) {
+    mbar_arrive_expect_tx(bar, kStageBytes);
+    tma_load_4d(dst, map, bar, 0, (int)(page * (2 * kPageSize)), 0, h, read_once_policy());
 }
 
 // Tensor map over the cache seen as [token rows = pages*2*16][Hkv][128], innermost first, in boxes of
 // 16 rows x 64 elements with the 128-byte swizzle.
 int make_kv_tensor_map(CUtensorMap* map, const DecodeParams& p);
+// ... as [Hkv][2 halves of 64][token rows][64], in boxes of one head, both halves and the 32 rows of a page.
+int make_page_tensor_map(CUtensorMap* map, const DecodeParams& p);
 
 int launch_decode_stream(const DecodeParams& p, int G, int max_entries, cudaStream_t st);
 int launch_decode_stream_mass(const DecodeParams& p, const MassParams& m, int G, int max_entries, cudaStream_t st);

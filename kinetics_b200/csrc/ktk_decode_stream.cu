@@ -103,7 +103,7 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                             issued = i + 1;
                         } else {
                             stage_tag[s] = i + 1;
-                            if (MASS) tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h, read_once_policy());
+                            if (MASS) tma_load_whole_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h);
                             else tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h);
                             issued = i + 1;
                         }
@@ -150,7 +150,7 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                         const int64_t position = cur.start + pc.e_lo + j;
                         float* at = p.m.scores + (position * kPageSize + gid) * G + 2 * tig;
                         const bool on = 2 * tig < G && position < p.m.positions;
-                        mma_consume_page_t<false, true>(
+                        mma_consume_page_t<false, true, true>(
                             ms, stages + s * kStageBytes, ntok, qb, d.scale_log2, lane, ntok, ntok,
                             [&](float s00, float s01, float s10, float s11) {
                                 if (!on) return;
@@ -369,7 +369,7 @@ size_t stream_workspace_bytes(int G) {
 template <bool MASS>
 static int launch_stream(const DecodeParams& p, const MassParams& m, int G, int max_entries, cudaStream_t st) {
     CUtensorMap map;
-    int rc = make_kv_tensor_map(&map, p);
+    int rc = MASS ? make_page_tensor_map(&map, p) : make_kv_tensor_map(&map, p);
     if (rc != KTK_OK) return rc;
     StreamParams sp;
     sp.d = p;

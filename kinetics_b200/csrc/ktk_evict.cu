@@ -491,20 +491,8 @@ evict_move_kernel(const EvictParams p, int parts) {
 
 template <int THREADS, int ITEMS>
 static cudaError_t launch_evict(const EvictParams& p, int64_t units, int cluster, bool fused, bool f32, cudaStream_t st) {
-    cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = (unsigned)(units * cluster);
-    cfg.blockDim = THREADS;
-    cfg.stream = st;
-    cfg.attrs = units * cluster <= sm_count() ? attr : attr + 1;                 // early, as launch_behind
-    cfg.numAttrs = (units * cluster <= sm_count() ? 1 : 0) + 1;
     const auto kernel = !fused ? evict_kernel<THREADS, ITEMS, 0> : f32 ? evict_kernel<THREADS, ITEMS, 32> : evict_kernel<THREADS, ITEMS, 16>;
-    return cudaLaunchKernelEx(&cfg, kernel, p, cluster);
+    return launch_cluster(units * cluster <= sm_count(), kernel, (unsigned)(units * cluster), THREADS, 0, cluster, st, p, cluster);
 }
 
 // CTAs per (sequence, kv head): more than one for long sequences where SMs would idle.  Two sequences of 32768 tokens, 8 kv heads, the

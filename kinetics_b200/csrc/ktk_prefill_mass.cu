@@ -125,18 +125,8 @@ static int launch_prefill_mass_simt(const PrefillMassParams& p, int64_t ctas, in
     int cluster = 1;
     while (cluster < 8 && ctas * cluster < 2 * sm_count() && rows > (int64_t)kPsRows * cluster) cluster *= 2;
     KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_mass_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPsSmem), who);
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = (unsigned)(ctas * cluster);
-    cfg.blockDim = kPsThreads;
-    cfg.dynamicSmemBytes = kPsSmem;
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    KTK_CUDA_TRY(cudaLaunchKernelEx(&cfg, prefill_mass_simt_kernel, p, chunks, cluster), who);
+    KTK_CUDA_TRY(launch_cluster(false, prefill_mass_simt_kernel, (unsigned)(ctas * cluster), kPsThreads, kPsSmem, cluster, st, p, chunks, cluster),
+                 who);
     return KTK_OK;
 }
 

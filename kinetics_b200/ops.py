@@ -494,14 +494,14 @@ def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_
         mass_out = mass
     else:
         _same(mass_out, mass, "mass_out")
-    if workspace is None:
+    if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     q_, kv_, i_, p_, l_, m_, mo_, o_, w_, s_, stream = _addresses(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, mass, mass_out,
                                                                  out, workspace, status)
     check(_lib.load().ktk_dense_decode_mass(
         q_, kv_, i_, p_, l_, None if view is None else view.c(), max_pages_per_seq, pages, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
-        _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], decay), o_, w_, workspace.nbytes, shp, s_, stream))
-    _launched(2)
+        _lib.Mass(m_, mo_, mass.shape[2], mass.shape[0], decay), o_, w_, 0 if workspace is None else workspace.nbytes, shp, s_, stream))
+    _launched(2 if need else 1)
     return out, mass_out
 
 

@@ -339,8 +339,8 @@ def test_refusals_on_the_device(cuda_device):
         call(out=torch.empty_like(s["q"], dtype=torch.float32))
     with pytest.raises(TypeError):
         call(mass_out=s["mass"][:, :, :100].contiguous())
-    with pytest.raises(_lib.KtkError, match="workspace"):
-        call(workspace=torch.empty(64, dtype=torch.uint8, device=cuda_device))
+    with pytest.raises(_lib.KtkError, match="workspace"):                # lists of a bound that needs one
+        ops.dense_decode_mass(s["q"], *s["table"], 30000, s["mass"], workspace=torch.empty(64, dtype=torch.uint8, device=cuda_device))
     odd = torch.empty(s["q"].numel() + 1, dtype=torch.bfloat16, device=cuda_device)[1:].view(s["q"].shape)
     with pytest.raises(_lib.KtkError, match="aligned"):
         call(q=odd)

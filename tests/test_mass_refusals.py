@@ -19,7 +19,7 @@ def _mass(a=ONE, b=ONE, stride=64, rows=2):
     return _lib.Mass(a, b, stride, rows, 1.0)
 
 
-def _decode(shape=None, mass=None, q=ONE, ws=ONE, bytes_=1 << 30, pages=4, total=-1, view=None, **kw):
+def _decode(shape=None, mass=None, q=ONE, ws=ONE, bytes_=1 << 30, pages=5000, total=-1, view=None, **kw):
     return _lib.load().ktk_dense_decode_mass(q, ONE, ONE, ONE, ONE, view, pages, total, 0.1, mass or _mass(), ONE, ws, bytes_,
                                              shape or _shape(**kw), NULL, NULL)
 
@@ -72,11 +72,12 @@ def test_each_ones_own():
 def test_workspaces_are_sized_by_what_is_given():
     lib = _lib.load()
     shp = _shape()
-    small = lib.ktk_decode_mass_workspace_bytes(shp, 100, 50)
-    assert lib.ktk_decode_mass_workspace_bytes(shp, 100, -1) - small == 150 * 16 * 4 * 4          # scores of 200 pages instead of 50
-    assert lib.ktk_decode_mass_workspace_bytes(shp, 100, 10 ** 9) == lib.ktk_decode_mass_workspace_bytes(shp, 100, -1)
-    assert ops.decode_mass_workspace_bytes(2, 1, 4, 100, torch.bfloat16, 50) == small
-    assert lib.ktk_decode_mass_workspace_bytes(_shape(head_dim=64), 100, -1) == 0
+    assert lib.ktk_decode_mass_workspace_bytes(shp, 100, -1) == 0                                  # short lists: a cluster each
+    small = lib.ktk_decode_mass_workspace_bytes(shp, 4000, 50)
+    assert lib.ktk_decode_mass_workspace_bytes(shp, 4000, -1) - small == 7950 * 16 * 4 * 4         # scores of 8000 pages instead of 50
+    assert lib.ktk_decode_mass_workspace_bytes(shp, 4000, 10 ** 9) == lib.ktk_decode_mass_workspace_bytes(shp, 4000, -1)
+    assert ops.decode_mass_workspace_bytes(2, 1, 4, 4000, torch.bfloat16, 50) == small
+    assert lib.ktk_decode_mass_workspace_bytes(_shape(head_dim=64), 4000, -1) == 0
     assert lib.ktk_evict_workspace_bytes(shp, 4, 40) == 2 * 4 * (1 + 2 * 24)                      # 24 of 64 tokens can move
     assert lib.ktk_evict_workspace_bytes(shp, 4, 10) == 2 * 4 * (1 + 2 * 10)
     # weights of few rows need their denominators only; of many, and few keys, sums over parts
