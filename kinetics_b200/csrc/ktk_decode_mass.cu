@@ -8,12 +8,14 @@
 //   the balanced partition (bf16) or splits (fp32): the decode kernels write the scores down as they go (4 G bytes per token beside
 //     the 512 of its bf16 key and value), and mass_finish_kernel turns them into weights.  It also merges the pieces of lists that
 //     the decode cut.
+#include <type_traits>
+
 #include "ktk_decode_mass.cuh"
 #include "ktk_decode_stream.cuh"
 
 namespace ktk {
 
-constexpr int kMassThreads = 256;
+constexpr int kMassThreads = 2 * kHeadDim;
 constexpr int kMassEach = 4;                              // tokens of a thread, their loads in flight together
 constexpr int kMassTokens = kMassThreads * kMassEach;     // of a CTA at a time
 
@@ -27,25 +29,28 @@ template <bool STREAM> struct Pieces {
     }
 };
 
-// One CTA per list and `rounds` times kMassTokens of its tokens, and one per list for its output.  A CTA's first loads, one behind the
+// One CTA per list and `rounds` times kMassTokens of its tokens, and `merges` per list for its output: one per head where there are few
+// lists, each of many pieces (one sequence of 8192 tokens, 8 kv heads, 74 pieces a list: 41.5 us with one CTA for the group's heads,
+// 20.6), else one (48 sequences of 2304: 80 us, 76).  A CTA's first loads, one behind the
 // other, take longer than a round does: about as many CTAs as the device holds, and the next round's loads in flight.
 template <typename T, bool STREAM, int G>
 __global__ void __launch_bounds__(kMassThreads)
-mass_finish_kernel(const StreamParams p, int chunks, int rounds, int decode_ctas) {
+mass_finish_kernel(const StreamParams p, int chunks, int rounds, int merges, int decode_ctas) {
     __shared__ float neg_lse[G];
     const DecodeParams& d = p.d;
     const MassParams& m = p.m;
     const int tid = threadIdx.x, lane = tid & 31;
     wait_for_front();
-    const int64_t unit = blockIdx.x / (chunks + 1);
-    const int part = (int)(blockIdx.x % (chunks + 1));
+    const int64_t unit = blockIdx.x / (chunks + merges);
+    const int part = (int)(blockIdx.x % (chunks + merges));
     const int b = (int)(unit / d.Hkv), h = (int)(unit % d.Hkv);
     bool bad;
     EntryList el = entry_list(d, b, h, bad);
     const int64_t qh = ((int64_t)b * d.Hkv + h) * G;
     if (el.cnt == 0) {                                    // no token: zeros
-        if (part == chunks)
-            for (int i = tid; i < G * kHeadDim; i += kMassThreads) ((T*)d.o)[qh * kHeadDim + i] = from_f32<T>(0.0f);
+        if (part >= chunks)
+            for (int i = (part - chunks) * kMassThreads + tid; i < G * kHeadDim; i += merges * kMassThreads)
+                ((T*)d.o)[qh * kHeadDim + i] = from_f32<T>(0.0f);
         return;
     }
     const int64_t start = list_position(d, m.wmax, b, h);
@@ -64,23 +69,43 @@ mass_finish_kernel(const StreamParams p, int chunks, int rounds, int decode_ctas
         pieces.first = unit;
         pieces.count = d.num_splits;
     }
-    if (part == chunks) {
+    if (part >= chunks) {
+        // a head's output: two threads to a dimension take every other piece, eight loads in flight
         if (pieces.count == 0) return;
-        for (int i = tid; i < G * kHeadDim; i += kMassThreads) {
-            const int g = i / kHeadDim, dd = i % kHeadDim;
+        __shared__ float other[3][kHeadDim];
+        const int dd = tid % kHeadDim, half = tid / kHeadDim;
+        for (int g = part - chunks; g < G; g += merges) {
             float M = -INFINITY, L = 0.0f, O = 0.0f;
-#pragma unroll 4
-            for (int k = 0; k < pieces.count; ++k) {
-                const int64_t row = pieces.row(k, G, g);
-                const float2 ml = *reinterpret_cast<const float2*>(d.ws_ml + row * 2);
-                const float o = d.ws_o[row * kHeadDim + dd];
-                if (ml.x == -INFINITY) continue;          // nothing seen: its partial row is unspecified
-                const float Mn = fmaxf(M, ml.x), a = exp2f(M - Mn), c = exp2f(ml.x - Mn);
-                L = L * a + ml.y * c;
-                O = O * a + o * c;
+            const auto join = [&](float m2, float l2, float o2) {
+                if (m2 == -INFINITY) return;              // nothing seen: its partial row is unspecified
+                const float Mn = fmaxf(M, m2), a = exp2f(M - Mn), c = exp2f(m2 - Mn);
+                L = L * a + l2 * c;
+                O = O * a + o2 * c;
                 M = Mn;
+            };
+            const auto some = [&](auto count, int k0) {
+                constexpr int kCount = decltype(count)::value;
+                float2 ml[kCount];
+                float o[kCount];
+#pragma unroll
+                for (int i = 0; i < kCount; ++i) {
+                    const int64_t at = pieces.row(min(k0 + 2 * i, pieces.count - 1), G, g);
+                    ml[i] = *reinterpret_cast<const float2*>(d.ws_ml + at * 2);
+                    o[i] = d.ws_o[at * kHeadDim + dd];
+                }
+#pragma unroll
+                for (int i = 0; i < kCount; ++i)
+                    if (k0 + 2 * i < pieces.count) join(ml[i].x, ml[i].y, o[i]);
+            };
+            some(std::integral_constant<int, 2>(), half);                       // most lists have few pieces
+            for (int k0 = half + 4; k0 < pieces.count; k0 += 16) some(std::integral_constant<int, 8>(), k0);
+            if (half == 1) { other[0][dd] = M; other[1][dd] = L; other[2][dd] = O; }
+            __syncthreads();
+            if (half == 0) {
+                join(other[0][dd], other[1][dd], other[2][dd]);
+                ((T*)d.o)[(qh + g) * kHeadDim + dd] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
             }
-            ((T*)d.o)[qh * kHeadDim + i] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
+            __syncthreads();
         }
         return;
     }
@@ -165,13 +190,13 @@ static int launch_finish(const StreamParams& p, int decode_ctas, cudaStream_t st
     const int64_t units = (int64_t)p.d.batch * p.d.Hkv, all = ((int64_t)p.m.max_pages * kPageSize + kMassTokens - 1) / kMassTokens;
     int64_t rounds = (units * all + sm_count() * 3 - 1) / (sm_count() * 3);      // CTAs that the device holds at once
     rounds = rounds < 1 ? 1 : rounds > all ? all : rounds;
-    const int64_t chunks = (all + rounds - 1) / rounds, ctas = (chunks + 1) * units;
+    const int64_t chunks = (all + rounds - 1) / rounds, merges = units < sm_count() ? p.G : 1, ctas = (chunks + merges) * units;
     if (ctas > 2147483647LL) {
         set_error("ktk_dense_decode_mass: batch * num_kv_heads * max_pages_per_seq exceeds the grid limit");
         return KTK_ERR_TOO_LARGE;
     }
     const auto go = [&](auto kernel) {
-        return launch_behind(true, kernel, (unsigned)ctas, kMassThreads, 0, st, p, (int)chunks, (int)rounds, decode_ctas);
+        return launch_behind(true, kernel, (unsigned)ctas, kMassThreads, 0, st, p, (int)chunks, (int)rounds, (int)merges, decode_ctas);
     };
     KTK_CUDA_TRY(p.G == 1 ? go(mass_finish_kernel<T, STREAM, 1>) : p.G == 2 ? go(mass_finish_kernel<T, STREAM, 2>)
                  : p.G == 4 ? go(mass_finish_kernel<T, STREAM, 4>) : go(mass_finish_kernel<T, STREAM, 8>),
@@ -200,9 +225,11 @@ static int mass_cluster(const ktk_shape* s, int max_pages) {
         best = c;
     }
     if (best == 0) return 0;
-    // the balanced partition where it would spread the pages over many more CTAs
+    // The balanced partition where it would leave its longest CTA far fewer pages.  Pages of a CTA, even share, us with clusters and
+    // balanced: 48 sequences of 2304 tokens and 8 kv heads 144, 93, 78.6 and 76.2; 55 of 1500 94, 70, 60.8 and 65.6; 48 of 2304 and one
+    // kv head 18, 12, 17.5 and 27.1; one of 8192 and 8 kv heads 64, 7, 18.7 and 20.6; one of 32768 256, 28, 53.8 and 34.8.
     const int64_t mine = (max_pages + best - 1) / best, even = units * max_pages / (4 * sms);
-    return mine <= 2 * even + 16 ? best : 0;
+    return 100 * mine <= 145 * even + 100 * (units * best >= 2 * sms ? 8 : 56) ? best : 0;
 }
 
 // Parts of the workspace, in bytes from its start

@@ -31,6 +31,8 @@ __global__ void __launch_bounds__(kMmaThreads, CTAS)
 decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map) {
     static_assert(STAGES % kMmaConsumers == 0, "a stage must belong to one consumer warp");
     constexpr int kMmaStages = STAGES;                     // shadows the default
+    constexpr int kIssuers = STAGES > 4 ? 8 : 1;           // MASS: lanes that issue loads
+    static_assert(STAGES % kIssuers == 0, "a stage must belong to one issuing lane");
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kMmaStages];
     __shared__ __align__(8) uint64_t empty_bar[kMmaStages];
@@ -85,35 +87,66 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
         // ---------------- producer warp ----------------
         if (lane == 0) prefetch_tensormap(&kv_map);
         int issued = 0;
-        int next_ids = (e0 + lane < e1) ? el.ptr[e0 + lane] : -1;
-        bool alive = true;
-        for (int base = e0; base < e1 && alive; base += 32) {
-            const int ids = next_ids;
-            next_ids = (base + 32 + lane < e1) ? el.ptr[base + 32 + lane] : -1;   // one chunk ahead
-            const int chunk = (e1 - base < 32) ? e1 - base : 32;
-            for (int j = 0; j < chunk && alive; ++j) {
-                const int64_t page = __shfl_sync(0xffffffffu, ids, j);
-                if (lane == 0) {
-                    const int i = issued;
+        if constexpr (MASS) {
+            // A load takes its thread some 600 cycles, whatever else is in flight: with a deep ring eight lanes issue in turn (one sequence
+            // of 8192 tokens, 8 kv heads, 64 CTAs: 29 us by one lane, 18.6); with four CTAs per SM one each is faster (48 of 2304: 77.9
+            // us, 80.6 by four).
+            if (lane < kIssuers) {
+                const uint64_t policy = read_once_policy();
+                int next = lane < n_entries ? el.ptr[e0 + lane] : -1;
+                for (int i = lane; i < n_entries; i += kIssuers) {
+                    const int64_t page = next;
+                    next = i + kIssuers < n_entries ? el.ptr[e0 + i + kIssuers] : -1;
                     const int s = i % kMmaStages;
-                    if (i >= kMmaStages && !mbar_wait(&empty_bar[s], ((i / kMmaStages) - 1) & 1, &abort_flag)) {
-                        alive = false;
-                    } else if (page < 0 || page >= d.num_pages) {
+                    if (i >= kMmaStages && !mbar_wait(&empty_bar[s], ((i / kMmaStages) - 1) & 1, &abort_flag)) break;
+                    if (page < 0 || page >= d.num_pages) {
                         report(d.status, KTK_STATUS_BAD_PAGE);
                         stage_tag[s] = -(i + 1);
-                        mbar_arrive(&full_bar[s]);          // nothing to load: release the consumer
-                        issued = i + 1;
+                        mbar_arrive(&full_bar[s]);              // nothing to load: release the consumer
                     } else {
                         stage_tag[s] = i + 1;
-                        if (MASS) tma_load_whole_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, h);
-                        else tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, h);
-                        issued = i + 1;
+                        tma_load_whole_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, h, policy);
                     }
+                    issued = i + 1;
                 }
-                alive = __shfl_sync(0xffffffffu, (int)alive, 0) != 0;
+                // the CTA gave up: its shared memory is written until the last copies have landed
+                if (abort_flag) {
+                    volatile int never = 0;
+                    for (int i = lane; i < issued; i += kIssuers)
+                        if (i + kMmaStages >= issued) mbar_wait(&full_bar[i % kMmaStages], (i / kMmaStages) & 1, &never);
+                }
             }
+            __syncwarp();
+        } else {
+            int next_ids = (e0 + lane < e1) ? el.ptr[e0 + lane] : -1;
+            bool alive = true;
+            for (int base = e0; base < e1 && alive; base += 32) {
+                const int ids = next_ids;
+                next_ids = (base + 32 + lane < e1) ? el.ptr[base + 32 + lane] : -1;   // one chunk ahead
+                const int chunk = (e1 - base < 32) ? e1 - base : 32;
+                for (int j = 0; j < chunk && alive; ++j) {
+                    const int64_t page = __shfl_sync(0xffffffffu, ids, j);
+                    if (lane == 0) {
+                        const int i = issued;
+                        const int s = i % kMmaStages;
+                        if (i >= kMmaStages && !mbar_wait(&empty_bar[s], ((i / kMmaStages) - 1) & 1, &abort_flag)) {
+                            alive = false;
+                        } else if (page < 0 || page >= d.num_pages) {
+                            report(d.status, KTK_STATUS_BAD_PAGE);
+                            stage_tag[s] = -(i + 1);
+                            mbar_arrive(&full_bar[s]);          // nothing to load: release the consumer
+                            issued = i + 1;
+                        } else {
+                            stage_tag[s] = i + 1;
+                            tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, h);
+                            issued = i + 1;
+                        }
+                    }
+                    alive = __shfl_sync(0xffffffffu, (int)alive, 0) != 0;
+                }
+            }
+            if (lane == 0) issued_total = issued;
         }
-        if (lane == 0) issued_total = issued;
     } else {
         // ---------------- consumer warps ----------------
         uint32_t qb[8][2];
@@ -157,7 +190,7 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
             // wait, again bounded, for copies still in flight before the CTA's shared memory is released
             volatile int never = 0;
             const int total = issued_total;
-            for (int i = (total > kMmaStages ? total - kMmaStages : 0); i < total; ++i)
+            for (int i = (MASS ? total : total > kMmaStages ? total - kMmaStages : 0); i < total; ++i)
                 mbar_wait(&full_bar[i % kMmaStages], (i / kMmaStages) & 1, &never);
         }
         if (!MASS) return;
@@ -266,7 +299,8 @@ int launch_decode_mma_mass(const DecodeParams& p, const MassParams& m, int G, cu
     const int64_t ctas = (int64_t)p.batch * p.Hkv * p.num_splits;
     const int per_sm = (int)((ctas + sm_count() - 1) / sm_count());
     const auto fits = [&](int stages) { return mma_mass_per_sm(stages, m.max_pages, p.num_splits, G) >= per_sm; };
-    const int stages = fits(16) ? 16 : fits(8) ? 8 : 4;
+    // one CTA per SM leaves clusters little choice of SMs: not for more CTAs than half of them
+    const int stages = 2 * ctas <= sm_count() && fits(16) ? 16 : fits(8) ? 8 : 4;
     const int smem = mma_mass_smem(stages, m.max_pages, p.num_splits, G);
     const auto kernel = stages == 16 ? decode_mma_kernel<16, 1, true> : stages == 8 ? decode_mma_kernel<8, 3, true> : decode_mma_kernel<4, 4, true>;
     KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);

@@ -162,11 +162,11 @@ __device__ __forceinline__ void tma_load_page(uint8_t* dst, const CUtensorMap* m
     tma_load_3d(dst + 3 * kHalfTile, map, bar, 64, h, y + kPageSize);
 }
 
-// A page by one load, through make_page_tensor_map's map; it is read once: it makes way in L2 before what is kept there.  The issuing
-// thread is what a CTA that streams alone waits for: MEASURE.
-__device__ __forceinline__ void tma_load_whole_page(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int64_t page, int h) {
+// A page by one load, through make_page_tensor_map's map.  policy: read_once_policy(), made once
+__device__ __forceinline__ void tma_load_whole_page(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int64_t page, int h,
+                                                    uint64_t policy) {
     mbar_arrive_expect_tx(bar, kStageBytes);
-    tma_load_4d(dst, map, bar, 0, (int)(page * (2 * kPageSize)), 0, h, read_once_policy());
+    tma_load_4d(dst, map, bar, 0, (int)(page * (2 * kPageSize)), 0, h, policy);
 }
 
 // Tensor map over the cache seen as [token rows = pages*2*16][Hkv][128], innermost first, in boxes of

@@ -78,6 +78,7 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
     if (warp == kMmaConsumers) {
         // ---------------- producer warp: one ring across all of the CTA's units ----------------
         if (lane == 0) prefetch_tensormap(&kv_map);
+        const uint64_t policy = MASS ? read_once_policy() : 0;
         int issued = 0;
         bool alive = true;
         for (Cursor cur = cursor_at(p, p0); cur.start < p1 && cur.b < d.batch && alive; cursor_next(p, cur)) {
@@ -103,7 +104,7 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                             issued = i + 1;
                         } else {
                             stage_tag[s] = i + 1;
-                            if (MASS) tma_load_whole_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h);
+                            if (MASS) tma_load_whole_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h, policy);
                             else tma_load_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, pc.h);
                             issued = i + 1;
                         }
