@@ -41,12 +41,20 @@ __device__ __forceinline__ void halve(float (&part)[kPageSize], int lane) {
     }
 }
 
-// MASS: weights are accumulated too.  kMassLong: the scores go to memory and all partials with them (ktk_decode_mass.cu); kMassCluster:
-// the splits of a list are a cluster, scores stay in (dynamic) shared memory.
-enum SimtMass { kMassNone, kMassLong, kMassCluster };
+// What a launch writes beside the outputs: nothing, minus log2 of the denominators (one split), or weights.  kMassLong: the scores go to
+// memory and all partials with them (ktk_decode_mass.cu); kMassCluster: the splits of a list are a cluster, scores stay in (dynamic)
+// shared memory.
+enum SimtMass { kMassNone, kMassLse, kMassLong, kMassCluster };
+struct NoMass {
+    static constexpr int max_pages = 0;
+};
+template <SimtMass MASS> struct MassArgument { using type = MassParams; };
+template <> struct MassArgument<kMassNone> { using type = NoMass; };
+template <> struct MassArgument<kMassLse> { using type = NoMass; };
+
 template <typename T, int G, SimtMass MASS>
 __global__ void __launch_bounds__(kSimtWarps * 32)
-decode_simt_kernel(const DecodeParams p, const MassParams mp) {
+decode_simt_kernel(const DecodeParams p, const typename MassArgument<MASS>::type mp) {
     using R = typename Raw4<T>::type;
     constexpr bool kPrefetch = sizeof(T) == 2;   // a page is 64 registers in bf16, 128 in fp32
     __shared__ __align__(16) float p_sm[kSimtWarps][kPageSize * G];   // probabilities [t][g]
@@ -111,7 +119,8 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
 
     // one page of the warp: scores, online softmax, weighted values
     extern __shared__ __align__(16) float simt_scores[];                      // kMassCluster
-    const int64_t position = MASS == kMassLong ? list_position(p, mp.wmax, b, h) : 0;
+    int64_t position = 0;
+    if constexpr (MASS == kMassLong) position = list_position(p, mp.wmax, b, h);
     auto consume = [&](int e, const R (&kr)[kPageSize], const R (&vr)[kPageSize]) {
         const int ntok = entry_tokens(el, e);
         const int tok = lane >> 1;               // the token this lane ends up holding
@@ -231,9 +240,9 @@ decode_simt_kernel(const DecodeParams p, const MassParams mp) {
         if constexpr (MASS == kMassCluster) {
             shared.o[g][d] = O;
             if (d == 0) { shared.ml[g][0] = M; shared.ml[g][1] = L; }
-        } else if (MASS == kMassNone && S == 1) {
+        } else if (MASS != kMassLong && S == 1) {
             ((T*)p.o)[qh * kHeadDim + d] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
-            if (p.neg_lse != nullptr && d == 0) p.neg_lse[qh] = -(M + log2f(L));
+            if (MASS == kMassLse && d == 0) p.neg_lse[qh] = -(M + log2f(L));
         } else {
             p.ws_o[(qh * S + split) * kHeadDim + d] = O;
             if (d == 0) {
@@ -272,21 +281,21 @@ combine_kernel(const float* __restrict__ ws_ml, const float* __restrict__ ws_o, 
 }
 
 template <typename T, int G, SimtMass MASS>
-static int simt_launch(const DecodeParams& p, const MassParams& m, cudaStream_t st) {
+static int simt_launch(const DecodeParams& p, const typename MassArgument<MASS>::type& m, cudaStream_t st) {
     const int64_t ctas = (int64_t)p.batch * p.Hkv * p.num_splits;
+    const auto kernel = decode_simt_kernel<T, G, MASS>;
     if constexpr (MASS == kMassCluster) {
         const size_t smem = (size_t)((m.max_pages + p.num_splits - 1) / p.num_splits) * kPageSize * G * sizeof(float);
-        KTK_CUDA_TRY(cudaFuncSetAttribute(decode_simt_kernel<T, G, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "ktk decode (simt)");
-        KTK_CUDA_TRY(launch_cluster(ctas <= sm_count(), decode_simt_kernel<T, G, MASS>, (unsigned)ctas, kSimtWarps * 32, smem, p.num_splits, st, p, m),
-                     "ktk decode (simt)");
-        return KTK_OK;
+        KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "ktk decode (simt)");
+        KTK_CUDA_TRY(launch_cluster(ctas <= sm_count(), kernel, (unsigned)ctas, kSimtWarps * 32, smem, p.num_splits, st, p, m), "ktk decode (simt)");
+    } else {
+        KTK_CUDA_TRY(launch_behind(ctas <= sm_count(), kernel, (unsigned)ctas, kSimtWarps * 32, 0, st, p, m), "ktk decode (simt)");
     }
-    KTK_CUDA_TRY(launch_behind(ctas <= sm_count(), decode_simt_kernel<T, G, MASS>, (unsigned)ctas, kSimtWarps * 32, 0, st, p, m), "ktk decode (simt)");
     return KTK_OK;
 }
 
 template <typename T, SimtMass MASS>
-static int simt_group(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st) {
+static int simt_group(const DecodeParams& p, const typename MassArgument<MASS>::type& m, int G, cudaStream_t st) {
     switch (G) {
         case 1: return simt_launch<T, 1, MASS>(p, m, st);
         case 2: return simt_launch<T, 2, MASS>(p, m, st);
@@ -296,8 +305,8 @@ static int simt_group(const DecodeParams& p, const MassParams& m, int G, cudaStr
 }
 
 int launch_decode_simt(const DecodeParams& p, int dtype, int G, cudaStream_t st) {
-    const MassParams none{};
-    return dtype == KTK_F32 ? simt_group<float, kMassNone>(p, none, G, st) : simt_group<__nv_bfloat16, kMassNone>(p, none, G, st);
+    if (p.neg_lse != nullptr) return simt_group<float, kMassLse>(p, {}, G, st);           // fp32, one split
+    return dtype == KTK_F32 ? simt_group<float, kMassNone>(p, {}, G, st) : simt_group<__nv_bfloat16, kMassNone>(p, {}, G, st);
 }
 
 int launch_decode_simt_mass(const DecodeParams& p, const MassParams& m, int G, bool cluster, cudaStream_t st) {

@@ -6,8 +6,8 @@
 
 namespace ktk {
 
-// Pages: below this a CTA is not worth its start-up.  Behind the form that accumulates weights pieces are joined by more CTAs, and one
-// page per consumer warp is (one sequence of 517 tokens, 8 kv heads: MEASURE).
+// Pages: below this a CTA is not worth its start-up.  The form that accumulates weights has a second launch anyway and joins pieces by
+// more CTAs: there one page per consumer warp is.
 constexpr int kStreamMinChunk = 16, kStreamMinChunkMass = kMmaConsumers;
 
 struct StreamParams {

@@ -74,7 +74,8 @@ __device__ __forceinline__ bool item_of_either(const PrefillUmmaParams& p, int& 
     return true;
 }
 
-template <Order ORDER>
+// LSE: the rows' denominators are written too
+template <Order ORDER, bool LSE>
 __global__ void __launch_bounds__(kFlThreads, 1)
 prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorMap kv_map) {
     extern __shared__ uint8_t um_raw[];
@@ -215,7 +216,7 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
         const bool done = fl.softmax<false>(tile, p.scale_log2, m_ref, l_run, prepare, [](float&, float&) {}, clear);
         if (done && fl.blocks_of(tile) > 0) {
             const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-            if (p.lse != nullptr && row_on) {
+            if (LSE && row_on) {
                 const float v = -(m_ref + log2f(l_run)) / p.scale_log2;
                 const float hi = __bfloat162float(__float2bfloat16_rn(v)), mid = __bfloat162float(__float2bfloat16_rn(v - hi));
                 p.lse[(int64_t)(q0 + my_tok) * Hq + my_head] = make_uint4(pack_bf16(hi, mid), pack_bf16(v - hi - mid, 0.0f), 0u, 0u);
@@ -265,7 +266,10 @@ int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st
     const int64_t about = p.total_new / (tpc * p.tiles) + p.batch / 2;
     const bool by_tile = pairs <= 65535;
     const bool either = by_tile && p.batch > 1 && p.batch <= kPuOrdered && about * p.Hkv > sm_count() && 2 * about * p.Hkv <= 5 * (int64_t)sm_count();
-    auto kernel = either ? prefill_umma_kernel<kByEither> : by_tile ? prefill_umma_kernel<kByTile> : prefill_umma_kernel<kBySequence>;
+    const bool lse = p.lse != nullptr;
+    auto kernel = either ? (lse ? prefill_umma_kernel<kByEither, true> : prefill_umma_kernel<kByEither, false>)
+                  : by_tile ? (lse ? prefill_umma_kernel<kByTile, true> : prefill_umma_kernel<kByTile, false>)
+                            : (lse ? prefill_umma_kernel<kBySequence, true> : prefill_umma_kernel<kBySequence, false>);
     KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPuSmem), who);
     const dim3 grid = by_tile ? dim3((unsigned)p.Hkv, (unsigned)p.batch, pairs) : dim3(pairs, (unsigned)p.Hkv, (unsigned)p.batch);
     DecodeParams d{};                               // only what the tensor map needs
