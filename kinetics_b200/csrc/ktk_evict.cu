@@ -335,6 +335,10 @@ __device__ __forceinline__ void copy_tokens(const EvictParams& p, int h, int sta
             if (dst[i][j] >= 0) cache[dst[i][j]] = v[i][j];
 }
 
+// The planning CTA copies at most this many tokens; more go to a launch of their own.  2049 tokens cut to 2048, 8 kv heads: 11.8 us in
+// one launch, 14 in two; 48 sequences of 2304 tokens cut to 2048: 48 us and 37; 7 of 700 cut to 333, fp32: 28 us and 13.
+constexpr int kEvFused = 64;
+
 // Sequences of at most THREADS * ITEMS tokens per CTA of the cluster, keys in registers.  CHUNKS: 16-byte pieces of a token's key; 0:
 // keys and values are left to evict_move_kernel.
 template <int THREADS, int ITEMS, int CHUNKS>
@@ -393,7 +397,8 @@ evict_kernel(const EvictParams p, int cluster) {
     __syncthreads();
     const int moves = number_moves<THREADS>(stay, level, first, n > 0 ? (n + 31) / 32 : 0, keep, keep - at.above, cl, shared, buf, turn);
     __syncthreads();
-    int32_t *from = p.from + unit * p.max_moves, *to = p.to + unit * p.max_moves;
+    __shared__ int32_t list[CHUNKS > 0 ? 2 * kEvFused : 1];
+    int32_t *from = CHUNKS > 0 ? list : p.from + unit * p.max_moves, *to = CHUNKS > 0 ? list + kEvFused : p.to + unit * p.max_moves;
     each_item([&](int, int i) {
         if (i < n) token_move(stay, level, first, t0 + i, keep, [&](int k) { to[k] = t0 + i; }, [&](int k) { from[k] = t0 + i; });
     });
@@ -495,6 +500,11 @@ static cudaError_t launch_evict(const EvictParams& p, int64_t units, int cluster
     return launch_cluster(units * cluster <= sm_count(), kernel, (unsigned)(units * cluster), THREADS, 0, cluster, st, p, cluster);
 }
 
+static int64_t evict_max_moves(int max_pages, int keep) {
+    const int64_t behind = (int64_t)max_pages * kPageSize - keep;
+    return behind < 1 ? 1 : behind < keep ? behind : keep;
+}
+
 // CTAs per (sequence, kv head): more than one for long sequences where SMs would idle.  Two sequences of 32768 tokens, 8 kv heads, the
 // plan alone: 48 us with one CTA of 1024 threads each, 30 with two, 26 with four, 46 with eight of 256 threads (which read 2048
 // counts of seven others, three times).
@@ -503,13 +513,22 @@ static int evict_cluster(int64_t units, int64_t most) {
     while (c < 4 && most > 4096 * c && units * c * 2 <= sm_count()) c *= 2;
     return most > 16384 * c ? 4 : c;
 }
-// The planning CTA copies at most this many tokens; more go to a launch of their own.  2049 tokens cut to 2048, 8 kv heads: 11.8 us in
-// one launch, 14 in two; 48 sequences of 2304 tokens cut to 2048: 48 us and 37; 7 of 700 cut to 333, fp32: 28 us and 13.
-constexpr int kEvFused = 64;
-
-static int64_t evict_max_moves(int max_pages, int keep) {
-    const int64_t behind = (int64_t)max_pages * kPageSize - keep;
-    return behind < 1 ? 1 : behind < keep ? behind : keep;
+// How an eviction is cut, by the caller's bounds
+struct EvictCut {
+    int64_t units, most, max_moves;
+    int cluster;
+    bool fused;                       // the planning CTA copies, from lists in its shared memory
+    size_t bytes;
+};
+static EvictCut evict_cut(const ktk_shape* s, int max_pages, int keep) {
+    EvictCut c;
+    c.units = (int64_t)s->batch * s->num_kv_heads;
+    c.most = (int64_t)max_pages * kPageSize;
+    c.max_moves = evict_max_moves(max_pages, keep);
+    c.cluster = evict_cluster(c.units, c.most);
+    c.fused = c.cluster == 1 && c.max_moves <= kEvFused;
+    c.bytes = c.fused ? 0 : (size_t)c.units * (1 + 2 * (size_t)c.max_moves) * sizeof(int32_t);
+    return c;
 }
 
 }  // namespace ktk
@@ -518,8 +537,7 @@ using namespace ktk;
 
 extern "C" size_t ktk_evict_workspace_bytes(const ktk_shape* shape, int32_t max_pages_per_seq, int32_t keep) {
     if (check_shape(shape, "ktk_evict_workspace_bytes") != KTK_OK || shape->batch == 0 || keep < 1 || max_pages_per_seq < 1) return 0;
-    const size_t units = (size_t)shape->batch * shape->num_kv_heads;
-    return units * (1 + 2 * (size_t)evict_max_moves(max_pages_per_seq, keep)) * sizeof(int32_t);
+    return evict_cut(shape, max_pages_per_seq, keep).bytes;
 }
 
 extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_t* kv_indptr, const int32_t* kv_last_page_len,
@@ -547,14 +565,14 @@ extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_
         return KTK_ERR_ARG;
     }
     if (max_pages_per_seq < 1) max_pages_per_seq = 1;
-    const int64_t units = (int64_t)s->batch * s->num_kv_heads;
-    if (max_pages_per_seq > kEvMaxPages || units > 2147483647LL) {
-        set_error("%s: %d pages per sequence (at most %d), %lld rows", who, max_pages_per_seq, kEvMaxPages, (long long)units);
+    const EvictCut cut = evict_cut(s, max_pages_per_seq, keep);
+    const int64_t parts = (cut.max_moves + kEvWarps * kEvEach - 1) / (kEvWarps * kEvEach);
+    if (max_pages_per_seq > kEvMaxPages || cut.units * (parts > 8 ? parts : 8) > 2147483647LL) {
+        set_error("%s: %d pages per sequence (at most %d), %lld rows", who, max_pages_per_seq, kEvMaxPages, (long long)cut.units);
         return KTK_ERR_TOO_LARGE;
     }
-    const size_t need = ktk_evict_workspace_bytes(s, max_pages_per_seq, keep);
-    if (workspace == nullptr || workspace_bytes < need) {
-        set_error("%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
+    if (cut.bytes > 0 && (workspace == nullptr || workspace_bytes < cut.bytes)) {
+        set_error("%s: workspace of %zu bytes needed, got %zu", who, cut.bytes, workspace ? workspace_bytes : (size_t)0);
         return KTK_ERR_WORKSPACE;
     }
     const View view = make_view(view_in);
@@ -565,32 +583,27 @@ extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_
     p.mass_in = mass->in; p.mass_out = mass->out; p.stride = mass->stride; p.rows = mass->rows;
     p.pos_in = positions_in; p.pos_out = positions_out; p.stored = stored; p.seen = seen;
     p.keep = keep; p.sink = sink; p.recent = recent; p.status = status;
-    p.max_moves = (int)evict_max_moves(max_pages_per_seq, keep);
+    p.max_moves = (int)cut.max_moves;
     p.count = (int32_t*)workspace;
-    p.from = p.count + units;
-    p.to = p.from + units * p.max_moves;
+    p.from = p.count + cut.units;
+    p.to = p.from + cut.units * p.max_moves;
+    p.smem_keys = 0;
 
-    const int64_t most = (int64_t)max_pages_per_seq * kPageSize;
     cudaStream_t st = (cudaStream_t)stream;
-    const int parts = (p.max_moves + kEvWarps * kEvEach - 1) / (kEvWarps * kEvEach);
-    if (units * (parts > 8 ? parts : 8) > 2147483647LL) {
-        set_error("%s: too many tokens to move in one launch", who);
-        return KTK_ERR_TOO_LARGE;
-    }
     const bool f32 = s->dtype == KTK_F32;
-    const int cluster = evict_cluster(units, most);
-    const bool fused = cluster == 1 && most <= 16384 && p.max_moves <= kEvFused;
-    if (most <= 4096) KTK_CUDA_TRY((launch_evict<256, 16>(p, units, cluster, fused, f32, st)), who);
-    else if (most <= 16384 * cluster) KTK_CUDA_TRY((launch_evict<1024, 16>(p, units, cluster, fused, f32, st)), who);
-    else {
-    const size_t bits = (size_t)((most + 31) / 32) * 2 * sizeof(uint32_t), room = 190 * 1024;
-    p.smem_keys = bits + most * sizeof(uint32_t) <= room ? (int)most : 0;
-    const size_t smem = bits + (size_t)p.smem_keys * sizeof(uint32_t);
-    KTK_CUDA_TRY(cudaFuncSetAttribute(evict_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
-    KTK_CUDA_TRY(launch_behind(false, evict_long_kernel, (unsigned)units, kEvLong, smem, st, p), who);
+    if (cut.most <= 4096) {
+        KTK_CUDA_TRY((launch_evict<256, 16>(p, cut.units, cut.cluster, cut.fused, f32, st)), who);
+    } else if (cut.most <= 16384 * cut.cluster) {
+        KTK_CUDA_TRY((launch_evict<1024, 16>(p, cut.units, cut.cluster, cut.fused, f32, st)), who);
+    } else {
+        const size_t bits = (size_t)((cut.most + 31) / 32) * 2 * sizeof(uint32_t), room = 190 * 1024;
+        p.smem_keys = bits + cut.most * sizeof(uint32_t) <= room ? (int)cut.most : 0;
+        const size_t smem = bits + (size_t)p.smem_keys * sizeof(uint32_t);
+        KTK_CUDA_TRY(cudaFuncSetAttribute(evict_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+        KTK_CUDA_TRY(launch_behind(false, evict_long_kernel, (unsigned)cut.units, kEvLong, smem, st, p), who);
     }
-    if (fused) return KTK_OK;
+    if (cut.fused) return KTK_OK;
     const auto move = f32 ? evict_move_kernel<32> : evict_move_kernel<16>;
-    KTK_CUDA_TRY(launch_behind(true, move, (unsigned)(units * parts), kEvWarps * 32, 0, st, p, parts), who);
+    KTK_CUDA_TRY(launch_behind(true, move, (unsigned)(cut.units * parts), kEvWarps * 32, 0, st, p, (int)parts), who);
     return KTK_OK;
 }

@@ -29,7 +29,7 @@ def _prefill(shape=None, mass=None, total=5, new=3, pages=4, window=0, scale=0.1
                                                   mass or _mass(), ONE, ws, bytes_, shape or _shape(**kw), NULL, NULL)
 
 
-def _evict(shape=None, mass=None, pos=ONE, pos_out=ONE, pages=4, keep=8, sink=0, recent=0, ws=ONE, bytes_=1 << 30, kv=ONE, **kw):
+def _evict(shape=None, mass=None, pos=ONE, pos_out=ONE, pages=40, keep=200, sink=0, recent=0, ws=ONE, bytes_=1 << 30, kv=ONE, **kw):
     return _lib.load().ktk_evict(kv, ONE, ONE, ONE, None, pages, mass or _mass(), pos, pos_out, ONE, ONE, keep, sink, recent, ws, bytes_,
                                  shape or _shape(**kw), NULL, NULL)
 
@@ -64,7 +64,7 @@ def test_each_ones_own():
     assert _evict(keep=8, sink=5, recent=4) == -1 and b"sink + recent" in text()
     assert _evict(sink=(1 << 31) - 1, recent=(1 << 31) - 1, keep=(1 << 31) - 1) == -1      # their sum passes 32 bits
     assert _evict(pos_out=ONE + 4) == -1 and b"positions" in text()
-    assert _evict(pages=40000) == -5
+    assert _evict(pages=40000) == -5 and _evict(pages=40000, keep=40000 * 16 - 1) == -5
     bad = _lib.View(16, 0, 0, 0, 0)
     assert _decode(view=bad) == -1
 
@@ -78,8 +78,9 @@ def test_workspaces_are_sized_by_what_is_given():
     assert lib.ktk_decode_mass_workspace_bytes(shp, 4000, 10 ** 9) == lib.ktk_decode_mass_workspace_bytes(shp, 4000, -1)
     assert ops.decode_mass_workspace_bytes(2, 1, 4, 4000, torch.bfloat16, 50) == small
     assert lib.ktk_decode_mass_workspace_bytes(_shape(head_dim=64), 4000, -1) == 0
-    assert lib.ktk_evict_workspace_bytes(shp, 4, 40) == 2 * 4 * (1 + 2 * 24)                      # 24 of 64 tokens can move
-    assert lib.ktk_evict_workspace_bytes(shp, 4, 10) == 2 * 4 * (1 + 2 * 10)
+    assert lib.ktk_evict_workspace_bytes(shp, 4, 40) == 0                                         # 24 of 64 tokens can move: one launch
+    assert lib.ktk_evict_workspace_bytes(shp, 40, 200) == 2 * 4 * (1 + 2 * 200)
+    assert lib.ktk_evict_workspace_bytes(shp, 40, 500) == 2 * 4 * (1 + 2 * 140)
     # weights of few rows need their denominators only; of many, and few keys, sums over parts
     rows = lib.ktk_prefill_mass_workspace_bytes(shp, 10, 10, 4, -1, 0)
     assert rows == 768 and lib.ktk_prefill_mass_workspace_bytes(shp, 10, 10, 4, -1, 3) == rows     # 40 rows of 16 bytes
