@@ -7,6 +7,10 @@
 // each, and prefix sums over the bits' words number the holes and the tokens that move.
 // Keys and values are copied a warp to a token: by the planning CTA where few can move, else by a launch of their own, whose many
 // warps hide the chain of loads (list, page table, cache) that each copy is.
+//
+// Two copies of a row per token are what an eviction cannot do without: 48 sequences of 2304 tokens cut to 2048, 8 kv heads, 101 MB: the
+// copies near HBM's rate (some 17 us), the plan in front of them some 13, most of it the latency of its steps (loads 4, three digits 3,
+// numbers and lists 3).
 #include <cooperative_groups.h>
 
 #include "ktk_decode.cuh"
@@ -295,48 +299,50 @@ __device__ __forceinline__ void token_move(const uint32_t* stay, const uint32_t*
     }
 }
 
-// Tokens of a warp's copies, their loads in flight together
-constexpr int kEvEach = 4;
-// Copies keys and values of moves first .. first + kEvEach - 1 (of `moves`): from(i) -> to(i).  CHUNKS: 16-byte pieces of a token's key
-// (as many of its value)
+// Tokens of a warp's copies, their loads in flight together: as many as two lanes each can look up
+constexpr int kEvEach = 8;
+// Copies keys and values of moves first .. first + kEvEach - 1 (of `moves`): from(i) -> to(i), by a whole warp.  Two lanes find where a move
+// leads, all lanes then copy.  CHUNKS: 16-byte pieces of a token's key (as many of its value)
 template <int CHUNKS, class From, class To>
 __device__ __forceinline__ void copy_tokens(const EvictParams& p, int h, int start, int first_fill, int first, int moves, From from, To to) {
     constexpr int kLoads = 2 * CHUNKS / 32;
     const int lane = threadIdx.x & 31;
     uint4* cache = (uint4*)p.cache;
-    // the 16-byte piece `c` of the token in place t: its key's, then its value's; -1: no such page
-    const auto piece = [&](int t, int c) -> int64_t {
+    int64_t at = -1;                                 // first piece of the token's key; -1: no such page
+    const int move = first + lane / 2;
+    if (lane < 2 * kEvEach && move < moves) {
         int e, slot;
-        page_of_pos(t, first_fill, e, slot);
+        page_of_pos(lane % 2 ? to(move) : from(move), first_fill, e, slot);
         const int64_t page = __ldg(p.kv_indices + start + e);
-        if (page < 0 || page >= p.num_pages) return -1;
-        return (((page * 2 + c / CHUNKS) * kPageSize + slot) * p.Hkv + h) * CHUNKS + c % CHUNKS;
-    };
+        if (page < 0 || page >= p.num_pages) report(p.status, KTK_STATUS_BAD_PAGE);
+        else at = ((page * 2 * kPageSize + slot) * p.Hkv + h) * CHUNKS;
+    }
+    const int64_t to_value = (int64_t)kPageSize * p.Hkv * CHUNKS;                // from a token's key to its value
+    int64_t mine[kLoads];                            // this lane's pieces from the first on
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+        const int c = j * 32 + lane;
+        mine[j] = c < CHUNKS ? c : to_value + c - CHUNKS;
+    }
     uint4 v[kEvEach][kLoads];
-    int64_t dst[kEvEach][kLoads];
 #pragma unroll
     for (int i = 0; i < kEvEach; ++i) {
-        const bool on = first + i < moves;
-        const int s = on ? from(first + i) : 0, d = on ? to(first + i) : 0;
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            dst[i][j] = -1;
-            if (!on) continue;
-            const int64_t src = piece(s, j * 32 + lane);
-            if (src >= 0) dst[i][j] = piece(d, j * 32 + lane);
-            if (dst[i][j] >= 0) v[i][j] = cache[src];
-            else report(p.status, KTK_STATUS_BAD_PAGE);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kEvEach; ++i)
+        const int64_t src = __shfl_sync(0xffffffffu, at, 2 * i);
 #pragma unroll
         for (int j = 0; j < kLoads; ++j)
-            if (dst[i][j] >= 0) cache[dst[i][j]] = v[i][j];
+            if (src >= 0) v[i][j] = cache[src + mine[j]];
+    }
+#pragma unroll
+    for (int i = 0; i < kEvEach; ++i) {
+        const int64_t src = __shfl_sync(0xffffffffu, at, 2 * i), dst = __shfl_sync(0xffffffffu, at, 2 * i + 1);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j)
+            if (src >= 0 && dst >= 0) cache[dst + mine[j]] = v[i][j];
+    }
 }
 
-// The planning CTA copies at most this many tokens; more go to a launch of their own.  2049 tokens cut to 2048, 8 kv heads: 11.8 us in
-// one launch, 14 in two; 48 sequences of 2304 tokens cut to 2048: 48 us and 37; 7 of 700 cut to 333, fp32: 28 us and 13.
+// The planning CTA copies at most this many tokens; more go to a launch of their own.  Device time, 8 kv heads, one launch and two: 2049
+// tokens cut to 2048 11.7 us and 12.8; 2304 cut to 2048 17.5 and 11.5, of 48 sequences 42.0 and 32.8.
 constexpr int kEvFused = 64;
 
 // Sequences of at most THREADS * ITEMS tokens per CTA of the cluster, keys in registers.  CHUNKS: 16-byte pieces of a token's key; 0:
@@ -397,8 +403,8 @@ evict_kernel(const EvictParams p, int cluster) {
     __syncthreads();
     const int moves = number_moves<THREADS>(stay, level, first, n > 0 ? (n + 31) / 32 : 0, keep, keep - at.above, cl, shared, buf, turn);
     __syncthreads();
-    __shared__ int32_t list[CHUNKS > 0 ? 2 * kEvFused : 1];
-    int32_t *from = CHUNKS > 0 ? list : p.from + unit * p.max_moves, *to = CHUNKS > 0 ? list + kEvFused : p.to + unit * p.max_moves;
+    extern __shared__ int32_t ev_list[];             // of a CTA that copies
+    int32_t *from = CHUNKS > 0 ? ev_list : p.from + unit * p.max_moves, *to = CHUNKS > 0 ? ev_list + p.max_moves : p.to + unit * p.max_moves;
     each_item([&](int, int i) {
         if (i < n) token_move(stay, level, first, t0 + i, keep, [&](int k) { to[k] = t0 + i; }, [&](int k) { from[k] = t0 + i; });
     });
@@ -497,7 +503,8 @@ evict_move_kernel(const EvictParams p, int parts) {
 template <int THREADS, int ITEMS>
 static cudaError_t launch_evict(const EvictParams& p, int64_t units, int cluster, bool fused, bool f32, cudaStream_t st) {
     const auto kernel = !fused ? evict_kernel<THREADS, ITEMS, 0> : f32 ? evict_kernel<THREADS, ITEMS, 32> : evict_kernel<THREADS, ITEMS, 16>;
-    return launch_cluster(units * cluster <= sm_count(), kernel, (unsigned)(units * cluster), THREADS, 0, cluster, st, p, cluster);
+    const size_t smem = fused ? 2 * (size_t)p.max_moves * sizeof(int32_t) : 0;
+    return launch_cluster(units * cluster <= sm_count(), kernel, (unsigned)(units * cluster), THREADS, smem, cluster, st, p, cluster);
 }
 
 static int64_t evict_max_moves(int max_pages, int keep) {
