@@ -560,7 +560,7 @@ typedef struct ktk_mass {
  * The weights are those of fp32 scores and denominators.
  *   total_pages  an upper bound of the entries in all lists (sizes the workspace), or -1: batch * max_pages_per_seq, which is
  *                also what counts with view->page_count
- *   max_pages_per_seq  at least every sequence's page count; a longer list reports KTK_STATUS_BAD_TABLE and its results are void
+ *   max_pages_per_seq  at least every sequence's page count; a longer list reports KTK_STATUS_BAD_TABLE and its results are void; 2^26 at most
  *   workspace    ktk_decode_mass_workspace_bytes() bytes: the scores of all tokens, and the partials of lists that are cut; 0, and then
  *                it may be null, for lists that the device holds all at once (a cluster of CTAs each)
  * q, kv_cache, o and workspace are 16-byte aligned.
@@ -576,8 +576,11 @@ KTK_API int ktk_dense_decode_mass(const void* q, const void* kv_cache, const int
  *   out[r, h, t] = decay * in[r, h, t] + sum over the last `window` new tokens and the heads of group h of p(t)
  * for the tokens t that were there before, and without the first term for the sequence's new ones.  window 0: all new tokens.
  * A sequence without new tokens is left as it is.
- *   max_pages_per_seq, total_pages   upper bounds of one list's entries and of all lists' together (-1: batch * max_pages_per_seq,
- *                as with view->page_count); they size the grid and the workspace
+ *   max_new_tokens, max_pages_per_seq, total_pages   upper bounds of one sequence's new tokens, of one list's entries (2^26 at most)
+ *                and of all lists' together (-1: batch * max_pages_per_seq, as with view->page_count); they size the grid and the
+ *                workspace.  A sequence beyond them, or of tokens outside total_new_tokens, reports KTK_STATUS_BAD_TABLE; its masses
+ *                stay as they are
+ *   sm_scale     at least 1e-30
  *   workspace    ktk_prefill_mass_workspace_bytes() bytes: the rows' denominators, and sums over parts of the rows
  * q, kv_cache, o and workspace are 16-byte aligned.
  */
@@ -604,6 +607,7 @@ KTK_API int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr, i
  *   max_pages_per_seq   an upper bound of a sequence's pages, at most 32768 (a longer sequence reports KTK_STATUS_BAD_TABLE and is
  *                 left alone)
  *   workspace     ktk_evict_workspace_bytes() bytes: which token moves where; 0, and then it may be null, where few can move
+ * A token whose page id is none of the cache's reports KTK_STATUS_BAD_PAGE; its keys and values are not copied.
  * sink + recent <= keep, keep >= 1.  shape->group_size plays no part.
  */
 KTK_API size_t ktk_evict_workspace_bytes(const ktk_shape* shape, int32_t max_pages_per_seq, int32_t keep);

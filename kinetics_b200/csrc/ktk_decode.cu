@@ -144,7 +144,7 @@ decode_simt_kernel(const DecodeParams p, const typename MassArgument<MASS>::type
             s[g] = (tok < ntok) ? part[0] : -INFINITY;
         }
         if constexpr (MASS == kMassLong) {
-            if ((lane & 1) == 0 && tok < ntok && position + e < mp.positions) {
+            if ((lane & 1) == 0 && tok < ntok && position + e >= 0 && position + e < mp.positions) {
 #pragma unroll
                 for (int g = 0; g < G; ++g) mp.scores[((position + e) * kPageSize + tok) * G + g] = s[g];
             }

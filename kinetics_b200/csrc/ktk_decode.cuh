@@ -47,6 +47,8 @@ struct MassParams {
     int max_pages;               // the caller's bound of a list
 };
 
+constexpr int kMassMaxPages = 1 << 26;       // of a list: its tokens are counted in 32 bits
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // How the pages of one sequence split into always-attended and scored ones.

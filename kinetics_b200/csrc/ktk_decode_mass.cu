@@ -114,7 +114,7 @@ mass_finish_kernel(const StreamParams p, int chunks, int rounds, int merges, int
     const int row = m.slot_index ? m.slot_index[b] : b;
     const int t_begin = part * rounds * kMassTokens, t_end = min(t_begin + rounds * kMassTokens, tokens);
     if (t_begin >= t_end) return;
-    if (row < 0 || row >= m.rows || tokens > m.stride || start + el.cnt > m.positions) {
+    if (row < 0 || row >= m.rows || tokens > m.stride || start < 0 || start + el.cnt > m.positions) {
         if (tid == 0 && part == 0) report(d.status, KTK_STATUS_BAD_TABLE);
         return;
     }
@@ -285,6 +285,10 @@ extern "C" int ktk_dense_decode_mass(const void* q, const void* kv_cache, const 
         (rc = check_apart(mass->in, mass->out, (size_t)mass->rows * s->num_kv_heads * mass->stride * sizeof(float), who, "mass")) != KTK_OK)
         return rc;
     if (max_pages_per_seq < 1) max_pages_per_seq = 1;
+    if (max_pages_per_seq > kMassMaxPages) {
+        set_error("%s: %d pages per sequence, at most %d", who, max_pages_per_seq, kMassMaxPages);
+        return KTK_ERR_TOO_LARGE;
+    }
     const View view = make_view(view_in);
     if (view.page_count) total_pages = -1;                // padded
     const MassWorkspace w = mass_workspace(s, max_pages_per_seq, total_pages);

@@ -12,12 +12,12 @@ constexpr int kMassMaxCluster = 8;
 // fed.
 constexpr int kMassPage = 2 * kPageSize * kHeadDim * 2;
 // dynamic shared memory of a bf16 CTA with its share of a list of max_pages
-inline int mma_mass_smem(int stages, int max_pages, int cluster, int G) {
-    return 1024 + stages * kMassPage + (max_pages + cluster - 1) / cluster * kPageSize * G * (int)sizeof(float);
+inline int64_t mma_mass_smem(int stages, int max_pages, int cluster, int G) {
+    return 1024 + stages * kMassPage + (max_pages + cluster - 1) / cluster * (int64_t)(kPageSize * G * sizeof(float));
 }
 // bf16 CTAs that an SM holds, beside their static shared memory and what the system takes of it
 inline int mma_mass_per_sm(int stages, int max_pages, int cluster, int G) {
-    return 228 * 1024 / (mma_mass_smem(stages, max_pages, cluster, G) + 6 * 1024);
+    return (int)(228 * 1024 / (mma_mass_smem(stages, max_pages, cluster, G) + 6 * 1024));
 }
 
 // A CTA's share of a list: entries [e0, e1)

@@ -301,7 +301,7 @@ int launch_decode_mma_mass(const DecodeParams& p, const MassParams& m, int G, cu
     const auto fits = [&](int stages) { return mma_mass_per_sm(stages, m.max_pages, p.num_splits, G) >= per_sm; };
     // one CTA per SM leaves clusters little choice of SMs: not for more CTAs than half of them
     const int stages = 2 * ctas <= sm_count() && fits(16) ? 16 : fits(8) ? 8 : 4;
-    const int smem = mma_mass_smem(stages, m.max_pages, p.num_splits, G);
+    const int smem = (int)mma_mass_smem(stages, m.max_pages, p.num_splits, G);
     const auto kernel = stages == 16 ? decode_mma_kernel<16, 1, true> : stages == 8 ? decode_mma_kernel<8, 3, true> : decode_mma_kernel<4, 4, true>;
     KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
     const MmaParams mp{p, m, G};

@@ -150,7 +150,7 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                         const int ntok = entry_tokens(pc.el, pc.e_lo + j);
                         const int64_t position = cur.start + pc.e_lo + j;
                         float* at = p.m.scores + (position * kPageSize + gid) * G + 2 * tig;
-                        const bool on = 2 * tig < G && position < p.m.positions;
+                        const bool on = 2 * tig < G && position >= 0 && position < p.m.positions;
                         mma_consume_page_t<false, true, true>(
                             ms, stages + s * kStageBytes, ntok, qb, d.scale_log2, lane, ntok, ntok,
                             [&](float s00, float s01, float s10, float s11) {

@@ -41,7 +41,6 @@ struct EvictParams {
     int32_t* from;                    // [units][max_moves] their places
     int32_t* to;                      // [units][max_moves] the holes
     int max_moves;
-    int smem_keys;                    // of evict_long_kernel: keys that shared memory holds (0: none)
     int32_t* status;
 };
 
@@ -424,7 +423,7 @@ evict_kernel(const EvictParams p, int cluster) {
     }
 }
 
-// Longer ones: keys in shared memory, or made again in every pass.
+// Longer ones, whose keys fit neither registers nor shared memory: they are made again in every pass.
 constexpr int kEvLong = 1024;
 __global__ void __launch_bounds__(kEvLong)
 evict_long_kernel(const EvictParams p) {
@@ -442,13 +441,8 @@ evict_long_kernel(const EvictParams p) {
         return;
     }
     const int n = u.n, keep = p.keep, words = (n + 31) / 32;
-    uint32_t *stay = ev_smem, *level = stay + words, *keys = level + words;
-    const bool held = n <= p.smem_keys;
-    for (int t = tid; t < n; t += kEvLong) {
-        const EvictToken x = read_token(u, t);
-        if (held && n > keep) keys[t] = key_of(p, u, x);
-        if (t < keep) keep_token(p, u, t, x);
-    }
+    uint32_t *stay = ev_smem, *level = stay + words;
+    for (int t = tid; t < min(n, keep); t += kEvLong) keep_token(p, u, t, read_token(u, t));
     if (n <= keep) {
         if (tid == 0) p.count[unit] = 0;
         return;
@@ -458,7 +452,7 @@ evict_long_kernel(const EvictParams p) {
     const auto each = [&](auto visit) {
         for (int t0 = tid - lane; t0 < n; t0 += kEvLong) {
             const int t = t0 + lane;
-            visit(t, t >= n ? 0 : held ? keys[t] : key_of(p, u, read_token(u, t)));
+            visit(t, t >= n ? 0 : key_of(p, u, read_token(u, t)));
         }
     };
     int turn = 0;
@@ -543,7 +537,9 @@ static EvictCut evict_cut(const ktk_shape* s, int max_pages, int keep) {
 using namespace ktk;
 
 extern "C" size_t ktk_evict_workspace_bytes(const ktk_shape* shape, int32_t max_pages_per_seq, int32_t keep) {
-    if (check_shape(shape, "ktk_evict_workspace_bytes") != KTK_OK || shape->batch == 0 || keep < 1 || max_pages_per_seq < 1) return 0;
+    if (check_shape(shape, "ktk_evict_workspace_bytes") != KTK_OK || shape->batch == 0 || keep < 1 || max_pages_per_seq < 1 ||
+        max_pages_per_seq > kEvMaxPages)
+        return 0;
     return evict_cut(shape, max_pages_per_seq, keep).bytes;
 }
 
@@ -594,7 +590,6 @@ extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_
     p.count = (int32_t*)workspace;
     p.from = p.count + cut.units;
     p.to = p.from + cut.units * p.max_moves;
-    p.smem_keys = 0;
 
     cudaStream_t st = (cudaStream_t)stream;
     const bool f32 = s->dtype == KTK_F32;
@@ -603,9 +598,7 @@ extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_
     } else if (cut.most <= 16384 * cut.cluster) {
         KTK_CUDA_TRY((launch_evict<1024, 16>(p, cut.units, cut.cluster, cut.fused, f32, st)), who);
     } else {
-        const size_t bits = (size_t)((cut.most + 31) / 32) * 2 * sizeof(uint32_t), room = 190 * 1024;
-        p.smem_keys = bits + cut.most * sizeof(uint32_t) <= room ? (int)cut.most : 0;
-        const size_t smem = bits + (size_t)p.smem_keys * sizeof(uint32_t);
+        const size_t smem = (size_t)((cut.most + 31) / 32) * 2 * sizeof(uint32_t);
         KTK_CUDA_TRY(cudaFuncSetAttribute(evict_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
         KTK_CUDA_TRY(launch_behind(false, evict_long_kernel, (unsigned)cut.units, kEvLong, smem, st, p), who);
     }

@@ -166,8 +166,8 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
     if ((rc = check_mass(mass, who)) != KTK_OK || (rc = check_aligned({q, kv_cache, o, workspace}, who)) != KTK_OK ||
         (rc = check_apart(mass->in, mass->out, (size_t)mass->rows * s->num_kv_heads * mass->stride * sizeof(float), who, "mass")) != KTK_OK)
         return rc;
-    if (!(sm_scale != 0.0f && sm_scale - sm_scale == 0.0f)) {
-        set_error("%s: sm_scale %g: finite, and not 0", who, (double)sm_scale);
+    if (!(sm_scale >= 1e-30f && sm_scale - sm_scale == 0.0f)) {          // denominators are divided by it
+        set_error("%s: sm_scale %g: finite, at least 1e-30", who, (double)sm_scale);
         return KTK_ERR_ARG;
     }
     if (total_new_tokens < 0 || max_new_tokens < 1 || window < 0 || max_pages_per_seq < 1) {
@@ -183,7 +183,7 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
         return KTK_ERR_WORKSPACE;
     }
     const int64_t chunks = (max_pages_per_seq * kPageSize + kPsKeys - 1) / kPsKeys, ctas = chunks * s->batch * s->num_kv_heads;
-    if (max_pages_per_seq > (1 << 27) || ctas > 2147483647LL / 8) {
+    if (max_pages_per_seq > kMassMaxPages || ctas > 2147483647LL / 8) {
         set_error("%s: batch * num_kv_heads * max_pages_per_seq exceeds the grid limit", who);
         return KTK_ERR_TOO_LARGE;
     }
@@ -196,6 +196,7 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
     p.q = q; p.cache = kv_cache; p.q_indptr = q_indptr; p.kv_indices = kv_indices; p.kv_indptr = kv_indptr;
     p.kv_last_page_len = kv_last_page_len; p.page_count = view.page_count; p.sink_tokens = view.sink_tokens;
     p.batch = s->batch; p.Hkv = s->num_kv_heads; p.G = s->group_size; p.num_pages = s->num_pages; p.total_new = total_new_tokens;
+    p.max_new = max_new_tokens; p.max_pages = (int)max_pages_per_seq;
     p.scale_log2 = sm_scale * kLog2e; p.lse = lse; p.window = window; p.status = status;
     p.m.in = mass->in; p.m.out = mass->out; p.m.stride = mass->stride; p.m.rows = mass->rows;
     p.m.slot_index = view.slot_index; p.m.decay = mass->decay;

@@ -17,6 +17,7 @@ struct PrefillMassParams {
     int batch, Hkv, G;
     int64_t num_pages;
     int64_t total_new;
+    int max_new, max_pages;     // the caller's bounds
     float scale_log2;
     const void* lse;            // of the rows [total_new, Hq], see prefill_attention (ktk_decode.cuh)
     int window;
@@ -41,7 +42,9 @@ __device__ __forceinline__ bool mass_sequence(const PrefillMassParams& p, int b,
     s.base_pos = s.sp.total - s.n_new;
     s.row = p.m.slot_index ? p.m.slot_index[b] : b;
     s.counted = p.window > 0 && p.window < s.n_new ? s.n_new - p.window : 0;
-    if (s.sp.bad || s.base_pos < 0 || s.row < 0 || s.row >= p.m.rows || s.sp.total > p.m.stride) {
+    if (s.sp.bad || s.base_pos < 0 || s.sp.n_pages > p.max_pages || s.n_new > p.max_new || s.q0 < 0 ||
+        s.q0 + (int64_t)s.n_new > p.total_new ||
+        s.row < 0 || s.row >= p.m.rows || s.sp.total > p.m.stride) {
         if (first && threadIdx.x == 0) report(p.status, KTK_STATUS_BAD_TABLE);
         return false;
     }

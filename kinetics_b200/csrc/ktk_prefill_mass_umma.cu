@@ -87,7 +87,7 @@ __device__ __forceinline__ bool find_group(const PrefillMassParams& p, int group
         int mine = 0;
         if (i < p.batch && p.q_indptr[i + 1] > p.q_indptr[i]) {
             const int pages = p.page_count ? p.page_count[i] : p.kv_indptr[i + 1] - p.kv_indptr[i];
-            mine = pages > 0 ? (pages + 2 * kPmPages - 1) / (2 * kPmPages) : 0;
+            mine = pages > p.max_pages ? 1 : pages > 0 ? (pages + 2 * kPmPages - 1) / (2 * kPmPages) : 0;     // too many: one to say so
         }
         int upto = mine;
 #pragma unroll

@@ -378,6 +378,15 @@ def _address(t, dev: int) -> int:
 _current_device, _current_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
 
 
+def _view_of(view, dev: int):
+    """The view as the library takes it, its tensors on device `dev`."""
+    if view is None:
+        return None
+    _address(view.page_count, dev)
+    _address(view.slot_index, dev)
+    return view.c()
+
+
 def _needs_cuda(t) -> None:
     if not t.is_cuda:
         raise RuntimeError("kinetics_b200 ops need CUDA tensors: this path has no CPU fallback")
@@ -426,13 +435,18 @@ def _decode_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dty
 
 @functools.lru_cache(maxsize=1024)
 def _prefill_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dtype, slots, padded, tables, max_new, window):
-    """(sizes, pages of the longest list, of all lists or -1, workspace bytes)"""
+    """(sizes, pages of the longest list, of all lists or -1, workspace bytes, launches)"""
     _check_queries(q_shape, q_dtype, kv_shape, kv_dtype)
     batch = tables[3][2] - 1
     shp = _mass_shape(batch, kv_shape, kv_dtype, q_shape[1], mass_shape, mass_dtype, slots, tables)
     pages = -1 if padded else tables[0][2]
-    most = mass_shape[2] // PAGE_SIZE + 2 if padded else max(pages, 1)
-    return shp, most, pages, int(_lib.load().ktk_prefill_mass_workspace_bytes(shp, q_shape[0], max_new, most, pages, window))
+    most = mass_shape[2] // PAGE_SIZE + 2              # a longer list than mass has places for is an error
+    if not padded:
+        most = max(min(most, pages), 1)
+    need = int(_lib.load().ktk_prefill_mass_workspace_bytes(shp, q_shape[0], max_new, most, pages, window))
+    # bf16: attention, sums, and where they come in parts their addition (beside 16 bytes a row, rounded up to 256); fp32: rows, attention, sums
+    parts = shp.dtype == _lib.KTK_F32 or need > (q_shape[0] * q_shape[1] * 16 + 255) // 256 * 256
+    return shp, most, pages, need, 3 if parts else 2
 
 
 @functools.lru_cache(maxsize=1024)
@@ -497,154 +511,9 @@ def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     check(_lib.load().ktk_dense_decode_mass(
         q_, _address(kv_cache, dev), _address(kv_indices, dev), _address(kv_indptr, dev), _address(kv_last_page_len, dev),
-        None if view is None else view.c(), max_pages_per_seq, pages, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
+        _view_of(view, dev), max_pages_per_seq, pages, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
         _lib.Mass(m_, mo_, mass_shape[2], mass_shape[0], decay), _address(out, dev), _address(workspace, dev),
         0 if workspace is None else workspace.nbytes, shp, _address(status, dev), _current_stream(dev)))
-    _launched(2 if need else 1)
-    return out
-
-
-# ---- a cache of bounded size: attention that adds up what tokens were paid, and the eviction that goes by it
-# A decode step of few sequences takes the device some ten microseconds, a Python attribute a tenth of one: these calls look at each
-# tensor once, and what follows from sizes and types alone (checks, the C struct, the workspace's size) is worked out once per set
-# of them.
-
-def _address(t, dev: int) -> int:
-    """Address of a contiguous tensor on device `dev` (None: 0)."""
-    if t is None:
-        return 0
-    if t.get_device() != dev:
-        _needs_cuda(t)
-        raise RuntimeError(f"kinetics_b200: a tensor on {t.device}, the current device is cuda:{dev}")
-    if not t.is_contiguous():
-        raise RuntimeError("kinetics_b200 ops need contiguous tensors")
-    return t.data_ptr()
-
-
-_current_device, _current_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
-
-
-def _needs_cuda(t) -> None:
-    if not t.is_cuda:
-        raise RuntimeError("kinetics_b200 ops need CUDA tensors: this path has no CPU fallback")
-
-
-def _mass_shape(batch, kv_shape, dtype, num_q_heads, mass_shape, mass_dtype, slots, tables) -> Shape:
-    """The sizes of a call over `batch` sequences, checked.  mass fp32 [rows, Hkv, places]; without slots (view.slot_index) one row
-    per sequence.  tables: (dtype, entries wanted or None, entries) of index tensors."""
-    if len(kv_shape) != 5 or kv_shape[1] != 2:
-        raise ValueError("kv_cache must be [num_pages, 2, page_size, num_kv_heads, head_dim]")
-    hkv = kv_shape[3]
-    if num_q_heads % hkv:
-        raise ValueError(f"{num_q_heads} query heads do not divide into {hkv} kv heads")
-    if dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"kinetics_b200: dtype {dtype} not supported (float32 or bfloat16)")
-    if mass_dtype != torch.float32:
-        raise TypeError("mass is fp32")
-    if len(mass_shape) != 3 or mass_shape[1] != hkv:
-        raise ValueError(f"mass must be [rows, {hkv}, places], got {tuple(mass_shape)}")
-    if mass_shape[0] < batch and not slots:
-        raise ValueError(f"mass of {mass_shape[0]} rows for {batch} sequences")
-    for index_dtype, want, have in tables:
-        if index_dtype != torch.int32:
-            raise TypeError("page tables, counts and positions are int32")
-        if want is not None and have < want:
-            raise ValueError(f"a table of {have} entries, {want} expected")
-    return Shape(batch, hkv, num_q_heads // hkv, kv_shape[4], kv_shape[2],
-                 _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32, kv_shape[0])
-
-
-def _check_queries(q_shape, q_dtype, kv_shape, kv_dtype) -> None:
-    if len(q_shape) != 3 or q_shape[2] != kv_shape[-1]:
-        raise ValueError(f"q must be [rows, Hq, {kv_shape[-1]}], got {tuple(q_shape)}")
-    if q_dtype != kv_dtype:
-        raise TypeError("q and kv_cache must share a dtype")
-
-
-@functools.lru_cache(maxsize=1024)
-def _decode_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dtype, slots, padded, tables, max_pages):
-    """(sizes, pages of all lists or -1, workspace bytes)"""
-    _check_queries(q_shape, q_dtype, kv_shape, kv_dtype)
-    shp = _mass_shape(q_shape[0], kv_shape, kv_dtype, q_shape[1], mass_shape, mass_dtype, slots, tables)
-    pages = -1 if padded else tables[0][2]
-    return shp, pages, int(_lib.load().ktk_decode_mass_workspace_bytes(shp, max_pages, pages))
-
-
-@functools.lru_cache(maxsize=1024)
-def _prefill_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dtype, slots, padded, tables, max_new, window):
-    """(sizes, pages of the longest list, of all lists or -1, workspace bytes)"""
-    _check_queries(q_shape, q_dtype, kv_shape, kv_dtype)
-    batch = tables[3][2] - 1
-    shp = _mass_shape(batch, kv_shape, kv_dtype, q_shape[1], mass_shape, mass_dtype, slots, tables)
-    pages = -1 if padded else tables[0][2]
-    most = mass_shape[2] // PAGE_SIZE + 2 if padded else max(pages, 1)
-    return shp, most, pages, int(_lib.load().ktk_prefill_mass_workspace_bytes(shp, q_shape[0], max_new, most, pages, window))
-
-
-@functools.lru_cache(maxsize=1024)
-def _evict_plan(batch, kv_shape, kv_dtype, mass_shape, mass_dtype, positions_shape, slots, tables, max_pages, keep):
-    """(sizes, workspace bytes)"""
-    shp = _mass_shape(batch, kv_shape, kv_dtype, kv_shape[3], mass_shape, mass_dtype, slots, tables)
-    if positions_shape != mass_shape:
-        raise ValueError(f"positions {tuple(positions_shape)} must have the shape of mass {tuple(mass_shape)}")
-    return shp, int(_lib.load().ktk_evict_workspace_bytes(shp, max_pages, keep))
-
-
-def _tables(batch, kv_indices, kv_indptr, kv_last_page_len, view):
-    """Types and sizes of a page table: ((dtype, entries wanted, entries), ...)."""
-    if view is None:
-        return ((kv_indices.dtype, None, kv_indices.numel()), (kv_indptr.dtype, batch + 1, kv_indptr.numel()),
-                (kv_last_page_len.dtype, batch, kv_last_page_len.numel()))
-    padded = view.page_count is not None
-    more = tuple((t.dtype, batch, t.numel()) for t in (view.page_count, view.slot_index) if t is not None)
-    return ((kv_indices.dtype, None, kv_indices.numel()), (kv_indptr.dtype, batch if padded else batch + 1, kv_indptr.numel()),
-            (kv_last_page_len.dtype, batch, kv_last_page_len.numel())) + more
-
-
-def _same(t, like, what) -> None:
-    if t.dtype != like.dtype or t.shape != like.shape:
-        raise TypeError(f"{what} must have the dtype and shape {like.dtype} {tuple(like.shape)}, got {t.dtype} {tuple(t.shape)}")
-
-
-def decode_mass_workspace_bytes(batch: int, num_kv_heads: int, group_size: int, max_pages_per_seq: int, dtype=torch.bfloat16,
-                                total_pages: int = -1) -> int:
-    """Bytes of workspace that ``dense_decode_mass`` needs; total_pages: entries of all page lists (-1, and always with a
-    view.page_count: batch * max_pages_per_seq)."""
-    shp = Shape(batch, num_kv_heads, group_size, HEAD_DIM, PAGE_SIZE, _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32, 0)
-    return int(_lib.load().ktk_decode_mass_workspace_bytes(shp, max_pages_per_seq, total_pages))
-
-
-def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: int, mass, decay: float = 1.0,
-                      sm_scale: Optional[float] = None, mass_out=None, workspace=None, out=None, status=None, view=None):
-    """``dense_decode`` that also accumulates the weights every cached token was given.
-
-    mass fp32 [rows, Hkv, places]: what the query heads of a group have paid the token in each place of its sequence
-    (row: view.slot_index, else the sequence's number; different rows for different sequences).  Writes
-    decay * mass + the weights of this step, and the weights alone for the newest token, to mass_out (None: mass itself);
-    places behind a sequence's length are left as they are.  workspace: ``ktk_decode_mass_workspace_bytes`` bytes, not shared
-    by calls that may overlap (None: from the allocator, which keeps streams and graphs apart).  Returns (out, mass_out)."""
-    _needs_cuda(q)
-    slots = view is not None and view.slot_index is not None
-    padded = view is not None and view.page_count is not None
-    shp, pages, need = _decode_mass_plan(q.shape, q.dtype, kv_cache.shape, kv_cache.dtype, mass.shape, mass.dtype, slots, padded,
-                                         _tables(len(q), kv_indices, kv_indptr, kv_last_page_len, view), max_pages_per_seq)
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        _same(out, q, "out")
-    if mass_out is None:
-        mass_out = mass
-    else:
-        _same(mass_out, mass, "mass_out")
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    dev = _current_device()
-    m_ = _address(mass, dev)
-    check(_lib.load().ktk_dense_decode_mass(
-        _address(q, dev), _address(kv_cache, dev), _address(kv_indices, dev), _address(kv_indptr, dev), _address(kv_last_page_len, dev),
-        None if view is None else view.c(), max_pages_per_seq, pages, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
-        _lib.Mass(m_, m_ if mass_out is mass else _address(mass_out, dev), mass.shape[2], mass.shape[0], decay), _address(out, dev),
-        _address(workspace, dev), 0 if workspace is None else workspace.nbytes, shp, _address(status, dev), _current_stream(dev)))
     _launched(2 if need else 1)
     return out, mass_out
 
@@ -657,7 +526,7 @@ def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indice
     weights alone.  Returns (out, mass_out)."""
     q_shape, mass_shape = q.shape, mass.shape
     i_, p_, l_, *more = _tables(q_indptr.numel() - 1, kv_indices, kv_indptr, kv_last_page_len, view)
-    shp, most, pages, need = _prefill_mass_plan(q_shape, q.dtype, kv_cache.shape, kv_cache.dtype, mass_shape, mass.dtype,
+    shp, most, pages, need, launches = _prefill_mass_plan(q_shape, q.dtype, kv_cache.shape, kv_cache.dtype, mass_shape, mass.dtype,
                                                 view is not None and view.slot_index is not None,
                                                 view is not None and view.page_count is not None,
                                                 (i_, p_, l_, (q_indptr.dtype, None, q_indptr.numel()), *more), max_new_tokens, window)
@@ -677,10 +546,10 @@ def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indice
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     check(_lib.load().ktk_prefill_attention_mass(
         q_, _address(q_indptr, dev), q_shape[0], max_new_tokens, _address(kv_cache, dev), _address(kv_indices, dev), _address(kv_indptr, dev),
-        _address(kv_last_page_len, dev), None if view is None else view.c(), most, pages, window,
+        _address(kv_last_page_len, dev), _view_of(view, dev), most, pages, window,
         HEAD_DIM ** -0.5 if sm_scale is None else sm_scale, _lib.Mass(m_, mo_, mass_shape[2], mass_shape[0], decay), _address(out, dev),
         _address(workspace, dev), workspace.nbytes, shp, _address(status, dev), _current_stream(dev)))
-    _launched(2 if shp.dtype == _lib.KTK_BF16 else 3)
+    _launched(launches)
     return out, mass_out
 
 
@@ -718,7 +587,7 @@ def evict(kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: 
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=kv_cache.device)
     check(_lib.load().ktk_evict(
-        kv_, _address(kv_indices, dev), _address(kv_indptr, dev), _address(kv_last_page_len, dev), None if view is None else view.c(),
+        kv_, _address(kv_indices, dev), _address(kv_indptr, dev), _address(kv_last_page_len, dev), _view_of(view, dev),
         max_pages_per_seq, _lib.Mass(m_, mo_, mass_shape[2], rows, 1.0), at_, ato_, _address(stored, dev), _address(seen, dev), keep, sink,
         recent, _address(workspace, dev), 0 if workspace is None else workspace.nbytes, shp, _address(status, dev), _current_stream(dev)))
     _launched(2 if need else 1)

@@ -327,6 +327,52 @@ def test_bad_tables_are_reported_and_touch_nothing_else(cuda_device, dtype, faul
         assert torch.equal(mass2[:, :, 700:width], bad["mass"][:, :, 700:width])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_new_tokens_than_the_bound(cuda_device, dtype):
+    # sequences of 33 and 40 new tokens are within it; the masses of the one of 200 stay as they are
+    from kinetics_b200 import ops
+    s, status = _state(8, cuda_device, dtype=dtype), ops.new_status(cuda_device)
+    _, mass = ops.prefill_attention_mass(s["qs"], s["indptr"], 40, *s["table"], s["mass"], mass_out=s["mass"].clone(), status=status)
+    assert int(status.item()) == 2
+    status.zero_()
+    _, want = ops.prefill_attention_mass(s["qs"], s["indptr"], 200, *s["table"], s["mass"], mass_out=s["mass"].clone(), status=status)
+    ops.raise_on_status(status)
+    assert torch.equal(mass[2], s["mass"][2])
+    torch.testing.assert_close(mass[:2], want[:2], rtol=1e-5, atol=1e-6)      # other parts, other orders of fp32 sums
+
+
+def test_nothing_to_do(cuda_device):
+    from kinetics_b200 import ops
+    s = _state(9, cuda_device)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    before, status = s["mass"].clone(), ops.new_status(cuda_device)
+    out, _ = ops.prefill_attention_mass(s["qs"][:0], i32(0, 0, 0, 0), 1, *s["table"], s["mass"], status=status)
+    assert out.shape == (0, 8, D)
+    none = (s["table"][0], i32(), i32(0), i32())
+    out, _ = ops.dense_decode_mass(s["q"][:0], *none, 1, s["mass"], status=status)
+    assert out.shape == (0, 8, D)
+    out, _ = ops.prefill_attention_mass(s["qs"][:0], i32(0), 1, *none, s["mass"], status=status)
+    ops.evict(*none, 1, s["mass"], s["positions"], s["stored"], s["seen"], 500, status=status)
+    ops.raise_on_status(status)
+    assert torch.equal(s["mass"], before)
+
+
+def test_launches_are_counted(cuda_device):
+    from kinetics_b200 import ops
+    s = _state(10, cuda_device)
+
+    def count(call):
+        before = ops.launch_count()
+        call()
+        return ops.launch_count() - before
+    decode = lambda most: ops.dense_decode_mass(s["q"], *s["table"], most, s["mass"])
+    prefill = lambda window: ops.prefill_attention_mass(s["qs"], s["indptr"], s["new"], *s["table"], s["mass"], window=window)
+    evict = lambda keep: ops.evict(*s["table"], s["most"], s["mass"], s["positions"], s["stored"], s["seen"], keep)
+    assert [count(lambda: decode(most)) for most in (s["most"], 30000)] == [1, 2]
+    assert [count(lambda: prefill(window)) for window in (20, 0)] == [2, 3]           # 800 rows in parts of 512
+    assert [count(lambda: evict(keep)) for keep in (1300, 500)] == [1, 2]
+
+
 def test_refusals_on_the_device(cuda_device):
     from kinetics_b200 import _lib, ops
     s = _state(7, cuda_device)

@@ -109,6 +109,29 @@ def test_decode_accumulates(cuda_device, lens, kv_heads, group, dtype, sink, pad
     assert inplace is mass and torch.equal(again, out) and torch.equal(mass.nan_to_num(-1), mass_out.nan_to_num(-1))
 
 
+@pytest.mark.parametrize("lens, kv_heads, group, dtype, sink, padded", [case for case in DECODE if case[0] != [20000]])
+def test_decode_with_a_bound_far_above_the_lists(cuda_device, lens, kv_heads, group, dtype, sink, padded):
+    # the form whose scores go to memory, of the same lists
+    from kinetics_b200 import ops
+    dev, new = cuda_device, [1 if n else 0 for n in lens]
+    c = _case(4, lens, new, kv_heads, group, dtype, sink, rows=len(lens) + 3)
+    c["q_indptr"] = torch.arange(len(lens) + 1, dtype=torch.int32)
+    q = torch.zeros(len(lens), kv_heads * group, D, dtype=dtype)
+    q[[b for b, w in enumerate(new) if w]] = c["q"]
+    c["q"] = q
+    d, view, status = to_dev(c["st"], dev), _view(c, lens, sink, dev, padded), ops.new_status(dev)
+    bound = 8000 if len(lens) < 10 else 1500
+    if dtype == torch.float32:
+        bound = 100000 // group
+    assert ops.decode_mass_workspace_bytes(len(lens), kv_heads, group, bound, dtype) > 0
+    indptr = d["kv_indptr"][:-1].contiguous() if padded else d["kv_indptr"]
+    out, mass_out = ops.dense_decode_mass(q.to(dev), d["kv_cache"], d["kv_indices"], indptr, d["kv_last_page_len"], bound, c["mass"].to(dev),
+                                          0.75, D ** -0.5, status=status, view=view)
+    ops.raise_on_status(status)
+    _check(c, out, mass_out, lens, new, kv_heads, group, dtype, 0, 0.75, D ** -0.5)
+    assert not out[[b for b, n in enumerate(lens) if n == 0]].any()
+
+
 PREFILL = [
     # tokens in all, new ones, kv heads, group, dtype, window, sink page, page counts
     ([1], [1], 1, 1, torch.bfloat16, 0, 0, False),
@@ -185,6 +208,9 @@ EVICT = [
     ([9000], 1, torch.float32, 4500, 4, 1000, 4000, 0, False, False),
     ([70000], 1, torch.bfloat16, 4096, 4, 512, 0, 0, False, True),
     ([31, 32, 33, 64, 65], 1, torch.bfloat16, 31, 2, 3, 7, 0, False, True),
+    ([40, 33, 31], 3, torch.float32, 32, 2, 3, 7, 0, False, True),
+    ([5040] + [100] * 39, 2, torch.bfloat16, 5000, 4, 100, 0, 0, False, True),
+    ([5040] + [100] * 39, 2, torch.float32, 4000, 4, 100, 2000, 0, False, True),
 ]
 
 

@@ -55,11 +55,11 @@ def test_sizes_and_pointers(call):
 def test_each_ones_own():
     text = _lib.load().ktk_last_error
     assert _decode(q=None) == -1 and _prefill(q=ONE + 2) == -1 and _evict(kv=ONE + 2) == -1
-    for scale in (0.0, float("nan"), float("inf")):
+    for scale in (0.0, -0.1, 1e-31, float("nan"), float("inf")):
         assert _prefill(scale=scale) == -1 and b"sm_scale" in text()
     assert _prefill(total=0) == 0
     assert _prefill(window=-1) == -1 and _prefill(new=0) == -1 and _prefill(pages=0) == -1
-    assert _prefill(pages=1 << 40) == -5
+    assert _prefill(pages=1 << 40) == -5 and _decode(pages=(1 << 26) + 1) == -5 and _decode(pages=(1 << 31) - 1) == -5
     assert _evict(keep=0) == -1 and _evict(sink=-1) == -1 and _evict(recent=-1) == -1
     assert _evict(keep=8, sink=5, recent=4) == -1 and b"sink + recent" in text()
     assert _evict(sink=(1 << 31) - 1, recent=(1 << 31) - 1, keep=(1 << 31) - 1) == -1      # their sum passes 32 bits
@@ -81,6 +81,9 @@ def test_workspaces_are_sized_by_what_is_given():
     assert lib.ktk_evict_workspace_bytes(shp, 4, 40) == 0                                         # 24 of 64 tokens can move: one launch
     assert lib.ktk_evict_workspace_bytes(shp, 40, 200) == 2 * 4 * (1 + 2 * 200)
     assert lib.ktk_evict_workspace_bytes(shp, 40, 500) == 2 * 4 * (1 + 2 * 140)
+    assert lib.ktk_evict_workspace_bytes(shp, 32769, 500) == 0                                    # refused
+    # a share of scores in bytes passes 32 bits: no list of that length is kept in shared memory
+    assert lib.ktk_decode_mass_workspace_bytes(_shape(group_size=8, batch=1), 1 << 26, 100) > 0
     # weights of few rows need their denominators only; of many, and few keys, sums over parts
     rows = lib.ktk_prefill_mass_workspace_bytes(shp, 10, 10, 4, -1, 0)
     assert rows == 768 and lib.ktk_prefill_mass_workspace_bytes(shp, 10, 10, 4, -1, 3) == rows     # 40 rows of 16 bytes
