@@ -260,13 +260,13 @@ extern "C" int ktk_prefill_attention(const void* q, const int32_t* q_indptr, int
                                      size_t workspace_bytes, int32_t variant, const ktk_shape* s, int32_t* status,
                                      void* stream) {
     return prefill_attention("ktk_prefill_attention", q, q_indptr, total_new_tokens, max_new_tokens, kv_cache, kv_indices, kv_indptr,
-                             kv_last_page_len, view_in, sm_scale, o, nullptr, workspace, workspace_bytes, variant, s, status, stream);
+                             kv_last_page_len, view_in, sm_scale, o, nullptr, 0, workspace, workspace_bytes, variant, s, status, stream);
 }
 
 int ktk::prefill_attention(const char* who, const void* q, const int32_t* q_indptr, int64_t total_new_tokens, int32_t max_new_tokens,
                            const void* kv_cache, const int32_t* kv_indices, const int32_t* kv_indptr,
                            const int32_t* kv_last_page_len, const ktk_view* view_in, float sm_scale, void* o, void* lse,
-                           void* workspace, size_t workspace_bytes, int32_t variant, const ktk_shape* s, int32_t* status,
+                           int64_t max_pages, void* workspace, size_t workspace_bytes, int32_t variant, const ktk_shape* s, int32_t* status,
                            void* stream) {
     int rc = check_shape(s, who);
     if (rc != KTK_OK) return rc;
@@ -302,6 +302,7 @@ int ktk::prefill_attention(const char* who, const void* q, const int32_t* q_indp
             u.kv_indptr = kv_indptr; u.kv_last_page_len = kv_last_page_len; u.page_count = view.page_count;
             u.sink_tokens = view.sink_tokens; u.batch = s->batch; u.total_new = total_new_tokens; u.Hkv = s->num_kv_heads; u.G = G;
             u.num_pages = s->num_pages; u.scale_log2 = sm_scale * kLog2e; u.status = status; u.lse = (uint4*)lse;
+            u.max_pages = max_pages;
             return launch_prefill_umma(u, max_new_tokens, st);
         }
         PrefillParams p;

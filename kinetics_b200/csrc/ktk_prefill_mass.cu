@@ -123,7 +123,7 @@ static int launch_prefill_mass_simt(const PrefillMassParams& p, int64_t ctas, in
     const char* who = "ktk_prefill_attention_mass";
     const int64_t rows = (int64_t)(p.window > 0 && p.window < max_new ? p.window : max_new) * p.G;
     int cluster = 1;
-    while (cluster < 8 && ctas * cluster < 2 * sm_count() && rows > (int64_t)kPsRows * cluster) cluster *= 2;
+    while (cluster < 8 && ctas * cluster <= sm_count() && rows > (int64_t)kPsRows * cluster) cluster *= 2;
     KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_mass_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPsSmem), who);
     KTK_CUDA_TRY(launch_cluster(false, prefill_mass_simt_kernel, (unsigned)(ctas * cluster), kPsThreads, kPsSmem, cluster, st, p, chunks, cluster),
                  who);
@@ -190,7 +190,7 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
     void* lse = workspace;
     char* behind = (char*)workspace + lse_bytes(s, total_new_tokens);
     rc = prefill_attention(who, q, q_indptr, total_new_tokens, max_new_tokens, kv_cache, kv_indices, kv_indptr, kv_last_page_len,
-                           view_in, sm_scale, o, lse, behind, need - lse_bytes(s, total_new_tokens), KTK_VARIANT_AUTO, s, status, stream);
+                           view_in, sm_scale, o, lse, max_pages_per_seq, behind, need - lse_bytes(s, total_new_tokens), KTK_VARIANT_AUTO, s, status, stream);
     if (rc != KTK_OK) return rc;
     PrefillMassParams p{};
     p.q = q; p.cache = kv_cache; p.q_indptr = q_indptr; p.kv_indices = kv_indices; p.kv_indptr = kv_indptr;

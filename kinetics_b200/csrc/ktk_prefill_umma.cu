@@ -7,6 +7,8 @@
 // is the operand layout tcgen05.mma reads).  The softmax and the order of the matrix instructions: ktk_flash.cuh.
 // Bound by the chain of a tile's block: matrix instructions, softmax, matrix instructions.  8192 tokens, 32 heads over 8 kv
 // heads: 489 us (1124 TFLOP/s), 855 us with one tile per CTA, blocks of 64 keys and two CTAs per SM.
+#include <cooperative_groups.h>
+
 #include "ktk_decode_mma.cuh"
 #include "ktk_flash.cuh"
 #include "ktk_prefill_umma.cuh"
@@ -74,16 +76,31 @@ __device__ __forceinline__ bool item_of_either(const PrefillUmmaParams& p, int& 
     return true;
 }
 
-// LSE: the rows' denominators are written too
-template <Order ORDER, bool LSE>
+// A row's minus log2 of its denominator over the scale, as three bf16 that add up to it
+__device__ __forceinline__ uint4 lse_of(float m, float l, float scale_log2) {
+    const float v = -(m + log2f(l)) / scale_log2;
+    const float hi = __bfloat162float(__float2bfloat16_rn(v)), mid = __bfloat162float(__float2bfloat16_rn(v - hi));
+    return make_uint4(pack_bf16(hi, mid), pack_bf16(v - hi - mid, 0.0f), 0u, 0u);
+}
+
+constexpr int kPuMaxCluster = 8, kPuSplit = 6;
+constexpr int kPuLd = kHeadDim + 4;                       // SPLIT: floats between a CTA's rows of outputs
+static_assert(2 * kUmRows * (kPuLd + 2 + kPuMaxCluster) * 4 <= kPuSmem - 1024, "outputs where queries and keys were");
+
+// LSE: the rows' denominators are written too.
+// SPLIT, for few rows behind many keys: each CTA of a cluster takes a part of the blocks of keys, at least two, and they join their outputs
+// through shared memory, every CTA some of the rows.  A block takes two tiles 2.1 us, the join 5, so a tile of fewer than kPuSplit blocks
+// stays with one CTA.  512 tokens of 32 heads over 8 behind 2048 46 us by one tile a CTA, 35 by two in clusters of two (10 blocks
+// each); 16 behind 8192 28.8 in clusters of eight.
+template <Order ORDER, bool LSE, bool SPLIT = false>
 __global__ void __launch_bounds__(kFlThreads, 1)
-prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorMap kv_map) {
+prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorMap kv_map, int cluster) {
     extern __shared__ uint8_t um_raw[];
     __shared__ __align__(8) FlashShared sh;
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(um_raw) + 1023) & ~uintptr_t(1023));
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int h = ORDER == kBySequence ? blockIdx.y : blockIdx.x;
+    const int h = ORDER == kBySequence ? blockIdx.y : SPLIT ? blockIdx.x / cluster : blockIdx.x;
     int b = ORDER == kBySequence ? blockIdx.z : blockIdx.y;
     int pair = ORDER == kBySequence ? (int)(gridDim.x - 1 - blockIdx.x) : (int)(gridDim.z - 1 - blockIdx.z);
     int item;
@@ -118,6 +135,18 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
         }
     }
 
+    int block0 = 0, ranks = 1;                      // SPLIT: the CTA's first block; CTAs of the cluster that have some
+    const int rank = SPLIT ? (int)(blockIdx.x % cluster) : 0;
+    if (SPLIT) {
+        const int blocks = (n_need + kPuPages - 1) / kPuPages;
+        ranks = blocks < kPuSplit ? 1 : min(cluster, blocks / 2);
+        if (ranks == 1 && rank > 0) return;         // the first CTA is alone
+        const int each = (blocks + ranks - 1) / ranks;
+        block0 = rank * each;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) keys[m] = max(min(keys[m] - block0 * kPuKeys, each * kPuKeys), 0);
+    }
+
     // a softmax thread's row
     const int tile = warp >> 2, row = tid & (kUmRows - 1);
     const int my_tok = tok0 + tile * tpc + row / G, my_head = h * G + row % G;
@@ -127,7 +156,7 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
     PrefillFlash fl(sh, sm, 2, 2, keys[0], keys[1]);
     // warp 9.  Lane i < 8: page i of a block; entries are read one block ahead of their first use
     auto entry = [&](int blk) {
-        const int e = blk * kPuPages + lane;
+        const int e = (block0 + blk) * kPuPages + lane;
         return lane < kPuPages && e < n_need ? p.kv_indices[sp.start + e] : -1;
     };
     int at[3], first = 0;                           // of blocks first, first + 1, first + 2
@@ -140,7 +169,7 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
         }
         const int pg = blk == first ? at[0] : (blk == first + 1 ? at[1] : at[2]);
         const bool on = pg >= 0 && pg < p.num_pages;
-        if (which == 0 && !on && lane < kPuPages && blk * kPuPages + lane < n_need) report(p.status, KTK_STATUS_BAD_PAGE);
+        if (which == 0 && !on && lane < kPuPages && (block0 + blk) * kPuPages + lane < n_need) report(p.status, KTK_STATUS_BAD_PAGE);
         const uint32_t pages = __popc(__ballot_sync(0xffffffffu, on));
         if (lane == 0) {
             if (pages) mbar_arrive_expect_tx(bar, pages * (2u * kPageSize * 128u));
@@ -174,7 +203,7 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
 #pragma unroll
         for (int i = 0; i < 3; ++i) at[i] = entry(i);
         __syncwarp();
-        fl.first_copies(load_k, load_v);
+        if (!SPLIT || fl.blocks() > 0) fl.first_copies(load_k, load_v);
     }
     tc_fence_before();
     __syncthreads();
@@ -190,7 +219,8 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
     } else {
         more_registers();
         const int tile_min_vis = base_pos + tok0 + tile * tpc + 1;
-        auto prepare = [&](float (&s)[kPuKeys], int j) {
+        auto prepare = [&](float (&s)[kPuKeys], int mine) {
+            const int j = block0 + mine;
             // column c of block j: position j * 128 + c - shift, but for the first page's own
             if ((j + 1) * kPuKeys - shift > tile_min_vis || (j == 0 && shift > 0)) {       // uniform for the tile
                 const int lim = (j == 0 && vis <= sp.first_fill) ? vis : vis + shift - j * kPuKeys;
@@ -205,7 +235,7 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
         };
         // the rows of V that hold no key: pages that are not read, the places of a page that is not full
         auto clear = [&](int j) {
-            const int e0 = j * kPuPages, e1 = e0 + kPuPages;
+            const int e0 = (block0 + j) * kPuPages, e1 = e0 + kPuPages;
             if (e1 <= n_need && !(e0 == 0 && shift > 0) && !(e1 == sp.n_pages && sp.last_fill != kPageSize)) return;
             fl.clear_rows(tile, j, [&](int r) {
                 const int e = e0 + r / kPageSize, slot = r % kPageSize;
@@ -214,13 +244,25 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
         };
         float m_ref = -INFINITY, l_run = 0.0f;
         const bool done = fl.softmax<false>(tile, p.scale_log2, m_ref, l_run, prepare, [](float&, float&) {}, clear);
-        if (done && fl.blocks_of(tile) > 0) {
-            const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-            if (LSE && row_on) {
-                const float v = -(m_ref + log2f(l_run)) / p.scale_log2;
-                const float hi = __bfloat162float(__float2bfloat16_rn(v)), mid = __bfloat162float(__float2bfloat16_rn(v - hi));
-                p.lse[(int64_t)(q0 + my_tok) * Hq + my_head] = make_uint4(pack_bf16(hi, mid), pack_bf16(v - hi - mid, 0.0f), 0u, 0u);
+        if (SPLIT && ranks > 1) {
+            // queries, keys and values of both tiles have been read
+            asm volatile("bar.sync 1, %0;" ::"n"(kFlSoftmaxWarps * 32) : "memory");
+            const bool some = done && fl.blocks_of(tile) > 0;
+            float* out = reinterpret_cast<float*>(sm) + tid * kPuLd;
+            const uint32_t o_at = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16) + kFlColO + tile * 128;
+            if (some) {
+#pragma unroll
+                for (int c = 0; c < kHeadDim; c += 32) {
+                    float o[32];
+                    tmem_ld32(o_at + c, o);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(out + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
             }
+            reinterpret_cast<float2*>(sm + 2 * kUmRows * kPuLd * 4)[tid] = make_float2(some ? m_ref : -INFINITY, l_run);
+        } else if (done && fl.blocks_of(tile) > 0) {
+            const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+            if (LSE && row_on) p.lse[(int64_t)(q0 + my_tok) * Hq + my_head] = lse_of(m_ref, l_run, p.scale_log2);
             const uint32_t o_at = sh.tmem + ((uint32_t)((warp & 3) * 32) << 16) + kFlColO + tile * 128;
             __nv_bfloat16* dst = (__nv_bfloat16*)p.o + ((int64_t)(q0 + (row_on ? my_tok : 0)) * Hq + my_head) * kHeadDim;
 #pragma unroll
@@ -241,6 +283,76 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
             }
         }
     }
+    if constexpr (SPLIT) {
+        if (ranks > 1) {
+            auto cl = cooperative_groups::this_cluster();
+            cl.sync();
+            const int rows = kUmRows * p.tiles, each = (rows + ranks - 1) / ranks, r0 = rank * each, n = min(each, rows - r0);
+            if (rank < ranks && warp < kFlSoftmaxWarps) {
+                constexpr int kAt = 2 * kUmRows * kPuLd;         // floats in front of maxima and sums
+                float* weights = reinterpret_cast<float*>(sm) + kAt + 4 * kUmRows;           // [row of this CTA][CTA], the outputs' factors
+                for (int i = tid; i < n; i += kFlSoftmaxWarps * 32) {
+                    const int r = r0 + i, tok = tok0 + r / kUmRows * tpc + r % kUmRows / G, head = h * G + r % G;
+                    float2 ml[kPuMaxCluster];
+                    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < kPuMaxCluster; ++k) {
+                        ml[k] = make_float2(-INFINITY, 0.0f);
+                        if (k < ranks) ml[k] = reinterpret_cast<const float2*>(cl.map_shared_rank(reinterpret_cast<const float*>(sm), k) + kAt)[r];
+                    }
+#pragma unroll
+                    for (int k = 0; k < kPuMaxCluster; ++k) M = fmaxf(M, ml[k].x);
+#pragma unroll
+                    for (int k = 0; k < kPuMaxCluster; ++k) {
+                        ml[k].x = ml[k].x == -INFINITY ? 0.0f : exp2f(ml[k].x - M);       // 0: a row that sees none of those keys
+                        L = fmaf(ml[k].y, ml[k].x, L);
+                    }
+                    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < kPuMaxCluster; ++k)
+                        if (k < ranks) weights[i * kPuMaxCluster + k] = ml[k].x * inv;
+                    if (tok < n_new) p.lse[(int64_t)(q0 + tok) * Hq + head] = lse_of(M, L, p.scale_log2);
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(kFlSoftmaxWarps * 32) : "memory");
+                // a warp to a row, four columns to a lane; kEach rows of all CTAs in flight
+                const auto join = [&](auto most) {
+                    constexpr int kMost = decltype(most)::value, kEach = 16 / kMost;
+                    const float* theirs[kMost];
+#pragma unroll
+                    for (int k = 0; k < kMost; ++k)
+                        theirs[k] = cl.map_shared_rank(reinterpret_cast<const float*>(sm), k < ranks ? k : 0) + r0 * kPuLd + lane * 4;
+                    for (int i0 = warp * kEach; i0 < n; i0 += kFlSoftmaxWarps * kEach) {
+                        float4 o[kEach][kMost];
+#pragma unroll
+                        for (int j = 0; j < kEach; ++j)
+#pragma unroll
+                            for (int k = 0; k < kMost; ++k) o[j][k] = *reinterpret_cast<const float4*>(theirs[k] + min(i0 + j, n - 1) * kPuLd);
+#pragma unroll
+                        for (int j = 0; j < kEach; ++j) {
+                            const int i = min(i0 + j, n - 1), r = r0 + i, tok = tok0 + r / kUmRows * tpc + r % kUmRows / G, head = h * G + r % G;
+                            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                            for (int k = 0; k < kMost; ++k) {
+                                const float a = k < ranks ? weights[i * kPuMaxCluster + k] : 0.0f;
+                                if (a == 0.0f) continue;                 // nothing was written there, or nothing that counts
+                                sum.x = fmaf(o[j][k].x, a, sum.x);
+                                sum.y = fmaf(o[j][k].y, a, sum.y);
+                                sum.z = fmaf(o[j][k].z, a, sum.z);
+                                sum.w = fmaf(o[j][k].w, a, sum.w);
+                            }
+                            if (i0 + j < n && tok < n_new)
+                                *reinterpret_cast<uint2*>((__nv_bfloat16*)p.o + ((int64_t)(q0 + tok) * Hq + head) * kHeadDim + lane * 4) =
+                                    make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
+                        }
+                    }
+                };
+                if (ranks <= 2) join(std::integral_constant<int, 2>());
+                else if (ranks <= 4) join(std::integral_constant<int, 4>());
+                else join(std::integral_constant<int, 8>());
+            }
+            cl.sync();                              // the others read until here
+        }
+    }
     tc_fence_before();
     __syncthreads();
     if (sh.abort && tid == 0) report(p.status, KTK_STATUS_TIMEOUT);
@@ -258,6 +370,12 @@ int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st
     const int64_t per_seq = ((int64_t)max_new_tokens + tpc - 1) / tpc, most = p.total_new / tpc + p.batch;
     const int64_t tiles = (p.batch * per_seq < most ? p.batch * per_seq : most) * p.Hkv;
     p.tiles = tiles <= sm_count() ? 1 : 2;
+    int cluster = 1;
+    if (p.lse != nullptr && p.max_pages >= kPuSplit * kPuPages) {        // as many CTAs as there are SMs, two blocks each
+        const int64_t ctas = (per_seq + 1) / 2 * p.batch * p.Hkv;
+        while (cluster < kPuMaxCluster && ctas * cluster * 2 <= sm_count() && p.max_pages >= 4 * kPuPages * cluster) cluster *= 2;
+        if (cluster > 1) p.tiles = 2;
+    }
     const unsigned pairs = (unsigned)((per_seq + p.tiles - 1) / p.tiles);
     // By length, if histories differ, where several sequences take between one round of CTAs and two and a half: the more rounds, the less
     // the last one leaves idle.  Six portions of 350 to 1050 tokens behind 2500 to 7500, 16 heads over 8: 255 us by tile, 229 by length
@@ -270,6 +388,7 @@ int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st
     auto kernel = either ? (lse ? prefill_umma_kernel<kByEither, true> : prefill_umma_kernel<kByEither, false>)
                   : by_tile ? (lse ? prefill_umma_kernel<kByTile, true> : prefill_umma_kernel<kByTile, false>)
                             : (lse ? prefill_umma_kernel<kBySequence, true> : prefill_umma_kernel<kBySequence, false>);
+    if (cluster > 1) kernel = prefill_umma_kernel<kByTile, true, true>;
     KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPuSmem), who);
     const dim3 grid = by_tile ? dim3((unsigned)p.Hkv, (unsigned)p.batch, pairs) : dim3(pairs, (unsigned)p.Hkv, (unsigned)p.batch);
     DecodeParams d{};                               // only what the tensor map needs
@@ -277,7 +396,12 @@ int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st
     CUtensorMap map;
     const int rc = make_kv_tensor_map(&map, d);
     if (rc != KTK_OK) return rc;
-    kernel<<<grid, kFlThreads, kPuSmem, st>>>(p, map);
+    if (cluster > 1) {
+        KTK_CUDA_TRY(launch_cluster(false, kernel, dim3((unsigned)(p.Hkv * cluster), (unsigned)p.batch, pairs), kFlThreads, kPuSmem, cluster,
+                                    st, p, map, cluster), who);
+        return KTK_OK;
+    }
+    kernel<<<grid, kFlThreads, kPuSmem, st>>>(p, map, 1);
     KTK_CUDA_TRY(cudaGetLastError(), who);
     return KTK_OK;
 }

@@ -22,6 +22,7 @@ struct PrefillUmmaParams {
     float scale_log2;
     int32_t* status;
     uint4* lse = nullptr;      // non-null: [total_new, Hq], see prefill_attention (ktk_decode.cuh)
+    int64_t max_pages = 0;     // with lse: a bound of a sequence's pages; 0: unknown
 };
 
 int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st);
