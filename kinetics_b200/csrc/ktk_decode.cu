@@ -41,16 +41,15 @@ __device__ __forceinline__ void halve(float (&part)[kPageSize], int lane) {
     }
 }
 
-// What a launch writes beside the outputs: nothing, minus log2 of the denominators (one split), or weights.  kMassLong: the scores go to
+// What a launch writes beside the outputs: nothing, or weights.  kMassLong: the scores go to
 // memory and all partials with them (ktk_decode_mass.cu); kMassCluster: the splits of a list are a cluster, scores stay in (dynamic)
 // shared memory.
-enum SimtMass { kMassNone, kMassLse, kMassLong, kMassCluster };
+enum SimtMass { kMassNone, kMassLong, kMassCluster };
 struct NoMass {
     static constexpr int max_pages = 0;
 };
 template <SimtMass MASS> struct MassArgument { using type = MassParams; };
 template <> struct MassArgument<kMassNone> { using type = NoMass; };
-template <> struct MassArgument<kMassLse> { using type = NoMass; };
 
 template <typename T, int G, SimtMass MASS>
 __global__ void __launch_bounds__(kSimtWarps * 32)
@@ -242,7 +241,6 @@ decode_simt_kernel(const DecodeParams p, const typename MassArgument<MASS>::type
             if (d == 0) { shared.ml[g][0] = M; shared.ml[g][1] = L; }
         } else if (MASS != kMassLong && S == 1) {
             ((T*)p.o)[qh * kHeadDim + d] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
-            if (MASS == kMassLse && d == 0) p.neg_lse[qh] = -(M + log2f(L));
         } else {
             p.ws_o[(qh * S + split) * kHeadDim + d] = O;
             if (d == 0) {
@@ -305,7 +303,6 @@ static int simt_group(const DecodeParams& p, const typename MassArgument<MASS>::
 }
 
 int launch_decode_simt(const DecodeParams& p, int dtype, int G, cudaStream_t st) {
-    if (p.neg_lse != nullptr) return simt_group<float, kMassLse>(p, {}, G, st);           // fp32, one split
     return dtype == KTK_F32 ? simt_group<float, kMassNone>(p, {}, G, st) : simt_group<__nv_bfloat16, kMassNone>(p, {}, G, st);
 }
 

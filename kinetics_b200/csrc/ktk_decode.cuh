@@ -163,8 +163,8 @@ int launch_decode_simt(const DecodeParams& p, int dtype, int G, cudaStream_t st)
 int launch_decode_simt_mass(const DecodeParams& p, const MassParams& m, int G, bool cluster, cudaStream_t st);    // fp32
 int launch_decode_mma_mass(const DecodeParams& p, const MassParams& m, int G, cudaStream_t st);                   // bf16, a cluster per list
 int launch_decode_mma(const DecodeParams& p, int G, cudaStream_t st);
-// What ktk_prefill_attention does, and with `lse`, for every variant but KTK_VARIANT_MMA, the logarithms of the rows' denominators
-// (and a bound of a sequence's pages, or 0) [total_new, Hq]: fp32 minus log2 of them; bf16 minus log2 of them over scale_log2, as 16 bytes: three bf16 that add up to it, and zeros.
+// What ktk_prefill_attention does, and with `lse`, bf16 and KTK_VARIANT_AUTO, minus the logarithms of the rows' denominators [total_new, Hq], over
+// scale_log2, as 16 bytes: three bf16 that add up to it, and zeros.  max_pages, with lse: a bound of a sequence's pages.
 int prefill_attention(const char* who, const void* q, const int32_t* q_indptr, int64_t total_new_tokens, int32_t max_new_tokens,
                       const void* kv_cache, const int32_t* kv_indices, const int32_t* kv_indptr, const int32_t* kv_last_page_len,
                       const ktk_view* view_in, float sm_scale, void* o, void* lse, int64_t max_pages, void* workspace, size_t workspace_bytes,

@@ -334,7 +334,7 @@ int ktk::prefill_attention(const char* who, const void* q, const int32_t* q_indp
     d.kv_indptr = rows; d.page_count = rows + total_new_tokens; d.kv_last_page_len = rows + 2 * total_new_tokens;
     d.topk = -1; d.entry_stride = 0; d.batch = (int)total_new_tokens; d.Hkv = s->num_kv_heads;
     d.num_pages = s->num_pages; d.scale_log2 = sm_scale * kLog2e; d.num_splits = 1;
-    d.ws_ml = nullptr; d.ws_o = nullptr; d.status = status; d.neg_lse = (float*)lse;
+    d.ws_ml = nullptr; d.ws_o = nullptr; d.status = status;
     d.sink_tokens = view.sink_tokens; d.local_tokens = view.local_tokens;
     return launch_decode_simt(d, s->dtype, G, st);
 }

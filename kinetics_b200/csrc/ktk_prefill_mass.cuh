@@ -7,6 +7,7 @@ namespace ktk {
 
 struct PrefillMassParams {
     const void* q;
+    void* o;                    // fp32
     const void* cache;
     const int32_t* q_indptr;
     const int32_t* kv_indices;
@@ -19,7 +20,7 @@ struct PrefillMassParams {
     int64_t total_new;
     int max_new, max_pages;     // the caller's bounds
     float scale_log2;
-    const void* lse;            // of the rows [total_new, Hq], see prefill_attention (ktk_decode.cuh)
+    void* lse;                  // of the rows [total_new, Hq]: bf16 see prefill_attention (ktk_decode.cuh), fp32 minus log2 of denominators
     int window;
     int32_t* status;
     MassParams m;
@@ -58,6 +59,7 @@ struct MassPlan {
     size_t partial;
 };
 MassPlan mass_plan(const ktk_shape* s, int max_new_tokens, int64_t max_pages, int64_t total_pages, int window);
+int launch_prefill_mass_f32(const PrefillMassParams& p, cudaStream_t st);      // attention and sums
 int launch_prefill_mass_umma(const PrefillMassParams& p, int64_t groups, cudaStream_t st);
 
 }  // namespace ktk

@@ -444,8 +444,8 @@ def _prefill_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dt
     if not padded:
         most = max(min(most, pages), 1)
     need = int(_lib.load().ktk_prefill_mass_workspace_bytes(shp, q_shape[0], max_new, most, pages, window))
-    # bf16: attention, sums, and where they come in parts their addition (beside 16 bytes a row, rounded up to 256); fp32: rows, attention, sums
-    parts = shp.dtype == _lib.KTK_F32 or need > (q_shape[0] * q_shape[1] * 16 + 255) // 256 * 256
+    # attention, sums, and where the workspace has parts of them beside the rows' 16 bytes, their addition
+    parts = need > (q_shape[0] * q_shape[1] * 16 + 255) // 256 * 256
     return shp, most, pages, need, 3 if parts else 2
 
 

@@ -26,8 +26,8 @@ def attend(q, k, v, n_new, window, scale, dtype):
     Scores: products of 16-bit values are exact in fp32, 128 of them are added with at most 2^-23 of the sum of their sizes each
     (tensor cores may truncate: twice a rounding's 2^-24).  fp32 inputs: the product's rounding joins.  A weight is 2^(s - lse): its
     relative error is that of the score times 1 / scale in absolute terms, twice (score and denominator), and one rounding per
-    addition that its sums see in a row: n / 16 pages, the counted rows, the merges of warps and pieces.  The output adds the
-    rounding of every weight to the values' type and its own."""
+    addition that its sums see in a row: bf16 n / 16 pages, fp32 the n keys one by one (2^-24 each), the counted rows, the merges of warps
+    and pieces.  The output adds the rounding of every weight to the values' type and its own."""
     q, k, v = q.double(), k.double(), v.double()
     n, (w, G, D) = k.shape[0], q.shape
     z = torch.einsum("wgd,td->gwt", q, k) * scale
@@ -39,7 +39,7 @@ def attend(q, k, v, n_new, window, scale, dtype):
     counted = horizon >= n - (window or w)
     paid = p[:, counted].sum((0, 1))
     rows = int(counted.sum()) * G
-    rel = 2.0 ** -23 * (2 * 132 * size + n / 16 + rows + 64)
+    rel = 2.0 ** -23 * (2 * 132 * size + n / (16 if dtype == torch.bfloat16 else 2) + rows + 64)
     o_bound = HALF[dtype] * (o.abs() + torch.einsum("gwt,td->wgd", p, v.abs())) + rel * torch.einsum("gwt,td->wgd", p, v.abs())
     return o, o_bound, paid, rel * paid + 1e-30
 

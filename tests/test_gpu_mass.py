@@ -152,6 +152,9 @@ PREFILL = [
     ([1], [1], 1, 1, torch.float32, 0, 0, False),
     ([140, 75, 9], [40, 75, 0], 2, 4, torch.float32, 0, 0, False),
     ([140, 75, 20], [40, 75, 1], 1, 2, torch.float32, 9, 4, True),
+    ([900, 1, 33, 32, 0, 97], [5, 1, 2, 32, 0, 97], 2, 1, torch.float32, 0, 0, False),
+    ([700, 64, 300], [9, 8, 130], 1, 8, torch.float32, 30, 12, True),
+    ([300] * 40, [70] * 40, 3, 4, torch.float32, 0, 0, False),
 ]
 
 
