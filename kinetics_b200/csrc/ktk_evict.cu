@@ -298,18 +298,16 @@ __device__ __forceinline__ void token_move(const uint32_t* stay, const uint32_t*
     }
 }
 
-// Tokens of a warp's copies, their loads in flight together: as many as two lanes each can look up
-constexpr int kEvEach = 8;
-// Copies keys and values of moves first .. first + kEvEach - 1 (of `moves`): from(i) -> to(i), by a whole warp.  Two lanes find where a move
-// leads, all lanes then copy.  CHUNKS: 16-byte pieces of a token's key (as many of its value)
-template <int CHUNKS, class From, class To>
+// Copies keys and values of moves first .. first + EACH - 1 (of `moves`): from(i) -> to(i), by a whole warp, their loads in flight
+// together.  Two lanes find where a move leads, all lanes then copy.  CHUNKS: 16-byte pieces of a token's key (as many of its value)
+template <int CHUNKS, int EACH, class From, class To>
 __device__ __forceinline__ void copy_tokens(const EvictParams& p, int h, int start, int first_fill, int first, int moves, From from, To to) {
     constexpr int kLoads = 2 * CHUNKS / 32;
     const int lane = threadIdx.x & 31;
     uint4* cache = (uint4*)p.cache;
     int64_t at = -1;                                 // first piece of the token's key; -1: no such page
     const int move = first + lane / 2;
-    if (lane < 2 * kEvEach && move < moves) {
+    if (lane < 2 * EACH && move < moves) {
         int e, slot;
         page_of_pos(lane % 2 ? to(move) : from(move), first_fill, e, slot);
         const int64_t page = __ldg(p.kv_indices + start + e);
@@ -323,16 +321,16 @@ __device__ __forceinline__ void copy_tokens(const EvictParams& p, int h, int sta
         const int c = j * 32 + lane;
         mine[j] = c < CHUNKS ? c : to_value + c - CHUNKS;
     }
-    uint4 v[kEvEach][kLoads];
+    uint4 v[EACH][kLoads];
 #pragma unroll
-    for (int i = 0; i < kEvEach; ++i) {
+    for (int i = 0; i < EACH; ++i) {
         const int64_t src = __shfl_sync(0xffffffffu, at, 2 * i);
 #pragma unroll
         for (int j = 0; j < kLoads; ++j)
             if (src >= 0) v[i][j] = cache[src + mine[j]];
     }
 #pragma unroll
-    for (int i = 0; i < kEvEach; ++i) {
+    for (int i = 0; i < EACH; ++i) {
         const int64_t src = __shfl_sync(0xffffffffu, at, 2 * i), dst = __shfl_sync(0xffffffffu, at, 2 * i + 1);
 #pragma unroll
         for (int j = 0; j < kLoads; ++j)
@@ -409,9 +407,9 @@ evict_kernel(const EvictParams p, int cluster) {
     });
     cl.sync();
     if constexpr (CHUNKS > 0) {                      // one CTA
-        constexpr int W = THREADS / 32;
-        for (int i = (tid >> 5) * kEvEach; i < moves; i += W * kEvEach)
-            copy_tokens<CHUNKS>(p, (int)(unit % p.Hkv), u.start, u.first_fill, i, moves, [&](int k) { return from[k]; },
+        constexpr int W = THREADS / 32, kEach = 4;   // eight took the planning's registers: 64 tokens of 384 CTAs 23.3 us, 20.4
+        for (int i = (tid >> 5) * kEach; i < moves; i += W * kEach)
+            copy_tokens<CHUNKS, kEach>(p, (int)(unit % p.Hkv), u.start, u.first_fill, i, moves, [&](int k) { return from[k]; },
                                 [&](int k) { return to[k]; });
     } else {
         if (cl.rank == 0 && tid == 0) p.count[unit] = moves;
@@ -480,7 +478,9 @@ evict_long_kernel(const EvictParams p) {
         p.pos_out[u.at + to[i]] = x.pos;
     }
 }
-constexpr int kEvWarps = 8;
+// 16 sequences of 2304 tokens cut to 2048: 17.6 us, 19.3 with four tokens of a warp in flight; CTAs of eight warps leave longer tails (100 fp32
+// sequences of 150 to 701 cut to 333: 25.0 us, 22.7).
+constexpr int kEvWarps = 4, kEvEach = 8;
 template <int CHUNKS>
 __global__ void __launch_bounds__(kEvWarps * 32)
 evict_move_kernel(const EvictParams p, int parts) {
@@ -490,7 +490,7 @@ evict_move_kernel(const EvictParams p, int parts) {
     const int moves = p.count[unit];
     if (first >= moves) return;
     const int32_t *from = p.from + unit * p.max_moves, *to = p.to + unit * p.max_moves;
-    copy_tokens<CHUNKS>(p, (int)(unit % p.Hkv), p.kv_indptr[unit / p.Hkv], p.sink_tokens > 0 ? p.sink_tokens : kPageSize, first, moves,
+    copy_tokens<CHUNKS, kEvEach>(p, (int)(unit % p.Hkv), p.kv_indptr[unit / p.Hkv], p.sink_tokens > 0 ? p.sink_tokens : kPageSize, first, moves,
                         [&](int k) { return from[k]; }, [&](int k) { return to[k]; });
 }
 
