@@ -338,9 +338,10 @@ __device__ __forceinline__ void copy_tokens(const EvictParams& p, int h, int sta
     }
 }
 
-// The planning CTA copies at most this many tokens; more go to a launch of their own.  Device time, 8 kv heads, one launch and two: 2049
-// tokens cut to 2048 11.7 us and 12.8; 2304 cut to 2048 17.5 and 11.5, of 48 sequences 42.0 and 32.8.
-constexpr int kEvFused = 64;
+// The planning CTA copies at most this many tokens; more go to a launch of their own.  Replayed from a graph, 8 kv heads, one launch and two:
+// sequences of 2048 + 64 tokens cut to 2048 12.5 us and 13.8, 2048 + 128 14.3 and 14.0 (48 sequences 25.8 and 27.2), 2048 + 256 14.6 and
+// 11.4 (16 sequences 22.9 and 17.9); a launch of its own costs the host 3 us.
+constexpr int kEvFused = 128;
 
 // Sequences of at most THREADS * ITEMS tokens per CTA of the cluster, keys in registers.  CHUNKS: 16-byte pieces of a token's key; 0:
 // keys and values are left to evict_move_kernel.
