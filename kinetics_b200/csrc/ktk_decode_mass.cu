@@ -8,6 +8,8 @@
 //   the balanced partition (bf16) or splits (fp32): the decode kernels write the scores down as they go (4 G bytes per token beside
 //     the 512 of its bf16 key and value), and mass_finish_kernel turns them into weights.  It also merges the pieces of lists that
 //     the decode cut.
+// Bound by HBM: 48 lists of 1790 to 2303 tokens, 32 heads over 8, 80 us (5.1 TB/s), 32 of 16 K 359 (5.8 TB/s); one of 517 tokens 7.6, a
+// chain of loads.
 #include <type_traits>
 
 #include "ktk_decode_mass.cuh"

@@ -32,7 +32,7 @@ constexpr int kPaMaxCluster = 8;
 // its weights pass through shared memory without a barrier.
 // Bound by shared memory: of a chunk's 6700 cycles of it 4100 are the scores' operands (32 bytes of them for 4 FMAs), 2600 the values';
 // the FMAs take 4100.  256 tokens of 32 heads over 8 behind 8192 1.06 ms (33 TFLOP/s), 2.2 by a CTA per token and kv head that
-// reads all its keys; 75 and 45 of 8 over 4 behind 200 and 333 23 us, 28.
+// reads all its keys; 75 and 52 of 8 over 4 behind 233 and 333 23 us, 28.
 __global__ void __launch_bounds__(kPaThreads, 2)
 prefill_attention_f32_kernel(const PrefillMassParams p, int cluster) {
     extern __shared__ __align__(16) float pa_smem[];

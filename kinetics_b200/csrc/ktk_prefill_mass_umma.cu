@@ -18,7 +18,8 @@
 // Every wait is bounded.
 //
 // Per 128 keys and 128 rows: 1024 cycles of the special-function units (16 exponentials a cycle) without kPmPoly, some 600 of the tensor
-// cores.
+// cores.  A prompt of 8192 tokens, 32 heads over 8: 279 us, special-function pipe 74 %, tensor pipe 55 %; 306 with the keys in
+// shared memory and no polynomials, 354 with denominators read from there too, 466 with one CTA per SM and unequal parts.
 #include "ktk_prefill_mass.cuh"
 #include "ktk_umma.cuh"
 
@@ -37,7 +38,7 @@ constexpr int kPmFirst = 2, kPmStages = 5;
 static_assert((kPmStages - kPmFirst) * kPmStage <= 4 * kPmKTile, "stages where the keys were");
 constexpr int kPmSmem = 4 * kPmKTile + kPmFirst * kPmStage + 2 * kPmOnes + 1024;
 constexpr int kPmTmemCols = 256, kPmColS = 128;          // keys m at column 64 m, scores m at 128 + 64 m
-constexpr int kPmPoly = 2;
+constexpr int kPmPoly = 2;                                // of eight pairs of exponentials; 0, 1, 2, 3, 4: 300, 281, 277, 290, 317 us
 
 struct PmShared {
     uint64_t k, k_moved, full[kPmStages], empty[kPmStages], s[2], s_free[2];
