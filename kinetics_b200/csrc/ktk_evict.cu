@@ -94,11 +94,11 @@ __device__ __forceinline__ bool evict_unit(const EvictParams& p, int64_t unit, i
     u.n = sp.total;
     u.start = sp.start;
     u.first_fill = sp.first_fill;
+    if (u.n <= 0 && !sp.bad) return false;           // an idle row: its slot may be none
     if (sp.bad || row < 0 || row >= p.rows || u.n > p.stride || sp.n_pages > p.max_pages || u.n > most) {
         if (threadIdx.x == 0) report(p.status, KTK_STATUS_BAD_TABLE);
         return false;
     }
-    if (u.n <= 0) return false;
     u.at = ((int64_t)row * p.Hkv + h) * p.stride;
     u.mass = p.mass_in + u.at;
     u.pos = p.pos_in + u.at;

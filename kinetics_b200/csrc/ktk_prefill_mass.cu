@@ -18,6 +18,7 @@ extern "C" size_t ktk_prefill_mass_workspace_bytes(const ktk_shape* shape, int64
     if (check_shape(shape, "ktk_prefill_mass_workspace_bytes") != KTK_OK || shape->batch == 0 || total_new_tokens <= 0 ||
         max_new_tokens < 1 || max_pages_per_seq < 1)
         return 0;
+    if (max_new_tokens > total_new_tokens) max_new_tokens = (int32_t)total_new_tokens;
     const size_t behind = shape->dtype == KTK_F32 ? 0 : mass_plan(shape, max_new_tokens, max_pages_per_seq, total_pages, window).partial * sizeof(float);
     return lse_bytes(shape, total_new_tokens) + up(behind);
 }
@@ -45,6 +46,7 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
                   (long long)total_new_tokens, max_new_tokens, window, (long long)max_pages_per_seq);
         return KTK_ERR_ARG;
     }
+    if (max_new_tokens > total_new_tokens) max_new_tokens = (int32_t)total_new_tokens;
     const View view = make_view(view_in);
     if (view.page_count) total_pages = -1;
     const size_t need = ktk_prefill_mass_workspace_bytes(s, total_new_tokens, max_new_tokens, max_pages_per_seq, total_pages, window);

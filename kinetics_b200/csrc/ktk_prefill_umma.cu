@@ -372,8 +372,9 @@ int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st
     p.tiles = tiles <= sm_count() ? 1 : 2;
     int cluster = 1;
     if (p.lse != nullptr && p.max_pages >= kPuSplit * kPuPages) {        // as many CTAs as there are SMs, two blocks each
-        const int64_t ctas = (per_seq + 1) / 2 * p.batch * p.Hkv;
-        while (cluster < kPuMaxCluster && ctas * cluster * 2 <= sm_count() && p.max_pages >= 4 * kPuPages * cluster) cluster *= 2;
+        const int64_t both = (per_seq + 1) / 2, some = p.total_new / (2 * tpc) + p.batch;
+        const int64_t ctas = (both * p.batch < some ? both * p.batch : some) * p.Hkv;
+        while (both <= 65535 && cluster < kPuMaxCluster && ctas * cluster * 2 <= sm_count() && p.max_pages >= 4 * kPuPages * cluster) cluster *= 2;
         if (cluster > 1) p.tiles = 2;
     }
     const unsigned pairs = (unsigned)((per_seq + p.tiles - 1) / p.tiles);

@@ -83,7 +83,7 @@ class EvictingKVManager:
         return np.stack((s * pages_per_slot, count, n - (count - 1) * PAGE, s)).astype(np.int32)
 
     def _table(self, slots, lengths):
-        key = (tuple(slots), tuple(lengths))
+        key = (tuple(slots), tuple(lengths), torch.cuda.current_stream(self.device).cuda_stream)
         if key != self._table_key:
             rows = torch.from_numpy(self._rows(slots, lengths, self.pages_per_slot)).pin_memory().to(self.device, non_blocking=True)
             self._table_key, self._table_val = key, (rows[0], rows[2], ops.PageView(0, 0, rows[1], rows[3]))

@@ -357,6 +357,67 @@ def test_nothing_to_do(cuda_device):
     assert torch.equal(s["mass"], before)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_idle_rows_of_a_padded_batch(cuda_device, dtype):
+    # a batch of five places, three of them idle: no pages, no new tokens, slots that are none
+    from kinetics_b200 import ops
+    s, status = _state(11, cuda_device, dtype=dtype), ops.new_status(cuda_device)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda_device)
+    cache, indices, indptr, last = s["table"]
+    view = ops.PageView(0, 0, i32(0, 44, 0, 82, 0), i32(-1, 2, 7, 0, -5))
+    padded = (i32(0, 0, 99, 47, 3), i32(99, 12, 0, 4, -1))               # starts; 700 and 1300 tokens
+    q = s["q"].new_zeros(5, 8, D)
+    q[1], q[3] = s["q"][0], s["q"][2]
+    rows = [0, 2]
+    mass = s["mass"].clone()
+    out, got = ops.dense_decode_mass(q, cache, indices, *padded, 82, mass, mass_out=mass.clone(), status=status, view=view)
+    plain = ops.PageView(0, 0, i32(44, 82), i32(2, 0))
+    two = (i32(0, 47), i32(12, 4))
+    want_out, want = ops.dense_decode_mass(s["q"][rows], cache, indices, *two, 82, mass, mass_out=mass.clone(), status=status, view=plain)
+    ops.raise_on_status(status)
+    assert not out[[0, 2, 4]].any()
+    torch.testing.assert_close(out[[1, 3]], want_out, rtol=2 ** -7, atol=1e-3)        # forms differ by the number of lists
+    torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-6)
+    new = torch.cat([s["qs"][:33], s["qs"][73:273]])
+    _, got = ops.prefill_attention_mass(new, i32(0, 0, 33, 33, 233, 233), 200, cache, indices, *padded, mass, mass_out=mass.clone(),
+                                        status=status, view=view)
+    _, want = ops.prefill_attention_mass(new, i32(0, 33, 233), 200, cache, indices, *two, mass, mass_out=mass.clone(), status=status, view=plain)
+    ops.raise_on_status(status)
+    torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-6)
+    runs = []
+    for table, v in ((padded, view), (two, plain)):
+        c, positions = cache.clone(), s["positions"].clone()
+        got, _ = ops.evict(c, indices, *table, 82, mass, positions, s["stored"], i32(1300, 40, 700), 500, 4, 64, mass_out=mass.clone(),
+                           status=status, view=v)
+        runs.append((c, positions, got))
+    ops.raise_on_status(status)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_pages_behind_2_31_elements(cuda_device, dtype):
+    # the same sequences in the last pages of a cache whose elements pass 31 bits (and bytes 32)
+    from kinetics_b200 import ops
+    small = _state(12, cuda_device, dtype=dtype)
+    cache, indices, indptr, last = small["table"]
+    shift = 2 ** 31 // cache[0].numel() + 64
+    big = torch.empty(shift + cache.shape[0], *cache.shape[1:], dtype=dtype, device=cuda_device)
+    big[shift:] = cache
+    status = ops.new_status(cuda_device)
+
+    def chain(kv, indices):
+        mass, positions = small["mass"].clone(), small["positions"].clone()
+        table = (kv, indices, indptr, last)
+        a, _ = ops.prefill_attention_mass(small["qs"], small["indptr"], small["new"], *table, mass, window=20, status=status)
+        b, _ = ops.dense_decode_mass(small["q"], *table, small["most"], mass, decay=0.9, status=status)
+        c, _ = ops.dense_decode_mass(small["q"], *table, 30000, mass, decay=0.9, status=status)
+        ops.evict(*table, small["most"], mass, positions, small["stored"], small["seen"], 500, 4, 64, status=status)
+        return a, b, c, mass, positions
+    want, got = chain(cache, indices), chain(big, indices + shift)
+    ops.raise_on_status(status)
+    assert all(torch.equal(x, y) for x, y in zip(want, got)) and torch.equal(big[shift:], cache)
+
+
 def test_launches_are_counted(cuda_device):
     from kinetics_b200 import ops
     s = _state(10, cuda_device)

@@ -45,6 +45,8 @@ def _view(c, lens, sink, dev, padded):
 def _check(c, out, mass_out, lens, new, kv_heads, group, dtype, window, decay, scale):
     first = c["q_indptr"].tolist()
     before = c["mass"]
+    others = [r for r in range(len(before)) if r not in c["slots"].tolist()]
+    assert torch.equal(mass_out[others].cpu().nan_to_num(-1), before[others].nan_to_num(-1))
     for b, (n, w) in enumerate(zip(lens, new)):
         row = int(c["slots"][b])
         got = mass_out[row].cpu()
