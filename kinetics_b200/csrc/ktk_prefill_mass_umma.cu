@@ -402,7 +402,7 @@ int launch_prefill_mass_umma(const PrefillMassParams& p, int64_t groups, cudaStr
         return KTK_ERR_TOO_LARGE;
     }
     KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_mass_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem), who);
-    KTK_CUDA_TRY(launch_behind(false, prefill_mass_umma_kernel, (unsigned)(units * p.splits), kPmThreads, kPmSmem, st, p, kv_map, q_map,
+    KTK_CUDA_TRY(launch_behind(true, prefill_mass_umma_kernel, (unsigned)(units * p.splits), kPmThreads, kPmSmem, st, p, kv_map, q_map,
                                lse_map), who);
     if (p.splits > 1)
         KTK_CUDA_TRY(launch_behind(true, prefill_mass_add_kernel, (unsigned)units, 2 * kPmBlock, 0, st, p), who);
