@@ -2,15 +2,15 @@
 // of largest mass stay, with the first and the newest.  The kept tokens behind place `keep` move into the holes in front of it.
 //
 // A CTA per (sequence, kv head), or a cluster of them, plans: every token has a 32-bit key whose order is that of the masses (the
-// first and newest: the largest key, NaN: the smallest).  The keep-th largest key is found by its digits, the first of 11 bits, from
-// counts of the keys with each digit; tokens at exactly that key stay from the lowest place on.  Which tokens stay is held as one bit
+// first and newest: the largest key, NaN: the smallest).  The keep-th largest key is found from counts of the keys in intervals; tokens at
+// exactly that key stay from the lowest place on.  Which tokens stay is held as one bit
 // each, and prefix sums over the bits' words number the holes and the tokens that move.
 // Keys and values are copied a warp to a token: by the planning CTA where few can move, else by a launch of their own, whose many
 // warps hide the chain of loads (list, page table, cache) that each copy is.
 //
 // Two copies of a row per token are what an eviction cannot do without: 48 sequences of 2304 tokens cut to 2048, 8 kv heads, 101 MB: the
-// copies at 4.8 TB/s (17 us), the plan in front of them 15, most of it the latency of its steps (loads 4, three digits 3, numbers and
-// lists 3).
+// copies at 4.8 TB/s (17 us), the plan in front of them 15, most of it the latency of its steps (loads 4, threshold 3, numbers and
+// lists 2).
 #include <cooperative_groups.h>
 
 #include "ktk_decode.cuh"
@@ -137,92 +137,195 @@ struct Cluster {
     }
 };
 
-// The keep-th largest key and how many keys are above it, digit by digit.  walk(visit): calls visit(key, there) for the CTA's keys, whole
-// warps together.  hist: zeros, kEvBins for each digit, the first twice; one, then the other half of a warp counts there, since many keys
-// share a first digit.  found: three words.  All CTAs of the cluster find the same.
-constexpr int kEvBins = 2048, kEvHists = 4;
+// The keep-th largest key and how many keys are above it.  walk(visit): calls visit(key, there) for the CTA's keys, whole warps together.
+// Counts of the keys in equal intervals from the smallest positive mass to the largest say in which it lies; up to kEvRanked keys there
+// are ranked directly, more are counted in intervals of that interval.  (Intervals of all 32-bit keys, which hold masses of a few
+// octaves in a dozen of them, took three rounds.)  All CTAs of the cluster find the same.
+constexpr int kEvRanked = 256;
+constexpr uint32_t kEvSafe = 0xffffffffu, kEvZero = 0x80000000u;        // keys of the first and newest tokens, and of a mass of 0
 struct Threshold {
     uint32_t key;
     int above;
 };
+template <int THREADS> struct ThresholdShared {
+    static constexpr int kBins = 2 * THREADS;         // a power of two; two of them to a thread
+    uint32_t hist[2][kBins];                          // begin as zeros; one, then the other half of a warp counts there
+    uint32_t some[kEvRanked], all[kEvRanked];
+    uint32_t found[3], count;                        // count begins as 0
+    uint4 range;
+};
+template <int THREADS> __device__ __forceinline__ void clear_counts(ThresholdShared<THREADS>& sh) {
+    reinterpret_cast<uint4*>(sh.hist[0])[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    if (threadIdx.x == 0) sh.count = 0;
+}
 template <int THREADS, class Walk>
-__device__ __forceinline__ Threshold find_threshold(int keep, const Cluster& cl, uint32_t (*hist)[kEvBins], uint32_t* found,
-                                                    uint64_t (*buf)[32], int& turn, Walk walk) {
-    constexpr int kEach = kEvBins / THREADS;
+__device__ __forceinline__ Threshold find_threshold(int keep, const Cluster& cl, ThresholdShared<THREADS>& sh, uint64_t (*buf)[32], int& turn, Walk walk) {
+    static_assert(kEvRanked <= THREADS, "a thread to a ranked key");
+    constexpr int kBins = ThresholdShared<THREADS>::kBins, kLog = THREADS == 256 ? 9 : 11, W = THREADS / 32;
+    static_assert(kBins == 1 << kLog, "intervals by shifts");
     const int tid = threadIdx.x, lane = tid & 31;
+    // smallest and largest key of the positive masses, and of the others
+    uint32_t lo = kEvSafe, hi = 0, low = kEvSafe, high = 0;
+    walk([&](uint32_t key, bool on) {
+        const bool positive = key > kEvZero;
+        if (on && positive && key != kEvSafe) {
+            lo = min(lo, key);
+            hi = max(hi, key);
+        }
+        if (on && !positive) {
+            low = min(low, key);
+            high = max(high, key);
+        }
+    });
+    const auto reduce = [&] {
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        low = __reduce_min_sync(0xffffffffu, low);
+        high = __reduce_max_sync(0xffffffffu, high);
+    };
+    reduce();
+    uint4* ranges = reinterpret_cast<uint4*>(sh.all);            // of the warps
+    if (lane == 0) ranges[tid >> 5] = make_uint4(lo, hi, low, high);
+    __syncthreads();
+    const auto take = [&](const uint4* from) {
+        const uint4 x = *from;
+        lo = x.x, hi = x.y, low = x.z, high = x.w;
+        reduce();
+    };
+    take(ranges + (lane < W ? lane : 0));
+    if (cl.size > 1) {
+        if (tid == 0) sh.range = make_uint4(lo, hi, low, high);
+        cl.sync();
+        take(cl.of(&sh.range, lane < cl.size ? lane : 0));
+    }
+    // The keys in question: base .. base + span.  In round 0 all of them: interval 0 is that of masses that are not positive, the last that
+    // of kEvSafe.
     Threshold r{0, 0};
-    uint32_t known = 0;                              // mask of the digits found
-    for (int digit = 0; ; ++digit) {
-        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
-        const uint32_t digits = digit == 2 ? 1023u : 2047u;
-        uint32_t* mine = hist[digit == 0 ? 0 : digit + 1];
-        if (digit == 0) {
-            uint32_t* copy = hist[lane >> 4];
+    uint32_t base = lo, span = lo < hi ? hi - lo : 0;
+    const auto inside = [&](uint32_t key) { return key - base <= span; };
+    for (int round = 0; ; ++round) {
+        int shift = max(32 - kLog - __clz(span | 1u), 0);
+        if (round == 0) {
+            if (span >> shift > kBins - 3) ++shift;
+            uint32_t* copy = sh.hist[lane >> 4];
             walk([&](uint32_t key, bool on) {
-                if (on) atomicAdd(&copy[key >> 21], 1u);
+                if (on) atomicAdd(&copy[key == kEvSafe ? kBins - 1 : key < base ? 0 : 1 + ((key - base) >> shift)], 1u);
             });
         } else {
+            if (cl.size > 1) {                       // zeros again, when all have read
+                cl.sync();
+                sh.hist[0][tid] = sh.hist[0][tid + THREADS] = 0;
+                __syncthreads();
+            }
             walk([&](uint32_t key, bool on) {
-                on = on && (key & known) == r.key;
+                on = on && inside(key);
                 const unsigned active = __ballot_sync(0xffffffffu, on);
                 if (active == 0) return;
-                // a warp whose keys share a digit (the same mass) adds once
-                const uint32_t bin = key >> shift & digits, one = __shfl_sync(0xffffffffu, bin, __ffs((int)active) - 1);
+                // a warp whose keys share an interval (the same mass) adds once
+                const uint32_t bin = (key - base) >> shift, one = __shfl_sync(0xffffffffu, bin, __ffs((int)active) - 1);
                 if (__all_sync(0xffffffffu, !on || bin == one)) {
-                    if (lane == 0) atomicAdd(&mine[one], (uint32_t)__popc(active));
+                    if (lane == 0) atomicAdd(&sh.hist[0][one], (uint32_t)__popc(active));
                 } else if (on) {
-                    atomicAdd(&mine[bin], 1u);
+                    atomicAdd(&sh.hist[0][bin], 1u);
                 }
             });
         }
-        if (cl.size > 1) {
-            if (digit == 0) {
+        if (cl.size > 1) {                           // sums over the CTAs to the second array
+            if (round == 0) {
                 __syncthreads();
-                for (int i = tid; i < kEvBins; i += THREADS) hist[0][i] += hist[1][i];
+                for (int i = tid; i < kBins; i += THREADS) sh.hist[0][i] += sh.hist[1][i];
             }
             cl.sync();
-            uint32_t sums[kEach];
+            uint32_t sums[2] = {0, 0};
 #pragma unroll
-            for (int k = 0; k < kEach; ++k) {
-                sums[k] = 0;
+            for (int i = 0; i < 4; ++i)
+                if (i < cl.size)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < cl.size) sums[k] += cl.of(mine, i)[k * THREADS + tid];
-            }
-            cl.sync();                               // all have read
-#pragma unroll
-            for (int k = 0; k < kEach; ++k) mine[k * THREADS + tid] = sums[k];
+                    for (int k = 0; k < 2; ++k) sums[k] += cl.of(sh.hist[0], i)[k * THREADS + tid];
+            sh.hist[1][tid] = sums[0];
+            sh.hist[1][tid + THREADS] = sums[1];
         }
         __syncthreads();
-        // from the largest digit on, kEach to a thread
-        const int bin0 = kEvBins - (tid + 1) * kEach;
-        uint32_t c[kEach], sum = 0, total;
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-            c[k] = mine[bin0 + k];
-            if (digit == 0 && cl.size == 1) c[k] += hist[1][bin0 + k];
-            sum += c[k];
+        // from the largest interval on, two to a thread, which leaves zeros
+        const int bin0 = kBins - (tid + 1) * 2;
+        uint2* at = reinterpret_cast<uint2*>(&sh.hist[1][bin0]);
+        uint2 c = *at;
+        *at = make_uint2(0u, 0u);
+        if (cl.size == 1) {
+            at = reinterpret_cast<uint2*>(&sh.hist[0][bin0]);
+            c.x += at->x;
+            c.y += at->y;
+            *at = make_uint2(0u, 0u);
         }
-        const uint32_t need = (uint32_t)(keep - r.above);
-        uint32_t before = block_prefix<THREADS>(sum, buf, turn, total);
+        uint32_t total;
+        const uint32_t sum = c.x + c.y;
+        uint32_t need = (uint32_t)(keep - r.above);
+        const uint32_t before = block_prefix<THREADS>(sum, buf, turn, total);
         if (before < need && need <= before + sum) {             // one thread
-#pragma unroll
-            for (int k = kEach - 1; k >= 0; --k) {
-                if (before < need && need <= before + c[k]) {
-                    found[0] = (uint32_t)(bin0 + k);
-                    found[1] = before;
-                    found[2] = c[k];
-                }
-                before += c[k];
-            }
+            const bool upper = need <= before + c.y;
+            sh.found[0] = (uint32_t)(bin0 + (upper ? 1 : 0));
+            sh.found[1] = upper ? before : before + c.y;
+            sh.found[2] = upper ? c.y : c.x;
         }
         __syncthreads();
-        r.key |= found[0] << shift;
-        r.above += (int)found[1];
-        known |= digits << shift;
-        const uint32_t here = found[2];
-        if (digit == 2) return r;
-        if (here == (uint32_t)(keep - r.above) && r.key != 0) return {r.key - 1, keep};          // all keys with these digits stay
+        const uint32_t bin = sh.found[0], here = sh.found[2];
+        r.above += (int)sh.found[1];
+        need -= sh.found[1];
+        if (round > 0) {
+            base += bin << shift;
+            span = (1u << shift) - 1u;
+        } else if (bin == kBins - 1) {
+            return {kEvSafe, 0};                     // as many first and newest ones as stay
+        } else if (bin > 0) {
+            base += (bin - 1) << shift;
+            span = (1u << shift) - 1u;
+        } else {
+            base = low;
+            span = high - low;
+        }
+        if (here == need) return {base - 1, keep};   // all of the interval stay; it is not that from 0 on: there are more than `keep` keys
+        if (span == 0) return {base, r.above};
+        if (here <= kEvRanked) {
+            uint32_t put = 0;                        // of the warp's keys, the first one's place
+            walk([&](uint32_t key, bool on) { put += __popc(__ballot_sync(0xffffffffu, on && inside(key))); });
+            if (lane == 0 && put > 0) put = atomicAdd(&sh.count, put);
+            put = __shfl_sync(0xffffffffu, put, 0);
+            walk([&](uint32_t key, bool on) {
+                on = on && inside(key);
+                const unsigned active = __ballot_sync(0xffffffffu, on);
+                if (on) sh.some[put + __popc(active & ((1u << lane) - 1u))] = key;
+                put += __popc(active);
+            });
+            if (tid < kEvRanked) sh.all[tid] = 0;
+            cl.sync();
+            if (tid < (int)here) {
+                int i = 0, at = tid;                 // the tid-th of the CTAs' keys, one CTA's behind the other's
+                for (; i + 1 < cl.size; ++i) {
+                    const int n = (int)*cl.of(&sh.count, i);
+                    if (at < n) break;
+                    at -= n;
+                }
+                sh.all[tid] = cl.of(sh.some, i)[at];
+            }
+            __syncthreads();
+            if (tid < (int)here) {
+                const uint32_t key = sh.all[tid];
+                uint32_t greater = 0, equal = 0;     // the zeros behind the last are equal to the smallest key at most
+#pragma unroll 4
+                for (uint32_t i = 0; i < here; i += 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(sh.all + i);
+                    greater += (v.x > key) + (v.y > key) + (v.z > key) + (v.w > key);
+                    equal += (v.x == key) + (v.y == key) + (v.z == key) + (v.w == key);
+                }
+                if (greater < need && need <= greater + equal) {                 // all that do hold the same key
+                    const bool stay = need == greater + equal;                   // all of that key do
+                    sh.found[0] = stay ? key - 1 : key;
+                    sh.found[1] = (uint32_t)(stay ? keep : r.above + (int)greater);
+                }
+            }
+            __syncthreads();
+            return {sh.found[0], (int)sh.found[1]};
+        }
         __syncthreads();                             // found may be written again
     }
 }
@@ -350,9 +453,10 @@ __global__ void __launch_bounds__(THREADS)
 evict_kernel(const EvictParams p, int cluster) {
     constexpr int kMost = THREADS * ITEMS, kWords = kMost / 32, kBatch = 8;
     __shared__ uint64_t buf[2][32], shared[2];
-    __shared__ uint32_t hist[kEvHists][kEvBins], found[3], stay[kWords], level[kWords];
+    __shared__ __align__(16) ThresholdShared<THREADS> counts;
+    __shared__ uint32_t stay[kWords], level[kWords];
     const int tid = threadIdx.x;
-    for (int i = tid; i < kEvHists * kEvBins; i += THREADS) hist[0][i] = 0;
+    clear_counts<THREADS>(counts);
     wait_for_front();
     const Cluster cl{cluster, (int)(blockIdx.x % cluster)};
     const int64_t unit = blockIdx.x / cluster;
@@ -388,7 +492,7 @@ evict_kernel(const EvictParams p, int cluster) {
         }
     };
     int turn = 0;
-    const Threshold at = find_threshold<THREADS>(keep, cl, hist, found, buf, turn, [&](auto visit) {
+    const Threshold at = find_threshold<THREADS>(keep, cl, counts, buf, turn, [&](auto visit) {
         each_item([&](int j, int i) { visit(key[j], i < n); });
     });
     each_item([&](int j, int i) {
@@ -428,10 +532,10 @@ __global__ void __launch_bounds__(kEvLong)
 evict_long_kernel(const EvictParams p) {
     extern __shared__ __align__(16) uint32_t ev_smem[];
     __shared__ uint64_t buf[2][32];
-    __shared__ uint32_t hist[kEvHists][kEvBins], found[3];
+    __shared__ __align__(16) ThresholdShared<kEvLong> counts;
     const int tid = threadIdx.x, lane = tid & 31;
     const Cluster alone{1, 0};
-    for (int i = tid; i < kEvHists * kEvBins; i += kEvLong) hist[0][i] = 0;
+    clear_counts<kEvLong>(counts);
     wait_for_front();
     const int64_t unit = blockIdx.x;
     EvictUnit u;
@@ -455,7 +559,7 @@ evict_long_kernel(const EvictParams p) {
         }
     };
     int turn = 0;
-    const Threshold at = find_threshold<kEvLong>(keep, alone, hist, found, buf, turn, [&](auto visit) {
+    const Threshold at = find_threshold<kEvLong>(keep, alone, counts, buf, turn, [&](auto visit) {
         each([&](int t, uint32_t key) { visit(key, t < n); });
     });
     each([&](int t, uint32_t key) {
@@ -499,7 +603,8 @@ template <int THREADS, int ITEMS>
 static cudaError_t launch_evict(const EvictParams& p, int64_t units, int cluster, bool fused, bool f32, cudaStream_t st) {
     const auto kernel = !fused ? evict_kernel<THREADS, ITEMS, 0> : f32 ? evict_kernel<THREADS, ITEMS, 32> : evict_kernel<THREADS, ITEMS, 16>;
     const size_t smem = fused ? 2 * (size_t)p.max_moves * sizeof(int32_t) : 0;
-    return launch_cluster(units * cluster <= sm_count(), kernel, (unsigned)(units * cluster), THREADS, smem, cluster, st, p, cluster);
+    // early only where no launch of copies comes behind: its CTAs would wait among this one's (4 sequences of 2304 cut to 2048 13.1 us, 12.1)
+    return launch_cluster(fused && units <= sm_count(), kernel, (unsigned)(units * cluster), THREADS, smem, cluster, st, p, cluster);
 }
 
 static int64_t evict_max_moves(int max_pages, int keep) {
@@ -508,8 +613,7 @@ static int64_t evict_max_moves(int max_pages, int keep) {
 }
 
 // CTAs per (sequence, kv head): more than one for long sequences where SMs would idle.  Two sequences of 32768 tokens, 8 kv heads, the
-// plan alone: 48 us with one CTA of 1024 threads each, 30 with two, 26 with four, 46 with eight of 256 threads (which read 2048
-// counts of seven others, three times).
+// plan alone: 24.4 us with two CTAs of 1024 threads each, 19.0 with four.
 static int evict_cluster(int64_t units, int64_t most) {
     int c = 1;
     while (c < 4 && most > 4096 * c && units * c * 2 <= sm_count()) c *= 2;

@@ -30,7 +30,7 @@ constexpr int kPaMaxCluster = 8;
 // One CTA, or a cluster of them that share the keys, per (sequence, kv head, 64 / G new tokens): running maximum and sum per row, two CTAs
 // per SM, a chunk's keys and values on their way while the one before is multiplied.  A row's eight threads lie in one warp, so that
 // its weights pass through shared memory without a barrier.
-// Bound by shared memory: of a chunk's 6700 cycles of it 4100 are the scores' operands (32 bytes of them for 4 FMAs), 2600 the values';
+// Bound by shared memory: of a chunk's 6700 cycles of it 4100 are the scores' operands (32 bytes of them a lane for 16 FMAs), 2600 the values';
 // the FMAs take 4100.  256 tokens of 32 heads over 8 behind 8192 1.06 ms (33 TFLOP/s), 2.2 by a CTA per token and kv head that
 // reads all its keys; 75 and 52 of 8 over 4 behind 233 and 333 23 us, 28.
 __global__ void __launch_bounds__(kPaThreads, 2)

@@ -226,9 +226,34 @@ EVICT = [
 @pytest.mark.parametrize("inplace", [False, True])
 @pytest.mark.parametrize("lens, kv_heads, dtype, keep, sink, recent, stored, sink_page, padded, odd", EVICT)
 def test_evict(cuda_device, lens, kv_heads, dtype, keep, sink, recent, stored, sink_page, padded, odd, inplace):
-    from kinetics_b200 import ops
-    dev = cuda_device
     c = _evict_case(7, lens, kv_heads, dtype, sink_page, keep, stored, odd)
+    _evict_equals(c, cuda_device, lens, kv_heads, keep, sink, recent, sink_page, padded, inplace)
+
+
+MASSES = {
+    "zeros": lambda u: torch.zeros_like(u),
+    "equal": lambda u: torch.full_like(u, 0.37),
+    "two": lambda u: torch.where(u < 0.4, 0.5, 0.25),
+    "near": lambda u: 1.0 + torch.floor(u * 3000) * 2.0 ** -23,               # neighbours
+    "octaves": lambda u: torch.exp2(250 * u - 126),
+    "small": lambda u: u * 1e-39,                                             # below the normal numbers
+    "negative": lambda u: -torch.exp2(40 * u - 20),
+    "mixed": lambda u: torch.where(u < 0.5, -u, torch.where(u < 0.6, torch.zeros_like(u), torch.exp2(20 * u))),
+    "infinite": lambda u: torch.where(u < 0.3, math.inf, torch.where(u < 0.6, -math.inf, u)),
+    "none": lambda u: torch.full_like(u, math.nan),
+}
+
+
+@pytest.mark.parametrize("lens, keep", [([700, 300, 257], 256), ([5000, 1100], 1000), ([40000], 3000), ([66000], 700)])
+@pytest.mark.parametrize("masses", sorted(MASSES))
+def test_evict_by_masses_of_any_range(cuda_device, masses, lens, keep):
+    c = _evict_case(8, lens, 1, torch.bfloat16, 0, keep, 0, False)
+    c["mass"] = MASSES[masses](torch.rand(c["mass"].shape, generator=torch.Generator().manual_seed(9)))
+    _evict_equals(c, cuda_device, lens, 1, keep, 2, 3, 0, False, True)
+
+
+def _evict_equals(c, dev, lens, kv_heads, keep, sink, recent, sink_page, padded, inplace):
+    from kinetics_b200 import ops
     st = c["st"]
     want_kv, want_mass, want_pos = st["kv_cache"].clone(), c["mass"].clone(), c["positions"].clone()
     moved = False
