@@ -606,7 +606,8 @@ KTK_API int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr, i
  *   mass->in/out  as above; `out` receives the masses of all min(n, keep) places; decay plays no part
  *   max_pages_per_seq   an upper bound of a sequence's pages, at most 32768 (a longer sequence reports KTK_STATUS_BAD_TABLE and is
  *                 left alone)
- *   workspace     ktk_evict_workspace_bytes() bytes: which token moves where; 0, and then it may be null, where few can move
+ *   workspace     ktk_evict_workspace_bytes() bytes: which token moves where; 0, and then it may be null, where few can move or rows
+ *                 are few
  * A token whose page id is none of the cache's reports KTK_STATUS_BAD_PAGE; its keys and values are not copied.
  * sink + recent <= keep, keep >= 1.  shape->group_size plays no part.
  */

@@ -5,7 +5,7 @@
 // first and newest: the largest key, NaN: the smallest).  The keep-th largest key is found from counts of the keys in intervals; tokens at
 // exactly that key stay from the lowest place on.  Which tokens stay is held as one bit
 // each, and prefix sums over the bits' words number the holes and the tokens that move.
-// Keys and values are copied a warp to a token: by the planning CTA where few can move, else by a launch of their own, whose many
+// Keys and values are copied a warp to a token: behind the plan where few can move or rows are few, else by a launch of their own, whose many
 // warps hide the chain of loads (list, page table, cache) that each copy is.
 //
 // Two copies of a row per token are what an eviction cannot do without: 48 sequences of 2304 tokens cut to 2048, 8 kv heads, 101 MB: the
@@ -441,16 +441,19 @@ __device__ __forceinline__ void copy_tokens(const EvictParams& p, int h, int sta
     }
 }
 
-// The planning CTA copies at most this many tokens; more go to a launch of their own.  Replayed from a graph, 8 kv heads, one launch and two:
-// sequences of 2048 + 64 tokens cut to 2048 12.5 us and 13.8, 2048 + 128 14.3 and 14.0 (48 sequences 25.8 and 27.2), 2048 + 256 14.6 and
-// 11.4 (16 sequences 22.9 and 17.9); a launch of its own costs the host 3 us.
-constexpr int kEvFused = 128;
+// Tokens that are copied behind the plan, in the same launch, where few rows leave SMs for more CTAs that copy (up to kEvCopiers a row) or few
+// tokens move; more go to a launch of their own, which costs the host 3 us and a workspace.  Replayed from a graph / called, one launch
+// and two, 8 kv heads, sequences of 2048 + 256 tokens cut to 2048: one, 8 copiers, 9.8 / 12.8 us and 11.3 / 16.3; four, 4 copiers, 12.3 / 12.8 and
+// 11.6 / 16.6; eight, 2 copiers, 14.9 / 15.6 and 12.4 / 16.4; seven fp32 ones of 150 to 701 cut to 333, 4 kv heads, 4 copiers, 10.1 / 11.0 and
+// 9.7 / 16.0; 48 of 2048 + 128, one copier, 25.8 / 27.0 and 27.2 / 29.1.
+constexpr int kEvFused = 128, kEvFusedEach = 96, kEvCopiers = 8;
 
-// Sequences of at most THREADS * ITEMS tokens per CTA of the cluster, keys in registers.  CHUNKS: 16-byte pieces of a token's key; 0:
-// keys and values are left to evict_move_kernel.
+// Sequences of at most THREADS * ITEMS tokens per CTA, keys in registers.  CHUNKS == 0: a cluster plans, keys and values are left to
+// evict_move_kernel.  Else CHUNKS is the number of 16-byte pieces of a token's key: one CTA plans, and with the others of its cluster, the
+// `copiers`, copies from the lists in its shared memory.
 template <int THREADS, int ITEMS, int CHUNKS>
 __global__ void __launch_bounds__(THREADS)
-evict_kernel(const EvictParams p, int cluster) {
+evict_kernel(const EvictParams p, int cluster, int copiers) {
     constexpr int kMost = THREADS * ITEMS, kWords = kMost / 32;
     // tokens of a thread whose loads are in flight together: of 256 threads 12 (48 sequences of 2304 tokens 31.9 us, 32.9
     // with 8; 100 of 150 to 701 21.9 us, 23.2 with 16); 1024 threads have registers for 8
@@ -461,72 +464,93 @@ evict_kernel(const EvictParams p, int cluster) {
     const int tid = threadIdx.x;
     clear_counts<THREADS>(counts);
     wait_for_front();
-    const Cluster cl{cluster, (int)(blockIdx.x % cluster)};
-    const int64_t unit = blockIdx.x / cluster;
+    const int copier = CHUNKS > 0 ? (int)(blockIdx.x % copiers) : 0;
+    const Cluster cl = CHUNKS > 0 ? Cluster{1, 0} : Cluster{cluster, (int)(blockIdx.x % cluster)};
+    const int64_t unit = blockIdx.x / (CHUNKS > 0 ? copiers : cluster);
     EvictUnit u;
-    const bool there = evict_unit(p, unit, kMost * cluster, u);                  // the same for the cluster
+    const bool there = evict_unit(p, unit, kMost * cl.size, u);                  // the same for the cluster
     if (CHUNKS == 0 && (!there || u.n <= p.keep) && tid == 0) p.count[unit] = 0;
     if (!there) return;
     const int keep = p.keep, front = u.n < keep ? u.n : keep;
     // the CTA's tokens: whole words
-    const int words = ((u.n + 31) / 32 + cluster - 1) / cluster, first = cl.rank * words, t0 = first * 32;
+    const int words = ((u.n + 31) / 32 + cl.size - 1) / cl.size, first = cl.rank * words, t0 = first * 32;
     const int n = min(u.n - t0, words * 32);         // may be negative
-    uint32_t key[ITEMS];
-#pragma unroll
-    for (int j0 = 0; j0 < ITEMS; j0 += kBatch) {     // reads of a batch, then its writes
-        if (j0 * THREADS >= n) break;
-        EvictToken x[kBatch];
-#pragma unroll
-        for (int j = 0; j < kBatch && j0 + j < ITEMS; ++j) x[j] = read_token(u, min(t0 + (j0 + j) * THREADS + tid, u.n - 1));
-#pragma unroll
-        for (int j = 0; j < kBatch && j0 + j < ITEMS; ++j) {
-            const int i = (j0 + j) * THREADS + tid;
-            key[j0 + j] = key_of(p, u, x[j]);
-            if (i < n && t0 + i < front) keep_token(p, u, t0 + i, x[j]);
-        }
-    }
-    if (u.n <= keep) return;
-    __syncthreads();
-    const auto each_item = [&](auto visit) {         // of the CTA's tokens, whole warps
-#pragma unroll
-        for (int j = 0; j < ITEMS; ++j) {
-            if (j * THREADS >= n) break;             // uniform
-            visit(j, j * THREADS + tid);
-        }
-    };
-    int turn = 0;
-    const Threshold at = find_threshold<THREADS>(keep, cl, counts, buf, turn, [&](auto visit) {
-        each_item([&](int j, int i) { visit(key[j], i < n); });
-    });
-    each_item([&](int j, int i) {
-        const uint32_t a = __ballot_sync(0xffffffffu, i < n && key[j] > at.key), l = __ballot_sync(0xffffffffu, i < n && key[j] == at.key);
-        if ((tid & 31) == 0) {
-            stay[i / 32] = a;
-            level[i / 32] = l;
-        }
-    });
-    __syncthreads();
-    const int moves = number_moves<THREADS>(stay, level, first, n > 0 ? (n + 31) / 32 : 0, keep, keep - at.above, cl, shared, buf, turn);
-    __syncthreads();
-    extern __shared__ int32_t ev_list[];             // of a CTA that copies
+    extern __shared__ int32_t ev_list[];             // of CTAs that copy
     int32_t *from = CHUNKS > 0 ? ev_list : p.from + unit * p.max_moves, *to = CHUNKS > 0 ? ev_list + p.max_moves : p.to + unit * p.max_moves;
-    each_item([&](int, int i) {
-        if (i < n) token_move(stay, level, first, t0 + i, keep, [&](int k) { to[k] = t0 + i; }, [&](int k) { from[k] = t0 + i; });
-    });
-    cl.sync();
-    if constexpr (CHUNKS > 0) {                      // one CTA
-        constexpr int W = THREADS / 32, kEach = 4;   // eight took the planning's registers: 64 tokens of 384 CTAs 23.3 us, 20.4
-        for (int i = (tid >> 5) * kEach; i < moves; i += W * kEach)
-            copy_tokens<CHUNKS, kEach>(p, (int)(unit % p.Hkv), u.start, u.first_fill, i, moves, [&](int k) { return from[k]; },
-                                [&](int k) { return to[k]; });
+    __shared__ int planned;
+    int moves = 0;
+    if (copier > 0) {
+        if (u.n <= keep) return;
     } else {
+        uint32_t key[ITEMS];
+#pragma unroll
+        for (int j0 = 0; j0 < ITEMS; j0 += kBatch) {     // reads of a batch, then its writes
+            if (j0 * THREADS >= n) break;
+            EvictToken x[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch && j0 + j < ITEMS; ++j) x[j] = read_token(u, min(t0 + (j0 + j) * THREADS + tid, u.n - 1));
+#pragma unroll
+            for (int j = 0; j < kBatch && j0 + j < ITEMS; ++j) {
+                const int i = (j0 + j) * THREADS + tid;
+                key[j0 + j] = key_of(p, u, x[j]);
+                if (i < n && t0 + i < front) keep_token(p, u, t0 + i, x[j]);
+            }
+        }
+        if (u.n <= keep) return;
+        __syncthreads();
+        const auto each_item = [&](auto visit) {         // of the CTA's tokens, whole warps
+#pragma unroll
+            for (int j = 0; j < ITEMS; ++j) {
+                if (j * THREADS >= n) break;             // uniform
+                visit(j, j * THREADS + tid);
+            }
+        };
+        int turn = 0;
+        const Threshold at = find_threshold<THREADS>(keep, cl, counts, buf, turn, [&](auto visit) {
+            each_item([&](int j, int i) { visit(key[j], i < n); });
+        });
+        each_item([&](int j, int i) {
+            const uint32_t a = __ballot_sync(0xffffffffu, i < n && key[j] > at.key), l = __ballot_sync(0xffffffffu, i < n && key[j] == at.key);
+            if ((tid & 31) == 0) {
+                stay[i / 32] = a;
+                level[i / 32] = l;
+            }
+        });
+        __syncthreads();
+        moves = number_moves<THREADS>(stay, level, first, n > 0 ? (n + 31) / 32 : 0, keep, keep - at.above, cl, shared, buf, turn);
+        __syncthreads();
+        each_item([&](int, int i) {
+            if (i < n) token_move(stay, level, first, t0 + i, keep, [&](int k) { to[k] = t0 + i; }, [&](int k) { from[k] = t0 + i; });
+        });
+    }
+    if constexpr (CHUNKS > 0) {
+        constexpr int W = THREADS / 32, kEach = 4;   // eight took the planning's registers: 64 tokens of 384 CTAs 23.3 us, 20.4
+        const int32_t *source = from, *hole = to;    // the planning CTA's
+        if (copiers > 1) {
+            if (tid == 0) planned = moves;
+            auto all = cooperative_groups::this_cluster();
+            all.sync();
+            moves = *all.map_shared_rank(&planned, 0);
+            source = all.map_shared_rank(from, 0);
+            hole = all.map_shared_rank(to, 0);
+        } else {
+            __syncthreads();
+        }
+        for (int i = (copier * W + (tid >> 5)) * kEach; i < moves; i += copiers * W * kEach)
+            copy_tokens<CHUNKS, kEach>(p, (int)(unit % p.Hkv), u.start, u.first_fill, i, moves, [&](int k) { return source[k]; },
+                                       [&](int k) { return hole[k]; });
+    } else {
+        cl.sync();
         if (cl.rank == 0 && tid == 0) p.count[unit] = moves;
     }
-    for (int i = cl.rank * THREADS + tid; i < moves; i += cluster * THREADS) {
-        const EvictToken x = read_token(u, from[i]);
-        p.mass_out[u.at + to[i]] = x.mass;
-        p.pos_out[u.at + to[i]] = x.pos;
+    if (copier == 0) {
+        for (int i = cl.rank * THREADS + tid; i < moves; i += cl.size * THREADS) {
+            const EvictToken x = read_token(u, from[i]);
+            p.mass_out[u.at + to[i]] = x.mass;
+            p.pos_out[u.at + to[i]] = x.pos;
+        }
     }
+    if (CHUNKS > 0 && copiers > 1) cooperative_groups::this_cluster().sync();    // the lists are read until here
 }
 
 // Longer ones, whose keys fit neither registers nor shared memory: they are made again in every pass.
@@ -602,14 +626,23 @@ evict_move_kernel(const EvictParams p, int parts) {
                         [&](int k) { return from[k]; }, [&](int k) { return to[k]; });
 }
 
+// How an eviction is cut, by the caller's bounds
+struct EvictCut {
+    int64_t units, most, max_moves;
+    int cluster;                      // CTAs that plan a unit
+    int copiers;                      // CTAs that copy behind the plan, from lists in shared memory
+    bool fused;                       // they do; else a launch of its own
+    size_t bytes;
+};
 template <int THREADS, int ITEMS>
-static cudaError_t launch_evict(const EvictParams& p, int64_t units, int cluster, bool fused, bool f32, cudaStream_t st) {
-    const auto kernel = !fused ? evict_kernel<THREADS, ITEMS, 0> : f32 ? evict_kernel<THREADS, ITEMS, 32> : evict_kernel<THREADS, ITEMS, 16>;
-    const size_t smem = fused ? 2 * (size_t)p.max_moves * sizeof(int32_t) : 0;
+static cudaError_t launch_evict(const EvictParams& p, const EvictCut& cut, bool f32, cudaStream_t st) {
+    const auto kernel = !cut.fused ? evict_kernel<THREADS, ITEMS, 0> : f32 ? evict_kernel<THREADS, ITEMS, 32> : evict_kernel<THREADS, ITEMS, 16>;
+    const size_t smem = cut.fused ? 2 * (size_t)p.max_moves * sizeof(int32_t) : 0;
+    const int ctas = cut.fused ? cut.copiers : cut.cluster;
     // Not early are small CTAs in front of a launch of copies, whose CTAs would wait among them (8 sequences of 2304 cut to 2048 13.9 us, 12.4);
     // of the large ones (8 of 16384 cut to 2048) early saves a call 43.2 us -> 40.5.
-    const bool early = (fused || THREADS == 1024) && units * cluster <= sm_count();
-    return launch_cluster(early, kernel, (unsigned)(units * cluster), THREADS, smem, cluster, st, p, cluster);
+    const bool early = (cut.fused || THREADS == 1024) && cut.units * ctas <= sm_count();
+    return launch_cluster(early, kernel, (unsigned)(cut.units * ctas), THREADS, smem, ctas, st, p, cut.cluster, cut.copiers);
 }
 
 static int64_t evict_max_moves(int max_pages, int keep) {
@@ -624,20 +657,16 @@ static int evict_cluster(int64_t units, int64_t most) {
     while (c < 4 && most > 4096 * c && units * c * 2 <= sm_count()) c *= 2;
     return most > 16384 * c ? 4 : c;
 }
-// How an eviction is cut, by the caller's bounds
-struct EvictCut {
-    int64_t units, most, max_moves;
-    int cluster;
-    bool fused;                       // the planning CTA copies, from lists in its shared memory
-    size_t bytes;
-};
 static EvictCut evict_cut(const ktk_shape* s, int max_pages, int keep) {
     EvictCut c;
     c.units = (int64_t)s->batch * s->num_kv_heads;
     c.most = (int64_t)max_pages * kPageSize;
     c.max_moves = evict_max_moves(max_pages, keep);
     c.cluster = evict_cluster(c.units, c.most);
-    c.fused = c.cluster == 1 && c.max_moves <= kEvFused;
+    c.copiers = 1;
+    if (c.cluster == 1)
+        while (c.copiers < kEvCopiers && c.max_moves > 32 * c.copiers && c.units * c.copiers * 2 <= sm_count()) c.copiers *= 2;
+    c.fused = c.cluster == 1 && (c.max_moves <= kEvFused || c.max_moves <= kEvFusedEach * c.copiers);
     c.bytes = c.fused ? 0 : (size_t)c.units * (1 + 2 * (size_t)c.max_moves) * sizeof(int32_t);
     return c;
 }
@@ -704,9 +733,9 @@ extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_
     cudaStream_t st = (cudaStream_t)stream;
     const bool f32 = s->dtype == KTK_F32;
     if (cut.most <= 4096) {
-        KTK_CUDA_TRY((launch_evict<256, 16>(p, cut.units, cut.cluster, cut.fused, f32, st)), who);
+        KTK_CUDA_TRY((launch_evict<256, 16>(p, cut, f32, st)), who);
     } else if (cut.most <= 16384 * cut.cluster) {
-        KTK_CUDA_TRY((launch_evict<1024, 16>(p, cut.units, cut.cluster, cut.fused, f32, st)), who);
+        KTK_CUDA_TRY((launch_evict<1024, 16>(p, cut, f32, st)), who);
     } else {
         const size_t smem = (size_t)((cut.most + 31) / 32) * 2 * sizeof(uint32_t);
         KTK_CUDA_TRY(cudaFuncSetAttribute(evict_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);

@@ -428,10 +428,10 @@ def test_launches_are_counted(cuda_device):
         return ops.launch_count() - before
     decode = lambda most: ops.dense_decode_mass(s["q"], *s["table"], most, s["mass"])
     prefill = lambda window: ops.prefill_attention_mass(s["qs"], s["indptr"], s["new"], *s["table"], s["mass"], window=window)
-    evict = lambda keep: ops.evict(*s["table"], s["most"], s["mass"], s["positions"], s["stored"], s["seen"], keep)
+    evict = lambda keep, most: ops.evict(*s["table"], most, s["mass"], s["positions"], s["stored"], s["seen"], keep)
     assert [count(lambda: decode(most)) for most in (s["most"], 30000)] == [1, 2]
     assert [count(lambda: prefill(window)) for window in (20, 0)] == [2, 3]           # 800 rows in parts of 512
-    assert [count(lambda: evict(keep)) for keep in (1300, 500)] == [1, 2]
+    assert [count(lambda: evict(keep, most)) for keep, most in ((1300, s["most"]), (500, s["most"]), (500, 4000))] == [1, 1, 2]
 
 
 def test_refusals_on_the_device(cuda_device):

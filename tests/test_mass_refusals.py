@@ -29,7 +29,7 @@ def _prefill(shape=None, mass=None, total=5, new=3, pages=4, window=0, scale=0.1
                                                   mass or _mass(), ONE, ws, bytes_, shape or _shape(**kw), NULL, NULL)
 
 
-def _evict(shape=None, mass=None, pos=ONE, pos_out=ONE, pages=40, keep=200, sink=0, recent=0, ws=ONE, bytes_=1 << 30, kv=ONE, **kw):
+def _evict(shape=None, mass=None, pos=ONE, pos_out=ONE, pages=400, keep=2000, sink=0, recent=0, ws=ONE, bytes_=1 << 30, kv=ONE, **kw):
     return _lib.load().ktk_evict(kv, ONE, ONE, ONE, None, pages, mass or _mass(), pos, pos_out, ONE, ONE, keep, sink, recent, ws, bytes_,
                                  shape or _shape(**kw), NULL, NULL)
 
@@ -79,8 +79,10 @@ def test_workspaces_are_sized_by_what_is_given():
     assert ops.decode_mass_workspace_bytes(2, 1, 4, 4000, torch.bfloat16, 50) == small
     assert lib.ktk_decode_mass_workspace_bytes(_shape(head_dim=64), 4000, -1) == 0
     assert lib.ktk_evict_workspace_bytes(shp, 4, 40) == 0                                         # 24 of 64 tokens can move: one launch
-    assert lib.ktk_evict_workspace_bytes(shp, 40, 200) == 2 * 4 * (1 + 2 * 200)
-    assert lib.ktk_evict_workspace_bytes(shp, 40, 500) == 2 * 4 * (1 + 2 * 140)
+    assert lib.ktk_evict_workspace_bytes(shp, 40, 200) == 0                                       # 200, and few rows: the same
+    assert lib.ktk_evict_workspace_bytes(_shape(batch=200), 40, 200) == 200 * 4 * (1 + 2 * 200)
+    assert lib.ktk_evict_workspace_bytes(shp, 256, 2000) == 2 * 4 * (1 + 2 * 2000)
+    assert lib.ktk_evict_workspace_bytes(shp, 256, 2500) == 2 * 4 * (1 + 2 * 1596)
     assert lib.ktk_evict_workspace_bytes(shp, 32769, 500) == 0                                    # refused
     # a share of scores in bytes passes 32 bits: no list of that length is kept in shared memory
     assert lib.ktk_decode_mass_workspace_bytes(_shape(group_size=8, batch=1), 1 << 26, 100) > 0
