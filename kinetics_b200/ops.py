@@ -375,13 +375,14 @@ def _address(t, dev: int) -> int:
     return t.data_ptr()
 
 
-_current_device, _current_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# a workspace for one call: given back when the launches are in the stream, whose next allocations come behind them (a tensor costs 1.1 us more)
+_take, _give_back = torch._C._cuda_cudaCachingAllocator_raw_alloc, torch._C._cuda_cudaCachingAllocator_raw_delete
+_SM_SCALE = HEAD_DIM ** -0.5
 
 
 def _view_of(view, dev: int):
     """The view as the library takes it, its tensors on device `dev`."""
-    if view is None:
-        return None
     _address(view.page_count, dev)
     _address(view.slot_index, dev)
     return view.c()
@@ -469,6 +470,14 @@ def _tables(batch, kv_indices, kv_indptr, kv_last_page_len, view):
             (kv_last_page_len.dtype, batch, kv_last_page_len.numel())) + more
 
 
+def _workspace(workspace, need: int, dev: int, stream: int):
+    """Address and bytes of a call's workspace, and the address to give back behind the launches (0: none)."""
+    if workspace is not None:
+        return _address(workspace, dev), workspace.nbytes, 0
+    at = _take(need, stream)
+    return at, need, at
+
+
 def _same(t, like, what) -> None:
     if t.dtype != like.dtype or t.shape != like.shape:
         raise TypeError(f"{what} must have the dtype and shape {like.dtype} {tuple(like.shape)}, got {t.dtype} {tuple(t.shape)}")
@@ -507,13 +516,16 @@ def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_
     else:
         _same(mass_out, mass, "mass_out")
         mo_ = _address(mass_out, dev)
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    check(_lib.load().ktk_dense_decode_mass(
-        q_, _address(kv_cache, dev), _address(kv_indices, dev), _address(kv_indptr, dev), _address(kv_last_page_len, dev),
-        _view_of(view, dev), max_pages_per_seq, pages, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
-        _lib.Mass(m_, mo_, mass_shape[2], mass_shape[0], decay), _address(out, dev), _address(workspace, dev),
-        0 if workspace is None else workspace.nbytes, shp, _address(status, dev), _current_stream(dev)))
+    stream = _current_stream(dev)
+    at, size, own = _workspace(workspace, need, dev, stream) if need else (0, 0, 0)
+    try:
+        check(_lib.load().ktk_dense_decode_mass(
+            q_, _address(kv_cache, dev), _address(kv_indices, dev), _address(kv_indptr, dev), _address(kv_last_page_len, dev),
+            view and _view_of(view, dev), max_pages_per_seq, pages, _SM_SCALE if sm_scale is None else sm_scale,
+            _lib.Mass(m_, mo_, mass_shape[2], mass_shape[0], decay), _address(out, dev), at, size, shp, _address(status, dev), stream))
+    finally:
+        if own:
+            _give_back(own)
     _launched(2 if need else 1)
     return out, mass_out
 
@@ -542,13 +554,17 @@ def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indice
     else:
         _same(mass_out, mass, "mass_out")
         mo_ = _address(mass_out, dev)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    check(_lib.load().ktk_prefill_attention_mass(
-        q_, _address(q_indptr, dev), q_shape[0], max_new_tokens, _address(kv_cache, dev), _address(kv_indices, dev), _address(kv_indptr, dev),
-        _address(kv_last_page_len, dev), _view_of(view, dev), most, pages, window,
-        HEAD_DIM ** -0.5 if sm_scale is None else sm_scale, _lib.Mass(m_, mo_, mass_shape[2], mass_shape[0], decay), _address(out, dev),
-        _address(workspace, dev), workspace.nbytes, shp, _address(status, dev), _current_stream(dev)))
+    stream = _current_stream(dev)
+    at, size, own = _workspace(workspace, need, dev, stream) if need else (0, 0, 0)
+    try:
+        check(_lib.load().ktk_prefill_attention_mass(
+            q_, _address(q_indptr, dev), q_shape[0], max_new_tokens, _address(kv_cache, dev), _address(kv_indices, dev),
+            _address(kv_indptr, dev), _address(kv_last_page_len, dev), view and _view_of(view, dev), most, pages, window,
+            _SM_SCALE if sm_scale is None else sm_scale, _lib.Mass(m_, mo_, mass_shape[2], mass_shape[0], decay), _address(out, dev), at,
+            size, shp, _address(status, dev), stream))
+    finally:
+        if own:
+            _give_back(own)
     _launched(launches)
     return out, mass_out
 
@@ -584,12 +600,16 @@ def evict(kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: 
     else:
         _same(positions_out, positions, "positions_out")
         ato_ = _address(positions_out, dev)
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=kv_cache.device)
-    check(_lib.load().ktk_evict(
-        kv_, _address(kv_indices, dev), _address(kv_indptr, dev), _address(kv_last_page_len, dev), _view_of(view, dev),
-        max_pages_per_seq, _lib.Mass(m_, mo_, mass_shape[2], rows, 1.0), at_, ato_, _address(stored, dev), _address(seen, dev), keep, sink,
-        recent, _address(workspace, dev), 0 if workspace is None else workspace.nbytes, shp, _address(status, dev), _current_stream(dev)))
+    stream = _current_stream(dev)
+    at, size, own = _workspace(workspace, need, dev, stream) if need else (0, 0, 0)
+    try:
+        check(_lib.load().ktk_evict(
+            kv_, _address(kv_indices, dev), _address(kv_indptr, dev), _address(kv_last_page_len, dev), view and _view_of(view, dev),
+            max_pages_per_seq, _lib.Mass(m_, mo_, mass_shape[2], rows, 1.0), at_, ato_, _address(stored, dev), _address(seen, dev), keep,
+            sink, recent, at, size, shp, _address(status, dev), stream))
+    finally:
+        if own:
+            _give_back(own)
     _launched(2 if need else 1)
     return mass_out, positions_out
 
