@@ -562,7 +562,9 @@ typedef struct ktk_mass {
  *                also what counts with view->page_count
  *   max_pages_per_seq  at least every sequence's page count; a longer list reports KTK_STATUS_BAD_TABLE and its results are void; 2^26 at most
  *   workspace    ktk_decode_mass_workspace_bytes() bytes: the scores of all tokens, and the partials of lists that are cut; 0, and then
- *                it may be null, for lists that the device holds all at once (a cluster of CTAs each)
+ *                it may be null, for lists that the device holds all at once (a cluster of CTAs each).  The need goes with the form that
+ *                the sizes call for: fewer sequences may need more.  A workspace for calls of several sizes is as large as the most of
+ *                them needs
  * q, kv_cache, o and workspace are 16-byte aligned.
  */
 KTK_API size_t ktk_decode_mass_workspace_bytes(const ktk_shape* shape, int32_t max_pages_per_seq, int64_t total_pages);

@@ -125,16 +125,17 @@ class EvictingKVManager:
         return self.decode(query_states, key_states, value_states, batch_idx, layer_idx).reshape(bsz, seq_len, self.hidden_size)
 
     def _decode_workspace(self):
-        """Sized for all slots once: captured steps keep its address."""
+        """Sized once for any number of active slots: captured steps keep its address."""
         if self._workspace is None:
             need = ops.decode_mass_workspace_bytes(self.max_batch_size, self.num_key_value_heads,
-                                                   self.num_attention_heads // self.num_key_value_heads, self.pages_per_slot, self.dtype)
+                                                   self.num_attention_heads // self.num_key_value_heads, self.pages_per_slot, self.dtype,
+                                                   fewer=True)
             self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
         return self._workspace
 
     def decode(self, query, key, value, batch_idx, layer_idx):
         """One token of every active slot: append, attend, accumulate."""
-        B = batch_idx.numel()
+        B, workspace = batch_idx.numel(), self._decode_workspace()           # before the slots count the token
         if self._step_table is None:
             slots = self._slots_of(batch_idx)
             self._evict(layer_idx, self._full(layer_idx, slots))
@@ -149,7 +150,7 @@ class EvictingKVManager:
         ops.append_kv(rows(key, self.num_key_value_heads), rows(value, self.num_key_value_heads), pages, None, self.kv_indices, start,
                       last, status=self.status, view=view)
         out, _ = ops.dense_decode_mass(rows(query, self.num_attention_heads), pages, self.kv_indices, start, last, self.pages_per_slot,
-                                       self.mass[layer_idx], self.decay, self.sm_scale, workspace=self._decode_workspace(),
+                                       self.mass[layer_idx], self.decay, self.sm_scale, workspace=workspace,
                                        status=self.status, view=view)
         return out
 

@@ -484,11 +484,14 @@ def _same(t, like, what) -> None:
 
 
 def decode_mass_workspace_bytes(batch: int, num_kv_heads: int, group_size: int, max_pages_per_seq: int, dtype=torch.bfloat16,
-                                total_pages: int = -1) -> int:
+                                total_pages: int = -1, fewer: bool = False) -> int:
     """Bytes of workspace that ``dense_decode_mass`` needs; total_pages: entries of all page lists (-1, and always with a
-    view.page_count: batch * max_pages_per_seq)."""
-    shp = Shape(batch, num_kv_heads, group_size, HEAD_DIM, PAGE_SIZE, _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32, 0)
-    return int(_lib.load().ktk_decode_mass_workspace_bytes(shp, max_pages_per_seq, total_pages))
+    view.page_count: batch * max_pages_per_seq).  The need goes with the form that the number of sequences calls for and does not grow with
+    it; fewer: what is enough for a call of any number of sequences up to ``batch``."""
+    code = _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32
+    need = lambda n: int(_lib.load().ktk_decode_mass_workspace_bytes(Shape(n, num_kv_heads, group_size, HEAD_DIM, PAGE_SIZE, code, 0),
+                                                                     max_pages_per_seq, total_pages))
+    return max(map(need, range(1, batch + 1)), default=0) if fewer else need(batch)
 
 
 def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: int, mass, decay: float = 1.0,

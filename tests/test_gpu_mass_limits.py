@@ -1,0 +1,98 @@
+"""The operators of a bounded cache at their limits: batches that shrink under a manager, sequences beyond a call's bounds, pages that are
+none, host threads; against plain fp64 forms."""
+import numpy as np
+import pytest
+import torch
+
+from helpers import paged_state, to_dev
+from mass_helpers import attend, mass_after
+
+pytestmark = pytest.mark.gpu
+D = 128
+
+
+def _lists(seed, device, lens, kv_heads, group, dtype, padded, new=None):
+    """Sequences of `lens` tokens whose last `new` (None: one each) have queries, in row b of the masses sequence b; the page table packed
+    or with page counts."""
+    from kinetics_b200 import ops
+    g = torch.Generator().manual_seed(seed)
+    new = new or [1] * len(lens)
+    cast = lambda t: t.to(dtype).float()
+    k, v = (cast(torch.randn(len(lens), kv_heads, max(lens), D, generator=g)) for _ in range(2))
+    q = cast(1.3 * torch.randn(sum(new), kv_heads * group, D, generator=g))
+    st = paged_state(k, v, lens, dtype, seed=seed, fill=0.5)
+    d = to_dev(st, device)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+    view = ops.PageView(0, 0, i32(st["npages"]) if padded else None, i32(range(len(lens))))
+    starts = d["kv_indptr"][:-1].contiguous() if padded else d["kv_indptr"]
+    mass = torch.rand(len(lens), kv_heads, max(lens) + 3, generator=g)
+    return dict(k=k, v=v, q=q, mass=mass, lens=lens, new=new, group=group, dtype=dtype, view=view, pages=st["npages"], first=st["kv_indptr"].tolist(),
+                table=[d["kv_cache"], d["kv_indices"], starts, d["kv_last_page_len"]], indptr=i32(np.concatenate([[0], np.cumsum(new)]).tolist()))
+
+
+def _equals(c, b, out, mass, window, decay, without=None):
+    """Outputs and masses of sequence b are those of the fp64 form, with the tokens `without` taking no part."""
+    n, w, G = c["lens"][b], c["new"][b], c["group"]
+    part = np.setdiff1d(np.arange(n), [] if without is None else without)
+    first = sum(c["new"][:b])
+    for h in range(c["k"].shape[1]):
+        q = c["q"][first:first + w, h * G:(h + 1) * G]
+        o, o_bound, some, some_bound = attend(q, c["k"][b, h, part], c["v"][b, h, part], w, window, D ** -0.5, c["dtype"])
+        err = (out[first:first + w, h * G:(h + 1) * G].double().cpu() - o).abs()
+        assert bool((err <= o_bound).all()), (b, h, float((err / o_bound).max()))
+        paid, bound = torch.zeros(n, dtype=torch.float64), torch.zeros(n, dtype=torch.float64)
+        paid[part], bound[part] = some, some_bound
+        want, more = mass_after(c["mass"], b, n, w, h, decay, paid)
+        err = (mass[b, h, :n].double().cpu() - want).abs()
+        assert bool((err <= bound + more).all()), (b, h, float((err - bound - more).max()))
+        assert torch.equal(mass[b, h, n:].cpu(), c["mass"][b, h, n:])
+
+
+# ---------------------------------------------------------------- a manager whose batch shrinks
+class Cfg:
+    hidden_size = 4096
+    num_attention_heads = 32
+    num_key_value_heads = 8
+    head_dim = 128
+    num_hidden_layers = 1
+
+
+@pytest.mark.parametrize("dtype, active", [(torch.bfloat16, (16, 10, 16, 10, 3)), (torch.float32, (16, 4, 7, 1, 2))])
+def test_a_manager_of_sixteen_slots_with_fewer_active(cuda_device, dtype, active):
+    from kinetics_b200 import EvictingKVManager
+    kv = EvictingKVManager(Cfg, 16, 4096, cuda_device, dtype, keep=2048)
+    g = torch.Generator().manual_seed(31)
+    keys, values = ([torch.zeros(0, 8, D) for _ in range(16)] for _ in range(2))
+    for n in active:
+        slots = torch.randperm(16, generator=g)[:n].tolist()
+        q, k, v = (torch.randn(n, heads, 1, D, generator=g).to(dtype) for heads in (32, 8, 8))
+        kv.begin_step(slots)
+        out = kv.compute_attention(*(t.to(cuda_device) for t in (q, k, v)), 0, torch.tensor(slots, device=cuda_device)).view(n, 32, D)
+        for i, s in enumerate(slots):
+            keys[s], values[s] = torch.cat((keys[s], k[i].float().transpose(0, 1))), torch.cat((values[s], v[i].float().transpose(0, 1)))
+            for h in range(8):
+                o, bound, _, _ = attend(q[i, 4 * h:4 * h + 4].float().transpose(0, 1), keys[s][:, h], values[s][:, h], 1, 0, D ** -0.5, dtype)
+                err = (out[i, 4 * h:4 * h + 4].double().cpu() - o[0]).abs()
+                assert bool((err <= bound[0]).all()), (n, s, h)
+    kv.check_status()
+
+
+def test_an_engine_that_drains_its_slots(cuda_device):
+    # requests of different lengths end one after the other: every number of active sequences from 16 down to 1
+    from kinetics_b200 import DecoderStack, Engine, EvictingKVManager
+    from kinetics_b200.config import LayerConfig
+    cfg, dtype = LayerConfig(hidden_size=256, num_attention_heads=8, num_key_value_heads=4, intermediate_size=512, num_hidden_layers=2,
+                             vocab_size=503), torch.float32
+    g = torch.Generator().manual_seed(32)
+    kv = EvictingKVManager(cfg, 16, 400, cuda_device, dtype, keep=2048)
+    eng = Engine(DecoderStack(cfg, cuda_device, dtype, max_positions=400, seed=3), kv, 400, cuda_device, temperature=0.0, repeat_check=False)
+    prompts = [torch.randint(0, 500, (1, 2 + i), generator=g) for i in range(16)]
+    for slot, p in enumerate(prompts):
+        eng.prefill(slot, p, 40)
+    for n in range(16, 0, -1):
+        eng.decode(list(range(n)))
+        if n % 3 == 0:
+            for _ in range(3):                                          # eager, captured, replayed
+                eng.decode_graphed(list(range(n)))
+    kv.check_status()
+    assert kv.cached(0) == 2 + 16 + 15
