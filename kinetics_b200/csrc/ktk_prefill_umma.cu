@@ -117,7 +117,7 @@ prefill_umma_kernel(const PrefillUmmaParams p, const __grid_constant__ CUtensorM
     if (tok0 >= n_new) return;                      // uniform for the CTA: nothing allocated yet
 
     const int base_pos = sp.total - n_new;          // position of the sequence's first new token
-    if (sp.bad || base_pos < 0) {
+    if (sp.bad || base_pos < 0 || q0 < 0 || q0 + (int64_t)n_new > p.total_new) {
         if (tid == 0) report(p.status, KTK_STATUS_BAD_TABLE);
         return;
     }

@@ -96,3 +96,27 @@ def test_an_engine_that_drains_its_slots(cuda_device):
                 eng.decode_graphed(list(range(n)))
     kv.check_status()
     assert kv.cached(0) == 2 + 16 + 15
+
+
+# ---------------------------------------------------------------- beyond a call's bounds
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens", [(300, 340), (2500, 3000)])             # a CTA per tile, CTAs that share the keys
+@pytest.mark.parametrize("indptr, good", [((0, 33, 133), 0), ((-7, 33, 73), 1), ((0, 33, 2 ** 31 - 1), 0)])
+def test_new_tokens_outside_the_queries_are_not_touched(cuda_device, indptr, good, lens, dtype):
+    from kinetics_b200 import _lib, ops
+    c, status = _lists(47, cuda_device, list(lens), 2, 4, dtype, False, new=[33, 40]), ops.new_status(cuda_device)
+    # outputs and workspace in the middle of more, which has to stay
+    rows = torch.full((73 + 400, 8, D), 7.0, dtype=dtype, device=cuda_device)
+    out = rows[200:273]
+    pages = min(c["mass"].shape[2] // 16 + 2, sum(c["pages"]))
+    shape = _lib.Shape(2, 2, 4, D, 16, 1 if dtype == torch.bfloat16 else 0, 0)
+    need = _lib.load().ktk_prefill_mass_workspace_bytes(shape, 73, 40, pages, sum(c["pages"]), 0)
+    space = torch.full((need + 2 ** 18,), 0x5a, dtype=torch.uint8, device=cuda_device)
+    at = 2 ** 17
+    _, mass = ops.prefill_attention_mass(c["q"].to(dtype).to(cuda_device), torch.tensor(indptr, dtype=torch.int32, device=cuda_device), 40,
+                                         *c["table"], c["mass"].to(cuda_device), 0, 0.75, out=out, workspace=space[at:at + need], status=status,
+                                         view=c["view"])
+    assert int(status.item()) == 2 and torch.equal(mass[1 - good].cpu(), c["mass"][1 - good])
+    assert bool((rows[:200] == 7).all()) and bool((rows[273:] == 7).all())
+    assert bool((space[:at] == 0x5a).all()) and bool((space[at + need:] == 0x5a).all())
+    _equals(c, good, out, mass, 0, 0.75)
