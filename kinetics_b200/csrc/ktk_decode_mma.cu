@@ -24,6 +24,10 @@ struct MmaParams {
     int G;
 };
 
+// Phase of a stage's barrier that ends with the last copy into it, by the stage's tag: issue index + 1 of its page, negated where there was
+// nothing to load, 0 before the first.  -1: the last one had nothing to load
+__host__ __device__ constexpr int last_copy(int tag, int stages) { return tag > 0 ? (tag - 1) / stages & 1 : -1; }
+
 // MASS: weights are accumulated too; the splits of a list are a cluster, and the scores of a CTA's tokens stay in shared memory, behind the
 // stages.
 template <int STAGES, int CTAS, bool MASS>
@@ -72,6 +76,7 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
         for (int s = 0; s < kMmaStages; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
+            if (MASS) stage_tag[s] = 0;
         }
         abort_flag = 0;
         issued_total = 0;
@@ -86,7 +91,6 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
     if (warp == kMmaConsumers) {
         // ---------------- producer warp ----------------
         if (lane == 0) prefetch_tensormap(&kv_map);
-        int issued = 0;
         if constexpr (MASS) {
             // A load takes its thread some 600 cycles, whatever else is in flight: with a deep ring eight lanes issue in turn (one sequence
             // of 8192 tokens, 8 kv heads, 64 CTAs: 29 us by one lane, 18.6); with four CTAs per SM one each is faster (48 of 2304: 77.9
@@ -107,17 +111,11 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
                         stage_tag[s] = i + 1;
                         tma_load_whole_page(stages + s * kStageBytes, &kv_map, &full_bar[s], page, h, policy);
                     }
-                    issued = i + 1;
-                }
-                // the CTA gave up: its shared memory is written until the last copies have landed
-                if (abort_flag) {
-                    volatile int never = 0;
-                    for (int i = lane; i < issued; i += kIssuers)
-                        if (i + kMmaStages >= issued) mbar_wait(&full_bar[i % kMmaStages], (i / kMmaStages) & 1, &never);
                 }
             }
             __syncwarp();
         } else {
+            int issued = 0;
             int next_ids = (e0 + lane < e1) ? el.ptr[e0 + lane] : -1;
             bool alive = true;
             for (int base = e0; base < e1 && alive; base += 32) {
@@ -189,9 +187,16 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
             report(d.status, KTK_STATUS_TIMEOUT);
             // wait, again bounded, for copies still in flight before the CTA's shared memory is released
             volatile int never = 0;
-            const int total = issued_total;
-            for (int i = (MASS ? total : total > kMmaStages ? total - kMmaStages : 0); i < total; ++i)
-                mbar_wait(&full_bar[i % kMmaStages], (i / kMmaStages) & 1, &never);
+            if constexpr (MASS) {                             // by several lanes, which may have stopped anywhere: each stage's last one
+                for (int s = 0; s < kMmaStages; ++s) {
+                    const int phase = last_copy(stage_tag[s], kMmaStages);
+                    if (phase >= 0) mbar_wait(&full_bar[s], phase, &never);
+                }
+            } else {
+                const int total = issued_total;
+                for (int i = (total > kMmaStages ? total - kMmaStages : 0); i < total; ++i)
+                    mbar_wait(&full_bar[i % kMmaStages], (i / kMmaStages) & 1, &never);
+            }
         }
         if (!MASS) return;
         __syncthreads();                                      // the cluster's other CTAs wait for this one: its results are void

@@ -1,8 +1,15 @@
 """The operators of a bounded cache at their limits, on the host."""
+import random
+import re
+import subprocess
+from pathlib import Path
+
 import pytest
 import torch
 
 from kinetics_b200 import EvictingKVManager, ops
+
+CSRC = Path(__file__).resolve().parent.parent / "kinetics_b200" / "csrc"
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -24,3 +31,35 @@ def test_a_size_for_fewer_sequences():
     assert size(16) == 0 < size(10)                                     # a cluster each; balanced
     assert size(16, fewer=True) == size(10) == size(10, fewer=True) and size(9, fewer=True) == 0
     assert size(0) == size(0, fewer=True) == 0
+
+
+def test_a_decode_that_gives_up_waits_for_the_copies_of_all_lanes(tmp_path):
+    """Lanes that issue in turn may stop anywhere; behind the barrier of the block each stage's last copy is waited for, by the stage's tag.
+    Compiled here from the source, against a ring that is filled step by step."""
+    text = (CSRC / "ktk_decode_mma.cu").read_text()
+    rule = re.search(r"^__host__ __device__ constexpr int last_copy\(.*$", text, re.M).group(0)
+    (tmp_path / "rule.cpp").write_text("#include <cstdio>\n#define __host__\n#define __device__\n" + rule + """
+int main() { int tag, stages; while (scanf("%d %d", &tag, &stages) == 2) printf("%d\\n", last_copy(tag, stages)); }
+""")
+    subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "rule"), str(tmp_path / "rule.cpp")], check=True)
+    rng, asked, want = random.Random(1), [], []
+    for stages, lanes in ((4, 1), (8, 8), (16, 8)):
+        for n in range(0, 70):
+            none = {i for i in range(n) if rng.random() < 0.2}           # pages with nothing to load
+            stop = [rng.randint(0, n) for _ in range(lanes)]             # where each lane stopped
+            tags, fills, loaded = [0] * stages, [0] * stages, [False] * stages
+            for i in range(n):
+                if i < stop[i % lanes]:
+                    s = i % stages
+                    tags[s], loaded[s], fills[s] = (-(i + 1) if i in none else i + 1), i not in none, fills[s] + 1
+            asked += [(tag, stages) for tag in tags]
+            # the f-th fill of a stage ends phase f - 1 of its barrier
+            want += [(f - 1) % 2 if there else -1 for f, there in zip(fills, loaded)]
+    out = subprocess.run([str(tmp_path / "rule")], input="\n".join(f"{t} {s}" for t, s in asked), capture_output=True, text=True, check=True)
+    assert list(map(int, out.stdout.split())) == want
+    kernel = text[text.index("decode_mma_kernel(const MmaParams"):text.index("// ---- merge the consumer warps")]
+    issue, behind = kernel.split("__syncthreads();   // every page consumed")
+    assert "if (MASS) stage_tag[s] = 0;" in issue and "never" not in issue          # nobody waits before the block has met
+    assert re.search(r"for \(int s = 0; s < kMmaStages; \+\+s\) \{\s*const int phase = last_copy\(stage_tag\[s\], kMmaStages\);\s*"
+                     r"if \(phase >= 0\) mbar_wait\(&full_bar\[s\], phase, &never\);", behind)
+    assert behind.index("last_copy(") < behind.index("if (!MASS) return;")
