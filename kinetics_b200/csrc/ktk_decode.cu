@@ -70,7 +70,8 @@ decode_simt_kernel(const DecodeParams p, const typename MassArgument<MASS>::type
 
     bool bad;
     EntryList el = entry_list(p, b, h, bad);
-    if (MASS == kMassCluster && el.cnt > mp.max_pages) {      // the scores of more do not fit
+    // the scores of more do not fit: shared memory, or the place of a padded list, behind which lies the next list's
+    if ((MASS == kMassCluster || (MASS == kMassLong && p.page_count != nullptr)) && el.cnt > mp.max_pages) {
         el.cnt = mp.max_pages;
         bad = true;
     }

@@ -120,3 +120,21 @@ def test_new_tokens_outside_the_queries_are_not_touched(cuda_device, indptr, goo
     assert bool((rows[:200] == 7).all()) and bool((rows[273:] == 7).all())
     assert bool((space[:at] == 0x5a).all()) and bool((space[at + need:] == 0x5a).all())
     _equals(c, good, out, mass, 0, 0.75)
+
+
+BEYOND = [(700, 30, 2), (8100, 500, 1)]            # tokens of the long list, bound in pages, kv heads: by clusters, with scores in memory
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("padded", [False, True])
+@pytest.mark.parametrize("long, most, kv_heads", BEYOND)
+def test_a_list_beyond_the_bound_leaves_the_others_alone(cuda_device, long, most, kv_heads, padded, dtype):
+    from kinetics_b200 import ops
+    c, status = _lists(41, cuda_device, [300, long, 90, 5], kv_heads, 4, dtype, padded), ops.new_status(cuda_device)
+    assert c["pages"][1] > most and (ops.decode_mass_workspace_bytes(4, kv_heads, 4, most, dtype) > 0) == (most > 30)
+    for _ in range(4):
+        out, mass = ops.dense_decode_mass(c["q"].to(dtype).to(cuda_device), *c["table"], most, c["mass"].to(cuda_device), 0.75, status=status,
+                                          view=c["view"])
+        assert int(status.item()) == 2
+        for b in (0, 2, 3):
+            _equals(c, b, out, mass, 0, 0.75)
