@@ -72,7 +72,8 @@ __device__ __forceinline__ bool item_of_either(const PrefillUmmaParams& p, int& 
     const int spread = (int)(__reduce_max_sync(0xffffffffu, n > 0 ? (unsigned)history : 0u) -
                              __reduce_min_sync(0xffffffffu, n > 0 ? (unsigned)history : 0x7fffffffu));
     if (spread <= longest / 4) return false;               // the same for all CTAs
-    item = item_by_length(blockIdx.z * gridDim.y + blockIdx.y, p.tiles * (kUmRows / p.G), p.batch, lane < p.batch && n > 0 ? n : 0, history);
+    item = item_by_length(blockIdx.z * gridDim.y + blockIdx.y, p.tiles * (kUmRows / p.G), p.batch,
+                          lane < p.batch && n > 0 ? min(n, p.max_new) : 0, history);       // those beyond the bound have no place in the grid
     return true;
 }
 
@@ -370,6 +371,7 @@ int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st
     const int64_t per_seq = ((int64_t)max_new_tokens + tpc - 1) / tpc, most = p.total_new / tpc + p.batch;
     const int64_t tiles = (p.batch * per_seq < most ? p.batch * per_seq : most) * p.Hkv;
     p.tiles = tiles <= sm_count() ? 1 : 2;
+    p.max_new = max_new_tokens;
     int cluster = 1;
     if (p.lse != nullptr && p.max_pages >= kPuSplit * kPuPages) {        // as many CTAs as there are SMs, two blocks each
         const int64_t both = (per_seq + 1) / 2, some = p.total_new / (2 * tpc) + p.batch;

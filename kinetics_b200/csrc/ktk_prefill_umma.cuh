@@ -18,6 +18,7 @@ struct PrefillUmmaParams {
     int batch, Hkv, G;
     int64_t total_new;
     int tiles;                 // of a CTA: 1 or 2 (set by launch_prefill_umma)
+    int max_new;               // the caller's bound of a sequence's new tokens (set by launch_prefill_umma)
     int64_t num_pages;
     float scale_log2;
     int32_t* status;

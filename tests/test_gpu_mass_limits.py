@@ -138,3 +138,16 @@ def test_a_list_beyond_the_bound_leaves_the_others_alone(cuda_device, long, most
         assert int(status.item()) == 2
         for b in (0, 2, 3):
             _equals(c, b, out, mass, 0, 0.75)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_new_tokens_than_the_bound_where_portions_go_by_length(cuda_device, dtype):
+    # the portion of 600 has the most keys; the two within the bound of 40 are attended and counted as ever
+    from kinetics_b200 import ops
+    c, status = _lists(43, cuda_device, [660, 340, 140], 4, 8, dtype, False, new=[600, 40, 40]), ops.new_status(cuda_device)
+    q = c["q"].to(dtype).to(cuda_device)
+    out, mass = ops.prefill_attention_mass(q, c["indptr"], 40, *c["table"], c["mass"].to(cuda_device), 0, 0.75,
+                                           out=torch.full_like(q, float("nan")), status=status, view=c["view"])
+    assert int(status.item()) == 2 and torch.equal(mass[0].cpu(), c["mass"][0])
+    for b in (1, 2):
+        _equals(c, b, out, mass, 0, 0.75)
