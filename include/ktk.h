@@ -560,7 +560,8 @@ typedef struct ktk_mass {
  * The weights are those of fp32 scores and denominators.
  *   total_pages  an upper bound of the entries in all lists (sizes the workspace), or -1: batch * max_pages_per_seq, which is
  *                also what counts with view->page_count
- *   max_pages_per_seq  at least every sequence's page count; a longer list reports KTK_STATUS_BAD_TABLE and its results are void; 2^26 at most
+ *   max_pages_per_seq  at least every sequence's page count; a longer list reports KTK_STATUS_BAD_TABLE, its masses stay as they are and its
+ *                output is void; 2^26 at most
  *   workspace    ktk_decode_mass_workspace_bytes() bytes: the scores of all tokens, and the partials of lists that are cut; 0, and then
  *                it may be null, for lists that the device holds all at once (a cluster of CTAs each).  The need goes with the form that
  *                the sizes call for: fewer sequences may need more.  A workspace for calls of several sizes is as large as the most of

@@ -72,7 +72,7 @@ decode_simt_kernel(const DecodeParams p, const typename MassArgument<MASS>::type
     EntryList el = entry_list(p, b, h, bad);
     // the scores of more do not fit: shared memory, or the place of a padded list, behind which lies the next list's
     if ((MASS == kMassCluster || (MASS == kMassLong && p.page_count != nullptr)) && el.cnt > mp.max_pages) {
-        el.cnt = mp.max_pages;
+        el.cnt = 0;
         bad = true;
     }
     if (bad && tid == 0 && split == 0) report(p.status, KTK_STATUS_BAD_TABLE);

@@ -56,9 +56,9 @@ mass_finish_kernel(const StreamParams p, int chunks, int rounds, int merges, int
         return;
     }
     const int64_t start = list_position(d, m.wmax, b, h);
-    if (el.cnt > m.max_pages) {
+    if (el.cnt > m.max_pages) {                           // masses stay as they are, and the output is void
         if (tid == 0 && part == chunks) report(d.status, KTK_STATUS_BAD_TABLE);
-        if (d.page_count) el.cnt = m.max_pages;           // padded lists are clipped by the decode
+        return;
     }
     Pieces<STREAM> pieces;
     if constexpr (STREAM) {

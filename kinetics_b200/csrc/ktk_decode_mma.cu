@@ -62,7 +62,7 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
     bool bad;
     EntryList el = entry_list(d, b, h, bad);
     if (MASS && el.cnt > p.m.max_pages) {                     // the scores of more do not fit
-        el.cnt = p.m.max_pages;
+        el.cnt = 0;
         bad = true;
     }
     if (bad && tid == 0 && split == 0) report(d.status, KTK_STATUS_BAD_TABLE);

@@ -151,3 +151,14 @@ def test_more_new_tokens_than_the_bound_where_portions_go_by_length(cuda_device,
     assert int(status.item()) == 2 and torch.equal(mass[0].cpu(), c["mass"][0])
     for b in (1, 2):
         _equals(c, b, out, mass, 0, 0.75)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("padded", [False, True])
+@pytest.mark.parametrize("long, most, kv_heads", BEYOND)
+def test_a_list_beyond_the_bound_keeps_its_masses(cuda_device, long, most, kv_heads, padded, dtype):
+    from kinetics_b200 import ops
+    c, status = _lists(42, cuda_device, [300, long, 90], kv_heads, 4, dtype, padded), ops.new_status(cuda_device)
+    _, mass = ops.dense_decode_mass(c["q"].to(dtype).to(cuda_device), *c["table"], most, c["mass"].to(cuda_device), 0.75, status=status,
+                                    view=c["view"])
+    assert int(status.item()) == 2 and torch.equal(mass[1].cpu(), c["mass"][1])
