@@ -64,6 +64,10 @@ mass_finish_kernel(const StreamParams p, int chunks, int rounds, int merges, int
     if constexpr (STREAM) {
         int64_t total, chunk;
         stream_extent(p, decode_ctas, total, chunk);
+        if (start < 0 || start + el.cnt > total) {        // starts that do not ascend: no CTA has written such pieces
+            if (tid == 0 && part == chunks) report(d.status, KTK_STATUS_BAD_TABLE);
+            return;
+        }
         pieces.first = start / chunk;
         const int64_t last = (start + el.cnt - 1) / chunk;
         pieces.count = last == pieces.first ? 0 : (int)(last - pieces.first + 1);

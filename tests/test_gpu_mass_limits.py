@@ -162,3 +162,14 @@ def test_a_list_beyond_the_bound_keeps_its_masses(cuda_device, long, most, kv_he
     _, mass = ops.dense_decode_mass(c["q"].to(dtype).to(cuda_device), *c["table"], most, c["mass"].to(cuda_device), 0.75, status=status,
                                     view=c["view"])
     assert int(status.item()) == 2 and torch.equal(mass[1].cpu(), c["mass"][1])
+
+
+def test_starts_that_do_not_ascend_are_refused(cuda_device):
+    # balanced partition: the list of sequence 0 passes the end that the table gives for all
+    from kinetics_b200 import ops
+    c, status = _lists(48, cuda_device, [16000, 640], 2, 4, torch.bfloat16, False), ops.new_status(cuda_device)
+    assert c["first"] == [0, 1000, 1040] and ops.decode_mass_workspace_bytes(2, 2, 4, 8000, torch.bfloat16) > 0
+    c["table"][2][2] = 40
+    _, mass = ops.dense_decode_mass(c["q"].to(torch.bfloat16).to(cuda_device), *c["table"], 8000, c["mass"].to(cuda_device), 0.75, status=status,
+                                    view=c["view"])
+    assert int(status.item()) == 2 and torch.equal(mass.cpu(), c["mass"])
