@@ -72,11 +72,11 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
     const int n_entries = (e1 > e0) ? e1 - e0 : 0;
     __shared__ MassShared<MASS ? 8 : 1> shared;
 
+    if (MASS && tid >= 32 && tid < 32 + kMmaStages) stage_tag[tid - 32] = 0;
     if (tid == 0) {
         for (int s = 0; s < kMmaStages; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
-            if (MASS) stage_tag[s] = 0;
         }
         abort_flag = 0;
         issued_total = 0;

@@ -59,7 +59,8 @@ int main() { int tag, stages; while (scanf("%d %d", &tag, &stages) == 2) printf(
     assert list(map(int, out.stdout.split())) == want
     kernel = text[text.index("decode_mma_kernel(const MmaParams"):text.index("// ---- merge the consumer warps")]
     issue, behind = kernel.split("__syncthreads();   // every page consumed")
-    assert "if (MASS) stage_tag[s] = 0;" in issue and "never" not in issue          # nobody waits before the block has met
+    clear = "if (MASS && tid >= 32 && tid < 32 + kMmaStages) stage_tag[tid - 32] = 0;"
+    assert issue.index(clear) < issue.index("__syncthreads();") and "never" not in issue      # nobody waits before the block has met
     assert re.search(r"for \(int s = 0; s < kMmaStages; \+\+s\) \{\s*const int phase = last_copy\(stage_tag\[s\], kMmaStages\);\s*"
                      r"if \(phase >= 0\) mbar_wait\(&full_bar\[s\], phase, &never\);", behind)
     assert behind.index("last_copy(") < behind.index("if (!MASS) return;")
