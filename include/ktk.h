@@ -557,7 +557,8 @@ typedef struct ktk_mass {
  * ktk_dense_decode_v that also accumulates: with p_hq(t) the softmax weights of query head hq,
  *   out[r, h, t] = decay * in[r, h, t] + sum_{hq of group h} p_hq(t)          for t < n - 1,
  * and without the first term for the newest token t = n - 1, whose place may still hold what an earlier token was paid.
- * The weights are those of fp32 scores and denominators.
+ * The weights are those of fp32 scores and denominators.  The tokens of a page id that is none of the cache's (KTK_STATUS_BAD_PAGE) take no
+ * part: their weights are 0.
  *   total_pages  an upper bound of the entries in all lists (sizes the workspace), or -1: batch * max_pages_per_seq, which is
  *                also what counts with view->page_count
  *   max_pages_per_seq  at least every sequence's page count; a longer list reports KTK_STATUS_BAD_TABLE, its masses stay as they are and its
@@ -578,7 +579,7 @@ KTK_API int ktk_dense_decode_mass(const void* q, const void* kv_cache, const int
  * ktk_prefill_attention that also accumulates what the new tokens pay:
  *   out[r, h, t] = decay * in[r, h, t] + sum over the last `window` new tokens and the heads of group h of p(t)
  * for the tokens t that were there before, and without the first term for the sequence's new ones.  window 0: all new tokens.
- * A sequence without new tokens is left as it is.
+ * A sequence without new tokens is left as it is.  The results of one with a page id that is none of the cache's (KTK_STATUS_BAD_PAGE) are void.
  *   max_new_tokens, max_pages_per_seq, total_pages   upper bounds of one sequence's new tokens, of one list's entries (2^26 at most)
  *                and of all lists' together (-1: batch * max_pages_per_seq, as with view->page_count); they size the grid and the
  *                workspace.  A sequence beyond them, or of tokens outside total_new_tokens, reports KTK_STATUS_BAD_TABLE; its masses

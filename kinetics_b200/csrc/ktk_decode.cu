@@ -191,6 +191,16 @@ decode_simt_kernel(const DecodeParams p, const typename MassArgument<MASS>::type
         __syncwarp();
     };
 
+    const auto no_page = [&](int e) {                                         // weights of 0
+        if constexpr (MASS == kMassLong) {
+            if (position + e >= 0 && position + e < mp.positions)
+                for (int x = lane; x < kPageSize * G; x += 32) mp.scores[(position + e) * kPageSize * G + x] = -INFINITY;
+        }
+        if constexpr (MASS == kMassCluster)
+            for (int x = lane; x < kPageSize * G; x += 32) simt_scores[(e - e0) * kPageSize * G + x] = -INFINITY;
+    };
+    static_assert(MASS == kMassNone || !kPrefetch, "no_page where pages are fetched");
+
     if constexpr (kPrefetch) {
         // two register buffers, alternated: the warp's next page is in flight
         // while the current one is reduced
@@ -209,8 +219,10 @@ decode_simt_kernel(const DecodeParams p, const typename MassArgument<MASS>::type
         }
     } else {
         R ka[kPageSize], va[kPageSize];
-        for (int e = e0 + warp; e < e1; e += kSimtWarps)
+        for (int e = e0 + warp; e < e1; e += kSimtWarps) {
             if (fetch(e, ka, va)) consume(e, ka, va);
+            else if constexpr (MASS != kMassNone) no_page(e);
+        }
     }
 
     // ---- merge the four warps ----

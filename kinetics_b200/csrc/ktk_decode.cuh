@@ -47,6 +47,9 @@ struct MassParams {
     int max_pages;               // the caller's bound of a list
 };
 
+// Minus log2 of a softmax's denominator by its maximum and sum.  A list whose pages are none has scores of -inf alone: weights of 0
+__device__ __forceinline__ float neg_log2_sum(float m, float l) { return m == -INFINITY ? 0.0f : -(m + log2f(l)); }
+
 constexpr int kMassMaxPages = 1 << 26;       // of a list: its tokens are counted in 32 bits
 
 constexpr float kLog2e = 1.4426950408889634f;

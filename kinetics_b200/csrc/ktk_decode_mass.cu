@@ -167,7 +167,7 @@ mass_finish_kernel(const StreamParams p, int chunks, int rounds, int merges, int
             const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
             join(m2, l2);
         }
-        if (lane < G) neg_lse[lane] = pieces.count == 0 ? d.neg_lse[qh + lane] : -(M + log2f(L));
+        if (lane < G) neg_lse[lane] = pieces.count == 0 ? d.neg_lse[qh + lane] : neg_log2_sum(M, L);
     }
     __syncthreads();
     float mine[G];

@@ -79,7 +79,7 @@ __device__ __forceinline__ void finish_cluster(const DecodeParams& p, const Mass
         const float inv = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
         for (int r = 0; r < kMassMaxCluster; ++r) sh.weight[r][tid] = mr[r] != -INFINITY ? exp2f(mr[r] - M) * inv : 0.0f;
-        sh.neg_lse[tid] = -(M + log2f(L));
+        sh.neg_lse[tid] = neg_log2_sum(M, L);
     }
     __syncthreads();
     T* o = (T*)p.o + ((int64_t)b * p.Hkv + h) * G * kHeadDim;

@@ -106,6 +106,7 @@ decode_mma_kernel(const MmaParams p, const __grid_constant__ CUtensorMap kv_map)
                     if (page < 0 || page >= d.num_pages) {
                         report(d.status, KTK_STATUS_BAD_PAGE);
                         stage_tag[s] = -(i + 1);
+                        for (int x = 0; x < kPageSize * G; ++x) scores[i * kPageSize * G + x] = -INFINITY;       // weights of 0
                         mbar_arrive(&full_bar[s]);              // nothing to load: release the consumer
                     } else {
                         stage_tag[s] = i + 1;

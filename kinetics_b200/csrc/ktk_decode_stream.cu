@@ -166,6 +166,10 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                     } else if (tag > 0) {
                         mma_consume_page(ms, stages + s * kStageBytes, entry_tokens(pc.el, pc.e_lo + j), qb,
                                          d.scale_log2, lane);
+                    } else if (MASS) {                                  // no page: weights of 0
+                        const int64_t position = cur.start + pc.e_lo + j;
+                        if (position >= 0 && position < p.m.positions)
+                            for (int x = lane; x < kPageSize * G; x += 32) p.m.scores[position * kPageSize * G + x] = -INFINITY;
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&empty_bar[s]);
@@ -211,7 +215,7 @@ decode_stream_kernel(const StreamParams p, const __grid_constant__ CUtensorMap k
                     if (whole) {
                         const int64_t qh = (int64_t)pc.b * Hq + (int64_t)pc.h * G + g;
                         ((__nv_bfloat16*)d.o)[qh * kHeadDim + dd] = __float2bfloat16_rn(L > 0.0f ? O / L : 0.0f);
-                        if (MASS && dd == 0) d.neg_lse[qh] = -(M + log2f(L));
+                        if (MASS && dd == 0) d.neg_lse[qh] = neg_log2_sum(M, L);
                     } else {
                         const int64_t row = (int64_t)slot * G + g;
                         d.ws_o[row * kHeadDim + dd] = O;

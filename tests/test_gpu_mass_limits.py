@@ -173,3 +173,48 @@ def test_starts_that_do_not_ascend_are_refused(cuda_device):
     _, mass = ops.dense_decode_mass(c["q"].to(torch.bfloat16).to(cuda_device), *c["table"], 8000, c["mass"].to(cuda_device), 0.75, status=status,
                                     view=c["view"])
     assert int(status.item()) == 2 and torch.equal(mass.cpu(), c["mass"])
+
+
+# ---------------------------------------------------------------- pages that are none
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("group", [1, 4, 8])
+@pytest.mark.parametrize("most", [0, 8000])
+def test_tokens_of_a_page_that_is_none_take_no_part(cuda_device, most, group, dtype):
+    # pages 2 and 17 of sequence 1; in the masses their tokens' are decayed, as those that were paid nothing
+    from kinetics_b200 import ops
+    c = _lists(44, cuda_device, [300, 700, 90], 2, group, dtype, False)
+    if most and dtype == torch.float32:
+        most = 100000 // group
+    assert (ops.decode_mass_workspace_bytes(3, 2, group, most or max(c["pages"]), dtype) > 0) == (most > 0)
+    for page, none in ((2, -1), (17, c["table"][0].shape[0])):
+        c["table"][1][c["first"][1] + page] = none
+    without = np.concatenate([np.arange(32, 48), np.arange(17 * 16, 18 * 16)])
+    status, q = ops.new_status(cuda_device), c["q"].to(dtype).to(cuda_device)
+    # what a page's scores may find in their places: those of an earlier call, or NaN
+    need = ops.decode_mass_workspace_bytes(3, 2, group, most or max(c["pages"]), dtype)
+    workspace = torch.full((max(need, 16) // 4,), float("nan"), device=cuda_device)
+    for _ in range(3):
+        out, mass = ops.dense_decode_mass(q, *c["table"], most or max(c["pages"]), c["mass"].to(cuda_device), 0.75, workspace=workspace,
+                                          status=status, view=c["view"])
+        assert int(status.item()) == 1
+        for b in range(3):
+            _equals(c, b, out, mass, 0, 0.75, without if b == 1 else None)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("most", [0, 8000])
+def test_a_list_whose_pages_are_all_none(cuda_device, most, dtype):
+    from kinetics_b200 import ops
+    c, status = _lists(49, cuda_device, [300, 700, 90], 2, 4, dtype, False), ops.new_status(cuda_device)
+    if most and dtype == torch.float32:
+        most = 25000
+    c["table"][1][c["first"][1]:c["first"][2]] = -1
+    out, mass = ops.dense_decode_mass(c["q"].to(dtype).to(cuda_device), *c["table"], most or max(c["pages"]), c["mass"].to(cuda_device), 0.75,
+                                      status=status, view=c["view"])
+    assert int(status.item()) == 1 and not out[1].any()
+    want = 0.75 * c["mass"][1]
+    want[:, 699] = 0                                                     # the newest starts from its weights alone
+    want[:, 700:] = c["mass"][1, :, 700:]
+    assert torch.equal(mass[1].cpu(), want)
+    for b in (0, 2):
+        _equals(c, b, out, mass, 0, 0.75)
