@@ -26,6 +26,11 @@ int check_mass(const ktk_mass* m, const char* who);
 int check_apart(const void* a, const void* b, size_t bytes, const char* who, const char* what);
 int check_aligned(std::initializer_list<const void*> pointers, const char* who);      // to 16 bytes
 
+// Lets launches of a kernel ask for `bytes` of dynamic shared memory.  The limit belongs to the kernel, not to the call or the thread: it is only
+// ever raised, for a lower one would refuse the launch of another host thread that has just set its own.
+cudaError_t raise_shared(const void* kernel, size_t bytes);
+template <typename K> inline cudaError_t allow_shared(K* kernel, size_t bytes) { return raise_shared((const void*)kernel, bytes); }
+
 // a ktk_view with the defaults filled in
 struct View {
     int sink_tokens = 0;

@@ -297,7 +297,7 @@ static int simt_launch(const DecodeParams& p, const typename MassArgument<MASS>:
     const auto kernel = decode_simt_kernel<T, G, MASS>;
     if constexpr (MASS == kMassCluster) {
         const size_t smem = (size_t)((m.max_pages + p.num_splits - 1) / p.num_splits) * kPageSize * G * sizeof(float);
-        KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "ktk decode (simt)");
+        KTK_CUDA_TRY(allow_shared(kernel, smem), "ktk decode (simt)");
         KTK_CUDA_TRY(launch_cluster(ctas <= sm_count(), kernel, (unsigned)ctas, kSimtWarps * 32, smem, p.num_splits, st, p, m), "ktk decode (simt)");
     } else {
         KTK_CUDA_TRY(launch_behind(ctas <= sm_count(), kernel, (unsigned)ctas, kSimtWarps * 32, 0, st, p, m), "ktk decode (simt)");

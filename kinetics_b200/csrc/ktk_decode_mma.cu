@@ -287,7 +287,7 @@ int launch_decode_mma(const DecodeParams& p, int G, cudaStream_t st) {
     if (rc != KTK_OK) return rc;
     const int smem = kMmaStages * kStageBytes + 1024;
     const auto kernel = decode_mma_kernel<kMmaStages, 3, false>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "ktk decode (mma)");
+    KTK_CUDA_TRY(allow_shared(kernel, smem), "ktk decode (mma)");
     MmaParams mp;
     mp.d = p;
     mp.m = MassParams{};
@@ -309,7 +309,7 @@ int launch_decode_mma_mass(const DecodeParams& p, const MassParams& m, int G, cu
     const int stages = 2 * ctas <= sm_count() && fits(16) ? 16 : fits(8) ? 8 : 4;
     const int smem = (int)mma_mass_smem(stages, m.max_pages, p.num_splits, G);
     const auto kernel = stages == 16 ? decode_mma_kernel<16, 1, true> : stages == 8 ? decode_mma_kernel<8, 3, true> : decode_mma_kernel<4, 4, true>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
+    KTK_CUDA_TRY(allow_shared(kernel, smem), who);
     const MmaParams mp{p, m, G};
     KTK_CUDA_TRY(launch_cluster(ctas <= sm_count(), kernel, (unsigned)ctas, kMmaThreads, smem, p.num_splits, st, mp, map), who);
     return KTK_OK;

@@ -343,7 +343,7 @@ static int stream_slots(int vi) {
     if (slots[dev][vi] == 0) {
         int per_sm = 0;
         const int smem = stream_smem(v.stages);
-        cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        allow_shared(v.kernel, smem);
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, v.kernel, kMmaThreads, smem) != cudaSuccess ||
             per_sm < 1)
             per_sm = 1;
@@ -399,7 +399,7 @@ static int launch_stream(const DecodeParams& p, const MassParams& m, int G, int 
     sp.chunk = (int)chunk;
     if (!sp.exact) grid = (int)((sp.total + chunk - 1) / chunk);            // no empty CTA
     const int smem = stream_smem(var.stages);
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+    KTK_CUDA_TRY(allow_shared(kernel, smem),
                  "ktk decode (balanced)");
     KTK_CUDA_TRY(launch_behind(grid <= sm_count(), kernel, grid, kMmaThreads, smem, st, sp, map), "ktk decode (balanced)");
     if (MASS) return launch_mass_finish(sp, grid, st);

@@ -311,7 +311,7 @@ extern "C" int ktk_block_topk_mask(float* logits, const int32_t* offset, int32_t
     }
     const size_t smem = (size_t)(max_len / kPageSize + 1) * sizeof(float);
     if (smem > 200 * 1024) { set_error("ktk_block_topk_mask: max_len %lld too long", (long long)max_len); return KTK_ERR_TOO_LARGE; }
-    KTK_CUDA_TRY(cudaFuncSetAttribute(block_topk_mask_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+    KTK_CUDA_TRY(allow_shared(block_topk_mask_kernel, smem),
                  "ktk_block_topk_mask");
     const dim3 grid((unsigned)rows, (unsigned)num_kv_heads);
     block_topk_mask_kernel<<<grid, kChainThreads, smem, (cudaStream_t)stream>>>(logits, offset, num_q_heads, num_kv_heads,

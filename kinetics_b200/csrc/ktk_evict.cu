@@ -738,7 +738,7 @@ extern "C" int ktk_evict(void* kv_cache, const int32_t* kv_indices, const int32_
         KTK_CUDA_TRY((launch_evict<1024, 16>(p, cut, f32, st)), who);
     } else {
         const size_t smem = (size_t)((cut.most + 31) / 32) * 2 * sizeof(uint32_t);
-        KTK_CUDA_TRY(cudaFuncSetAttribute(evict_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+        KTK_CUDA_TRY(allow_shared(evict_long_kernel, smem), who);
         KTK_CUDA_TRY(launch_behind(false, evict_long_kernel, (unsigned)cut.units, kEvLong, smem, st, p), who);
     }
     if (cut.fused) return KTK_OK;

@@ -2,6 +2,9 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <mutex>
+#include <unordered_map>
+
 #include "ktk_common.cuh"
 #include "ktk_pipeline.cuh"
 
@@ -85,6 +88,17 @@ int check_aligned(std::initializer_list<const void*> pointers, const char* who) 
             return KTK_ERR_ARG;
         }
     return KTK_OK;
+}
+
+cudaError_t raise_shared(const void* kernel, size_t bytes) {
+    static std::mutex mu;
+    static std::unordered_map<const void*, size_t> most;
+    std::lock_guard<std::mutex> lock(mu);
+    size_t& have = most[kernel];
+    // set on every call: the current device may be another one
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes > have ? bytes : have));
+    if (e == cudaSuccess && bytes > have) have = bytes;
+    return e;
 }
 
 int sm_count() {

@@ -234,7 +234,7 @@ static int launch_prefill_mma(const PrefillParams& p, const void* cache, int max
     int rc = make_kv_tensor_map(&map, d);
     if (rc != KTK_OK) return rc;
     const int smem = kPfStages * kStageBytes + 1024;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+    KTK_CUDA_TRY(allow_shared(prefill_mma_kernel, smem),
                  "ktk_prefill_attention");
     const int tpc = (8 / p.G) * kPfConsumers;
     const dim3 grid((unsigned)((max_new_tokens + tpc - 1) / tpc), (unsigned)p.Hkv, (unsigned)p.batch);

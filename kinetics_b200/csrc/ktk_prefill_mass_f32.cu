@@ -335,13 +335,13 @@ int launch_prefill_mass_f32(const PrefillMassParams& p, cudaStream_t st) {
     const int64_t tiles = (per_seq * p.batch < p.total_new / tpc + p.batch ? per_seq * p.batch : p.total_new / tpc + p.batch) * p.Hkv;
     int cluster = 1;
     while (cluster < kPaMaxCluster && tiles * cluster <= sm_count() && key_chunks > cluster) cluster *= 2;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_attention_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPaSmem), who);
+    KTK_CUDA_TRY(allow_shared(prefill_attention_f32_kernel, kPaSmem), who);
     KTK_CUDA_TRY(launch_cluster(false, prefill_attention_f32_kernel, (unsigned)(per_seq * units * cluster), kPaThreads,
                                 kPaSmem, cluster, st, p, cluster), who);
     const int64_t rows = (int64_t)(p.window > 0 && p.window < p.max_new ? p.window : p.max_new) * p.G;
     cluster = 1;
     while (cluster < 8 && ctas * cluster <= sm_count() && rows > (int64_t)kPsRows * cluster) cluster *= 2;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_sums_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPsSmem), who);
+    KTK_CUDA_TRY(allow_shared(prefill_sums_f32_kernel, kPsSmem), who);
     KTK_CUDA_TRY(launch_cluster(false, prefill_sums_f32_kernel, (unsigned)(ctas * cluster), kPsThreads, kPsSmem, cluster, st, p, (int)key_chunks,
                                 cluster), who);
     return KTK_OK;

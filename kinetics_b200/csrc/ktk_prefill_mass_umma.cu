@@ -401,7 +401,7 @@ int launch_prefill_mass_umma(const PrefillMassParams& p, int64_t groups, cudaStr
         set_error("%s: num_kv_heads * tokens exceed the grid limit", who);
         return KTK_ERR_TOO_LARGE;
     }
-    KTK_CUDA_TRY(cudaFuncSetAttribute(prefill_mass_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem), who);
+    KTK_CUDA_TRY(allow_shared(prefill_mass_umma_kernel, kPmSmem), who);
     KTK_CUDA_TRY(launch_behind(true, prefill_mass_umma_kernel, (unsigned)(units * p.splits), kPmThreads, kPmSmem, st, p, kv_map, q_map,
                                lse_map), who);
     if (p.splits > 1)

@@ -392,7 +392,7 @@ int launch_prefill_umma(PrefillUmmaParams p, int max_new_tokens, cudaStream_t st
                   : by_tile ? (lse ? prefill_umma_kernel<kByTile, true> : prefill_umma_kernel<kByTile, false>)
                             : (lse ? prefill_umma_kernel<kBySequence, true> : prefill_umma_kernel<kBySequence, false>);
     if (cluster > 1) kernel = prefill_umma_kernel<kByTile, true, true>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPuSmem), who);
+    KTK_CUDA_TRY(allow_shared(kernel, kPuSmem), who);
     const dim3 grid = by_tile ? dim3((unsigned)p.Hkv, (unsigned)p.batch, pairs) : dim3(pairs, (unsigned)p.Hkv, (unsigned)p.batch);
     DecodeParams d{};                               // only what the tensor map needs
     d.cache = p.cache; d.Hkv = p.Hkv; d.num_pages = p.num_pages;

@@ -510,7 +510,7 @@ static int select_launch(const void* q, const void* summaries, int64_t summary_s
     const size_t smem = (size_t)kSelStages * SelStage<T>::kRows * kHeadDim * sizeof(T) + (size_t)kp * 8 +
                         (size_t)key_cap * sizeof(uint32_t);
     auto kern = select_kernel<T, G>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+    KTK_CUDA_TRY(allow_shared(kern, smem),
                  "ktk_select");
     const int64_t items = (int64_t)s->batch * s->num_kv_heads;
     int64_t grid = (int64_t)sm_count() * kSelCtasPerSm;

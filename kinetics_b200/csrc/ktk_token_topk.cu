@@ -227,7 +227,7 @@ extern "C" int ktk_token_topk_mask(float* logits, const int32_t* offset, int32_t
         return KTK_ERR_TOO_LARGE;
     }
     const int smem = (int)dyn * (int)sizeof(uint32_t);
-    KTK_CUDA_TRY(cudaFuncSetAttribute(token_topk_mask_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+    KTK_CUDA_TRY(allow_shared(token_topk_mask_kernel, smem),
                  "ktk_token_topk_mask");
     token_topk_mask_kernel<<<dim3((unsigned)rows, (unsigned)num_kv_heads), kTokThreads, smem, (cudaStream_t)stream>>>(
         logits, offset, num_q_heads, num_kv_heads, max_len, topk, local, sink, status);

@@ -452,7 +452,7 @@ template <int DC, int VC, bool FIXED, int CTAS> static int decode_launch(const A
     if (rc != KTK_OK) return rc;
     constexpr int smem = ad_smem<DC, VC>();
     auto kernel = attn_decode_kernel<DC, VC, FIXED, CTAS>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
+    KTK_CUDA_TRY(allow_shared(kernel, smem), who);
     const int group = p.a.heads / p.a.kv_heads;
     const dim3 grid((unsigned)p.splits, (unsigned)(p.a.kv_heads * ((group + 7) / 8)), (unsigned)p.t.batch);
     kernel<<<grid, kAdThreads, smem, st>>>(p, km, vm);

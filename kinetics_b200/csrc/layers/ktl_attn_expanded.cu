@@ -199,7 +199,7 @@ static int expanded_launch(const ExpandedParams& p, const __nv_bfloat16* kv, con
     int64_t heads_per = kAeGroupBytes / per_head;
     heads_per = heads_per < 1 ? 1 : (heads_per > a.heads ? a.heads : heads_per);
     auto kernel = attn_expanded_kernel<VC, NK>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
+    KTK_CUDA_TRY(allow_shared(kernel, smem), who);
     kernel<<<(unsigned)(pairs * a.heads), kFlThreads, smem, st>>>(p, (int)heads_per, km, rm, vm);
     KTK_CUDA_TRY(cudaGetLastError(), who);
     return KTK_OK;

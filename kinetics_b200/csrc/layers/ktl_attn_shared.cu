@@ -760,7 +760,7 @@ template <int N> static int shared_launch(const AttnParams& p, const Packing& k,
         set_error("%s: more than 65535 groups of rows in one launch", who);
         return KTK_ERR_TOO_LARGE;
     }
-    KTK_CUDA_TRY(cudaFuncSetAttribute(attn_shared_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
+    KTK_CUDA_TRY(allow_shared(attn_shared_kernel<N>, smem), who);
     const bool balanced = p.splits < 0;
     const int ctas = balanced_ctas(a);
     const dim3 grid((unsigned)(balanced ? ctas : p.splits), (unsigned)k.chunks, (unsigned)(balanced ? 1 : groups * p.t.batch));

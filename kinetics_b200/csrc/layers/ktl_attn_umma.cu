@@ -220,7 +220,7 @@ template <int DC, int VC, bool FIXED> static int umma_launch(const AttnParams& p
     const unsigned tiles = (unsigned)(((int64_t)p.max_new + tpc - 1) / tpc), heads = (unsigned)p.a.kv_heads, batch = (unsigned)p.t.batch;
     const bool tile_major = tiles <= 65535;
     auto kernel = tile_major ? attn_umma_kernel<DC, VC, FIXED, true> : attn_umma_kernel<DC, VC, FIXED, false>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
+    KTK_CUDA_TRY(allow_shared(kernel, smem), who);
     kernel<<<tile_major ? dim3(heads, batch, tiles) : dim3(tiles, heads, batch), kFlThreads, smem, st>>>(p, km, vm);
     KTK_CUDA_TRY(cudaGetLastError(), who);
     return KTK_OK;

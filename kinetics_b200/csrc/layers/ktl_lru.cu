@@ -582,7 +582,7 @@ template <typename T> static int scan_launch(const LruParams& p, cudaStream_t st
         const auto kernel = one ? (aligned ? lru_scan_kernel<T, true, kHasOne> : lru_scan_kernel<T, false, kHasOne>)
                                 : (aligned ? lru_scan_kernel<T, true, false> : lru_scan_kernel<T, false, false>);
         if (one) cfg.dynamicSmemBytes /= 2;
-        KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes), "ktk_lru_scan");
+        KTK_CUDA_TRY(allow_shared(kernel, cfg.dynamicSmemBytes), "ktk_lru_scan");
         KTK_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p), "ktk_lru_scan");
     }
     else
@@ -663,7 +663,7 @@ extern "C" int ktk_lru_decode(const void* proj, int64_t row_stride, int64_t y_co
     const int chan = narrow ? 32 : 64, smem = lf_smem(shape->block_stride, chan), slices = (shape->block_stride + chan - 1) / chan;
     auto kernel = shape->taps == 4 ? (narrow ? lru_decode_kernel<4, 32> : lru_decode_kernel<4, 64>)
                                    : (narrow ? lru_decode_kernel<0, 32> : lru_decode_kernel<0, 64>);
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), who);
+    KTK_CUDA_TRY(allow_shared(kernel, smem), who);
     kernel<<<dim3((unsigned)(shape->blocks * slices), (unsigned)groups), kLfThreads, smem, (cudaStream_t)stream>>>(q);
     KTK_CUDA_TRY(cudaGetLastError(), who);
     return KTK_OK;

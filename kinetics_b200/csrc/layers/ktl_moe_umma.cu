@@ -426,7 +426,7 @@ template <int STAGE> static int moe_umma(const MoeParams& p, cudaStream_t st) {
     }
     const int64_t units = tiles * per < sm_count() / ctas ? tiles * per : sm_count() / ctas;
     auto kernel = pair ? moe_umma_kernel<STAGE, true> : moe_umma_kernel<STAGE, false>;
-    KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMuRing + 1024), who);
+    KTK_CUDA_TRY(allow_shared(kernel, kMuRing + 1024), who);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(units * ctas));
     cfg.blockDim = dim3(STAGE == 0 ? 320 : 192);

@@ -277,7 +277,7 @@ static int residual_norm_launch(const ResidualNormParams& p, cudaStream_t st) {
         p.rows >= (narrow ? 16 : 12) * (int64_t)sm_count()) {
         const size_t stage = (size_t)p.stride * (TOKENS ? sizeof(T) : 4) + (p.y ? (size_t)p.stride * sizeof(T) : 0);
         const auto walk = [&](auto kernel, int threads_of, int resident) {
-            KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kRnStages * stage)), who);
+            KTK_CUDA_TRY(allow_shared(kernel, kRnStages * stage), who);
             kernel<<<(unsigned)(sm_count() * resident), threads_of, kRnStages * stage, st>>>(p);
             KTK_CUDA_TRY(cudaGetLastError(), who);
             return (int)KTK_OK;

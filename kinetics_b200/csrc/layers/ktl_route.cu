@@ -333,7 +333,7 @@ extern "C" int ktk_moe_route(const void* h, const void* w, const float* b, int32
         const size_t smem = ((shape->experts + 3) / 4 * 4 + shape->width_stride + shape->top) * sizeof(float);
         if (smem > 200 * 1024) { set_error("%s: rows of %d columns", who, shape->width); return KTK_ERR_UNSUPPORTED; }
         auto kernel = shape->dtype == KTK_F32 ? route_row_kernel<float> : route_row_kernel<__nv_bfloat16>;
-        KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+        KTK_CUDA_TRY(allow_shared(kernel, smem), who);
         kernel<<<(unsigned)rows, kRtRowThreads, smem, st>>>(p);
     } else {
         const size_t ring = (size_t)kRtStageElems * 2;    // of a stage
@@ -346,7 +346,7 @@ extern "C" int ktk_moe_route(const void* h, const void* w, const float* b, int32
             return KTK_ERR_UNSUPPORTED;
         }
         auto kernel = stages == 3 ? route_mma_kernel<3> : route_mma_kernel<2>;
-        KTK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who);
+        KTK_CUDA_TRY(allow_shared(kernel, smem), who);
         kernel<<<(unsigned)((rows + kRtRows - 1) / kRtRows), kRtThreads, smem, st>>>(p);
     }
     KTK_CUDA_TRY(cudaGetLastError(), who);

@@ -1,5 +1,7 @@
 """The operators of a bounded cache at their limits: batches that shrink under a manager, sequences beyond a call's bounds, pages that are
 none, host threads; against plain fp64 forms."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -218,3 +220,72 @@ def test_a_list_whose_pages_are_all_none(cuda_device, most, dtype):
     assert torch.equal(mass[1].cpu(), want)
     for b in (0, 2):
         _equals(c, b, out, mass, 0, 0.75)
+
+
+# ---------------------------------------------------------------- host threads
+def _together(calls, rounds):
+    """Each call(stream), which returns 0 or an error's code, `rounds` times in a thread and a stream of its own; the errors."""
+    from kinetics_b200 import _lib
+    errors, start = [], threading.Barrier(len(calls))
+
+    def work(call):
+        torch.cuda.set_device(0)
+        stream = torch.cuda.Stream()
+        start.wait()
+        for i in range(rounds):
+            if call(stream.cuda_stream) != 0:
+                errors.append((i, _lib.load().ktk_last_error()))
+                return
+            if i % 500 == 499:
+                stream.synchronize()
+    workers = [threading.Thread(target=work, args=(call,)) for call in calls]
+    torch.cuda.synchronize()
+    for t in workers:
+        t.start()
+    for t in workers:
+        t.join()
+    torch.cuda.synchronize()
+    return errors
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_threads_whose_lists_have_other_bounds(cuda_device, dtype):
+    # the same kernels with other amounts of shared memory at once
+    from kinetics_b200 import _lib, ops
+    lens, heads, group = ([90, 33], 2, 4) if dtype == torch.bfloat16 else ([90, 33, 1, 2, 3, 4, 5, 6], 8, 8)
+    c = _lists(45, cuda_device, lens, heads, group, dtype, False)
+    cache, indices, starts, last = c["table"]
+    q = c["q"].to(dtype).to(cuda_device)
+    shape = _lib.Shape(len(lens), heads, group, D, 16, 1 if dtype == torch.bfloat16 else 0, cache.shape[0])
+    bounds = (8, 400, 60, 300) if dtype == torch.bfloat16 else (200, 2500, 1200, 1900)
+    call, kept = _lib.load().ktk_dense_decode_mass, []
+
+    def of(most):
+        mass, out = c["mass"].to(cuda_device), torch.empty_like(q)
+        need = ops.decode_mass_workspace_bytes(len(lens), heads, group, most, dtype)
+        assert need == 0
+        m = _lib.Mass(mass.data_ptr(), mass.data_ptr(), mass.shape[2], len(lens), 1.0)
+        kept.append((mass, out, m))
+        args = (q.data_ptr(), cache.data_ptr(), indices.data_ptr(), starts.data_ptr(), last.data_ptr(), None, most, -1, 0.1, m, out.data_ptr(), 0, 0,
+                shape, 0)
+        return lambda stream: call(*args, stream)
+    assert _together([of(most) for most in bounds], 10000) == []
+
+
+def test_threads_that_evict_from_lists_of_other_bounds(cuda_device):
+    from kinetics_b200 import _lib, ops
+    c = _lists(46, cuda_device, [90, 33], 2, 4, torch.bfloat16, False)
+    shape = _lib.Shape(2, 2, 1, D, 16, 1, c["table"][0].shape[0])
+    seen, stored = torch.tensor([90, 33], dtype=torch.int32, device=cuda_device), torch.zeros(2, dtype=torch.int32, device=cuda_device)
+    call, kept = _lib.load().ktk_evict, []
+
+    def of(most):
+        cache, mass = c["table"][0].clone(), c["mass"].to(cuda_device)
+        positions = torch.zeros(mass.shape, dtype=torch.int32, device=cuda_device)
+        space = torch.empty(_lib.load().ktk_evict_workspace_bytes(shape, most, 64), dtype=torch.uint8, device=cuda_device)
+        m = _lib.Mass(mass.data_ptr(), mass.data_ptr(), mass.shape[2], 2, 1.0)
+        kept.append((cache, mass, positions, space, m))
+        args = (cache.data_ptr(), *(t.data_ptr() for t in c["table"][1:]), None, most, m, positions.data_ptr(), positions.data_ptr(), stored.data_ptr(),
+                seen.data_ptr(), 64, 4, 0, space.data_ptr(), space.nbytes, shape, 0)
+        return lambda stream: call(*args, stream)
+    assert _together([of(most) for most in (4200, 32768, 9000)], 5000) == []

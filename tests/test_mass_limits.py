@@ -64,3 +64,10 @@ int main() { int tag, stages; while (scanf("%d %d", &tag, &stages) == 2) printf(
     assert re.search(r"for \(int s = 0; s < kMmaStages; \+\+s\) \{\s*const int phase = last_copy\(stage_tag\[s\], kMmaStages\);\s*"
                      r"if \(phase >= 0\) mbar_wait\(&full_bar\[s\], phase, &never\);", behind)
     assert behind.index("last_copy(") < behind.index("if (!MASS) return;")
+
+
+def test_kernels_share_their_limits_of_shared_memory():
+    """The limit belongs to the kernel: set per call, it is lowered under a launch of another thread.  One place sets it, and only raises it."""
+    sources = [p for suffix in ("cu", "cuh") for p in CSRC.rglob(f"*.{suffix}")]
+    assert [p.name for p in sources if "cudaFuncAttributeMaxDynamicSharedMemorySize" in p.read_text()] == ["ktk_host.cu"]
+    assert sum("allow_shared(" in p.read_text() for p in sources) > 15
