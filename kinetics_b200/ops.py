@@ -375,9 +375,15 @@ def _address(t, dev: int) -> int:
     return t.data_ptr()
 
 
-_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-# a workspace for one call: given back when the launches are in the stream, whose next allocations come behind them (a tensor costs 1.1 us more)
-_take, _give_back = torch._C._cuda_cudaCachingAllocator_raw_alloc, torch._C._cuda_cudaCachingAllocator_raw_delete
+# The short ways that torch's own calls take, where this torch has them: a device's number and a raw stream; and a workspace for one call, given back
+# when the launches are in the stream, whose next allocations come behind them (a tensor costs 1.1 us more).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_take = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None)
+_give_back = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None)
+if _take is None or _give_back is None:
+    _take = lambda size, stream: torch.cuda.caching_allocator_alloc(size, None, stream)
+    _give_back = torch.cuda.caching_allocator_delete
 _SM_SCALE = HEAD_DIM ** -0.5
 
 

@@ -289,3 +289,30 @@ def test_threads_that_evict_from_lists_of_other_bounds(cuda_device):
                 seen.data_ptr(), 64, 4, 0, space.data_ptr(), space.nbytes, shape, 0)
         return lambda stream: call(*args, stream)
     assert _together([of(most) for most in (4200, 32768, 9000)], 5000) == []
+
+
+def test_calls_by_the_public_names_of_torch(cuda_device, monkeypatch):
+    # what stands in for the private names where a torch lacks them: the same results, on a stream of their own and captured
+    from kinetics_b200 import ops
+    c, status = _lists(50, cuda_device, [300, 8100, 90], 1, 4, torch.bfloat16, False), ops.new_status(cuda_device)
+    q, most = c["q"].to(torch.bfloat16).to(cuda_device), max(c["pages"])
+    assert ops.decode_mass_workspace_bytes(3, 1, 4, most) > 0
+    call = lambda: ops.dense_decode_mass(q, *c["table"], most, c["mass"].to(cuda_device), 0.75, status=status, view=c["view"])
+    want = call()
+    monkeypatch.setattr(ops, "_current_device", torch.cuda.current_device)
+    monkeypatch.setattr(ops, "_current_stream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+    monkeypatch.setattr(ops, "_take", lambda size, stream: torch.cuda.caching_allocator_alloc(size, None, stream))
+    monkeypatch.setattr(ops, "_give_back", torch.cuda.caching_allocator_delete)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    mass, graph = c["mass"].to(cuda_device), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.dense_decode_mass(q, *c["table"], most, mass, 0.75, mass_out=torch.empty_like(mass), status=status, view=c["view"])
+    got[1].copy_(mass)
+    graph.replay()
+    ops.raise_on_status(status)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))

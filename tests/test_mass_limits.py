@@ -2,6 +2,7 @@
 import random
 import re
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -71,3 +72,11 @@ def test_kernels_share_their_limits_of_shared_memory():
     sources = [p for suffix in ("cu", "cuh") for p in CSRC.rglob(f"*.{suffix}")]
     assert [p.name for p in sources if "cudaFuncAttributeMaxDynamicSharedMemorySize" in p.read_text()] == ["ktk_host.cu"]
     assert sum("allow_shared(" in p.read_text() for p in sources) > 15
+
+
+def test_the_package_needs_no_private_names_of_torch():
+    names = ("_cuda_getDevice", "_cuda_getCurrentRawStream", "_cuda_cudaCachingAllocator_raw_alloc", "_cuda_cudaCachingAllocator_raw_delete")
+    for gone in (names, *((name,) for name in names)):
+        code = (f"import torch\nfor name in {gone!r}:\n    if hasattr(torch._C, name):\n        delattr(torch._C, name)\n"
+                "from kinetics_b200 import ops\nassert all(map(callable, (ops._current_device, ops._current_stream, ops._take, ops._give_back)))\n")
+        subprocess.run([sys.executable, "-c", code], check=True, cwd=CSRC.parent.parent)
