@@ -440,6 +440,14 @@ def _decode_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dty
     return shp, pages, int(_lib.load().ktk_decode_mass_workspace_bytes(shp, max_pages, pages))
 
 
+def _prefill_mass_need(shp, total_new, max_new, places, pages, window):
+    """(pages of the longest list, workspace bytes)"""
+    most = places // PAGE_SIZE + 2                     # a longer list than mass has places for is an error
+    if pages >= 0:
+        most = max(min(most, pages), 1)
+    return most, int(_lib.load().ktk_prefill_mass_workspace_bytes(shp, total_new, max_new, most, pages, window))
+
+
 @functools.lru_cache(maxsize=1024)
 def _prefill_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dtype, slots, padded, tables, max_new, window):
     """(sizes, pages of the longest list, of all lists or -1, workspace bytes, launches)"""
@@ -447,10 +455,7 @@ def _prefill_mass_plan(q_shape, q_dtype, kv_shape, kv_dtype, mass_shape, mass_dt
     batch = tables[3][2] - 1
     shp = _mass_shape(batch, kv_shape, kv_dtype, q_shape[1], mass_shape, mass_dtype, slots, tables)
     pages = -1 if padded else tables[0][2]
-    most = mass_shape[2] // PAGE_SIZE + 2              # a longer list than mass has places for is an error
-    if not padded:
-        most = max(min(most, pages), 1)
-    need = int(_lib.load().ktk_prefill_mass_workspace_bytes(shp, q_shape[0], max_new, most, pages, window))
+    most, need = _prefill_mass_need(shp, q_shape[0], max_new, mass_shape[2], pages, window)
     # attention, sums, and where the workspace has parts of them beside the rows' 16 bytes, their addition
     parts = need > (q_shape[0] * q_shape[1] * 16 + 255) // 256 * 256
     return shp, most, pages, need, 3 if parts else 2
@@ -489,15 +494,31 @@ def _same(t, like, what) -> None:
         raise TypeError(f"{what} must have the dtype and shape {like.dtype} {tuple(like.shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
+def _size_shape(batch, num_kv_heads, group_size, dtype) -> Shape:
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"kinetics_b200: dtype {dtype} not supported (float32 or bfloat16)")
+    return Shape(batch, num_kv_heads, group_size, HEAD_DIM, PAGE_SIZE, _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32, 0)
+
+
 def decode_mass_workspace_bytes(batch: int, num_kv_heads: int, group_size: int, max_pages_per_seq: int, dtype=torch.bfloat16,
                                 total_pages: int = -1, fewer: bool = False) -> int:
     """Bytes of workspace that ``dense_decode_mass`` needs; total_pages: entries of all page lists (-1, and always with a
     view.page_count: batch * max_pages_per_seq).  The need goes with the form that the number of sequences calls for and does not grow with
     it; fewer: what is enough for a call of any number of sequences up to ``batch``."""
-    code = _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32
-    need = lambda n: int(_lib.load().ktk_decode_mass_workspace_bytes(Shape(n, num_kv_heads, group_size, HEAD_DIM, PAGE_SIZE, code, 0),
-                                                                     max_pages_per_seq, total_pages))
+    need = lambda n: int(_lib.load().ktk_decode_mass_workspace_bytes(_size_shape(n, num_kv_heads, group_size, dtype), max_pages_per_seq, total_pages))
     return max(map(need, range(1, batch + 1)), default=0) if fewer else need(batch)
+
+
+def prefill_mass_workspace_bytes(batch: int, total_new_tokens: int, max_new_tokens: int, num_kv_heads: int, group_size: int, places: int,
+                                 dtype=torch.bfloat16, total_pages: int = -1, window: int = 0) -> int:
+    """Bytes of workspace that ``prefill_attention_mass`` needs for these sizes; places: of a row of mass, total_pages: length of kv_indices (-1
+    with a view.page_count).  Smaller sizes may need more: one for several has the most of theirs."""
+    return _prefill_mass_need(_size_shape(batch, num_kv_heads, group_size, dtype), total_new_tokens, max_new_tokens, places, total_pages, window)[1]
+
+
+def evict_workspace_bytes(batch: int, num_kv_heads: int, max_pages_per_seq: int, keep: int) -> int:
+    """Bytes of workspace that ``evict`` needs for these sizes.  Smaller sizes may need more: one for several has the most of theirs."""
+    return int(_lib.load().ktk_evict_workspace_bytes(_size_shape(batch, num_kv_heads, 1, torch.bfloat16), max_pages_per_seq, keep))
 
 
 def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: int, mass, decay: float = 1.0,
@@ -507,7 +528,7 @@ def dense_decode_mass(q, kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_
     mass fp32 [rows, Hkv, places]: what the query heads of a group have paid the token in each place of its sequence
     (row: view.slot_index, else the sequence's number; different rows for different sequences).  Writes
     decay * mass + the weights of this step, and the weights alone for the newest token, to mass_out (None: mass itself);
-    places behind a sequence's length are left as they are.  workspace: ``ktk_decode_mass_workspace_bytes`` bytes, not shared
+    places behind a sequence's length are left as they are.  workspace: ``decode_mass_workspace_bytes`` bytes, not shared
     by calls that may overlap (None: from the allocator, which keeps streams and graphs apart).  Returns (out, mass_out)."""
     q_shape, mass_shape = q.shape, mass.shape
     shp, pages, need = _decode_mass_plan(q_shape, q.dtype, kv_cache.shape, kv_cache.dtype, mass_shape, mass.dtype,
@@ -543,8 +564,8 @@ def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indice
                            window: int = 0, decay: float = 1.0, sm_scale: Optional[float] = None, mass_out=None,
                            workspace=None, out=None, status=None, view=None):
     """``prefill_attention`` that also accumulates the weights that the last ``window`` new tokens of every sequence (0: all
-    of them) give each cached token; mass and workspace as in ``dense_decode_mass``, the sequence's new tokens start from their
-    weights alone.  Returns (out, mass_out)."""
+    of them) give each cached token; mass as in ``dense_decode_mass``, the sequence's new tokens start from their weights alone.
+    workspace: ``prefill_mass_workspace_bytes`` bytes, as there.  Returns (out, mass_out)."""
     q_shape, mass_shape = q.shape, mass.shape
     i_, p_, l_, *more = _tables(q_indptr.numel() - 1, kv_indices, kv_indptr, kv_last_page_len, view)
     shp, most, pages, need, launches = _prefill_mass_plan(q_shape, q.dtype, kv_cache.shape, kv_cache.dtype, mass_shape, mass.dtype,
@@ -588,7 +609,7 @@ def evict(kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: 
     [rows, Hkv, places]: where the tokens of the first stored[row] places were in the sequence; those behind were appended in
     order, up to position seen[row] - 1 (stored, seen: int32 [rows]).  Afterwards a sequence holds min(n, keep) tokens: that
     is ``stored`` of the next call, and what the next page table has to say.  Page summaries have to be rebuilt.
-    workspace: ``ktk_evict_workspace_bytes`` bytes, as in ``dense_decode_mass``.  Returns (mass_out, positions_out)."""
+    workspace: ``evict_workspace_bytes`` bytes, as in ``dense_decode_mass``.  Returns (mass_out, positions_out)."""
     batch, mass_shape = _batch_of(kv_indptr, view), mass.shape
     rows = mass_shape[0]
     shp, need = _evict_plan(batch, kv_cache.shape, kv_cache.dtype, mass_shape, mass.dtype, positions.shape,

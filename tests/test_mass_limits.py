@@ -8,7 +8,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from kinetics_b200 import EvictingKVManager, ops
+from kinetics_b200 import EvictingKVManager, _lib, ops
 
 CSRC = Path(__file__).resolve().parent.parent / "kinetics_b200" / "csrc"
 
@@ -80,3 +80,19 @@ def test_the_package_needs_no_private_names_of_torch():
         code = (f"import torch\nfor name in {gone!r}:\n    if hasattr(torch._C, name):\n        delattr(torch._C, name)\n"
                 "from kinetics_b200 import ops\nassert all(map(callable, (ops._current_device, ops._current_stream, ops._take, ops._give_back)))\n")
         subprocess.run([sys.executable, "-c", code], check=True, cwd=CSRC.parent.parent)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_workspaces_are_sized_from_python(dtype):
+    i32, lib, code = (lambda n: (torch.int32, None, n)), _lib.load(), _lib.KTK_BF16 if dtype == torch.bfloat16 else _lib.KTK_F32
+    for batch, new, most_new, heads, group, places, pages, window in ((1, 512, 512, 8, 4, 3000, 160, 64), (6, 3000, 700, 8, 8, 2600, 500, 0), (3, 7, 5, 2, 1, 90, -1, 0)):
+        q, kv, mass = torch.Size((new, heads * group, 128)), torch.Size((999, 2, 16, heads, 128)), torch.Size((batch, heads, places))
+        tables = (i32(pages if pages >= 0 else 77), i32(batch + 1), i32(batch), i32(batch + 1))
+        need = ops._prefill_mass_plan(q, dtype, kv, dtype, mass, torch.float32, False, pages < 0, tables, most_new, window)[3]
+        assert need > 0 and ops.prefill_mass_workspace_bytes(batch, new, most_new, heads, group, places, dtype, pages, window) == need
+    shape = lambda n: _lib.Shape(n, 8, 4, 128, 16, code, 999)
+    for batch, most, keep in ((1, 144, 2048), (48, 144, 2048), (2, 2048, 4096), (1, 40000, 4096)):
+        assert ops.evict_workspace_bytes(batch, 8, most, keep) == lib.ktk_evict_workspace_bytes(shape(batch), most, keep)
+    assert ops.evict_workspace_bytes(48, 8, 144, 2048) > 0 == ops.evict_workspace_bytes(1, 8, 144, 2048)
+    with pytest.raises(TypeError, match="not supported"):
+        ops.prefill_mass_workspace_bytes(1, 1, 1, 1, 1, 16, torch.float16)
