@@ -603,6 +603,8 @@ KTK_API int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr, i
  * The kept tokens behind place `keep` move, in their order, into the places in front of it that became free, in theirs: only their
  * keys, values, masses and positions are copied.  Attention does not depend on the order of cached tokens.  The sequence then
  * holds min(n, keep) tokens: the caller's next page table says so.  Summaries of its pages (ktk_build_summaries) are out of date.
+ * Pages are written in place: those of a sequence with more than `keep` tokens are in no other list, in this call or outside it (a prefix that
+ * sequences share is copied first).
  *   positions_in  int32 [mass->rows, Hkv, mass->stride]: positions of the tokens in the first stored[row] places; the token in
  *                 place t >= stored[row] of n was appended in order and has position seen[row] - n + t
  *   positions_out the same array, or memory apart from it: receives the positions of all min(n, keep) places

@@ -608,7 +608,8 @@ def evict(kv_cache, kv_indices, kv_indptr, kv_last_page_len, max_pages_per_seq: 
     positions of the kept places go to mass_out and positions_out (None: mass and positions themselves).  positions int32
     [rows, Hkv, places]: where the tokens of the first stored[row] places were in the sequence; those behind were appended in
     order, up to position seen[row] - 1 (stored, seen: int32 [rows]).  Afterwards a sequence holds min(n, keep) tokens: that
-    is ``stored`` of the next call, and what the next page table has to say.  Page summaries have to be rebuilt.
+    is ``stored`` of the next call, and what the next page table has to say.  Page summaries have to be rebuilt.  Pages are written
+    in place: those of a sequence that is cut must be in no other sequence's list (copy a shared prefix first).
     workspace: ``evict_workspace_bytes`` bytes, as in ``dense_decode_mass``.  Returns (mass_out, positions_out)."""
     batch, mass_shape = _batch_of(kv_indptr, view), mass.shape
     rows = mass_shape[0]
