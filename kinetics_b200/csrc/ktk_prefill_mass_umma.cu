@@ -288,7 +288,7 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.s_free[m]);
             // columns that see the key, and those that are rows at all
-            const int c_lo = (t - s.base_pos - tok0) * G, c_hi = (s.n_new - tok0) * G;
+            const int c_lo = max(t - s.base_pos - tok0, 0) * G, c_hi = (s.n_new - tok0) * G;
             uint64_t acc[4] = {0, 0, 0, 0};
             auto sum = [&](auto masked) {
 #pragma unroll

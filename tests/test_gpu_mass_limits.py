@@ -316,3 +316,29 @@ def test_calls_by_the_public_names_of_torch(cuda_device, monkeypatch):
     graph.replay()
     ops.raise_on_status(status)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_prompt_behind_more_than_2_28_tokens(cuda_device):
+    """Rows are counted in (token, head) pairs: eight heads behind 2^28 tokens pass 31 bits.  The cache is five pages, listed over and over.
+    A weight's error: the denominators add 2^18 blocks of keys a CTA, half a step of 2^-23 of their sum each (2^-6); the rest is below 2^-10."""
+    from kinetics_b200 import ops
+    g = torch.Generator().manual_seed(51)
+    n, G = 2 ** 28 + 40, 8
+    kv = (0.3 * torch.randn(5, 2, 16, 1, D, generator=g)).to(torch.bfloat16)
+    q = torch.randn(1, G, D, generator=g).to(torch.bfloat16)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda_device)
+    pages, status = (n + 15) // 16, ops.new_status(cuda_device)
+    indices = torch.arange(pages, device=cuda_device, dtype=torch.int32) % 5
+    mass = torch.zeros(1, 1, n + 8, device=cuda_device)
+    ops.prefill_attention_mass(q.to(cuda_device), i32(0, 1), 1, kv.to(cuda_device), indices, i32(0, pages), i32(n - 16 * (pages - 1)), mass, status=status)
+    ops.raise_on_status(status)
+    # the 80 tokens of the five pages, each listed `often` times
+    score = torch.einsum("gd,td->gt", q[0].double(), kv[:, 0, :, 0].reshape(80, D).double()) * D ** -0.5
+    often = torch.full((80,), n // 80, dtype=torch.float64)
+    often[:n % 80] += 1
+    weight = score.exp()
+    want = (weight / (weight * often).sum(1, keepdim=True)).sum(0).to(cuda_device)
+    for first in range(0, n - 80, 80 * 2 ** 20):                         # piece by piece
+        got = mass[0, 0, first:min(first + 80 * 2 ** 20, n // 80 * 80)].view(-1, 80).double()
+        assert bool(((got - want).abs() <= 2.0 ** -5 * want).all()), (first, float(((got - want) / want).abs().max()))
+    assert not mass[0, 0, n:].any()
