@@ -8,7 +8,7 @@
 //   the balanced partition (bf16) or splits (fp32): the decode kernels write the scores down as they go (4 G bytes per token beside
 //     the 512 of its bf16 key and value), and mass_finish_kernel turns them into weights.  It also merges the pieces of lists that
 //     the decode cut.
-// Bound by HBM: 48 lists of 1790 to 2303 tokens, 32 heads over 8, 80 us (5.1 TB/s), 32 of 16 K 359 (5.8 TB/s); one of 517 tokens 7.6, a
+// Bound by HBM: 48 lists of 1790 to 2303 tokens, 32 heads over 8, 80 us (5.1 TB/s), 32 of 16 K 359 (5.8 TB/s); one of 517 tokens 7.7, a
 // chain of loads.
 #include <type_traits>
 
@@ -234,6 +234,9 @@ static int mass_cluster(const ktk_shape* s, int max_pages) {
     // The balanced partition where it would leave its longest CTA far fewer pages.  Pages of a CTA, even share, us with clusters and
     // balanced: 48 sequences of 2304 tokens and 8 kv heads 144, 93, 78.6 and 76.2; 55 of 1500 94, 70, 60.8 and 65.6; 48 of 2304 and one
     // kv head 18, 12, 17.5 and 27.1; one of 8192 and 8 kv heads 64, 7, 18.7 and 20.6; one of 32768 256, 28, 53.8 and 34.8.
+    // It follows these, and misses the faster form in places between them.  Lists of 2049 to 2304 tokens, clusters and balanced, * what the rule
+    // takes: 8 kv heads, 8 sequences 18.8* and 23.8 us, 9 30.8* and 25.0, 10 24.1 and 26.9*, 11 24.7* and 29.3, 16 29.5* and 36.2, 20 39.8 and
+    // 43.0*, 24 43.0* and 46.6, 48 76.8 and 80.5*; 4 kv heads, 16 20.8* and 32.7, 20 25.9 and 35.8*, 24 27.4* and 40.2, 48 45.8* and 58.8.
     const int64_t mine = (max_pages + best - 1) / best, even = units * max_pages / (4 * sms);
     return 100 * mine <= 145 * even + 100 * (units * best >= 2 * sms ? 8 : 56) ? best : 0;
 }
