@@ -586,7 +586,7 @@ KTK_API int ktk_dense_decode_mass(const void* q, const void* kv_cache, const int
  *                stay as they are
  *   sm_scale     at least 1e-30
  *   workspace    ktk_prefill_mass_workspace_bytes() bytes: the rows' denominators, and sums over parts of the rows
- * q, kv_cache, o and workspace are 16-byte aligned.
+ * q, kv_cache, o and workspace are 16-byte aligned; q and o lie apart.
  */
 KTK_API size_t ktk_prefill_mass_workspace_bytes(const ktk_shape* shape, int64_t total_new_tokens, int32_t max_new_tokens,
                                                 int64_t max_pages_per_seq, int64_t total_pages, int32_t window);

@@ -62,6 +62,12 @@ extern "C" int ktk_prefill_attention_mass(const void* q, const int32_t* q_indptr
         set_error("%s: null pointer argument", who);
         return KTK_ERR_ARG;
     }
+    // the attention may be done with a query when it writes its output, the weights are not
+    const size_t bytes = (size_t)total_new_tokens * s->num_kv_heads * s->group_size * kHeadDim * (s->dtype == KTK_F32 ? 4 : 2);
+    if ((uintptr_t)q < (uintptr_t)o + bytes && (uintptr_t)o < (uintptr_t)q + bytes) {
+        set_error("%s: q and o overlap", who);
+        return KTK_ERR_ARG;
+    }
     void* lse = workspace;
     PrefillMassParams p{};
     p.q = q; p.o = o; p.cache = kv_cache; p.q_indptr = q_indptr; p.kv_indices = kv_indices; p.kv_indptr = kv_indptr;

@@ -565,7 +565,7 @@ def prefill_attention_mass(q, q_indptr, max_new_tokens: int, kv_cache, kv_indice
                            workspace=None, out=None, status=None, view=None):
     """``prefill_attention`` that also accumulates the weights that the last ``window`` new tokens of every sequence (0: all
     of them) give each cached token; mass as in ``dense_decode_mass``, the sequence's new tokens start from their weights alone.
-    workspace: ``prefill_mass_workspace_bytes`` bytes, as there.  Returns (out, mass_out)."""
+    workspace: ``prefill_mass_workspace_bytes`` bytes, as there.  out lies apart from q.  Returns (out, mass_out)."""
     q_shape, mass_shape = q.shape, mass.shape
     i_, p_, l_, *more = _tables(q_indptr.numel() - 1, kv_indices, kv_indptr, kv_last_page_len, view)
     shp, most, pages, need, launches = _prefill_mass_plan(q_shape, q.dtype, kv_cache.shape, kv_cache.dtype, mass_shape, mass.dtype,

@@ -96,3 +96,18 @@ def test_workspaces_are_sized_from_python(dtype):
     assert ops.evict_workspace_bytes(48, 8, 144, 2048) > 0 == ops.evict_workspace_bytes(1, 8, 144, 2048)
     with pytest.raises(TypeError, match="not supported"):
         ops.prefill_mass_workspace_bytes(1, 1, 1, 1, 1, 16, torch.float16)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_a_prompts_outputs_may_not_lie_on_its_queries(dtype):
+    """The weights read the queries again.  Addresses are never dereferenced: what is not refused fails at the launch, which has no device."""
+    lib, shape, one = _lib.load(), _lib.Shape(1, 2, 4, 128, 16, dtype, 8), 1 << 20
+    bytes_ = 5 * 8 * 128 * (2 if dtype else 4)
+
+    def call(o):
+        return lib.ktk_prefill_attention_mass(one, 4096, 5, 5, 4096, 4096, 4096, 4096, None, 4, -1, 0, 0.1, _lib.Mass(4096, 4096, 64, 1, 1.0), o, 4096,
+                                              1 << 20, shape, None, None)
+    for o in (one, one + 256, one - 256, one + bytes_ - 16, one - bytes_ + 16):
+        assert call(o) == -1 and b"q and o overlap" in lib.ktk_last_error()
+    if not torch.cuda.is_available():
+        assert call(one + bytes_) != -1 and call(one - bytes_) != -1
