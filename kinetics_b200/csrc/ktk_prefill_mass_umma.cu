@@ -108,6 +108,11 @@ __device__ __forceinline__ bool find_group(const PrefillMassParams& p, int group
     return false;
 }
 
+// Whether all groups of the sequence of group `item` are among the launch's: else its masses stay as they are
+__device__ __forceinline__ bool all_groups(const MassSequence& s, int item, int group, int items) {
+    return item - group + (s.sp.n_pages + 2 * kPmPages - 1) / (2 * kPmPages) <= items;
+}
+
 // Tiles of rows of a group of pages: those from the first that sees its first key on, cut into equal parts
 struct PmTiles {
     int first, all, each;
@@ -139,7 +144,7 @@ prefill_mass_umma_kernel(const PrefillMassParams p, const __grid_constant__ CUte
         report(p.status, KTK_STATUS_BAD_TABLE);           // more than the caller's bounds
     if (!find_group(p, item, b, group)) return;           // uniform for the CTA, as all that follows: nothing set up yet
     MassSequence s;
-    if (!mass_sequence(p, b, group == 0 && split == 0 && h == 0, s)) return;
+    if (!mass_sequence(p, b, group == 0 && split == 0 && h == 0, s) || !all_groups(s, item, group, items)) return;
     const int e0 = group * 2 * kPmPages;
     const PmTiles tiles = tiles_of(p, s, group, tpc);
     const int t_begin = tiles.first + split * tiles.each, t_end = min(t_begin + tiles.each, tiles.all);
@@ -348,7 +353,7 @@ prefill_mass_add_kernel(const PrefillMassParams p) {
     const int h = blockIdx.x % p.Hkv, item = blockIdx.x / p.Hkv, tid = threadIdx.x;
     int b, group;
     MassSequence s;
-    if (!find_group(p, item, b, group) || !mass_sequence(p, b, false, s)) return;
+    if (!find_group(p, item, b, group) || !mass_sequence(p, b, false, s) || !all_groups(s, item, group, (int)(gridDim.x / p.Hkv))) return;
     const int e = group * 2 * kPmPages + tid / kPageSize, slot = tid % kPageSize;
     if (e >= s.sp.n_pages || slot >= (e == s.sp.n_pages - 1 ? s.sp.last_fill : (e == 0 ? s.sp.first_fill : kPageSize))) return;
     const int t = page_first_pos(e, s.sp.first_fill) + slot;

@@ -176,6 +176,23 @@ def test_starts_that_do_not_ascend_are_refused(cuda_device):
                                     view=c["view"])
     assert int(status.item()) == 2 and torch.equal(mass.cpu(), c["mass"])
 
+@pytest.mark.parametrize("window", [0, 20])                              # parts of the rows that are added, one part
+def test_lists_beyond_the_bound_of_all_keep_their_masses(cuda_device, window):
+    # eleven groups of sixteen pages where there are three, ten and ten: no sequence is counted in part
+    from kinetics_b200 import _lib
+    c, status = _lists(52, cuda_device, [700, 2400, 2400], 2, 8, torch.bfloat16, False, new=[5, 600, 40]), torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    q, lib = c["q"].to(torch.bfloat16).to(cuda_device), _lib.load()
+    shape, most, total = _lib.Shape(3, 2, 8, D, 16, 1, c["table"][0].shape[0]), 150, 130
+    space = torch.empty(lib.ktk_prefill_mass_workspace_bytes(shape, 645, 600, most, total, window), dtype=torch.uint8, device=cuda_device)
+    mass, out = c["mass"].to(cuda_device), torch.empty_like(q)
+    view = c["view"].c()
+    assert lib.ktk_prefill_attention_mass(
+        q.data_ptr(), c["indptr"].data_ptr(), 645, 600, *(t.data_ptr() for t in c["table"]), view, most, total, window, D ** -0.5,
+        _lib.Mass(mass.data_ptr(), mass.data_ptr(), mass.shape[2], 3, 0.75), out.data_ptr(), space.data_ptr(), space.nbytes, shape, status.data_ptr(),
+        torch.cuda.current_stream().cuda_stream) == 0
+    assert int(status.item()) == 2 and torch.equal(mass[1:].cpu(), c["mass"][1:])
+    _equals(c, 0, out, mass, window, 0.75)
+
 
 # ---------------------------------------------------------------- pages that are none
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
