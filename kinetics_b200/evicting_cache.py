@@ -89,10 +89,17 @@ class EvictingKVManager:
             self._table_key, self._table_val = key, (rows[0], rows[2], ops.PageView(0, 0, rows[1], rows[3]))
         return self._table_val
 
+    def _checked(self, slots) -> List[int]:
+        """A row each: two rows of one slot would append to and count the same places."""
+        slots = [int(s) for s in slots]
+        if len(set(slots)) != len(slots) or any(not 0 <= s < self.max_batch_size for s in slots):
+            raise ValueError(f"slots {slots}: different ones of {self.max_batch_size}")
+        return slots
+
     def _slots_of(self, batch_idx) -> List[int]:
         if self._active is not None and len(self._active) == batch_idx.numel():
             return self._active
-        return [int(s) for s in batch_idx.tolist()]
+        return self._checked(batch_idx.tolist())
 
     def cached(self, slot: int, layer_idx: int = 0) -> int:
         """Tokens that the slot's cache holds."""
@@ -183,13 +190,14 @@ class EvictingKVManager:
 
     # ---- a decode step whose device work can sit in a CUDA graph (Engine.decode_graphed)
     def begin_step(self, slots: Sequence[int]) -> None:
-        self._active = list(slots)
+        """The slots of the calls that follow, in the order of their batch_idx, which is then not read."""
+        self._active = self._checked(slots)
 
     def prepare_step(self, slots: Sequence[int]) -> None:
         """The host work of one decode step over `slots`, and the evictions it needs, of all layers: the step itself is then the
         same launches whatever the lengths, with the page table in buffers whose addresses never change.  `end_step()` closes
         the step."""
-        slots = list(slots)
+        slots = self._checked(slots)
         n = len(slots)
         for layer in range(self.num_layers):
             self._evict(layer, self._full(layer, slots))

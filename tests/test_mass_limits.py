@@ -111,3 +111,17 @@ def test_a_prompts_outputs_may_not_lie_on_its_queries(dtype):
         assert call(o) == -1 and b"q and o overlap" in lib.ktk_last_error()
     if not torch.cuda.is_available():
         assert call(one + bytes_) != -1 and call(one - bytes_) != -1
+
+
+def test_a_slot_has_one_row():
+    class Cfg:
+        hidden_size, num_attention_heads, num_key_value_heads, head_dim, num_hidden_layers = 512, 4, 2, 128, 2
+
+    kv = EvictingKVManager(Cfg, 3, 512, "meta", torch.bfloat16, keep=128)
+    for slots in ([0, 0], [2, 1, 2], [3], [-1]):
+        for call in (kv.begin_step, kv.prepare_step, lambda slots: kv._slots_of(torch.tensor(slots))):
+            with pytest.raises(ValueError, match="different ones of 3"):
+                call(slots)
+    assert not kv._held.any() and not kv._seen.any()
+    kv.begin_step(torch.tensor([2, 0]).tolist())
+    assert kv._active == [2, 0]
