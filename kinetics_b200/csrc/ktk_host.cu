@@ -93,12 +93,16 @@ int check_aligned(std::initializer_list<const void*> pointers, const char* who) 
 cudaError_t raise_shared(const void* kernel, size_t bytes) {
     static std::mutex mu;
     static std::unordered_map<const void*, size_t> most;
-    std::lock_guard<std::mutex> lock(mu);
-    size_t& have = most[kernel];
-    // set on every call: the current device may be another one
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes > have ? bytes : have));
-    if (e == cudaSuccess && bytes > have) have = bytes;
-    return e;
+    try {                                    // nothing is thrown through the C entry points
+        std::lock_guard<std::mutex> lock(mu);
+        size_t& have = most[kernel];
+        // set on every call: the current device may be another one
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes > have ? bytes : have));
+        if (e == cudaSuccess && bytes > have) have = bytes;
+        return e;
+    } catch (...) {
+        return cudaErrorMemoryAllocation;
+    }
 }
 
 int sm_count() {

@@ -74,6 +74,13 @@ def test_kernels_share_their_limits_of_shared_memory():
     assert sum("allow_shared(" in p.read_text() for p in sources) > 15
 
 
+def test_nothing_is_thrown_where_kernels_limits_are_kept():
+    text = (CSRC / "ktk_host.cu").read_text()
+    body = text[text.index("cudaError_t raise_shared("):text.index("int sm_count()")]
+    guarded = body[body.index("try {"):body.index("} catch (...) {")]
+    assert all(x in guarded and x not in body.replace(guarded, "") for x in ("lock_guard", "most[kernel]", "cudaFuncSetAttribute"))
+
+
 def test_the_package_needs_no_private_names_of_torch():
     names = ("_cuda_getDevice", "_cuda_getCurrentRawStream", "_cuda_cudaCachingAllocator_raw_alloc", "_cuda_cudaCachingAllocator_raw_delete")
     for gone in (names, *((name,) for name in names)):
