@@ -580,6 +580,8 @@ KTK_API int ktk_dense_decode_mass(const void* q, const void* kv_cache, const int
  *   out[r, h, t] = decay * in[r, h, t] + sum over the last `window` new tokens and the heads of group h of p(t)
  * for the tokens t that were there before, and without the first term for the sequence's new ones.  window 0: all new tokens.
  * A sequence without new tokens is left as it is.  The results of one with a page id that is none of the cache's (KTK_STATUS_BAD_PAGE) are void.
+ * Values of later new tokens have weights of 0 in the products of up to 128 rows: an infinity or NaN there reaches outputs of the
+ * sequence's earlier ones (masses it does not).
  *   max_new_tokens, max_pages_per_seq, total_pages   upper bounds of one sequence's new tokens, of one list's entries (2^26 at most)
  *                and of all lists' together (-1: batch * max_pages_per_seq, as with view->page_count); they size the grid and the
  *                workspace.  A sequence beyond them, or of tokens outside total_new_tokens, reports KTK_STATUS_BAD_TABLE; its masses
