@@ -62,7 +62,7 @@ class Cfg:
 @pytest.mark.parametrize("dtype, active", [(torch.bfloat16, (16, 10, 16, 10, 3)), (torch.float32, (16, 4, 7, 1, 2))])
 def test_a_manager_of_sixteen_slots_with_fewer_active(cuda_device, dtype, active):
     from kinetics_b200 import EvictingKVManager
-    kv = EvictingKVManager(Cfg, 16, 4096, cuda_device, dtype, keep=2048)
+    kv = EvictingKVManager(Cfg, 16, 4096, cuda_device, dtype, keep=2000)
     g = torch.Generator().manual_seed(31)
     keys, values = ([torch.zeros(0, 8, D) for _ in range(16)] for _ in range(2))
     for n in active:
@@ -86,7 +86,7 @@ def test_an_engine_that_drains_its_slots(cuda_device):
     cfg, dtype = LayerConfig(hidden_size=256, num_attention_heads=8, num_key_value_heads=4, intermediate_size=512, num_hidden_layers=2,
                              vocab_size=503), torch.float32
     g = torch.Generator().manual_seed(32)
-    kv = EvictingKVManager(cfg, 16, 400, cuda_device, dtype, keep=2048)
+    kv = EvictingKVManager(cfg, 16, 400, cuda_device, dtype, keep=2000)
     eng = Engine(DecoderStack(cfg, cuda_device, dtype, max_positions=400, seed=3), kv, 400, cuda_device, temperature=0.0, repeat_check=False)
     prompts = [torch.randint(0, 500, (1, 2 + i), generator=g) for i in range(16)]
     for slot, p in enumerate(prompts):
